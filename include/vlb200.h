@@ -503,6 +503,110 @@ int vlb_router_logits_device(vlb_handle* h, const float* x_dev, const float* w_d
 int vlb_rms_norm_device(vlb_handle* h, const float* x_dev, const float* w_dev, uint32_t rows,
                         uint32_t width, float eps, float* out_dev, void* stream);
 
+/* ---- products on 8-bit integers ------------------------------------------------------------
+ * Element types of the row operators below. */
+enum { VLB_DTYPE_F32 = 0, VLB_DTYPE_F16 = 1, VLB_DTYPE_BF16 = 2, VLB_DTYPE_I8 = 3 };
+
+/* Rows to int8 with one scale each, in 32-bit steps:
+ *     a = max_c |x_rc|,   scale_r = a / 127,   q_rc = rint(x_rc * (127 / a))   (ties to even)
+ * A row of zeros has q = 0 and scale 0; a row that is not finite has q = 0 and scale NaN, so that
+ * products of it are NaN in that row and nowhere else. Weight matrices are quantized by the same
+ * call (rows = output channels). Strides are in elements, 0 = cols. row_index_dev (u32 [rows] or
+ * NULL): row r is x row row_index[r]; an index >= x_rows gives a row of zeros. x_rows 0 = rows.
+ * up_dev (or NULL; type and stride of x): the row is silu(min(x, L)) * clamp(up, -L, L), the
+ * experts' SwiGLU (execute_expert, deepseek_v4_graph.cpp:1826-1895), L = swiglu_limit, 0 = no
+ * clamp. x_type F32, F16 or BF16. Enqueued on `stream` (NULL = the handle's; 1 =
+ * cudaStreamLegacy). */
+int vlb_int8_quantize_device(vlb_handle* h, int x_type, const void* x_dev, uint64_t x_stride, uint64_t x_rows,
+                             const uint32_t* row_index_dev, const void* up_dev, float swiglu_limit, uint32_t rows,
+                             uint32_t cols, int8_t* q_dev, uint64_t q_stride, float* scale_dev, void* stream);
+
+/* y[r][n] = (sum_k q[r][k] w[g][n][k]) * x_scale[r] * w_scale[g][n] (* row_weight[r]): the sum is
+ * exact in 32-bit integers, rounded to f32 once. x_type F32 / F16 / BF16: the rows are quantized
+ * first as vlb_int8_quantize_device does (row_index, up and swiglu_limit as there), into ws.
+ * x_type I8: x holds the integers and x_scale their scales. groups > 1 (or offsets given): rows
+ * offsets[g] .. offsets[g + 1] (device u32 [groups + 1], not falling) use matrix g; rows of y
+ * outside every group are left as they are. Offsets are read on the device and kept inside
+ * [0, rows]. groups <= 1024, cols <= 131071, groups * out_cols < 2^31, rows < 2^31. Any stride and
+ * alignment of the elements' own size works; rows of w (and of int8 x) that start on 16-byte
+ * boundaries (pointer and stride multiples of 16) run on the tensor cores, others do not. y must
+ * not overlap an input. Deterministic. Enqueued on `stream`; nothing is allocated and the host is
+ * not synchronised, so the call can be captured in a graph. */
+typedef struct vlb_int8_linear_desc {
+    const void* x;             /* [x_rows] rows of x_type */
+    uint64_t x_stride;         /* elements; 0 = cols */
+    uint64_t x_rows;           /* rows that row_index may name; 0 = rows */
+    const uint32_t* row_index; /* [rows] or NULL */
+    const void* up;            /* second SwiGLU operand or NULL */
+    const float* x_scale;      /* [rows], x_type I8 only */
+    const float* row_weight;   /* [rows] or NULL (a route weight) */
+    const int8_t* w;           /* [groups x out_cols] rows */
+    const float* w_scale;      /* [groups x out_cols] */
+    uint64_t w_stride;         /* elements; 0 = cols */
+    const uint32_t* offsets;   /* [groups + 1] or NULL (groups == 1: every row) */
+    void* y;                   /* [rows] rows of y_type */
+    uint64_t y_stride;         /* elements; 0 = out_cols */
+    void* ws;                  /* vlb_int8_workspace_bytes(rows, cols), 16-byte aligned; unused for I8 */
+    uint64_t ws_bytes;
+    uint32_t rows;
+    uint32_t cols;             /* K */
+    uint32_t out_cols;         /* N */
+    uint32_t groups;
+    int32_t x_type;
+    int32_t y_type;            /* F32, F16 or BF16 */
+    float swiglu_limit;
+    uint32_t reserved0;
+} vlb_int8_linear_desc;
+uint64_t vlb_int8_workspace_bytes(uint32_t rows, uint32_t cols);
+int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void* stream);
+
+/* The plan of a grouped product from a route (idx u32 [T x k], weights f32 [T x k]): the pairs in
+ * the dispatch's stable order (expert, then token, then slot): row_index_dev [T*k] = the pair's
+ * token, row_weight_dev [T*k] = its weight, elem_row_dev [T*k] = the row of element t * k + slot,
+ * offsets_dev [E + 2] = the experts' starts. ws_dev: vlb_ep_workspace_bytes(T, k, E). An id >= E
+ * returns VLB_ERR_INVALID_FORMAT (one host synchronisation reads the check). */
+int vlb_route_plan_device(vlb_handle* h, const uint32_t* idx_dev, const float* weights_dev, uint32_t T, uint32_t k,
+                          uint32_t E, void* ws_dev, uint32_t* row_index_dev, float* row_weight_dev,
+                          uint32_t* elem_row_dev, uint32_t* offsets_dev, void* stream);
+
+/* ---- the router's load-balance loss ---------------------------------------------------------
+ * For sequence s with n_s live tokens, c_se their (token, slot) pairs on expert e, and the token's
+ * normalised scores p_te = u(z_te) / sum_j u(z_tj) (u = exp, sigmoid or sqrt(softplus) by `score`;
+ * the f64 softmax modes are exp):
+ *     f_se = E c_se / (k n_s),   L = coefficient * mean over sequences with n_s > 0 of
+ *                                    (1 / n_s) sum_t sum_e f_se p_te
+ * loss = L; counts[s][e] = c_se; dlogits = upstream * dL/dz (the counts carry no gradient). A token
+ * is live when mask[t] != 0 (NULL: all) and a sequence holds it; others give nothing, their logits
+ * are not read and their gradient is 0. A slot whose id is >= E was dropped: it is not counted. A
+ * live token whose logits are all -inf counts in n_s, adds 0 and gets gradient 0. No live token:
+ * L = 0. Sums of any order-dependent kind run in a fixed order: equal inputs give equal bits.
+ * E <= 512, k <= 64, k <= E. T = 0 is valid. The reference does not train; its routers' scores are
+ * cited at VLB_SCORE_*. Enqueued on `stream`; allocates nothing and does not synchronise. */
+typedef struct vlb_balance_desc {
+    const void* logits;          /* [T] rows of logits_type */
+    uint64_t logits_stride;      /* elements; 0 = E */
+    const uint32_t* idx;         /* [T x k] */
+    const uint8_t* mask;         /* [T] or NULL */
+    const uint32_t* seq_offsets; /* [n_seqs + 1], not falling, or NULL (n_seqs == 1: every token) */
+    const float* upstream;       /* device scalar, NULL = 1 */
+    float* loss;                 /* device scalar or NULL */
+    uint32_t* counts;            /* [n_seqs x E] */
+    void* dlogits;               /* [T] rows of logits_type, or NULL */
+    uint64_t dlogits_stride;     /* elements; 0 = E */
+    void* ws;                    /* vlb_balance_workspace_bytes(T, E, n_seqs), 16-byte aligned */
+    uint64_t ws_bytes;
+    uint32_t T;
+    uint32_t E;
+    uint32_t k;
+    uint32_t n_seqs;
+    int32_t score;
+    int32_t logits_type;         /* F32, F16 or BF16 */
+    float coefficient;
+    uint32_t reserved0;
+} vlb_balance_desc;
+uint64_t vlb_balance_workspace_bytes(uint32_t T, uint32_t E, uint32_t n_seqs);
+int vlb_balance_loss_device(vlb_handle* h, const vlb_balance_desc* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -43,6 +43,12 @@ TYPE_Q6_K = 14
 TYPE_IQ2_S = 22
 TYPE_MXFP4 = 39
 
+# element types of the row operators
+DTYPE_F32 = 0
+DTYPE_F16 = 1
+DTYPE_BF16 = 2
+DTYPE_I8 = 3
+
 SCORE_SQRT_SOFTPLUS = 0
 SCORE_SIGMOID = 1
 SCORE_SOFTMAX = 2
@@ -124,6 +130,24 @@ class _HcDesc(C.Structure):
                 ("base", C.c_void_p), ("norm_weight", C.c_void_p)]
 
 
+class _Int8LinearDesc(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_uint64), ("x_rows", C.c_uint64), ("row_index", C.c_void_p),
+                ("up", C.c_void_p), ("x_scale", C.c_void_p), ("row_weight", C.c_void_p), ("w", C.c_void_p),
+                ("w_scale", C.c_void_p), ("w_stride", C.c_uint64), ("offsets", C.c_void_p), ("y", C.c_void_p),
+                ("y_stride", C.c_uint64), ("ws", C.c_void_p), ("ws_bytes", C.c_uint64), ("rows", C.c_uint32),
+                ("cols", C.c_uint32), ("out_cols", C.c_uint32), ("groups", C.c_uint32), ("x_type", C.c_int32),
+                ("y_type", C.c_int32), ("swiglu_limit", C.c_float), ("reserved0", C.c_uint32)]
+
+
+class _BalanceDesc(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("logits_stride", C.c_uint64), ("idx", C.c_void_p), ("mask", C.c_void_p),
+                ("seq_offsets", C.c_void_p), ("upstream", C.c_void_p), ("loss", C.c_void_p), ("counts", C.c_void_p),
+                ("dlogits", C.c_void_p), ("dlogits_stride", C.c_uint64), ("ws", C.c_void_p), ("ws_bytes", C.c_uint64),
+                ("T", C.c_uint32), ("E", C.c_uint32), ("k", C.c_uint32), ("n_seqs", C.c_uint32),
+                ("score", C.c_int32), ("logits_type", C.c_int32), ("coefficient", C.c_float),
+                ("reserved0", C.c_uint32)]
+
+
 class _LayerDesc(C.Structure):
     _fields_ = [
         ("hidden", C.c_uint32),
@@ -165,7 +189,9 @@ EXPORTS = (
     "vlb_ep_nccl_version vlb_ep_unique_id vlb_ep_comm_init vlb_ep_comm_destroy vlb_ep_comm_abort "
     "vlb_ep_all_to_all_device vlb_ep_layer_create vlb_ep_layer_destroy vlb_ep_forward_device vlb_ep_last_phases "
     "vlb_upload_record_async vlb_upload_query vlb_upload_finish vlb_host_alloc vlb_host_free "
-    "vlb_layer_set_hyper_connection vlb_layer_last_hyper_split"
+    "vlb_layer_set_hyper_connection vlb_layer_last_hyper_split "
+    "vlb_int8_quantize_device vlb_int8_workspace_bytes vlb_int8_linear_device vlb_route_plan_device "
+    "vlb_balance_workspace_bytes vlb_balance_loss_device"
 ).split()
 
 
@@ -243,6 +269,12 @@ def load_library() -> C.CDLL:
         "vlb_host_free": (I, [P, P]),
         "vlb_layer_set_hyper_connection": (I, [P, P, C.POINTER(_HcDesc)]),
         "vlb_layer_last_hyper_split": (I, [P, P, U32, P, P, P]),
+        "vlb_int8_quantize_device": (I, [P, I, P, U64, U64, P, P, F, U32, U32, P, U64, P, P]),
+        "vlb_int8_workspace_bytes": (U64, [U32, U32]),
+        "vlb_int8_linear_device": (I, [P, C.POINTER(_Int8LinearDesc), P]),
+        "vlb_route_plan_device": (I, [P, P, P, U32, U32, U32, P, P, P, P, P, P]),
+        "vlb_balance_workspace_bytes": (U64, [U32, U32, U32]),
+        "vlb_balance_loss_device": (I, [P, C.POINTER(_BalanceDesc), P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -288,6 +320,30 @@ class Matrix:
     cols: int
     identity: int
     payload_bytes: int
+
+
+@dataclass
+class Int8Weights:
+    """Int8 weight rows on the device: `groups` matrices of `rows` output channels x `cols`, row
+    stride `stride` elements (0: cols), and one f32 scale a channel ([groups x rows]). Rows that
+    start on 16-byte boundaries (address and stride multiples of 16) run on the tensor cores."""
+
+    ptr: int
+    scale_ptr: int
+    rows: int
+    cols: int
+    groups: int = 1
+    stride: int = 0
+
+
+def int8_workspace_bytes(rows: int, cols: int) -> int:
+    """Workspace of one int8 product whose rows are quantized in the call."""
+    return int(load_library().vlb_int8_workspace_bytes(rows, cols))
+
+
+def balance_workspace_bytes(T: int, E: int, n_seqs: int = 1) -> int:
+    """Workspace of one balance-loss call."""
+    return int(load_library().vlb_balance_workspace_bytes(T, E, n_seqs))
 
 
 class DeviceBuffer:
@@ -547,6 +603,121 @@ class Device:
             return ob.download(np.float32, rows * width).reshape(rows, width)
         finally:
             for b in (xb, wb, ob):
+                b.free()
+
+    # -- products on 8-bit integers --
+    def int8_quantize_device(self, x_ptr: int, rows: int, cols: int, q_ptr: int, scale_ptr: int, *,
+                             x_type: int = DTYPE_F32, x_stride: int = 0, x_rows: int = 0, row_index_ptr: int = 0,
+                             up_ptr: int = 0, swiglu_limit: float = 0.0, q_stride: int = 0, stream: int = 0) -> None:
+        """Rows to int8 with one scale each (vlb_int8_quantize_device), on raw device pointers."""
+        self._check(self.lib.vlb_int8_quantize_device(
+            self.h, x_type, x_ptr, x_stride, x_rows, row_index_ptr or None, up_ptr or None, swiglu_limit, rows, cols,
+            q_ptr, q_stride, scale_ptr, stream or None))
+
+    def int8_linear_device(self, weights: Int8Weights, x_ptr: int, rows: int, y_ptr: int, *, x_type: int = DTYPE_F32,
+                           y_type: int = DTYPE_F32, x_stride: int = 0, x_rows: int = 0, row_index_ptr: int = 0,
+                           up_ptr: int = 0, swiglu_limit: float = 0.0, x_scale_ptr: int = 0, row_weight_ptr: int = 0,
+                           offsets_ptr: int = 0, y_stride: int = 0, ws_ptr: int = 0, ws_bytes: int = 0,
+                           stream: int = 0) -> None:
+        """y = x W^T on 8-bit integers (vlb_int8_linear_device) on raw device pointers, enqueued on
+        `stream` (0: the handle's, 1: the legacy default stream). Float rows are quantized in the
+        call and need a workspace (int8_workspace_bytes); int8 rows bring x_scale_ptr."""
+        w = weights
+        st = self.lib.vlb_int8_linear_device(
+            self.h, _Int8LinearDesc(x_ptr, x_stride, x_rows, row_index_ptr, up_ptr, x_scale_ptr, row_weight_ptr, w.ptr,
+                                    w.scale_ptr, w.stride, offsets_ptr, y_ptr, y_stride, ws_ptr, ws_bytes, rows,
+                                    w.cols, w.rows, w.groups, x_type, y_type, swiglu_limit, 0), stream or None)
+        if st:
+            self._check(st)
+
+    def int8_quantize(self, x: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+        """Host form: (q int8 [rows, cols], scale f32 [rows]) of f32 or f16 rows."""
+        x = np.ascontiguousarray(x)
+        if x.dtype not in (np.float32, np.float16) or x.ndim != 2:
+            raise ValueError("x must be a float32 or float16 matrix")
+        rows, cols = x.shape
+        xb, qb, sb = self.to_device(x), self.buffer(max(1, x.size)), self.buffer(max(4, rows * 4))
+        try:
+            self.int8_quantize_device(xb.address, rows, cols, qb.address, sb.address,
+                                      x_type=DTYPE_F16 if x.dtype == np.float16 else DTYPE_F32)
+            self.synchronize()
+            return qb.download(np.int8, rows * cols).reshape(rows, cols), sb.download(np.float32, rows)
+        finally:
+            for b in (xb, qb, sb):
+                b.free()
+
+    def int8_linear(self, weights: Int8Weights, x: np.ndarray) -> np.ndarray:
+        """Host form of one matrix's product: f32 rows [n, cols] -> f32 [n, rows]."""
+        x = np.ascontiguousarray(x, dtype=np.float32)
+        if x.ndim != 2 or x.shape[1] != weights.cols or weights.groups != 1:
+            raise ValueError("x must have `cols` columns, and the weights one matrix")
+        n = x.shape[0]
+        ws = int8_workspace_bytes(n, weights.cols)
+        bufs = [self.to_device(x), self.buffer(max(4, n * weights.rows * 4)), self.buffer(max(16, ws))]
+        try:
+            self.int8_linear_device(weights, bufs[0].address, n, bufs[1].address, ws_ptr=bufs[2].address, ws_bytes=ws)
+            self.synchronize()
+            return bufs[1].download(np.float32, n * weights.rows).reshape(n, weights.rows)
+        finally:
+            for b in bufs:
+                b.free()
+
+    def route_plan_device(self, idx_ptr: int, weights_ptr: int, T: int, k: int, E: int, ws_ptr: int, row_index_ptr: int,
+                          row_weight_ptr: int, elem_row_ptr: int, offsets_ptr: int, stream: int = 0) -> None:
+        """The rows of a grouped product from a route (vlb_route_plan_device), on raw device pointers."""
+        self._check(self.lib.vlb_route_plan_device(self.h, idx_ptr, weights_ptr, T, k, E, ws_ptr, row_index_ptr,
+                                                   row_weight_ptr, elem_row_ptr, offsets_ptr, stream or None))
+
+    # -- the router's balance loss --
+    def balance_loss_device(self, logits_ptr: int, idx_ptr: int, T: int, E: int, k: int, *, counts_ptr: int, ws_ptr: int,
+                            ws_bytes: int, logits_type: int = DTYPE_F32, logits_stride: int = 0,
+                            score: int = SCORE_SOFTMAX, coefficient: float = 1.0, mask_ptr: int = 0,
+                            seq_offsets_ptr: int = 0, n_seqs: int = 1, upstream_ptr: int = 0, loss_ptr: int = 0,
+                            dlogits_ptr: int = 0, dlogits_stride: int = 0, stream: int = 0) -> None:
+        """Load-balance loss, per-expert counts and the logits' gradient (vlb_balance_loss_device) on
+        raw device pointers; a loss or gradient pointer of 0 leaves that output out."""
+        st = self.lib.vlb_balance_loss_device(
+            self.h, _BalanceDesc(logits_ptr, logits_stride, idx_ptr, mask_ptr, seq_offsets_ptr, upstream_ptr, loss_ptr,
+                                 counts_ptr, dlogits_ptr, dlogits_stride, ws_ptr, ws_bytes, T, E, k, n_seqs, score,
+                                 logits_type, coefficient, 0), stream or None)
+        if st:
+            self._check(st)
+
+    def balance_loss(self, logits: np.ndarray, idx: np.ndarray, score: int = SCORE_SOFTMAX, coefficient: float = 1.0,
+                     mask: Optional[np.ndarray] = None, seq_offsets: Optional[np.ndarray] = None,
+                     upstream: float = 1.0):
+        """Host form: (loss, counts u32 [n_seqs, E], dlogits f32 [T, E]) of f32 logits and the routed
+        experts idx [T, k]."""
+        logits = np.ascontiguousarray(logits, dtype=np.float32)
+        idx = np.ascontiguousarray(idx, dtype=np.uint32)
+        T, E = logits.shape
+        if idx.ndim != 2 or idx.shape[0] != T:
+            raise ValueError("idx must have one row for each token")
+        S = 1 if seq_offsets is None else len(seq_offsets) - 1
+        bufs = [self.to_device(logits), self.to_device(idx), self.to_device(np.array([upstream], np.float32)),
+                self.buffer(4), self.buffer(max(4, S * E * 4)), self.buffer(max(4, T * E * 4))]
+        m = o = None
+        ws = balance_workspace_bytes(T, E, S)
+        try:
+            bufs.append(self.buffer(ws))
+            if mask is not None:
+                m = np.ascontiguousarray(mask).astype(np.uint8)
+                if m.shape != (T,):
+                    raise ValueError("mask must have one entry for each token")
+                bufs.append(self.to_device(m))
+                m = bufs[-1].address
+            if seq_offsets is not None:
+                bufs.append(self.to_device(np.ascontiguousarray(seq_offsets, dtype=np.uint32)))
+                o = bufs[-1].address
+            self.balance_loss_device(bufs[0].address, bufs[1].address, T, E, idx.shape[1], counts_ptr=bufs[4].address,
+                                     ws_ptr=bufs[6].address, ws_bytes=ws, score=score, coefficient=coefficient,
+                                     mask_ptr=m or 0, seq_offsets_ptr=o or 0, n_seqs=S, upstream_ptr=bufs[2].address,
+                                     loss_ptr=bufs[3].address, dlogits_ptr=bufs[5].address)
+            self.synchronize()
+            return (float(bufs[3].download(np.float32, 1)[0]), bufs[4].download(np.uint32, S * E).reshape(S, E),
+                    bufs[5].download(np.float32, T * E).reshape(T, E))
+        finally:
+            for b in bufs:
                 b.free()
 
 

@@ -1658,4 +1658,255 @@ int vlb_ep_combine_device(vlb_handle* h, const float* y_rows, const uint32_t* el
     return VLB_OK;
 }
 
+// ---- products on 8-bit integers, route plan, balance loss -----------------------------------------
+
+// Nothing may leave these entries as a C++ exception (a message that cannot be allocated).
+#define VLB_GUARDED(...)                   \
+    try {                                  \
+        __VA_ARGS__                        \
+    } catch (...) {                        \
+        return VLB_ERR_RESOURCE_EXHAUSTED; \
+    }
+
+static size_t dtype_size(int t) {
+    return t == VLB_DTYPE_F32 ? 4 : t == VLB_DTYPE_F16 || t == VLB_DTYPE_BF16 ? 2 : t == VLB_DTYPE_I8 ? 1 : 0;
+}
+static bool float_type(int t) { return t == VLB_DTYPE_F32 || t == VLB_DTYPE_F16 || t == VLB_DTYPE_BF16; }
+static bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+constexpr uint32_t kInt8MaxCols = 131071;  // 128 * 128 * cols stays below 2^31
+
+// The workspace of a product: the int8 rows at a pitch of whole 16-byte pieces, then their scales.
+static size_t int8_pitch(uint32_t cols) { return ((size_t)cols + 15) / 16 * 16; }
+static size_t int8_rows_bytes(uint32_t rows, uint32_t cols) { return ((size_t)rows * int8_pitch(cols) + 255) / 256 * 256; }
+
+uint64_t vlb_int8_workspace_bytes(uint32_t rows, uint32_t cols) {
+    return int8_rows_bytes(rows, cols) + ((uint64_t)rows * 4 + 255) / 256 * 256;
+}
+
+// What is wrong with the float rows of a quantizing call, or null.
+static const char* bad_float_rows(int x_type, const void* x, uint64_t x_stride, uint64_t x_rows,
+                                  const uint32_t* row_index, const void* up, float limit, uint32_t rows, uint32_t cols) {
+    if (!float_type(x_type)) return "x_type must be F32, F16 or BF16";
+    const size_t es = dtype_size(x_type);
+    if (rows && (!x || !aligned(x, es))) return "x is null or not aligned to its elements";
+    if (!aligned(up, es)) return "up is not aligned to its elements";
+    if (!aligned(row_index, 4)) return "row_index is not aligned to its elements";
+    if (x_stride < cols) return "x_stride is below cols";
+    if (!row_index && x_rows < rows) return "x has fewer rows than the call";
+    if (x_rows > 0x7fffffffull || x_stride > (1ull << 40)) return "x is too large";
+    if (!(limit >= 0.f) || !std::isfinite(limit)) return "swiglu_limit must be finite and not negative";
+    return nullptr;
+}
+
+int vlb_int8_quantize_device(vlb_handle* h, int x_type, const void* x, uint64_t x_stride, uint64_t x_rows,
+                             const uint32_t* row_index, const void* up, float swiglu_limit, uint32_t rows,
+                             uint32_t cols, int8_t* q, uint64_t q_stride, float* scale, void* stream) {
+    VLB_GUARDED({
+        VLB_LOCK(h);
+        if (x_stride == 0) x_stride = cols;
+        if (x_rows == 0) x_rows = rows;
+        if (q_stride == 0) q_stride = cols;
+        if (cols == 0 || rows > 0x7fffffffu)
+            return h->fail(VLB_ERR_INVALID_ARGUMENT, "int8 quantize: cols must be positive and rows below 2^31");
+        if (const char* why = bad_float_rows(x_type, x, x_stride, x_rows, row_index, up, swiglu_limit, rows, cols))
+            return h->fail(VLB_ERR_INVALID_ARGUMENT, std::string("int8 quantize: ") + why);
+        if (rows && (!q || !scale || !aligned(scale, 4)))
+            return h->fail(VLB_ERR_INVALID_ARGUMENT, "int8 quantize: q or scale is null or not aligned");
+        if (q_stride < cols || q_stride > (1ull << 40))
+            return h->fail(VLB_ERR_INVALID_ARGUMENT, "int8 quantize: q_stride is out of range");
+        if (rows == 0) return VLB_OK;
+        Int8QuantParams p{};
+        p.x = x;
+        p.up = up;
+        p.row_index = row_index;
+        p.q = q;
+        p.scale = scale;
+        p.x_stride = x_stride;
+        p.q_stride = q_stride;
+        p.x_rows = x_rows;
+        p.rows = rows;
+        p.cols = cols;
+        p.fill_cols = cols;
+        p.limit = swiglu_limit;
+        VLB_CUDA(h, launch_int8_quantize(p, x_type, h->pick(stream)));
+        return VLB_OK;
+    })
+}
+
+int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void* stream) {
+    VLB_GUARDED({
+        VLB_LOCK(h);
+        if (!desc) return h->fail(VLB_ERR_INVALID_ARGUMENT, "int8 linear: null description");
+        vlb_int8_linear_desc d = *desc;
+        if (d.x_stride == 0) d.x_stride = d.cols;
+        if (d.w_stride == 0) d.w_stride = d.cols;
+        if (d.y_stride == 0) d.y_stride = d.out_cols;
+        if (d.x_rows == 0) d.x_rows = d.rows;
+        auto bad = [&](const char* why) { return h->fail(VLB_ERR_INVALID_ARGUMENT, std::string("int8 linear: ") + why); };
+        if (d.cols == 0 || d.out_cols == 0 || d.groups == 0) return bad("cols, out_cols and groups must be positive");
+        if (d.cols > kInt8MaxCols)
+            return h->fail(VLB_ERR_UNSUPPORTED, "int8 linear: a sum of more than 131071 products can pass 32 bits");
+        if (d.groups > kInt8MaxGroups) return h->fail(VLB_ERR_UNSUPPORTED, "int8 linear: more than 1024 groups");
+        if (d.rows > 0x7fffffffu || (uint64_t)d.groups * d.out_cols > 0x7fffffffull)
+            return h->fail(VLB_ERR_UNSUPPORTED, "int8 linear: rows or groups x out_cols pass 2^31");
+        if (d.groups > 1 && !d.offsets) return bad("groups need offsets");
+        if (!float_type(d.y_type)) return bad("y_type must be F32, F16 or BF16");
+        if (!d.w || !d.w_scale || (d.rows && !d.y)) return bad("w, w_scale or y is null");
+        if (!aligned(d.w_scale, 4) || !aligned(d.x_scale, 4) || !aligned(d.row_weight, 4) || !aligned(d.offsets, 4) ||
+            !aligned(d.y, dtype_size(d.y_type)))
+            return bad("a pointer is not aligned to its elements");
+        if (d.w_stride < d.cols || d.y_stride < d.out_cols || d.w_stride > (1ull << 38) || d.y_stride > (1ull << 38))
+            return bad("a stride is out of range");
+        Int8LinearParams p{};
+        p.row_weight = d.row_weight;
+        p.w = d.w;
+        p.w_scale = d.w_scale;
+        p.offsets = d.offsets;
+        p.y = d.y;
+        p.w_stride = d.w_stride;
+        p.y_stride = d.y_stride;
+        p.rows = d.rows;
+        p.cols = d.cols;
+        p.out_cols = d.out_cols;
+        p.groups = d.groups;
+        cudaStream_t s = h->pick(stream);
+        if (d.x_type == VLB_DTYPE_I8) {
+            if (d.row_index || d.up) return bad("int8 rows take neither row_index nor up");
+            if (d.rows && (!d.x || !d.x_scale)) return bad("x or x_scale is null");
+            if (d.x_stride < d.cols || d.x_stride > (1ull << 38)) return bad("a stride is out of range");
+            p.x = static_cast<const int8_t*>(d.x);
+            p.x_scale = d.x_scale;
+            p.x_stride = d.x_stride;
+            if (d.rows == 0) return VLB_OK;
+        } else {
+            if (const char* why =
+                    bad_float_rows(d.x_type, d.x, d.x_stride, d.x_rows, d.row_index, d.up, d.swiglu_limit, d.rows, d.cols))
+                return bad(why);
+            if (d.x_scale) return bad("x_scale belongs to int8 rows");
+            if (d.rows == 0) return VLB_OK;
+            if (!d.ws || !aligned(d.ws, 16) || d.ws_bytes < vlb_int8_workspace_bytes(d.rows, d.cols))
+                return bad("the workspace is null, not 16-byte aligned or below vlb_int8_workspace_bytes");
+            Int8QuantParams q{};
+            q.x = d.x;
+            q.up = d.up;
+            q.row_index = d.row_index;
+            q.q = static_cast<int8_t*>(d.ws);
+            q.scale = reinterpret_cast<float*>(static_cast<char*>(d.ws) + int8_rows_bytes(d.rows, d.cols));
+            q.x_stride = d.x_stride;
+            q.q_stride = int8_pitch(d.cols);
+            q.x_rows = d.x_rows;
+            q.rows = d.rows;
+            q.cols = d.cols;
+            q.fill_cols = (uint32_t)int8_pitch(d.cols);
+            q.limit = d.swiglu_limit;
+            VLB_CUDA(h, launch_int8_quantize(q, d.x_type, s));
+            p.x = q.q;
+            p.x_scale = q.scale;
+            p.x_stride = q.q_stride;
+        }
+        VLB_CUDA(h, launch_int8_linear(p, d.y_type, s));
+        return VLB_OK;
+    })
+}
+
+int vlb_route_plan_device(vlb_handle* h, const uint32_t* idx, const float* weights, uint32_t T, uint32_t k, uint32_t E,
+                          void* ws, uint32_t* row_index, float* row_weight, uint32_t* elem_row, uint32_t* offsets,
+                          void* stream) {
+    VLB_GUARDED({
+        VLB_LOCK(h);
+        if (!offsets || !ws || k == 0 || k > 64 || E == 0 || E > 512 || (uint64_t)T * k > 0x7fffffffull ||
+            (T && (!idx || !weights || !row_index || !row_weight || !elem_row)))
+            return h->fail(VLB_ERR_INVALID_ARGUMENT, "invalid route plan argument");
+        cudaStream_t s = h->pick(stream);
+        if (T == 0) {
+            VLB_CUDA(h, cudaMemsetAsync(offsets, 0, (E + 2) * 4, s));
+            return VLB_OK;
+        }
+        const size_t n = (size_t)T * k;
+        char* w = static_cast<char*>(ws);
+        uint32_t* flag = reinterpret_cast<uint32_t*>(w);
+        uint32_t* slots = reinterpret_cast<uint32_t*>(w + 256);
+        uint32_t* pair_slot = reinterpret_cast<uint32_t*>(w + 256 + ep_round(n * 4));
+        uint32_t* counts = reinterpret_cast<uint32_t*>(w + 256 + 2 * ep_round(n * 4));
+        VLB_CUDA(h, cudaMemsetAsync(flag, 0, 4, s));
+        VLB_CUDA(h, launch_ep_slots(idx, n, E, nullptr, slots, flag, s));
+        MoeParams p{};
+        p.T = T;
+        p.k = k;
+        p.E = E;
+        p.idx = slots;
+        p.weights = const_cast<float*>(weights);
+        p.offsets = offsets;
+        p.pair_token = row_index;
+        p.pair_slot = pair_slot;
+        p.pair_weight = row_weight;
+        p.combine_pairs = elem_row;
+        p.disp_counts = counts;
+        p.has_shared = 0;
+        VLB_CUDA(h, launch_stable_sort(p, s));
+        uint32_t bad = 0;
+        VLB_CUDA(h, cudaMemcpyAsync(&bad, flag, 4, cudaMemcpyDeviceToHost, s));
+        VLB_CUDA(h, cudaStreamSynchronize(s));
+        if (bad) return h->fail(VLB_ERR_INVALID_FORMAT, "a route selects an out-of-range expert");
+        return VLB_OK;
+    })
+}
+
+uint64_t vlb_balance_workspace_bytes(uint32_t T, uint32_t E, uint32_t n_seqs) {
+    (void)T;
+    (void)E;
+    return kBalanceBlocks * 8 + ((uint64_t)n_seqs * 4 + 255) / 256 * 256;
+}
+
+int vlb_balance_loss_device(vlb_handle* h, const vlb_balance_desc* desc, void* stream) {
+    VLB_GUARDED({
+        VLB_LOCK(h);
+        if (!desc) return h->fail(VLB_ERR_INVALID_ARGUMENT, "balance loss: null description");
+        vlb_balance_desc d = *desc;
+        auto bad = [&](const char* why) { return h->fail(VLB_ERR_INVALID_ARGUMENT, std::string("balance loss: ") + why); };
+        if (d.E == 0 || d.k == 0 || d.k > d.E || d.n_seqs == 0) return bad("E, k and n_seqs must be positive and k <= E");
+        if (d.E > 512 || d.k > 64 || (uint64_t)d.T * d.k > 0x7fffffffull || d.n_seqs > (1u << 20))
+            return h->fail(VLB_ERR_UNSUPPORTED, "balance loss: E > 512, k > 64, T x k >= 2^31 or n_seqs > 2^20");
+        if (d.logits_stride == 0) d.logits_stride = d.E;
+        if (d.dlogits_stride == 0) d.dlogits_stride = d.E;
+        if (d.score < VLB_SCORE_SQRT_SOFTPLUS || d.score > VLB_SCORE_SOFTMAX_F64_NORM) return bad("unknown score");
+        if (!float_type(d.logits_type)) return bad("logits_type must be F32, F16 or BF16");
+        if (d.n_seqs > 1 && !d.seq_offsets) return bad("sequences need seq_offsets");
+        if (!d.counts || (d.T && (!d.logits || !d.idx))) return bad("logits, idx or counts is null");
+        const size_t es = dtype_size(d.logits_type);
+        if (!aligned(d.logits, es) || !aligned(d.dlogits, es) || !aligned(d.idx, 4) || !aligned(d.seq_offsets, 4) ||
+            !aligned(d.upstream, 4) || !aligned(d.loss, 4) || !aligned(d.counts, 4))
+            return bad("a pointer is not aligned to its elements");
+        if (d.logits_stride < d.E || d.dlogits_stride < d.E || d.logits_stride > (1ull << 32) ||
+            d.dlogits_stride > (1ull << 32))
+            return bad("a stride is out of range");
+        if (!std::isfinite(d.coefficient)) return bad("the coefficient must be finite");
+        if (!d.ws || !aligned(d.ws, 16) || d.ws_bytes < vlb_balance_workspace_bytes(d.T, d.E, d.n_seqs))
+            return bad("the workspace is null, not 16-byte aligned or below vlb_balance_workspace_bytes");
+        BalanceParams p{};
+        p.logits = d.logits;
+        p.idx = d.idx;
+        p.mask = d.mask;
+        p.seq_offsets = d.seq_offsets;
+        p.upstream = d.upstream;
+        p.loss = d.loss;
+        p.counts = d.counts;
+        p.dlogits = d.dlogits;
+        p.partial = static_cast<double*>(d.ws);
+        p.live = reinterpret_cast<uint32_t*>(p.partial + kBalanceBlocks);
+        p.stride = d.logits_stride;
+        p.grad_stride = d.dlogits_stride;
+        p.T = d.T;
+        p.E = d.E;
+        p.k = d.k;
+        p.S = d.n_seqs;
+        p.score = d.score >= VLB_SCORE_SOFTMAX ? VLB_SCORE_SOFTMAX : d.score;
+        p.logits_type = d.logits_type;
+        p.coefficient = d.coefficient;
+        VLB_CUDA(h, launch_balance(p, h->pick(stream)));
+        return VLB_OK;
+    })
+}
+
 }  // extern "C"

@@ -73,4 +73,52 @@ bool hc_entry_fits(uint32_t m, uint32_t H);
 cudaError_t launch_rms_norm(const float* x, const float* w, uint32_t rows, uint32_t width,
                             float eps, float* out, uint32_t* xmax, double* out_d, cudaStream_t s);
 
+// ---- products on 8-bit integers (vlb_int8.cu) ----
+struct Int8QuantParams {
+    const void* x;             // rows of VLB_DTYPE_F32 / F16 / BF16
+    const void* up;            // SwiGLU's second operand (same type and stride), or null
+    const uint32_t* row_index; // row r is x's row row_index[r] (none there: zeros), or null
+    int8_t* q;
+    float* scale;
+    size_t x_stride, q_stride; // elements
+    uint64_t x_rows;
+    uint32_t rows, cols;
+    uint32_t fill_cols;        // columns written: cols, then zeros
+    float limit;               // SwiGLU clamp, 0: none
+};
+struct Int8LinearParams {
+    const int8_t* x;           // [rows] of x_stride
+    const float* x_scale;
+    const float* row_weight;   // or null
+    const int8_t* w;           // [groups x out_cols] of w_stride
+    const float* w_scale;      // [groups x out_cols]
+    const uint32_t* offsets;   // [groups + 1] or null (one group, every row)
+    void* y;
+    size_t x_stride, w_stride, y_stride;
+    uint32_t rows, cols, out_cols, groups;
+};
+constexpr uint32_t kInt8MaxGroups = 1024;
+cudaError_t launch_int8_quantize(const Int8QuantParams& p, int x_type, cudaStream_t s);
+cudaError_t launch_int8_linear(const Int8LinearParams& p, int y_type, cudaStream_t s);
+
+// ---- the router's balance loss (vlb_balance.cu) ----
+struct BalanceParams {
+    const void* logits;
+    const uint32_t* idx;         // [T x k]
+    const uint8_t* mask;         // [T] or null
+    const uint32_t* seq_offsets; // [S + 1] or null (S == 1, every token)
+    const float* upstream;       // or null: 1
+    float* loss;                 // or null
+    uint32_t* counts;            // [S x E]
+    void* dlogits;               // or null
+    uint32_t* live;              // [S] workspace
+    double* partial;             // [kBalanceBlocks] workspace
+    size_t stride, grad_stride;
+    uint32_t T, E, k, S;
+    int score, logits_type;
+    float coefficient;
+};
+constexpr uint32_t kBalanceBlocks = 1184;  // 8 blocks of 256 threads on each of 148 SMs
+cudaError_t launch_balance(const BalanceParams& p, cudaStream_t s);
+
 }  // namespace vlb
