@@ -190,7 +190,7 @@ EXPORTS = (
     "vlb_ep_all_to_all_device vlb_ep_layer_create vlb_ep_layer_destroy vlb_ep_forward_device vlb_ep_last_phases "
     "vlb_upload_record_async vlb_upload_query vlb_upload_finish vlb_host_alloc vlb_host_free "
     "vlb_layer_set_hyper_connection vlb_layer_last_hyper_split "
-    "vlb_int8_quantize_device vlb_int8_workspace_bytes vlb_int8_linear_device vlb_route_plan_device "
+    "vlb_int8_quantize_device vlb_int8_workspace_bytes vlb_int8_linear_device vlb_int8_status vlb_route_plan_device "
     "vlb_balance_workspace_bytes vlb_balance_loss_device"
 ).split()
 
@@ -272,6 +272,7 @@ def load_library() -> C.CDLL:
         "vlb_int8_quantize_device": (I, [P, I, P, U64, U64, P, P, F, U32, U32, P, U64, P, P]),
         "vlb_int8_workspace_bytes": (U64, [U32, U32]),
         "vlb_int8_linear_device": (I, [P, C.POINTER(_Int8LinearDesc), P]),
+        "vlb_int8_status": (I, [P, P]),
         "vlb_route_plan_device": (I, [P, P, P, U32, U32, U32, P, P, P, P, P, P]),
         "vlb_balance_workspace_bytes": (U64, [U32, U32, U32]),
         "vlb_balance_loss_device": (I, [P, C.POINTER(_BalanceDesc), P]),
@@ -629,6 +630,10 @@ class Device:
                                     w.cols, w.rows, w.groups, x_type, y_type, swiglu_limit, 0), stream or None)
         if st:
             self._check(st)
+
+    def int8_status(self, stream: int = 0) -> None:
+        """Raises if a wait inside an int8 product ran out since the last call (synchronises `stream`)."""
+        self._check(self.lib.vlb_int8_status(self.h, stream or None))
 
     def int8_quantize(self, x: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
         """Host form: (q int8 [rows, cols], scale f32 [rows]) of f32 or f16 rows."""

@@ -1805,7 +1805,17 @@ int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void
             p.x_scale = q.scale;
             p.x_stride = q.q_stride;
         }
-        VLB_CUDA(h, launch_int8_linear(p, d.y_type, s));
+        VLB_CUDA(h, launch_int8_linear(p, d.y_type, d.x_type != VLB_DTYPE_I8, s));
+        return VLB_OK;
+    })
+}
+
+int vlb_int8_status(vlb_handle* h, void* stream) {
+    VLB_GUARDED({
+        VLB_LOCK(h);
+        uint32_t bits = 0;
+        VLB_CUDA(h, int8_take_error(&bits, h->pick(stream)));
+        if (bits) return h->fail(VLB_ERR_INTERNAL_ERROR, "a wait inside an int8 product ran out");
         return VLB_OK;
     })
 }

@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "vlb_launch.h"
+#include "vlb_tcgen05.cuh"
 
 namespace vlb {
 namespace {
@@ -87,6 +88,7 @@ template <typename T, bool SWIGLU>
 __global__ void __launch_bounds__(256) int8_quantize_kernel(const Int8QuantParams p) {
     __shared__ uint32_t top[8];
     const uint32_t tid = threadIdx.x;
+    tc::grid_launch_dependents();
     for (size_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const uint64_t src = p.row_index ? p.row_index[r] : r;
         const bool have = src < p.x_rows;
@@ -182,6 +184,375 @@ __global__ void __launch_bounds__(256) int8_linear_kernel(const Int8LinearParams
     }
 }
 
+// ---- product on the tensor cores ---------------------------------------------------------------
+//
+// D[channel][token] = W X^T by tcgen05.mma kind::i8: a tile is 128 channels (the TMEM lanes) by up
+// to 256 tokens of one group (the columns), so a lane of the epilogue holds one channel's scale and
+// a warp's stores are 32 neighbouring channels of one token; few tokens cost few columns.
+// K runs in chunks of 128 bytes (one 128-byte swizzle row) through a ring of TMA stages.
+// Roles: warps 0-7 epilogue, warp 8 TMA, warp 9 MMA; two accumulators, so a tile's epilogue runs
+// beside the next tile's products. Persistent CTAs, tiles in order, a group's token tiles
+// innermost (its weights come from HBM once).
+// SPLIT: a cluster shares a tile, each CTA a part of K; the partial sums are integers, so their
+// order does not matter, and are added through distributed shared memory.
+
+constexpr uint32_t kMmChannels = 128, kMmMaxTokens = 256, kMmKc = 128;
+constexpr uint32_t kMmEpiWarps = 8, kMmThreads = (kMmEpiWarps + 2) * 32;
+constexpr uint32_t kMmWStage = kMmChannels * kMmKc;
+constexpr uint32_t kMmMaxStages = 12;
+constexpr uint32_t kMmSmemLimit = 227u * 1024u;
+constexpr uint64_t kMmWaitNs = 2000000000ull;
+
+struct Int8MmaParams {
+    CUtensorMap wmap, xmap;
+    Int8LinearParams l;
+    uint32_t width;     // most tokens a tile takes (a multiple of 16)
+    uint32_t box;       // rows of the token operand's TMA box
+    uint32_t stages, x_stage;
+    uint32_t ct, nk;    // channel tiles, K chunks
+    uint32_t tmem_cols, acc_cols;
+    uint32_t split;
+};
+
+// A wait that ran out (a fault of this code: every wait's event is this CTA's own copies or
+// products); sticky until read.
+__device__ uint32_t g_int8_error;
+
+struct MmTile {
+    uint32_t g, row0, count, channel0;
+};
+
+struct MmShared {
+    uint32_t* first;  // [groups + 1] token tiles before group g
+    uint32_t* lo;     // [groups] first row
+    uint32_t* cnt;    // [groups] rows
+    float* scale;     // [2][256] the tile's token scales
+    uint64_t *full, *empty, *acc_full, *acc_empty;
+    uint32_t* tmem;
+    volatile uint32_t* abort;
+};
+
+__host__ __device__ constexpr uint32_t mm_table_bytes(uint32_t groups) { return (3u * groups + 1u) * 4u; }
+__host__ __device__ constexpr uint32_t mm_fixed_bytes(uint32_t groups) {
+    return 2u * kMmMaxTokens * 4u + (2u * kMmMaxStages + 4u) * 8u + 16u + mm_table_bytes(groups) + 16u;
+}
+
+// Bounded: false once the time limit has passed or another role has given up.
+__device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
+    if (tc::mbar_try(bar, parity)) return true;
+    const uint64_t t0 = tc::global_ns();
+    for (;;) {
+        for (uint32_t i = 0; i < 64u; ++i) {
+            if (tc::mbar_try(bar, parity)) return true;
+            if (*abort) return false;
+        }
+        if (tc::global_ns() - t0 > kMmWaitNs) return false;
+    }
+}
+
+__device__ __forceinline__ void mm_fail(volatile uint32_t* abort) {
+    *abort = 1u;
+    atomicOr(&g_int8_error, 1u);
+}
+
+__device__ __forceinline__ MmTile mm_tile(const MmShared& sh, const Int8MmaParams& p, uint32_t t) {
+    const uint32_t u = t / p.ct;
+    uint32_t a = 0, b = p.l.groups;  // last g with first[g] <= u; groups without rows have no tiles
+    while (b - a > 1u) {
+        const uint32_t mid = (a + b) / 2u;
+        if (sh.first[mid] <= u) a = mid;
+        else b = mid;
+    }
+    const uint32_t tt = sh.first[a + 1] - sh.first[a], local = t - sh.first[a] * p.ct;
+    const uint32_t c = local / tt, j = local - c * tt;
+    const uint32_t n = sh.cnt[a];  // balanced: the group's tiles differ by one row at most
+    const uint32_t from = (uint32_t)((uint64_t)n * j / tt), to = (uint32_t)((uint64_t)n * (j + 1u) / tt);
+    return MmTile{a, sh.lo[a] + from, to - from, c * kMmChannels};
+}
+
+// One K chunk's operands: 128 rows of w, and the tile's tokens in boxes (rows past the tile's are
+// loaded and not used; past the matrix the TMA unit fills zeros, also past K).
+__device__ __forceinline__ void mm_load_w(const Int8MmaParams& p, uint32_t smem, uint64_t* full, const MmTile& t,
+                                          uint32_t boxes, uint32_t kc) {
+    tc::mbar_arrive_expect_tx(full, kMmWStage + boxes * p.box * kMmKc);
+    tc::tma_load_2d(smem, &p.wmap, (int32_t)(kc * kMmKc), (int32_t)(t.g * p.l.out_cols + t.channel0), full);
+}
+__device__ __forceinline__ void mm_load_x(const Int8MmaParams& p, uint32_t smem, uint64_t* full, const MmTile& t,
+                                          uint32_t boxes, uint32_t kc) {
+    for (uint32_t b = 0; b < boxes; ++b)
+        tc::tma_load_2d(smem + kMmWStage + b * p.box * kMmKc, &p.xmap, (int32_t)(kc * kMmKc),
+                        (int32_t)(t.row0 + b * p.box), full);
+}
+
+template <typename TY>
+__device__ __forceinline__ void mm_store(const Int8LinearParams& l, uint32_t row, uint32_t n, int32_t acc, float s,
+                                         float t) {
+    static_cast<TY*>(l.y)[(size_t)row * l.y_stride + n] = from_float<TY>((float)acc * s * t);
+}
+
+template <typename TY, bool SPLIT>
+__global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_constant__ Int8MmaParams p) {
+    extern __shared__ __align__(1024) unsigned char mm_smem[];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t smem = tc::smem_u32(mm_smem), stage_bytes = kMmWStage + p.x_stage;
+    const Int8LinearParams& l = p.l;
+    MmShared sh;
+    {
+        unsigned char* at = mm_smem + p.stages * stage_bytes;
+        sh.scale = reinterpret_cast<float*>(at);
+        sh.full = reinterpret_cast<uint64_t*>(at + 2u * kMmMaxTokens * 4u);
+        sh.empty = sh.full + kMmMaxStages;
+        sh.acc_full = sh.empty + kMmMaxStages;
+        sh.acc_empty = sh.acc_full + 2;
+        sh.tmem = reinterpret_cast<uint32_t*>(sh.acc_empty + 2);
+        sh.abort = sh.tmem + 1;
+        sh.first = sh.tmem + 4;
+        sh.lo = sh.first + l.groups + 1;
+        sh.cnt = sh.lo + l.groups;
+    }
+    if (smem & 1023u) {  // the swizzle atoms need it; the same in every CTA of the launch
+        if (tid == 0) atomicOr(&g_int8_error, 2u);
+        return;
+    }
+    if (warp == kMmEpiWarps) tc::tmem_alloc(sh.tmem, p.tmem_cols);
+    if (tid == 0) {
+        for (uint32_t i = 0; i < p.stages; ++i) {
+            tc::mbar_init(sh.full + i, 1);
+            tc::mbar_init(sh.empty + i, 1);
+        }
+        for (uint32_t i = 0; i < 2u; ++i) {
+            tc::mbar_init(sh.acc_full + i, 1);
+            tc::mbar_init(sh.acc_empty + i, kMmEpiWarps);
+        }
+        *sh.abort = 0;
+        tc::mbar_fence_init();
+    }
+    for (uint32_t g = tid; g < l.groups; g += kMmThreads) {
+        uint32_t lo, hi;
+        group_range(l, g, lo, hi);
+        sh.lo[g] = lo;
+        sh.cnt[g] = hi - lo;
+    }
+    __syncthreads();
+    if (warp == kMmEpiWarps + 1u) {
+        // token tiles before each group, 32 groups a step
+        uint32_t run = 0;
+        for (uint32_t g0 = 0; g0 < l.groups; g0 += 32u) {
+            const uint32_t g = g0 + lane;
+            const uint32_t tiles = g < l.groups ? (sh.cnt[g] + p.width - 1u) / p.width : 0u;
+            uint32_t incl = tiles;
+#pragma unroll
+            for (uint32_t d = 1; d < 32u; d <<= 1) {
+                const uint32_t v = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= d) incl += v;
+            }
+            if (g < l.groups) sh.first[g] = run + incl - tiles;
+            run += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) sh.first[l.groups] = run;
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = *sh.tmem;
+    const uint32_t total = sh.first[l.groups] * p.ct;
+    const uint32_t rank = SPLIT ? tc::cluster_rank() : 0u;
+    const uint32_t step = SPLIT ? gridDim.x / p.split : gridDim.x;
+    const uint32_t begin = SPLIT ? blockIdx.x / p.split : blockIdx.x;
+    const uint32_t k_lo = SPLIT ? p.nk * rank / p.split : 0u, k_hi = SPLIT ? p.nk * (rank + 1u) / p.split : p.nk;
+    const uint32_t nk = k_hi - k_lo;
+    bool dirty = false, pending = false;  // copies / products under way when a role gave up
+    uint32_t pending_bar = 0, pending_parity = 0;
+
+    // ---- roles; in SPLIT mode each returns to the common tile loop after one tile -------------
+    uint32_t stage = 0, phase = 0, it = 0;
+    bool waited = false;  // on the kernel ahead
+    auto next_stage = [&] {
+        if (++stage == p.stages) stage = 0, phase ^= 1u;
+    };
+    auto produce = [&](uint32_t t) -> bool {
+        const MmTile tile = mm_tile(sh, p, t);
+        const uint32_t boxes = (tile.count + p.box - 1u) / p.box;
+        dirty = true;
+        uint32_t done = 0;
+        if (!waited) {
+            // the weights are no kernel's output: the first stages' are on their way while the
+            // kernel ahead still quantizes the tokens
+            done = nk < p.stages ? nk : p.stages;
+            for (uint32_t i = 0; i < done; ++i)
+                mm_load_w(p, smem + i * stage_bytes, sh.full + i, tile, boxes, k_lo + i);
+            tc::grid_dependency_wait();
+            waited = true;
+            for (uint32_t i = 0; i < done; ++i) {
+                mm_load_x(p, smem + i * stage_bytes, sh.full + i, tile, boxes, k_lo + i);
+                next_stage();
+            }
+        }
+        for (uint32_t i = done; i < nk; ++i) {
+            if (!mm_wait(sh.empty + stage, phase ^ 1u, sh.abort)) return false;
+            mm_load_w(p, smem + stage * stage_bytes, sh.full + stage, tile, boxes, k_lo + i);
+            mm_load_x(p, smem + stage * stage_bytes, sh.full + stage, tile, boxes, k_lo + i);
+            next_stage();
+        }
+        dirty = false;
+        return true;
+    };
+    auto multiply = [&](uint32_t t) -> bool {
+        const MmTile tile = mm_tile(sh, p, t);
+        const uint32_t buf = SPLIT ? 0u : it & 1u, use = SPLIT ? it : it >> 1;
+        if (!SPLIT && !mm_wait(sh.acc_empty + buf, (use & 1u) ^ 1u, sh.abort)) return false;
+        tc::fence_after_sync();
+        const uint32_t idesc = tc::idesc_i8(kMmChannels, (tile.count + 15u) & ~15u);
+        const uint32_t acc = tmem + buf * p.acc_cols;
+        for (uint32_t i = 0; i < nk; ++i) {
+            if (!mm_wait(sh.full + stage, phase, sh.abort)) return false;
+            tc::fence_after_sync();
+            const uint32_t ws = smem + stage * stage_bytes, xs = ws + kMmWStage;
+            pending = true;
+            pending_bar = buf;
+            pending_parity = use & 1u;
+#pragma unroll
+            for (uint32_t ks = 0; ks < kMmKc / 32u; ++ks)
+                tc::mma_i8(acc, tc::sw128_desc(ws + ks * 32u), tc::sw128_desc(xs + ks * 32u), idesc, (i | ks) ? 1u : 0u);
+            tc::mma_commit(sh.empty + stage);
+            next_stage();
+        }
+        tc::mma_commit(sh.acc_full + buf);
+        pending = false;
+        ++it;
+        return true;
+    };
+    const uint32_t quad = warp & 3u, half = warp >> 2;
+    auto epilogue = [&](uint32_t t) -> bool {
+        const MmTile tile = mm_tile(sh, p, t);
+        const uint32_t buf = it & 1u, use = it >> 1;
+        float* ts = sh.scale + buf * kMmMaxTokens;
+        if (!waited) {
+            tc::grid_dependency_wait();
+            waited = true;
+        }
+        if (tid < tile.count) {
+            const uint32_t r = tile.row0 + tid;
+            ts[tid] = l.row_weight ? l.x_scale[r] * l.row_weight[r] : l.x_scale[r];
+        }
+        const uint32_t n = tile.channel0 + 32u * quad + lane;
+        const float cs = n < l.out_cols ? l.w_scale[(size_t)tile.g * l.out_cols + n] : 0.f;
+        asm volatile("bar.sync 1, %0;" ::"n"(kMmEpiWarps * 32) : "memory");
+        const bool ok = __all_sync(0xffffffffu, mm_wait(sh.acc_full + buf, use & 1u, sh.abort));
+        if (ok) {
+            tc::fence_after_sync();
+            const uint32_t src = tmem + buf * p.acc_cols + ((32u * quad) << 16);
+            for (uint32_t c = 16u * half; c < tile.count; c += 32u) {
+                float v[16];
+                tc::tmem_ld16(src + c, v);
+                tc::tmem_wait_ld();
+                TY* y = static_cast<TY*>(l.y) + (size_t)(tile.row0 + c) * l.y_stride + n;
+                const uint32_t m = min(16u, tile.count - c);
+#pragma unroll
+                for (uint32_t i = 0; i < 16u; ++i)
+                    if (i < m && n < l.out_cols)
+                        y[i * l.y_stride] = from_float<TY>((float)__float_as_int(v[i]) * ts[c + i] * cs);
+            }
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(sh.acc_empty + buf);
+            ++it;
+        }
+        return ok;
+    };
+
+    if (!SPLIT) {
+        if (warp < kMmEpiWarps) {
+            // after a role has given up the epilogue warps still walk every tile (their waits end at
+            // once), so that all of them meet at each tile's named barrier
+            for (uint32_t t = begin; t < total; t += step)
+                if (!epilogue(t) && lane == 0) mm_fail(sh.abort);
+        } else if (warp == kMmEpiWarps) {
+            if (lane == 0)
+                for (uint32_t t = begin; t < total; t += step)
+                    if (!produce(t)) {
+                        mm_fail(sh.abort);
+                        break;
+                    }
+        } else if (lane == 0) {
+            for (uint32_t t = begin; t < total; t += step)
+                if (!multiply(t)) {
+                    mm_fail(sh.abort);
+                    break;
+                }
+        }
+    } else {
+        int32_t* part = reinterpret_cast<int32_t*>(mm_smem);  // [token][128], over the idle ring
+        for (uint32_t t = begin; t < total; t += step) {
+            // every CTA of the cluster takes part in both barriers of every tile, also after a
+            // role has given up
+            const MmTile tile = mm_tile(sh, p, t);
+            bool ok = true;
+            if (warp == kMmEpiWarps) {
+                if (lane == 0) ok = *sh.abort ? false : produce(t);
+            } else if (warp == kMmEpiWarps + 1u) {
+                if (lane == 0) ok = *sh.abort ? false : multiply(t);
+            } else {
+                if (!waited) {
+                    tc::grid_dependency_wait();
+                    waited = true;
+                }
+                ok = __all_sync(0xffffffffu, *sh.abort == 0 && mm_wait(sh.acc_full, it & 1u, sh.abort));
+                ++it;
+                if (ok) {
+                    tc::fence_after_sync();
+                    const uint32_t src = tmem + ((32u * quad) << 16);
+                    for (uint32_t c = 16u * half; c < tile.count; c += 32u) {
+                        float v[16];
+                        tc::tmem_ld16(src + c, v);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (uint32_t i = 0; i < 16u; ++i)
+                            part[(c + i) * kMmChannels + 32u * quad + lane] = __float_as_int(v[i]);
+                    }
+                    tc::fence_before_sync();
+                }
+            }
+            if (!ok && (warp < kMmEpiWarps ? lane == 0 : true)) mm_fail(sh.abort);
+            __syncwarp();
+            tc::cluster_sync();
+            if (warp < kMmEpiWarps) {
+                const uint32_t c = 32u * quad + lane, n = tile.channel0 + c;
+                const float cs = n < l.out_cols ? l.w_scale[(size_t)tile.g * l.out_cols + n] : 0.f;
+                for (uint32_t j = rank * 2u + half; j < tile.count; j += 2u * p.split) {
+                    const uint32_t at = smem + (j * kMmChannels + c) * 4u;
+                    int32_t sum = 0;
+                    for (uint32_t r = 0; r < p.split; ++r) sum += (int32_t)tc::cluster_ld(at, r);
+                    const uint32_t row = tile.row0 + j;
+                    const float s = l.row_weight ? l.x_scale[row] * l.row_weight[row] : l.x_scale[row];
+                    if (n < l.out_cols) mm_store<TY>(l, row, n, sum, s, cs);
+                }
+            }
+            tc::fence_proxy_async();
+            tc::fence_after_sync();
+            tc::cluster_sync();
+        }
+    }
+    __syncthreads();
+    if (warp == kMmEpiWarps && lane == 0 && dirty) {
+        // after giving up: copies already issued land before the CTA's shared memory goes away
+        const uint64_t t0 = tc::global_ns();
+        while (tc::global_ns() - t0 < 1000000ull) {
+        }
+    }
+    if (warp == kMmEpiWarps + 1u && lane == 0 && pending) {
+        tc::mma_commit(sh.acc_full + pending_bar);
+        const uint64_t t0 = tc::global_ns();
+        while (!tc::mbar_try(sh.acc_full + pending_bar, pending_parity) && tc::global_ns() - t0 < kMmWaitNs) {
+        }
+    }
+    __syncthreads();
+    if (warp == kMmEpiWarps) {
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tmem, p.tmem_cols);
+    }
+}
+
 template <typename T>
 cudaError_t quantize_type(const Int8QuantParams& p, cudaStream_t s) {
     const unsigned grid = p.rows < 65535u ? p.rows : 65535u;
@@ -193,11 +564,157 @@ cudaError_t quantize_type(const Int8QuantParams& p, cudaStream_t s) {
 }
 
 template <typename TY>
-cudaError_t linear_type(const Int8LinearParams& p, cudaStream_t s) {
+cudaError_t general_type(const Int8LinearParams& p, cudaStream_t s) {
     const uint32_t tiles_n = (p.out_cols + kGenTile - 1u) / kGenTile, tiles_r = (p.rows + kGenTile - 1u) / kGenTile;
     const dim3 grid(tiles_n, tiles_r < 1024u ? tiles_r : 1024u, p.groups < 1024u ? p.groups : 1024u);
     int8_linear_kernel<TY><<<grid, 256, 0, s>>>(p);
     return cudaGetLastError();
+}
+
+template <typename K>
+cudaError_t smem_once(K kernel, size_t bytes) {
+    static std::mutex mu;
+    static std::vector<std::pair<int, const void*>> done;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mu);
+    for (auto& d : done)
+        if (d.first == dev && d.second == (const void*)kernel) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done.emplace_back(dev, (const void*)kernel);
+    return e;
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(f);
+    });
+    return fn;
+}
+
+// Rows of bytes read as boxes of 128 columns x box_rows with the 128-byte swizzle.
+bool encode_rows(CUtensorMap* map, const int8_t* base, uint64_t rows, uint64_t cols, uint64_t stride, uint32_t box_rows) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {cols, rows};
+    const cuuint64_t strides[1] = {stride};
+    const cuuint32_t box[2] = {kMmKc, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool tma_rows(const int8_t* p, size_t stride) {
+    return reinterpret_cast<uintptr_t>(p) % 16u == 0 && stride % 16u == 0;
+}
+
+uint32_t round16(uint32_t v) { return (v + 15u) / 16u * 16u; }
+
+// Tile width and split of a product on the tensor cores.
+void mma_plan(Int8MmaParams& p, uint32_t sms) {
+    const Int8LinearParams& l = p.l;
+    p.ct = (l.out_cols + kMmChannels - 1u) / kMmChannels;
+    p.nk = (l.cols + kMmKc - 1u) / kMmKc;
+    const uint32_t used = l.groups < l.rows ? l.groups : l.rows;
+    const uint32_t mean = (l.rows + used - 1u) / used;
+    const auto split_of = [&](uint64_t tiles) {
+        uint32_t split = 1;
+        while (split < 8u && tiles * split * 2u <= sms && p.nk >= split * 2u) split *= 2u;
+        return split;
+    };
+    if (l.groups == 1) {
+        // the width whose waves of tiles pass the fewest columns x K chunks; one tile of tokens
+        // where they fit one (narrower ones would read the weights again)
+        uint64_t best = ~0ull;
+        const uint32_t most = round16(l.rows < kMmMaxTokens ? l.rows : kMmMaxTokens);
+        for (uint32_t w = most; w >= 128u || w == most; w -= 16u) {
+            const uint64_t n = (l.rows + w - 1u) / w, tiles = n * p.ct, waves = (tiles + sms - 1u) / sms;
+            const uint32_t balanced = round16((uint32_t)((l.rows + n - 1u) / n)), split = split_of(tiles);
+            const uint64_t cost = waves * balanced * ((p.nk + split - 1u) / split);
+            if (cost < best) best = cost, p.width = w, p.split = split;
+            if (w == most && l.rows <= kMmMaxTokens) break;
+        }
+    } else {
+        // unknown rows a group: room for the usual spread around the mean, or a second tile would
+        // read the group's weights again
+        uint32_t spread = 1;
+        while (spread * spread < mean) ++spread;
+        const uint32_t want = round16(mean + 3u * spread);
+        p.width = want < kMmMaxTokens ? want : kMmMaxTokens;
+        p.split = split_of((uint64_t)used * ((mean + p.width - 1u) / p.width) * p.ct);
+    }
+    p.box = p.width < 64u ? p.width : 64u;
+    p.x_stage = (p.width + p.box - 1u) / p.box * p.box * kMmKc;
+    p.acc_cols = p.width < 32u ? 32u : p.width;
+    p.tmem_cols = 32;
+    while (p.tmem_cols < (p.split > 1 ? 1u : 2u) * p.acc_cols) p.tmem_cols *= 2u;
+    const uint32_t room = kMmSmemLimit - 1024u - mm_fixed_bytes(l.groups);
+    p.stages = room / (kMmWStage + p.x_stage);
+    if (p.stages > kMmMaxStages) p.stages = kMmMaxStages;
+}
+
+template <typename TY, bool SPLIT>
+cudaError_t mma_launch(const Int8MmaParams& p, uint32_t sms, bool after_quantize, cudaStream_t s) {
+    auto* kernel = int8_mma_kernel<TY, SPLIT>;
+    cudaError_t e = smem_once(kernel, kMmSmemLimit);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[2];
+    cfg.gridDim = dim3(sms / p.split * p.split);
+    cfg.blockDim = dim3(kMmThreads);
+    cfg.dynamicSmemBytes = p.stages * (kMmWStage + p.x_stage) + mm_fixed_bytes(p.l.groups);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    if (SPLIT) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = p.split;
+        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    if (after_quantize) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
+    }
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+uint32_t sm_count() {
+    static uint32_t n = 0;
+    if (n == 0) {
+        int dev = 0, v = 0;
+        if (cudaGetDevice(&dev) == cudaSuccess &&
+            cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0)
+            n = (uint32_t)v;
+    }
+    return n ? n : 148u;
+}
+
+template <typename TY>
+cudaError_t linear_type(const Int8LinearParams& l, bool after_quantize, cudaStream_t s) {
+    if (tma_rows(l.w, l.w_stride) && tma_rows(l.x, l.x_stride)) {
+        Int8MmaParams p{};
+        p.l = l;
+        const uint32_t sms = sm_count();
+        mma_plan(p, sms);
+        if (encode_rows(&p.wmap, l.w, (uint64_t)l.groups * l.out_cols, l.cols, l.w_stride, kMmChannels) &&
+            encode_rows(&p.xmap, l.x, l.rows, l.cols, l.x_stride, p.box))
+            return p.split > 1 ? mma_launch<TY, true>(p, sms, after_quantize, s)
+                               : mma_launch<TY, false>(p, sms, after_quantize, s);
+    }
+    return general_type<TY>(l, s);
 }
 
 }  // namespace
@@ -211,13 +728,21 @@ cudaError_t launch_int8_quantize(const Int8QuantParams& p, int x_type, cudaStrea
     }
 }
 
-cudaError_t launch_int8_linear(const Int8LinearParams& p, int y_type, cudaStream_t s) {
+cudaError_t launch_int8_linear(const Int8LinearParams& p, int y_type, bool after_quantize, cudaStream_t s) {
     switch (y_type) {
-        case VLB_DTYPE_F32: return linear_type<float>(p, s);
-        case VLB_DTYPE_F16: return linear_type<__half>(p, s);
-        case VLB_DTYPE_BF16: return linear_type<__nv_bfloat16>(p, s);
+        case VLB_DTYPE_F32: return linear_type<float>(p, after_quantize, s);
+        case VLB_DTYPE_F16: return linear_type<__half>(p, after_quantize, s);
+        case VLB_DTYPE_BF16: return linear_type<__nv_bfloat16>(p, after_quantize, s);
         default: return cudaErrorInvalidValue;
     }
+}
+
+cudaError_t int8_take_error(uint32_t* bits, cudaStream_t s) {
+    void* at = nullptr;
+    cudaError_t e = cudaGetSymbolAddress(&at, g_int8_error);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(bits, at, 4, cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaMemsetAsync(at, 0, 4, s);
+    return e == cudaSuccess ? cudaStreamSynchronize(s) : e;
 }
 
 }  // namespace vlb

@@ -99,7 +99,10 @@ struct Int8LinearParams {
 };
 constexpr uint32_t kInt8MaxGroups = 1024;
 cudaError_t launch_int8_quantize(const Int8QuantParams& p, int x_type, cudaStream_t s);
-cudaError_t launch_int8_linear(const Int8LinearParams& p, int y_type, cudaStream_t s);
+// after_quantize: launch_int8_quantize went before it on the stream (the product may start beside it)
+cudaError_t launch_int8_linear(const Int8LinearParams& p, int y_type, bool after_quantize, cudaStream_t s);
+// reads and clears the error bits of the products on the current device (synchronises s)
+cudaError_t int8_take_error(uint32_t* bits, cudaStream_t s);
 
 // ---- the router's balance loss (vlb_balance.cu) ----
 struct BalanceParams {

@@ -145,6 +145,17 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
         : "memory");
 }
 
+// The same for signed 8-bit integers, 32-bit integer accumulators (K = 32 per instruction).
+__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // 32 lanes x 16 columns of 32-bit values from registers: thread i of the warp writes its TMEM
 // lane's 16 consecutive columns.
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -229,6 +240,40 @@ __host__ __device__ constexpr uint32_t idesc_f16(uint32_t M, uint32_t N) {
     return (1u << 4)            // D format f32 (A and B format 0 = f16)
            | ((N >> 3) << 17)   // N / 8
            | ((M >> 4) << 24);  // M / 16
+}
+
+// Instruction descriptor, kind::i8: signed A and B, 32-bit integer accumulator.
+__host__ __device__ constexpr uint32_t idesc_i8(uint32_t M, uint32_t N) {
+    return (2u << 4)             // D format s32
+           | (1u << 7)           // A signed
+           | (1u << 10)          // B signed
+           | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+
+// ---- a grid that may start before the kernel ahead of it has ended ------------------------------
+// Waits for that kernel's end and its writes (nothing to wait for in an ordinary launch).
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets a dependent grid start once every block of this one has got here.
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
+
+// ---- thread-block clusters ------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// All threads of the cluster; shared-memory writes before it are seen by the peers after it.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// 32 bits from the shared memory of block `rank` of the cluster, at this block's address `addr`.
+__device__ __forceinline__ uint32_t cluster_ld(uint32_t addr, uint32_t rank) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u32 %0, [a];\n\t}"
+                 : "=r"(v)
+                 : "r"(addr), "r"(rank)
+                 : "memory");
+    return v;
 }
 
 }  // namespace tc
