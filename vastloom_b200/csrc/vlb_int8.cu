@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 
 #include <mutex>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -42,13 +43,14 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
 }
 
 // silu(g) * u with the clamp of the layer's experts (gate from above, up on both sides). The
-// comparisons keep a NaN, which fminf / fmaxf would drop.
+// comparisons keep a NaN, which fminf / fmaxf would drop. The quotient by the approximate
+// reciprocal is within 2 units of 2^-23; a gate below -87 gives 0 (its true value is under 1e-35).
 __device__ __forceinline__ float swiglu(float g, float u, float limit) {
     if (limit > 0.f) {
         g = g > limit ? limit : g;
         u = u > limit ? limit : (u < -limit ? -limit : u);
     }
-    return g / (1.f + expf(-g)) * u;
+    return __fdividef(g, 1.f + expf(-g)) * u;
 }
 
 // ---- row quantizer ---------------------------------------------------------------------------
@@ -108,6 +110,179 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(const Int8QuantParam
         for (uint32_t c = tid; c < p.fill_cols; c += blockDim.x) {
             const bool in = have && c < p.cols;
             p.q[r * p.q_stride + c] = (int8_t)(in ? quant_byte(row_value<T, SWIGLU>(p, base + c), st) : 0u);
+        }
+    }
+}
+
+// ---- row quantizer, rows on 16-byte boundaries ---------------------------------------------------
+//
+// HBM-bound: every element is read once (16 bytes a load) and kept in registers between the row's
+// maximum and its rounding; rows longer than the registers hold are read twice, the second time
+// mostly from L2. A warp takes a row of up to 8 loads a lane (8 rows a CTA: no barrier, all loads
+// in flight at once); longer rows, and calls of too few rows to fill the GPU with warps, take a
+// CTA a row.
+
+template <typename T>
+struct RowVec {
+    static constexpr uint32_t kN = 16u / sizeof(T);
+    uint4 raw;
+    __device__ __forceinline__ void load(const T* p) { raw = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void clear() { raw = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ float get(uint32_t i) const {
+        const uint32_t w = (&raw.x)[i * sizeof(T) / 4u];
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+        else if constexpr (std::is_same<T, __half>::value)
+            return __half2float(__ushort_as_half((unsigned short)(i & 1u ? w >> 16 : w & 0xffffu)));
+        else
+            return __uint_as_float(i & 1u ? w & 0xffff0000u : w << 16);
+    }
+    // the last vector of a row that ends inside it
+    __device__ __forceinline__ void load_part(const T* p, uint32_t n) {
+        clear();
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i)
+            if (i < n) {
+                if constexpr (sizeof(T) == 4) (&raw.x)[i] = __float_as_uint(p[i]);
+                else {
+                    const uint32_t v = reinterpret_cast<const unsigned short*>(p)[i];
+                    (&raw.x)[i / 2u] |= i & 1u ? v << 16 : v;
+                }
+            }
+    }
+};
+
+// Largest |x| of a vector, as float bits. 16-bit types compare two magnitudes an instruction; their
+// bit patterns order like their values, a NaN above infinity.
+template <typename T>
+struct RowMax {
+    uint32_t m = 0;
+    __device__ __forceinline__ void add(const RowVec<T>& v) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            const uint32_t w = (&v.raw.x)[i];
+            m = sizeof(T) == 4 ? max(m, w & 0x7fffffffu) : __vmaxu2(m, w & 0x7fff7fffu);
+        }
+    }
+    __device__ __forceinline__ uint32_t bits() const {
+        if constexpr (sizeof(T) == 4) return m;
+        const uint32_t top = max(m & 0xffffu, m >> 16);
+        if constexpr (std::is_same<T, __half>::value)
+            return __float_as_uint(__half2float(__ushort_as_half((unsigned short)top)));
+        return top << 16;
+    }
+};
+
+// A vector's bytes at q; `n` of them (N but at a row's end).
+template <uint32_t N>
+__device__ __forceinline__ void store_bytes(int8_t* q, const float (&x)[N], const RowStep& st, uint32_t n) {
+    uint32_t w[N / 4];
+#pragma unroll
+    for (uint32_t i = 0; i < N; i += 4u) {
+        uint32_t b[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; ++j) b[j] = __float_as_uint(__fadd_rn(__fmul_rn(x[i + j], st.inv), 12582912.f));
+        w[i / 4u] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    }
+    if (n < N) {
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i)
+            if (i < n) q[i] = (int8_t)(w[i / 4u] >> (8u * (i % 4u)));
+    } else if constexpr (N == 8) *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(q) = w[0];
+}
+
+// ROW: threads of a row (32 or the CTA's 256); KEEP: vectors a thread keeps.
+template <typename T, bool SWIGLU, uint32_t ROW, uint32_t KEEP>
+__global__ void __launch_bounds__(256) int8_quantize_vec_kernel(const Int8QuantParams p) {
+    constexpr uint32_t N = RowVec<T>::kN;
+    __shared__ uint32_t top[8];
+    tc::grid_launch_dependents();
+    const uint32_t tid = threadIdx.x % ROW;
+    const uint32_t vecs = (p.cols + N - 1u) / N, all = (p.fill_cols + N - 1u) / N;  // of x; of q
+    for (size_t r = (size_t)blockIdx.x * (256u / ROW) + threadIdx.x / ROW; r < p.rows;
+         r += (size_t)gridDim.x * (256u / ROW)) {
+        const uint64_t src = p.row_index ? p.row_index[r] : r;
+        const uint32_t have = src < p.x_rows ? vecs : 0u;
+        const T* x = static_cast<const T*>(p.x) + src * p.x_stride;
+        const T* up = SWIGLU ? static_cast<const T*>(p.up) + src * p.x_stride : nullptr;
+        auto fetch = [&](const T* row, uint32_t v) {
+            RowVec<T> a;
+            if (v >= have) a.clear();
+            else if ((v + 1u) * N <= p.cols) a.load(row + (size_t)v * N);
+            else a.load_part(row + (size_t)v * N, p.cols - v * N);
+            return a;
+        };
+        RowVec<T> a[KEEP];
+        float f[SWIGLU ? KEEP : 1][N];
+        uint32_t m = 0;
+        if constexpr (SWIGLU) {
+            RowVec<T> b[KEEP];
+#pragma unroll
+            for (uint32_t i = 0; i < KEEP; ++i) {
+                a[i] = fetch(x, tid + i * ROW);
+                b[i] = fetch(up, tid + i * ROW);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < KEEP; ++i)
+#pragma unroll
+                for (uint32_t j = 0; j < N; ++j) {
+                    f[i][j] = swiglu(a[i].get(j), b[i].get(j), p.limit);
+                    m = max(m, __float_as_uint(f[i][j]) & 0x7fffffffu);
+                }
+            for (uint32_t v = tid + KEEP * ROW; v < have; v += ROW) {
+                const RowVec<T> c = fetch(x, v), d = fetch(up, v);
+#pragma unroll
+                for (uint32_t j = 0; j < N; ++j)
+                    m = max(m, __float_as_uint(swiglu(c.get(j), d.get(j), p.limit)) & 0x7fffffffu);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < KEEP; ++i) a[i] = fetch(x, tid + i * ROW);
+            RowMax<T> t;
+#pragma unroll
+            for (uint32_t i = 0; i < KEEP; ++i) t.add(a[i]);
+            for (uint32_t v = tid + KEEP * ROW; v < have; v += ROW) t.add(fetch(x, v));
+            m = t.bits();
+        }
+        m = __reduce_max_sync(0xffffffffu, m);
+        if constexpr (ROW == 256) {
+            __syncthreads();
+            if ((tid & 31u) == 0) top[tid >> 5] = m;
+            __syncthreads();
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) m = max(m, top[i]);
+        }
+        const RowStep st = row_step(m);
+        if (tid == 0) p.scale[r] = st.scale;
+        int8_t* q = p.q + r * p.q_stride;
+        auto put = [&](uint32_t v, float (&y)[N]) {
+            if (st.lift != 1.f) {  // a row of zeros, of tiny values, or not finite
+#pragma unroll
+                for (uint32_t j = 0; j < N; ++j) y[j] = st.inv == 0.f ? 0.f : y[j] * st.lift;
+            }
+            store_bytes<N>(q + (size_t)v * N, y, st, min(N, p.fill_cols - v * N));
+        };
+#pragma unroll
+        for (uint32_t i = 0; i < KEEP; ++i) {
+            const uint32_t v = tid + i * ROW;
+            if (v < all) {
+                float y[N];
+#pragma unroll
+                for (uint32_t j = 0; j < N; ++j) {
+                    if constexpr (SWIGLU) y[j] = f[i][j];
+                    else y[j] = a[i].get(j);
+                }
+                put(v, y);
+            }
+        }
+        for (uint32_t v = tid + KEEP * ROW; v < all; v += ROW) {
+            const RowVec<T> c = fetch(x, v);
+            RowVec<T> d = c;
+            if constexpr (SWIGLU) d = fetch(up, v);
+            float y[N];
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j) y[j] = SWIGLU ? swiglu(c.get(j), d.get(j), p.limit) : c.get(j);
+            put(v, y);
         }
     }
 }
@@ -553,14 +728,34 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
     }
 }
 
+template <typename T, bool SWIGLU>
+cudaError_t quantize_rows(const Int8QuantParams& p, cudaStream_t s) {
+    constexpr uint32_t N = RowVec<T>::kN;
+    auto on = [](const void* at, size_t stride_bytes, size_t n) {
+        return reinterpret_cast<uintptr_t>(at) % n == 0 && stride_bytes % n == 0;
+    };
+    const bool vec = on(p.x, p.x_stride * sizeof(T), 16) && on(p.up, 0, 16) && on(p.q, p.q_stride, N);
+    if (!vec) {
+        int8_quantize_kernel<T, SWIGLU><<<p.rows < 65535u ? p.rows : 65535u, 256, 0, s>>>(p);
+    } else if (p.cols <= 32u * 8u * N && p.rows >= 2048u) {
+        const uint32_t grid = (p.rows + 7u) / 8u;
+        if (p.cols <= 32u * 4u * N)
+            int8_quantize_vec_kernel<T, SWIGLU, 32, 4><<<grid, 256, 0, s>>>(p);
+        else
+            int8_quantize_vec_kernel<T, SWIGLU, 32, 8><<<grid, 256, 0, s>>>(p);
+    } else {
+        const uint32_t grid = p.rows < 65535u ? p.rows : 65535u;
+        if (p.cols <= 256u * 2u * N)
+            int8_quantize_vec_kernel<T, SWIGLU, 256, 2><<<grid, 256, 0, s>>>(p);
+        else
+            int8_quantize_vec_kernel<T, SWIGLU, 256, 4><<<grid, 256, 0, s>>>(p);
+    }
+    return cudaGetLastError();
+}
+
 template <typename T>
 cudaError_t quantize_type(const Int8QuantParams& p, cudaStream_t s) {
-    const unsigned grid = p.rows < 65535u ? p.rows : 65535u;
-    if (p.up)
-        int8_quantize_kernel<T, true><<<grid, 256, 0, s>>>(p);
-    else
-        int8_quantize_kernel<T, false><<<grid, 256, 0, s>>>(p);
-    return cudaGetLastError();
+    return p.up ? quantize_rows<T, true>(p, s) : quantize_rows<T, false>(p, s);
 }
 
 template <typename TY>
