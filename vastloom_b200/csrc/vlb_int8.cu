@@ -368,9 +368,12 @@ __global__ void __launch_bounds__(256) int8_linear_kernel(const Int8LinearParams
 // Roles: warps 0-7 epilogue, warp 8 TMA, warp 9 MMA; two accumulators, so a tile's epilogue runs
 // beside the next tile's products. Persistent CTAs, tiles in order, a group's token tiles
 // innermost (its weights come from HBM once).
+// PAIR: two CTAs share a tile of 256 channels (cta_group::2): each loads its own 128 channels and half
+// the tokens, which is two thirds of the operand bytes a CTA alone takes from L2 for the same products.
 // SPLIT: a cluster shares a tile, each CTA a part of K; the partial sums are integers, so their
 // order does not matter, and are added through distributed shared memory.
 
+enum class Mm { kOne, kSplit, kPair };
 constexpr uint32_t kMmChannels = 128, kMmMaxTokens = 256, kMmKc = 128;
 constexpr uint32_t kMmEpiWarps = 8, kMmThreads = (kMmEpiWarps + 2) * 32;
 constexpr uint32_t kMmWStage = kMmChannels * kMmKc;
@@ -384,6 +387,7 @@ struct Int8MmaParams {
     uint32_t width;     // most tokens a tile takes (a multiple of 16)
     uint32_t box;       // rows of the token operand's TMA box
     uint32_t stages, x_stage;
+    uint32_t channels;  // of a tile: 128, a pair's 256
     uint32_t ct, nk;    // channel tiles, K chunks
     uint32_t tmem_cols, acc_cols;
     uint32_t split;
@@ -412,13 +416,22 @@ __host__ __device__ constexpr uint32_t mm_fixed_bytes(uint32_t groups) {
     return 2u * kMmMaxTokens * 4u + (2u * kMmMaxStages + 4u) * 8u + 16u + mm_table_bytes(groups) + 16u;
 }
 
-// Bounded: false once the time limit has passed or another role has given up.
+// Columns of a tile's products: the shapes' steps are 16 for one CTA, 32 for a pair.
+template <bool PAIR>
+__device__ __forceinline__ uint32_t mm_columns(uint32_t count) {
+    return PAIR ? (count + 31u) & ~31u : (count + 15u) & ~15u;
+}
+
+// Bounded: false once the time limit has passed or another role has given up. CLUSTER: the arrivals
+// come from the peer CTA too.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
-    if (tc::mbar_try(bar, parity)) return true;
+    auto done = [&] { return CLUSTER ? tc::mbar_try_cluster(bar, parity) : tc::mbar_try(bar, parity); };
+    if (done()) return true;
     const uint64_t t0 = tc::global_ns();
     for (;;) {
         for (uint32_t i = 0; i < 64u; ++i) {
-            if (tc::mbar_try(bar, parity)) return true;
+            if (done()) return true;
             if (*abort) return false;
         }
         if (tc::global_ns() - t0 > kMmWaitNs) return false;
@@ -442,21 +455,7 @@ __device__ __forceinline__ MmTile mm_tile(const MmShared& sh, const Int8MmaParam
     const uint32_t c = local / tt, j = local - c * tt;
     const uint32_t n = sh.cnt[a];  // balanced: the group's tiles differ by one row at most
     const uint32_t from = (uint32_t)((uint64_t)n * j / tt), to = (uint32_t)((uint64_t)n * (j + 1u) / tt);
-    return MmTile{a, sh.lo[a] + from, to - from, c * kMmChannels};
-}
-
-// One K chunk's operands: 128 rows of w, and the tile's tokens in boxes (rows past the tile's are
-// loaded and not used; past the matrix the TMA unit fills zeros, also past K).
-__device__ __forceinline__ void mm_load_w(const Int8MmaParams& p, uint32_t smem, uint64_t* full, const MmTile& t,
-                                          uint32_t boxes, uint32_t kc) {
-    tc::mbar_arrive_expect_tx(full, kMmWStage + boxes * p.box * kMmKc);
-    tc::tma_load_2d(smem, &p.wmap, (int32_t)(kc * kMmKc), (int32_t)(t.g * p.l.out_cols + t.channel0), full);
-}
-__device__ __forceinline__ void mm_load_x(const Int8MmaParams& p, uint32_t smem, uint64_t* full, const MmTile& t,
-                                          uint32_t boxes, uint32_t kc) {
-    for (uint32_t b = 0; b < boxes; ++b)
-        tc::tma_load_2d(smem + kMmWStage + b * p.box * kMmKc, &p.xmap, (int32_t)(kc * kMmKc),
-                        (int32_t)(t.row0 + b * p.box), full);
+    return MmTile{a, sh.lo[a] + from, to - from, c * p.channels};
 }
 
 template <typename TY>
@@ -465,8 +464,9 @@ __device__ __forceinline__ void mm_store(const Int8LinearParams& l, uint32_t row
     static_cast<TY*>(l.y)[(size_t)row * l.y_stride + n] = from_float<TY>((float)acc * s * t);
 }
 
-template <typename TY, bool SPLIT>
+template <typename TY, Mm MODE>
 __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_constant__ Int8MmaParams p) {
+    constexpr bool SPLIT = MODE == Mm::kSplit, PAIR = MODE == Mm::kPair;
     extern __shared__ __align__(1024) unsigned char mm_smem[];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t smem = tc::smem_u32(mm_smem), stage_bytes = kMmWStage + p.x_stage;
@@ -489,7 +489,10 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         if (tid == 0) atomicOr(&g_int8_error, 2u);
         return;
     }
-    if (warp == kMmEpiWarps) tc::tmem_alloc(sh.tmem, p.tmem_cols);
+    if (warp == kMmEpiWarps) {
+        if (PAIR) tc::tmem_alloc_pair(sh.tmem, p.tmem_cols);
+        else tc::tmem_alloc(sh.tmem, p.tmem_cols);
+    }
     if (tid == 0) {
         for (uint32_t i = 0; i < p.stages; ++i) {
             tc::mbar_init(sh.full + i, 1);
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         }
         for (uint32_t i = 0; i < 2u; ++i) {
             tc::mbar_init(sh.acc_full + i, 1);
-            tc::mbar_init(sh.acc_empty + i, kMmEpiWarps);
+            tc::mbar_init(sh.acc_empty + i, PAIR ? 2u * kMmEpiWarps : kMmEpiWarps);
         }
         *sh.abort = 0;
         tc::mbar_fence_init();
@@ -528,12 +531,12 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
     }
     tc::fence_before_sync();
     __syncthreads();
+    if (PAIR) tc::cluster_sync();  // the peer's barriers and TMEM are ready too
     tc::fence_after_sync();
     const uint32_t tmem = *sh.tmem;
     const uint32_t total = sh.first[l.groups] * p.ct;
-    const uint32_t rank = SPLIT ? tc::cluster_rank() : 0u;
-    const uint32_t step = SPLIT ? gridDim.x / p.split : gridDim.x;
-    const uint32_t begin = SPLIT ? blockIdx.x / p.split : blockIdx.x;
+    const uint32_t rank = MODE != Mm::kOne ? tc::cluster_rank() : 0u, in_cluster = SPLIT ? p.split : PAIR ? 2u : 1u;
+    const uint32_t step = gridDim.x / in_cluster, begin = blockIdx.x / in_cluster;
     const uint32_t k_lo = SPLIT ? p.nk * rank / p.split : 0u, k_hi = SPLIT ? p.nk * (rank + 1u) / p.split : p.nk;
     const uint32_t nk = k_hi - k_lo;
     bool dirty = false, pending = false;  // copies / products under way when a role gave up
@@ -545,39 +548,65 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
     auto next_stage = [&] {
         if (++stage == p.stages) stage = 0, phase ^= 1u;
     };
+    // One K chunk's operands: 128 rows of w, and the tile's tokens (a pair: this CTA's half of them) in
+    // boxes. Rows past the tile's are loaded and not used; past the matrix, also past K, the TMA unit
+    // fills zeros. A pair's bytes all complete on the first CTA's barrier.
+    auto load_w = [&](uint32_t st, const MmTile& tile, uint32_t boxes, uint32_t kc) {
+        if (!PAIR || rank == 0)
+            tc::mbar_arrive_expect_tx(sh.full + st, (PAIR ? 2u : 1u) * (boxes * p.box * kMmKc + kMmWStage));
+        const int32_t x = (int32_t)(kc * kMmKc);
+        const int32_t y = (int32_t)(tile.g * l.out_cols + tile.channel0 + (PAIR ? rank * kMmChannels : 0u));
+        if (PAIR) tc::tma_load_2d_pair(smem + st * stage_bytes, &p.wmap, x, y, tc::cluster_map(tc::smem_u32(sh.full + st), 0));
+        else tc::tma_load_2d(smem + st * stage_bytes, &p.wmap, x, y, sh.full + st);
+    };
+    auto load_x = [&](uint32_t st, const MmTile& tile, uint32_t boxes, uint32_t kc) {
+        const uint32_t dst = smem + st * stage_bytes + kMmWStage;
+        const uint32_t row0 = tile.row0 + (PAIR ? rank * (mm_columns<PAIR>(tile.count) / 2u) : 0u);
+        for (uint32_t b = 0; b < boxes; ++b) {
+            const int32_t x = (int32_t)(kc * kMmKc), y = (int32_t)(row0 + b * p.box);
+            if (PAIR)
+                tc::tma_load_2d_pair(dst + b * p.box * kMmKc, &p.xmap, x, y, tc::cluster_map(tc::smem_u32(sh.full + st), 0));
+            else
+                tc::tma_load_2d(dst + b * p.box * kMmKc, &p.xmap, x, y, sh.full + st);
+        }
+    };
     auto produce = [&](uint32_t t) -> bool {
         const MmTile tile = mm_tile(sh, p, t);
-        const uint32_t boxes = (tile.count + p.box - 1u) / p.box;
+        const uint32_t own = PAIR ? mm_columns<PAIR>(tile.count) / 2u : tile.count;
+        const uint32_t boxes = (own + p.box - 1u) / p.box;
         dirty = true;
         uint32_t done = 0;
         if (!waited) {
             // the weights are no kernel's output: the first stages' are on their way while the
             // kernel ahead still quantizes the tokens
             done = nk < p.stages ? nk : p.stages;
-            for (uint32_t i = 0; i < done; ++i)
-                mm_load_w(p, smem + i * stage_bytes, sh.full + i, tile, boxes, k_lo + i);
+            for (uint32_t i = 0; i < done; ++i) load_w(i, tile, boxes, k_lo + i);
             tc::grid_dependency_wait();
             waited = true;
             for (uint32_t i = 0; i < done; ++i) {
-                mm_load_x(p, smem + i * stage_bytes, sh.full + i, tile, boxes, k_lo + i);
+                load_x(i, tile, boxes, k_lo + i);
                 next_stage();
             }
         }
         for (uint32_t i = done; i < nk; ++i) {
             if (!mm_wait(sh.empty + stage, phase ^ 1u, sh.abort)) return false;
-            mm_load_w(p, smem + stage * stage_bytes, sh.full + stage, tile, boxes, k_lo + i);
-            mm_load_x(p, smem + stage * stage_bytes, sh.full + stage, tile, boxes, k_lo + i);
+            load_w(stage, tile, boxes, k_lo + i);
+            load_x(stage, tile, boxes, k_lo + i);
             next_stage();
         }
         dirty = false;
         return true;
     };
+    auto commit = [&](uint64_t* bar) {
+        if (PAIR) tc::mma_commit_pair(bar);
+        else tc::mma_commit(bar);
+    };
     auto multiply = [&](uint32_t t) -> bool {
         const MmTile tile = mm_tile(sh, p, t);
         const uint32_t buf = SPLIT ? 0u : it & 1u, use = SPLIT ? it : it >> 1;
-        if (!SPLIT && !mm_wait(sh.acc_empty + buf, (use & 1u) ^ 1u, sh.abort)) return false;
+        if (!SPLIT && !mm_wait<PAIR>(sh.acc_empty + buf, (use & 1u) ^ 1u, sh.abort)) return false;
         tc::fence_after_sync();
-        const uint32_t idesc = tc::idesc_i8(kMmChannels, (tile.count + 15u) & ~15u);
+        const uint32_t idesc = tc::idesc_i8(PAIR ? 2u * kMmChannels : kMmChannels, mm_columns<PAIR>(tile.count));
         const uint32_t acc = tmem + buf * p.acc_cols;
         for (uint32_t i = 0; i < nk; ++i) {
             if (!mm_wait(sh.full + stage, phase, sh.abort)) return false;
@@ -587,12 +616,15 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
             pending_bar = buf;
             pending_parity = use & 1u;
 #pragma unroll
-            for (uint32_t ks = 0; ks < kMmKc / 32u; ++ks)
-                tc::mma_i8(acc, tc::sw128_desc(ws + ks * 32u), tc::sw128_desc(xs + ks * 32u), idesc, (i | ks) ? 1u : 0u);
-            tc::mma_commit(sh.empty + stage);
+            for (uint32_t ks = 0; ks < kMmKc / 32u; ++ks) {
+                const uint64_t wd = tc::sw128_desc(ws + ks * 32u), xd = tc::sw128_desc(xs + ks * 32u);
+                if (PAIR) tc::mma_i8_pair(acc, wd, xd, idesc, (i | ks) ? 1u : 0u);
+                else tc::mma_i8(acc, wd, xd, idesc, (i | ks) ? 1u : 0u);
+            }
+            commit(sh.empty + stage);
             next_stage();
         }
-        tc::mma_commit(sh.acc_full + buf);
+        commit(sh.acc_full + buf);
         pending = false;
         ++it;
         return true;
@@ -610,7 +642,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
             const uint32_t r = tile.row0 + tid;
             ts[tid] = l.row_weight ? l.x_scale[r] * l.row_weight[r] : l.x_scale[r];
         }
-        const uint32_t n = tile.channel0 + 32u * quad + lane;
+        const uint32_t n = tile.channel0 + (PAIR ? rank * kMmChannels : 0u) + 32u * quad + lane;
         const float cs = n < l.out_cols ? l.w_scale[(size_t)tile.g * l.out_cols + n] : 0.f;
         asm volatile("bar.sync 1, %0;" ::"n"(kMmEpiWarps * 32) : "memory");
         const bool ok = __all_sync(0xffffffffu, mm_wait(sh.acc_full + buf, use & 1u, sh.abort));
@@ -630,7 +662,10 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
             }
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(sh.acc_empty + buf);
+            if (lane == 0) {
+                if (PAIR) tc::mbar_arrive_cluster(tc::cluster_map(tc::smem_u32(sh.acc_empty + buf), 0));
+                else tc::mbar_arrive(sh.acc_empty + buf);
+            }
             ++it;
         }
         return ok;
@@ -649,7 +684,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
                         mm_fail(sh.abort);
                         break;
                     }
-        } else if (lane == 0) {
+        } else if (lane == 0 && rank == 0) {
             for (uint32_t t = begin; t < total; t += step)
                 if (!multiply(t)) {
                     mm_fail(sh.abort);
@@ -716,15 +751,21 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         }
     }
     if (warp == kMmEpiWarps + 1u && lane == 0 && pending) {
-        tc::mma_commit(sh.acc_full + pending_bar);
+        commit(sh.acc_full + pending_bar);
         const uint64_t t0 = tc::global_ns();
         while (!tc::mbar_try(sh.acc_full + pending_bar, pending_parity) && tc::global_ns() - t0 < kMmWaitNs) {
         }
     }
     __syncthreads();
+    if (PAIR) {
+        // the peer may still be read by products or signal this CTA's barriers
+        tc::fence_before_sync();
+        tc::cluster_sync();
+    }
     if (warp == kMmEpiWarps) {
         tc::fence_after_sync();
-        tc::tmem_dealloc(tmem, p.tmem_cols);
+        if (PAIR) tc::tmem_dealloc_pair(tmem, p.tmem_cols);
+        else tc::tmem_dealloc(tmem, p.tmem_cols);
     }
 }
 
@@ -815,10 +856,8 @@ bool tma_rows(const int8_t* p, size_t stride) {
     return reinterpret_cast<uintptr_t>(p) % 16u == 0 && stride % 16u == 0;
 }
 
-uint32_t round16(uint32_t v) { return (v + 15u) / 16u * 16u; }
-
-// Tile width and split of a product on the tensor cores.
-void mma_plan(Int8MmaParams& p, uint32_t sms) {
+// Tile width, split or pairs of a product on the tensor cores. Returns the mode.
+Mm mma_plan(Int8MmaParams& p, uint32_t sms) {
     const Int8LinearParams& l = p.l;
     p.ct = (l.out_cols + kMmChannels - 1u) / kMmChannels;
     p.nk = (l.cols + kMmKc - 1u) / kMmKc;
@@ -829,14 +868,25 @@ void mma_plan(Int8MmaParams& p, uint32_t sms) {
         while (split < 8u && tiles * split * 2u <= sms && p.nk >= split * 2u) split *= 2u;
         return split;
     };
+    Mm mode = Mm::kOne;
+    if (mean > kMmMaxTokens / 2u && (uint64_t)l.rows * p.ct >= (uint64_t)kMmMaxTokens * sms / 2u) mode = Mm::kPair;
+    const uint32_t step = mode == Mm::kPair ? 32u : 16u, units = mode == Mm::kPair ? sms / 2u : sms;
+    if (mode == Mm::kPair) {
+        p.channels = 2u * kMmChannels;
+        p.ct = (l.out_cols + p.channels - 1u) / p.channels;
+    } else {
+        p.channels = kMmChannels;
+    }
+    const auto up = [&](uint32_t v) { return (v + step - 1u) / step * step; };
     if (l.groups == 1) {
         // the width whose waves of tiles pass the fewest columns x K chunks; one tile of tokens
         // where they fit one (narrower ones would read the weights again)
         uint64_t best = ~0ull;
-        const uint32_t most = round16(l.rows < kMmMaxTokens ? l.rows : kMmMaxTokens);
-        for (uint32_t w = most; w >= 128u || w == most; w -= 16u) {
-            const uint64_t n = (l.rows + w - 1u) / w, tiles = n * p.ct, waves = (tiles + sms - 1u) / sms;
-            const uint32_t balanced = round16((uint32_t)((l.rows + n - 1u) / n)), split = split_of(tiles);
+        const uint32_t most = up(l.rows < kMmMaxTokens ? l.rows : kMmMaxTokens);
+        for (uint32_t w = most; w >= 128u || w == most; w -= step) {
+            const uint64_t n = (l.rows + w - 1u) / w, tiles = n * p.ct, waves = (tiles + units - 1u) / units;
+            const uint32_t balanced = up((uint32_t)((l.rows + n - 1u) / n));
+            const uint32_t split = mode == Mm::kPair ? 1u : split_of(tiles);
             const uint64_t cost = waves * balanced * ((p.nk + split - 1u) / split);
             if (cost < best) best = cost, p.width = w, p.split = split;
             if (w == most && l.rows <= kMmMaxTokens) break;
@@ -846,35 +896,39 @@ void mma_plan(Int8MmaParams& p, uint32_t sms) {
         // read the group's weights again
         uint32_t spread = 1;
         while (spread * spread < mean) ++spread;
-        const uint32_t want = round16(mean + 3u * spread);
+        const uint32_t want = up(mean + 3u * spread);
         p.width = want < kMmMaxTokens ? want : kMmMaxTokens;
-        p.split = split_of((uint64_t)used * ((mean + p.width - 1u) / p.width) * p.ct);
+        p.split = mode == Mm::kPair ? 1u : split_of((uint64_t)used * ((mean + p.width - 1u) / p.width) * p.ct);
     }
-    p.box = p.width < 64u ? p.width : 64u;
-    p.x_stage = (p.width + p.box - 1u) / p.box * p.box * kMmKc;
+    if (p.split > 1) mode = Mm::kSplit;
+    const uint32_t held = mode == Mm::kPair ? p.width / 2u : p.width;  // token rows in one CTA's stage
+    p.box = held < 64u ? held : 64u;
+    p.x_stage = (held + p.box - 1u) / p.box * p.box * kMmKc;
     p.acc_cols = p.width < 32u ? 32u : p.width;
     p.tmem_cols = 32;
-    while (p.tmem_cols < (p.split > 1 ? 1u : 2u) * p.acc_cols) p.tmem_cols *= 2u;
+    while (p.tmem_cols < (mode == Mm::kSplit ? 1u : 2u) * p.acc_cols) p.tmem_cols *= 2u;
     const uint32_t room = kMmSmemLimit - 1024u - mm_fixed_bytes(l.groups);
     p.stages = room / (kMmWStage + p.x_stage);
     if (p.stages > kMmMaxStages) p.stages = kMmMaxStages;
+    return mode;
 }
 
-template <typename TY, bool SPLIT>
+template <typename TY, Mm MODE>
 cudaError_t mma_launch(const Int8MmaParams& p, uint32_t sms, bool after_quantize, cudaStream_t s) {
-    auto* kernel = int8_mma_kernel<TY, SPLIT>;
+    auto* kernel = int8_mma_kernel<TY, MODE>;
+    const uint32_t in_cluster = MODE == Mm::kSplit ? p.split : MODE == Mm::kPair ? 2u : 1u;
     cudaError_t e = smem_once(kernel, kMmSmemLimit);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[2];
-    cfg.gridDim = dim3(sms / p.split * p.split);
+    cfg.gridDim = dim3(sms / in_cluster * in_cluster);
     cfg.blockDim = dim3(kMmThreads);
     cfg.dynamicSmemBytes = p.stages * (kMmWStage + p.x_stage) + mm_fixed_bytes(p.l.groups);
     cfg.stream = s;
     cfg.attrs = attr;
-    if (SPLIT) {
+    if (MODE != Mm::kOne) {
         attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attr[cfg.numAttrs].val.clusterDim.x = p.split;
+        attr[cfg.numAttrs].val.clusterDim.x = in_cluster;
         attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
         ++cfg.numAttrs;
     }
@@ -903,11 +957,12 @@ cudaError_t linear_type(const Int8LinearParams& l, bool after_quantize, cudaStre
         Int8MmaParams p{};
         p.l = l;
         const uint32_t sms = sm_count();
-        mma_plan(p, sms);
+        const Mm mode = mma_plan(p, sms);
         if (encode_rows(&p.wmap, l.w, (uint64_t)l.groups * l.out_cols, l.cols, l.w_stride, kMmChannels) &&
             encode_rows(&p.xmap, l.x, l.rows, l.cols, l.x_stride, p.box))
-            return p.split > 1 ? mma_launch<TY, true>(p, sms, after_quantize, s)
-                               : mma_launch<TY, false>(p, sms, after_quantize, s);
+            return mode == Mm::kPair    ? mma_launch<TY, Mm::kPair>(p, sms, after_quantize, s)
+                   : mode == Mm::kSplit ? mma_launch<TY, Mm::kSplit>(p, sms, after_quantize, s)
+                                        : mma_launch<TY, Mm::kOne>(p, sms, after_quantize, s);
     }
     return general_type<TY>(l, s);
 }
