@@ -62,7 +62,7 @@ def quantized(x):
 
 
 def product(q, s, w, ws, rw=None):
-    y = (q.astype(np.int64) @ w.astype(np.int64).T).astype(np.float64) * s.astype(np.float64)[:, None]
+    y = (q.astype(np.float64) @ w.astype(np.float64).T) * s.astype(np.float64)[:, None]
     y *= ws.astype(np.float64)[None, :]
     return y if rw is None else y * rw.astype(np.float64)[:, None]
 
@@ -330,6 +330,39 @@ def test_groups(dev, torch, counts, N, K):
     xc, ic, rc, oc, wc, swc = (cuda(torch, a) for a in (x, index, rw, off, w, sw))
     y = run_linear(dev, torch, xc, wc, swc, rows=rows, cols=K, x_rows=T, row_index_ptr=ic.data_ptr() if rows else 0,
                    row_weight_ptr=rc.data_ptr() if rows else 0, offsets_ptr=oc.data_ptr())
+    q, s = quantized(x)
+    out = y.cpu().numpy()
+    for g in range(G):
+        sl = slice(off[g], off[g + 1])
+        check_product(out[sl], product(q[index[sl]], s[index[sl]], w[g, :, :K], sw[g], rw[sl]), "f32")
+
+
+@pytest.mark.parametrize("M,N,K", [(2049, 2600, 160), (1500, 4097, 400), (300, 20000, 129), (5000, 1030, 1024)])
+def test_linear_large(dev, torch, M, N, K):
+    """Products of many tiles: several a CTA, ragged at every edge."""
+    rng = np.random.default_rng(M)
+    ld = (K + 15) // 16 * 16
+    x, w = (rng.integers(-128, 128, (n, ld), dtype=np.int8) for n in (M, N))
+    sx, sw = rng.random(M, np.float32) + np.float32(0.1), rng.standard_normal(N).astype(np.float32)
+    xc, wc, sxc, swc = (cuda(torch, a) for a in (x, w[None], sx, sw[None]))
+    y = run_linear(dev, torch, xc, wc, swc, x_type="i8", x_stride=ld, cols=K, x_scale_ptr=sxc.data_ptr())
+    check_product(y.cpu().numpy(), product(x[:, :K], sx, w[:, :K], sw), "f32")
+
+
+@pytest.mark.parametrize("counts,N,K", [([700, 0, 300, 513, 1, 2000], 1100, 300), ([0, 1300, 1300], 2000, 64),
+                                        ([400] * 20, 1000, 96), ([0, 5000, 3], 700, 500)])
+def test_large_groups(dev, torch, counts, N, K):
+    rng = np.random.default_rng(N)
+    G, rows, T = len(counts), sum(counts), 900
+    ld = (K + 15) // 16 * 16
+    off = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    x = rng.standard_normal((T, K)).astype(np.float32)
+    index = rng.integers(0, T, rows).astype(np.int32)
+    rw = rng.random(rows, np.float32)
+    w, sw = rng.integers(-127, 128, (G, N, ld), dtype=np.int8), rng.random((G, N), np.float32)
+    xc, ic, rc, oc, wc, swc = (cuda(torch, a) for a in (x, index, rw, off, w, sw))
+    y = run_linear(dev, torch, xc, wc, swc, rows=rows, cols=K, x_rows=T, row_index_ptr=ic.data_ptr(),
+                   row_weight_ptr=rc.data_ptr(), offsets_ptr=oc.data_ptr())
     q, s = quantized(x)
     out = y.cpu().numpy()
     for g in range(G):

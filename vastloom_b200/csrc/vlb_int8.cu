@@ -468,7 +468,7 @@ template <typename TY, Mm MODE>
 __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_constant__ Int8MmaParams p) {
     constexpr bool SPLIT = MODE == Mm::kSplit, PAIR = MODE == Mm::kPair;
     extern __shared__ __align__(1024) unsigned char mm_smem[];
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
     const uint32_t smem = tc::smem_u32(mm_smem), stage_bytes = kMmWStage + p.x_stage;
     const Int8LinearParams& l = p.l;
     MmShared sh;
@@ -493,6 +493,8 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         if (PAIR) tc::tmem_alloc_pair(sh.tmem, p.tmem_cols);
         else tc::tmem_alloc(sh.tmem, p.tmem_cols);
     }
+    if (warp == kMmEpiWarps + 1u && lane < 2u)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane ? &p.xmap : &p.wmap)) : "memory");
     if (tid == 0) {
         for (uint32_t i = 0; i < p.stages; ++i) {
             tc::mbar_init(sh.full + i, 1);
@@ -550,48 +552,57 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
     };
     // One K chunk's operands: 128 rows of w, and the tile's tokens (a pair: this CTA's half of them) in
     // boxes. Rows past the tile's are loaded and not used; past the matrix, also past K, the TMA unit
-    // fills zeros. A pair's bytes all complete on the first CTA's barrier.
-    auto load_w = [&](uint32_t st, const MmTile& tile, uint32_t boxes, uint32_t kc) {
-        if (!PAIR || rank == 0)
-            tc::mbar_arrive_expect_tx(sh.full + st, (PAIR ? 2u : 1u) * (boxes * p.box * kMmKc + kMmWStage));
-        const int32_t x = (int32_t)(kc * kMmKc);
-        const int32_t y = (int32_t)(tile.g * l.out_cols + tile.channel0 + (PAIR ? rank * kMmChannels : 0u));
-        if (PAIR) tc::tma_load_2d_pair(smem + st * stage_bytes, &p.wmap, x, y, tc::cluster_map(tc::smem_u32(sh.full + st), 0));
-        else tc::tma_load_2d(smem + st * stage_bytes, &p.wmap, x, y, sh.full + st);
+    // fills zeros. A pair's bytes all complete on the first CTA's barrier. One lane of a warp in step
+    // runs these, as the products.
+    struct Source {
+        int32_t w_row, x_row;
+        uint32_t boxes;
     };
-    auto load_x = [&](uint32_t st, const MmTile& tile, uint32_t boxes, uint32_t kc) {
+    const uint32_t full0 = PAIR ? tc::cluster_map(tc::smem_u32(sh.full), 0) : tc::smem_u32(sh.full);
+    auto load_w = [&](uint32_t st, const Source& src, uint32_t kc) {
+        if (!PAIR || rank == 0)
+            tc::mbar_arrive_expect_tx(sh.full + st, (PAIR ? 2u : 1u) * (src.boxes * p.box * kMmKc + kMmWStage));
+        if (PAIR) tc::tma_load_2d_pair(smem + st * stage_bytes, &p.wmap, (int32_t)(kc * kMmKc), src.w_row, full0 + st * 8u);
+        else tc::tma_load_2d(smem + st * stage_bytes, &p.wmap, (int32_t)(kc * kMmKc), src.w_row, sh.full + st);
+    };
+    auto load_x = [&](uint32_t st, const Source& src, uint32_t kc) {
         const uint32_t dst = smem + st * stage_bytes + kMmWStage;
-        const uint32_t row0 = tile.row0 + (PAIR ? rank * (mm_columns<PAIR>(tile.count) / 2u) : 0u);
-        for (uint32_t b = 0; b < boxes; ++b) {
-            const int32_t x = (int32_t)(kc * kMmKc), y = (int32_t)(row0 + b * p.box);
-            if (PAIR)
-                tc::tma_load_2d_pair(dst + b * p.box * kMmKc, &p.xmap, x, y, tc::cluster_map(tc::smem_u32(sh.full + st), 0));
-            else
-                tc::tma_load_2d(dst + b * p.box * kMmKc, &p.xmap, x, y, sh.full + st);
+        for (uint32_t b = 0; b < src.boxes; ++b) {
+            const int32_t x = (int32_t)(kc * kMmKc), y = src.x_row + (int32_t)(b * p.box);
+            if (PAIR) tc::tma_load_2d_pair(dst + b * p.box * kMmKc, &p.xmap, x, y, full0 + st * 8u);
+            else tc::tma_load_2d(dst + b * p.box * kMmKc, &p.xmap, x, y, sh.full + st);
         }
     };
     auto produce = [&](uint32_t t) -> bool {
         const MmTile tile = mm_tile(sh, p, t);
         const uint32_t own = PAIR ? mm_columns<PAIR>(tile.count) / 2u : tile.count;
-        const uint32_t boxes = (own + p.box - 1u) / p.box;
+        Source src;
+        src.w_row = (int32_t)(tile.g * l.out_cols + tile.channel0 + (PAIR ? rank * kMmChannels : 0u));
+        src.x_row = (int32_t)(tile.row0 + (PAIR ? rank * own : 0u));
+        src.boxes = (own + p.box - 1u) / p.box;
         dirty = true;
         uint32_t done = 0;
         if (!waited) {
             // the weights are no kernel's output: the first stages' are on their way while the
             // kernel ahead still quantizes the tokens
             done = nk < p.stages ? nk : p.stages;
-            for (uint32_t i = 0; i < done; ++i) load_w(i, tile, boxes, k_lo + i);
+            if (tc::elect_lane())
+                for (uint32_t i = 0; i < done; ++i) load_w(i, src, k_lo + i);
+            __syncwarp();
             tc::grid_dependency_wait();
             waited = true;
-            for (uint32_t i = 0; i < done; ++i) {
-                load_x(i, tile, boxes, k_lo + i);
-                next_stage();
-            }
+            if (tc::elect_lane())
+                for (uint32_t i = 0; i < done; ++i) load_x(i, src, k_lo + i);
+            __syncwarp();
+            for (uint32_t i = 0; i < done; ++i) next_stage();
         }
         for (uint32_t i = done; i < nk; ++i) {
-            if (!mm_wait(sh.empty + stage, phase ^ 1u, sh.abort)) return false;
-            load_w(stage, tile, boxes, k_lo + i);
-            load_x(stage, tile, boxes, k_lo + i);
+            if (!__all_sync(0xffffffffu, mm_wait(sh.empty + stage, phase ^ 1u, sh.abort))) return false;
+            if (tc::elect_lane()) {
+                load_w(stage, src, k_lo + i);
+                load_x(stage, src, k_lo + i);
+            }
+            __syncwarp();
             next_stage();
         }
         dirty = false;
@@ -601,30 +612,34 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         if (PAIR) tc::mma_commit_pair(bar);
         else tc::mma_commit(bar);
     };
+    // the whole warp, in step
     auto multiply = [&](uint32_t t) -> bool {
         const MmTile tile = mm_tile(sh, p, t);
         const uint32_t buf = SPLIT ? 0u : it & 1u, use = SPLIT ? it : it >> 1;
-        if (!SPLIT && !mm_wait<PAIR>(sh.acc_empty + buf, (use & 1u) ^ 1u, sh.abort)) return false;
+        if (!SPLIT && !__all_sync(0xffffffffu, mm_wait<PAIR>(sh.acc_empty + buf, (use & 1u) ^ 1u, sh.abort))) return false;
         tc::fence_after_sync();
         const uint32_t idesc = tc::idesc_i8(PAIR ? 2u * kMmChannels : kMmChannels, mm_columns<PAIR>(tile.count));
         const uint32_t acc = tmem + buf * p.acc_cols;
+        pending_bar = buf;
+        pending_parity = use & 1u;
         for (uint32_t i = 0; i < nk; ++i) {
-            if (!mm_wait(sh.full + stage, phase, sh.abort)) return false;
+            if (!__all_sync(0xffffffffu, mm_wait(sh.full + stage, phase, sh.abort))) return false;
             tc::fence_after_sync();
-            const uint32_t ws = smem + stage * stage_bytes, xs = ws + kMmWStage;
             pending = true;
-            pending_bar = buf;
-            pending_parity = use & 1u;
+            if (tc::elect_lane()) {
+                const uint64_t wd = tc::sw128_desc(smem + stage * stage_bytes);
+                const uint64_t xd = tc::sw128_desc(smem + stage * stage_bytes + kMmWStage);
 #pragma unroll
-            for (uint32_t ks = 0; ks < kMmKc / 32u; ++ks) {
-                const uint64_t wd = tc::sw128_desc(ws + ks * 32u), xd = tc::sw128_desc(xs + ks * 32u);
-                if (PAIR) tc::mma_i8_pair(acc, wd, xd, idesc, (i | ks) ? 1u : 0u);
-                else tc::mma_i8(acc, wd, xd, idesc, (i | ks) ? 1u : 0u);
+                for (uint32_t ks = 0; ks < kMmKc / 32u; ++ks) {  // 32 bytes on: 2 of the descriptor's 16-byte units
+                    if (PAIR) tc::mma_i8_pair(acc, wd + 2u * ks, xd + 2u * ks, idesc, (i | ks) ? 1u : 0u);
+                    else tc::mma_i8(acc, wd + 2u * ks, xd + 2u * ks, idesc, (i | ks) ? 1u : 0u);
+                }
+                commit(sh.empty + stage);
+                if (i + 1u == nk) commit(sh.acc_full + buf);
             }
-            commit(sh.empty + stage);
+            __syncwarp();
             next_stage();
         }
-        commit(sh.acc_full + buf);
         pending = false;
         ++it;
         return true;
@@ -649,16 +664,31 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         if (ok) {
             tc::fence_after_sync();
             const uint32_t src = tmem + buf * p.acc_cols + ((32u * quad) << 16);
-            for (uint32_t c = 16u * half; c < tile.count; c += 32u) {
-                float v[16];
-                tc::tmem_ld16(src + c, v);
+            // 32 columns (tokens) at a time, the warps of a lane quarter taking turns
+            for (uint32_t c = 32u * half; c < tile.count; c += 64u) {
+                uint32_t v[32];
+                tc::tmem_ld32(src + c, v);
                 tc::tmem_wait_ld();
                 TY* y = static_cast<TY*>(l.y) + (size_t)(tile.row0 + c) * l.y_stride + n;
-                const uint32_t m = min(16u, tile.count - c);
+                const float4* t4 = reinterpret_cast<const float4*>(ts + c);
+                if (tile.count - c >= 32u && n - lane + 32u <= l.out_cols) {
 #pragma unroll
-                for (uint32_t i = 0; i < 16u; ++i)
-                    if (i < m && n < l.out_cols)
-                        y[i * l.y_stride] = from_float<TY>((float)__float_as_int(v[i]) * ts[c + i] * cs);
+                    for (uint32_t i = 0; i < 32u; i += 4u) {
+                        const float4 t = t4[i / 4u];
+                        y[0] = from_float<TY>((float)(int32_t)v[i] * t.x * cs);
+                        y += l.y_stride;
+                        y[0] = from_float<TY>((float)(int32_t)v[i + 1] * t.y * cs);
+                        y += l.y_stride;
+                        y[0] = from_float<TY>((float)(int32_t)v[i + 2] * t.z * cs);
+                        y += l.y_stride;
+                        y[0] = from_float<TY>((float)(int32_t)v[i + 3] * t.w * cs);
+                        y += l.y_stride;
+                    }
+                } else if (n < l.out_cols) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 32u; ++i)
+                        if (c + i < tile.count) y[i * l.y_stride] = from_float<TY>((float)(int32_t)v[i] * ts[c + i] * cs);
+                }
             }
             tc::fence_before_sync();
             __syncwarp();
@@ -678,16 +708,15 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
             for (uint32_t t = begin; t < total; t += step)
                 if (!epilogue(t) && lane == 0) mm_fail(sh.abort);
         } else if (warp == kMmEpiWarps) {
-            if (lane == 0)
-                for (uint32_t t = begin; t < total; t += step)
-                    if (!produce(t)) {
-                        mm_fail(sh.abort);
-                        break;
-                    }
-        } else if (lane == 0 && rank == 0) {
+            for (uint32_t t = begin; t < total; t += step)
+                if (!produce(t)) {
+                    if (lane == 0) mm_fail(sh.abort);
+                    break;
+                }
+        } else if (!PAIR || rank == 0) {
             for (uint32_t t = begin; t < total; t += step)
                 if (!multiply(t)) {
-                    mm_fail(sh.abort);
+                    if (lane == 0) mm_fail(sh.abort);
                     break;
                 }
         }
@@ -698,17 +727,25 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
             // role has given up
             const MmTile tile = mm_tile(sh, p, t);
             bool ok = true;
+            float cs = 0.f;
+            float* ts = sh.scale;
             if (warp == kMmEpiWarps) {
-                if (lane == 0) ok = *sh.abort ? false : produce(t);
+                ok = __all_sync(0xffffffffu, *sh.abort == 0) && produce(t);
             } else if (warp == kMmEpiWarps + 1u) {
-                if (lane == 0) ok = *sh.abort ? false : multiply(t);
+                ok = __all_sync(0xffffffffu, *sh.abort == 0) && multiply(t);
             } else {
                 if (!waited) {
                     tc::grid_dependency_wait();
                     waited = true;
                 }
+                if (tid < tile.count) {
+                    const uint32_t r = tile.row0 + tid;
+                    ts[tid] = l.row_weight ? l.x_scale[r] * l.row_weight[r] : l.x_scale[r];
+                }
                 ok = __all_sync(0xffffffffu, *sh.abort == 0 && mm_wait(sh.acc_full, it & 1u, sh.abort));
                 ++it;
+                const uint32_t n = tile.channel0 + 32u * quad + lane;
+                cs = n < l.out_cols ? l.w_scale[(size_t)tile.g * l.out_cols + n] : 0.f;
                 if (ok) {
                     tc::fence_after_sync();
                     const uint32_t src = tmem + ((32u * quad) << 16);
@@ -723,19 +760,30 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
                     tc::fence_before_sync();
                 }
             }
-            if (!ok && (warp < kMmEpiWarps ? lane == 0 : true)) mm_fail(sh.abort);
+            if (!ok && lane == 0) mm_fail(sh.abort);
             __syncwarp();
             tc::cluster_sync();
             if (warp < kMmEpiWarps) {
                 const uint32_t c = 32u * quad + lane, n = tile.channel0 + c;
-                const float cs = n < l.out_cols ? l.w_scale[(size_t)tile.g * l.out_cols + n] : 0.f;
-                for (uint32_t j = rank * 2u + half; j < tile.count; j += 2u * p.split) {
-                    const uint32_t at = smem + (j * kMmChannels + c) * 4u;
-                    int32_t sum = 0;
-                    for (uint32_t r = 0; r < p.split; ++r) sum += (int32_t)tc::cluster_ld(at, r);
-                    const uint32_t row = tile.row0 + j;
-                    const float s = l.row_weight ? l.x_scale[row] * l.row_weight[row] : l.x_scale[row];
-                    if (n < l.out_cols) mm_store<TY>(l, row, n, sum, s, cs);
+                // two columns at a time, so that up to 16 loads from the peers are in flight
+                const uint32_t pace = 2u * p.split;
+                for (uint32_t j = rank * 2u + half; j < tile.count; j += 2u * pace) {
+                    uint32_t v[2][8];
+#pragma unroll
+                    for (uint32_t u = 0; u < 2u; ++u)
+#pragma unroll
+                        for (uint32_t r = 0; r < 8u; ++r)
+                            v[u][r] = r < p.split && j + u * pace < tile.count
+                                          ? tc::cluster_ld(smem + ((j + u * pace) * kMmChannels + c) * 4u, r) : 0u;
+#pragma unroll
+                    for (uint32_t u = 0; u < 2u; ++u) {
+                        if (j + u * pace >= tile.count) break;
+                        uint32_t sum = 0;
+#pragma unroll
+                        for (uint32_t r = 0; r < 8u; ++r) sum += v[u][r];
+                        const uint32_t row = tile.row0 + j + u * pace;
+                        if (n < l.out_cols) mm_store<TY>(l, row, n, (int32_t)sum, ts[j + u * pace], cs);
+                    }
                 }
             }
             tc::fence_proxy_async();
@@ -750,7 +798,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         while (tc::global_ns() - t0 < 1000000ull) {
         }
     }
-    if (warp == kMmEpiWarps + 1u && lane == 0 && pending) {
+    if (warp == kMmEpiWarps + 1u && pending && tc::elect_lane()) {
         commit(sh.acc_full + pending_bar);
         const uint64_t t0 = tc::global_ns();
         while (!tc::mbar_try(sh.acc_full + pending_bar, pending_parity) && tc::global_ns() - t0 < kMmWaitNs) {
@@ -879,15 +927,16 @@ Mm mma_plan(Int8MmaParams& p, uint32_t sms) {
     }
     const auto up = [&](uint32_t v) { return (v + step - 1u) / step * step; };
     if (l.groups == 1) {
-        // the width whose waves of tiles pass the fewest columns x K chunks; one tile of tokens
-        // where they fit one (narrower ones would read the weights again)
+        // the width whose waves of tiles take the least time, a K chunk of a tile taking about its
+        // columns + 240 cycles (424 at 128 columns, 525 at 256: its weights' bytes and the products'
+        // issue do not shrink with the width); one tile of tokens where they fit one
         uint64_t best = ~0ull;
         const uint32_t most = up(l.rows < kMmMaxTokens ? l.rows : kMmMaxTokens);
         for (uint32_t w = most; w >= 128u || w == most; w -= step) {
             const uint64_t n = (l.rows + w - 1u) / w, tiles = n * p.ct, waves = (tiles + units - 1u) / units;
             const uint32_t balanced = up((uint32_t)((l.rows + n - 1u) / n));
             const uint32_t split = mode == Mm::kPair ? 1u : split_of(tiles);
-            const uint64_t cost = waves * balanced * ((p.nk + split - 1u) / split);
+            const uint64_t cost = waves * (balanced + 240u) * ((p.nk + split - 1u) / split);
             if (cost < best) best = cost, p.width = w, p.split = split;
             if (w == most && l.rows <= kMmMaxTokens) break;
         }
@@ -902,7 +951,7 @@ Mm mma_plan(Int8MmaParams& p, uint32_t sms) {
     }
     if (p.split > 1) mode = Mm::kSplit;
     const uint32_t held = mode == Mm::kPair ? p.width / 2u : p.width;  // token rows in one CTA's stage
-    p.box = held < 64u ? held : 64u;
+    p.box = held < 128u ? held : 128u;
     p.x_stage = (held + p.box - 1u) / p.box * p.box * kMmKc;
     p.acc_cols = p.width < 32u ? 32u : p.width;
     p.tmem_cols = 32;
