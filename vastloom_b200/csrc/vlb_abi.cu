@@ -1864,9 +1864,9 @@ int vlb_route_plan_device(vlb_handle* h, const uint32_t* idx, const float* weigh
 }
 
 uint64_t vlb_balance_workspace_bytes(uint32_t T, uint32_t E, uint32_t n_seqs) {
-    (void)T;
-    (void)E;
-    return kBalanceBlocks * 8 + ((uint64_t)n_seqs * 4 + 255) / 256 * 256;
+    if (n_seqs == 0) return 0;
+    // ticket | the blocks' losses | the parts' counts
+    return 256 + kBalanceBlocks * 8 + (uint64_t)n_seqs * balance_parts(T, n_seqs) * ((uint64_t)E + 1) * 4;
 }
 
 int vlb_balance_loss_device(vlb_handle* h, const vlb_balance_desc* desc, void* stream) {
@@ -1903,8 +1903,10 @@ int vlb_balance_loss_device(vlb_handle* h, const vlb_balance_desc* desc, void* s
         p.loss = d.loss;
         p.counts = d.counts;
         p.dlogits = d.dlogits;
-        p.partial = static_cast<double*>(d.ws);
-        p.live = reinterpret_cast<uint32_t*>(p.partial + kBalanceBlocks);
+        p.ticket = static_cast<uint32_t*>(d.ws);
+        p.partial = reinterpret_cast<double*>(static_cast<char*>(d.ws) + 256);
+        p.part = reinterpret_cast<uint32_t*>(p.partial + kBalanceBlocks);
+        p.parts = balance_parts(d.T, d.n_seqs);
         p.stride = d.logits_stride;
         p.grad_stride = d.dlogits_stride;
         p.T = d.T;

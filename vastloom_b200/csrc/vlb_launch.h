@@ -114,14 +114,18 @@ struct BalanceParams {
     float* loss;                 // or null
     uint32_t* counts;            // [S x E]
     void* dlogits;               // or null
-    uint32_t* live;              // [S] workspace
-    double* partial;             // [kBalanceBlocks] workspace
+    // workspace
+    uint32_t* ticket;
+    double* partial;             // [kBalanceBlocks] the blocks' losses
+    uint32_t* part;              // [S x parts x (E + 1)] counts and live tokens of a sequence's parts
     size_t stride, grad_stride;
-    uint32_t T, E, k, S;
+    uint32_t T, E, k, S, parts;
     int score, logits_type;
     float coefficient;
 };
-constexpr uint32_t kBalanceBlocks = 1184;  // 8 blocks of 256 threads on each of 148 SMs
+constexpr uint32_t kBalanceBlocks = 444;  // 3 blocks of 512 threads on each of 148 SMs
+constexpr uint32_t kBalOneTokens = 128;   // up to here one block does the whole call
+uint32_t balance_parts(uint32_t T, uint32_t S);
 cudaError_t launch_balance(const BalanceParams& p, cudaStream_t s);
 
 }  // namespace vlb
