@@ -45,109 +45,201 @@ __device__ __forceinline__ void bl_set(__half& p, float v) { p = __float2half_rn
 __device__ __forceinline__ void bl_set(__nv_bfloat16& p, float v) { p = __float2bfloat16_rn(v); }
 
 constexpr uint32_t kBalThreads = 512, kBalWarps = kBalThreads / 32u;
+constexpr uint32_t kBalCluster = 8, kBalParts = 16;  // most blocks of a counting cluster, parts of a sequence
+constexpr uint32_t kBalSeqs = 512;                  // offsets held in shared memory
 
 // The first sequence that ends after token t (S: none does).
-__device__ __forceinline__ uint32_t sequence_after(const BalanceParams& p, uint32_t t) {
-    if (!p.seq_offsets) return 0;
-    uint32_t lo = 0, hi = p.S;
+__device__ __forceinline__ uint32_t sequence_after(const uint32_t* offsets, uint32_t S, uint32_t t) {
+    uint32_t lo = 0, hi = S;
     while (lo < hi) {
         const uint32_t mid = (lo + hi) / 2u;
-        if (p.seq_offsets[mid + 1] > t) hi = mid;
+        if (offsets[mid + 1] > t) hi = mid;
         else lo = mid + 1;
     }
     return lo;
 }
-// Whether sequence s holds token t.
-__device__ __forceinline__ bool holds(const BalanceParams& p, uint32_t s, uint32_t t) {
-    return sequence_after(p, t) == s && (!p.seq_offsets || p.seq_offsets[s] <= t);
+// The offsets from shared memory where they fit (a search in memory is one round trip a step).
+__device__ __forceinline__ const uint32_t* near_offsets(const BalanceParams& p, uint32_t* shared) {
+    if (!p.seq_offsets || p.S > kBalSeqs) return p.seq_offsets;
+    for (uint32_t s = threadIdx.x; s <= p.S; s += kBalThreads) shared[s] = p.seq_offsets[s];
+    __syncthreads();
+    return shared;
 }
 
-// Adds the routes of the live tokens in [lo, hi) to hist[E] (shared) and returns this thread's
-// share of the live tokens.
-__device__ __forceinline__ uint32_t count_routes(const BalanceParams& p, uint32_t lo, uint32_t hi, uint32_t* hist) {
+// Adds the routes of the live tokens in [lo, hi) to hist[E] (shared), and the live tokens to hist[E]'s
+// next entry: 16 bytes of routes a load, four loads a thread in flight.
+__device__ __forceinline__ void count_routes(const BalanceParams& p, uint32_t lo, uint32_t hi, uint32_t* hist) {
+    const uint32_t tid = threadIdx.x;
     uint32_t live = 0;
-    for (uint32_t t = lo + threadIdx.x; t < hi; t += blockDim.x) live += !p.mask || p.mask[t];
-    const uint32_t end = hi * p.k;
-    for (uint32_t i = lo * p.k + threadIdx.x; i < end; i += blockDim.x) {
-        const uint32_t e = p.idx[i];
-        if (e < p.E && (!p.mask || p.mask[i / p.k])) atomicAdd(hist + e, 1u);
+    if (p.mask)
+        for (uint32_t t = lo + tid; t < hi; t += blockDim.x) live += p.mask[t] != 0;
+    else if (tid == 0)
+        live = hi - lo;
+    live = __reduce_add_sync(0xffffffffu, live);
+    if ((tid & 31u) == 0 && live) atomicAdd(hist + p.E, live);
+    // the expert of pair i, or E when its token is not live
+    const auto live_expert = [&](uint32_t i, uint32_t e) { return !p.mask || p.mask[i / p.k] ? e : p.E; };
+    const auto add = [&](uint32_t e) {
+        if (e < p.E) atomicAdd(hist + e, 1u);
+    };
+    const uint32_t first = lo * p.k, end = hi * p.k;
+    const uint32_t head = min((4u - (uint32_t)(reinterpret_cast<uintptr_t>(p.idx + first) / 4u) % 4u) % 4u, end - first);
+    const uint32_t body = first + head, quads = (end - body) / 4u, tail = body + 4u * quads;
+    if (tid < head) add(live_expert(first + tid, p.idx[first + tid]));
+    if (tid < end - tail) add(live_expert(tail + tid, p.idx[tail + tid]));
+    const uint4* q = reinterpret_cast<const uint4*>(p.idx + body);
+    for (uint32_t i0 = tid; i0 < quads; i0 += 4u * blockDim.x) {
+        uint4 v[4];
+#pragma unroll
+        for (uint32_t u = 0; u < 4u; ++u)
+            if (i0 + u * blockDim.x < quads) v[u] = __ldg(q + i0 + u * blockDim.x);
+        if (p.mask) {
+#pragma unroll
+            for (uint32_t u = 0; u < 4u; ++u) {
+                const uint32_t i = i0 + u * blockDim.x, at = body + 4u * i;
+                if (i < quads)
+                    v[u] = make_uint4(live_expert(at, v[u].x), live_expert(at + 1u, v[u].y), live_expert(at + 2u, v[u].z),
+                                      live_expert(at + 3u, v[u].w));
+            }
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < 4u; ++u) {
+            if (i0 + u * blockDim.x >= quads) break;
+            add(v[u].x);
+            add(v[u].y);
+            add(v[u].z);
+            add(v[u].w);
+        }
     }
-    return live;
 }
 
-// Part blockIdx.x % parts of sequence blockIdx.x / parts: its counts and, behind them, its live tokens.
-__global__ void __launch_bounds__(kBalThreads) balance_count_kernel(const BalanceParams p) {
-    __shared__ uint32_t hist[512], range[2], live_s;
+// Block b counts piece b mod 2^log_pieces of sequence b >> log_pieces; the blocks of a cluster add theirs through
+// distributed shared memory to one part: E counts and, behind them, the live tokens.
+__global__ void __launch_bounds__(kBalThreads) balance_count_kernel(const BalanceParams p, uint32_t log_pieces, uint32_t cluster) {
+    __shared__ uint32_t hist[513], foreign, offsets_s[kBalSeqs + 1];
     tc::grid_launch_dependents();
-    const uint32_t tid = threadIdx.x, s = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
-    for (uint32_t e = tid; e < p.E; e += kBalThreads) hist[e] = 0;
-    if (tid == 0) {
-        uint32_t lo = 0, hi = p.T;
-        if (p.seq_offsets) lo = min(p.seq_offsets[s], p.T), hi = max(lo, min(p.seq_offsets[s + 1], p.T));
-        const uint32_t from = lo + (uint32_t)((uint64_t)(hi - lo) * part / p.parts);
-        const uint32_t to = lo + (uint32_t)((uint64_t)(hi - lo) * (part + 1u) / p.parts);
+    const uint32_t tid = threadIdx.x, s = blockIdx.x >> log_pieces;
+    const uint32_t piece = blockIdx.x & ((1u << log_pieces) - 1u);
+    for (uint32_t e = tid; e <= p.E; e += kBalThreads) hist[e] = 0;
+    if (tid == 0) foreign = 0;
+    __syncthreads();
+    const uint32_t* offsets = near_offsets(p, offsets_s);
+    uint32_t lo = 0, hi = p.T;
+    if (offsets) lo = min(offsets[s], p.T), hi = max(lo, min(offsets[s + 1], p.T));
+    const uint32_t from = lo + (uint32_t)(((uint64_t)(hi - lo) * piece) >> log_pieces);
+    const uint32_t to = lo + (uint32_t)(((uint64_t)(hi - lo) * (piece + 1u)) >> log_pieces);
+    if ((tid == 0 || tid == 32u) && offsets && from < to) {
         // offsets that fall: a range whose ends another sequence holds is empty
-        const bool ours = from < to && holds(p, s, from) && holds(p, s, to - 1u);
-        range[0] = from;
-        range[1] = ours ? to : from;
-        live_s = 0;
-        if (blockIdx.x == 0) *p.ticket = 0;
+        const uint32_t t = tid ? to - 1u : from;
+        if (sequence_after(offsets, p.S, t) != s || offsets[s] > t) foreign = 1;
     }
+    if (blockIdx.x == 0 && tid == 0) *p.ticket = 0;
     __syncthreads();
-    const uint32_t live = __reduce_add_sync(0xffffffffu, count_routes(p, range[0], range[1], hist));
-    if ((tid & 31u) == 0 && live) atomicAdd(&live_s, live);
-    __syncthreads();
-    uint32_t* out = p.part + (size_t)blockIdx.x * (p.E + 1u);
-    for (uint32_t e = tid; e < p.E; e += kBalThreads) out[e] = hist[e];
-    if (tid == 0) out[p.E] = live_s;
+    count_routes(p, from, foreign ? from : to, hist);
+    uint32_t* out = p.part + (size_t)(blockIdx.x / cluster) * (p.E + 1u);
+    if (cluster == 1u) {
+        __syncthreads();
+        for (uint32_t e = tid; e <= p.E; e += kBalThreads) out[e] = hist[e];
+        return;
+    }
+    tc::cluster_sync();
+    const uint32_t base = tc::smem_u32(hist);
+    for (uint32_t e = tc::cluster_rank() * kBalThreads + tid; e <= p.E; e += cluster * kBalThreads) {
+        uint32_t v[kBalCluster], sum = 0;
+#pragma unroll
+        for (uint32_t r = 0; r < kBalCluster; ++r) v[r] = r < cluster ? tc::cluster_ld(base + e * 4u, r) : 0u;
+#pragma unroll
+        for (uint32_t r = 0; r < kBalCluster; ++r) sum += v[r];
+        out[e] = sum;
+    }
+    tc::cluster_sync();  // no block leaves while its counts are read
 }
 
 // Entry e of sequence s (e == E: its live tokens), summed over the parts.
 __device__ __forceinline__ uint32_t part_sum(const BalanceParams& p, uint32_t s, uint32_t e) {
     const uint32_t* at = p.part + (size_t)s * p.parts * (p.E + 1u) + e;
-    uint32_t sum = 0;
-#pragma unroll 8
-    for (uint32_t i = 0; i < p.parts; ++i) sum += at[(size_t)i * (p.E + 1u)];
+    uint32_t v[kBalParts], sum = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kBalParts; ++i) v[i] = i < p.parts ? at[(size_t)i * (p.E + 1u)] : 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < kBalParts; ++i) sum += v[i];
     return sum;
 }
 
-// log(1 + e) for e in [0, 1] as 2 artanh(e / (2 + e)): the series' next term is below 2^-26 of it,
+// The row's arithmetic is what bounds the kernel next to HBM, so it uses the approximate reciprocal,
+// root and power of two (2 units of 2^-23 each; subnormals are 0).
+__device__ __forceinline__ float fast_rcp(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float fast_rsqrt(float x) {
+    float r;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// e^x as 2^(x log2 e). The rounding of the exponent's product, which grows with |x|, is put back:
+// 2^(t + c) = 2^t (1 + c ln 2), c the product's rest.
+__device__ __forceinline__ float fast_exp(float x) {
+    const float t = x * 1.44269504f;
+    const float c = fmaf(x, 1.44269504f, -t);
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    return x < -1000.f ? 0.f : fmaf(e, c * 0.693147181f, e);
+}
+
+// log(1 + e) / 2 for e in [0, 1] as artanh(e / (2 + e)): the series' next term is below 2^-26 of it,
 // and small e keep their bits.
-__device__ __forceinline__ float log1p_unit(float e) {
-    const float s = __fdividef(e, 2.f + e), q = s * s;
+__device__ __forceinline__ float half_log1p(float e) {
+    const float s = e * fast_rcp(2.f + e), q = s * s;
     float v = fmaf(q, 1.f / 13.f, 1.f / 11.f);
     v = fmaf(q, v, 1.f / 9.f);
     v = fmaf(q, v, 1.f / 7.f);
     v = fmaf(q, v, 1.f / 5.f);
     v = fmaf(q, v, 1.f / 3.f);
-    return 2.f * fmaf(s * q, v, s);
+    return fmaf(s * q, v, s);
 }
 
 // u(z) / U and u(z) r(z) / U, U a power that only depends on m = min(0, largest z) (softmax: m the
 // largest z): with it taken out the sums stay normal numbers however low a row's logits are.
-// ZERO: m is 0, as in every row with a logit that is not negative.
-template <int SCORE, bool ZERO>
+// PLAIN: m is 0 and every z is above -80, as in nearly every row.
+template <int SCORE, bool PLAIN>
 __device__ __forceinline__ void balance_score(float z, float m, float& u, float& ur) {
     if (SCORE == VLB_SCORE_SOFTMAX) {
-        u = expf(z - m);
+        u = fast_exp(z - m);
         ur = u;
         return;
     }
-    const float e = expf(-fabsf(z)), d = __fdividef(1.f, 1.f + e);
+    const float e = fast_exp(-fabsf(z)), d = fast_rcp(1.f + e);
     if (SCORE == VLB_SCORE_SIGMOID) {
-        const float low = ZERO ? e : expf(z - m);  // of a negative z; without ZERO all are
-        u = (ZERO && z > 0.f ? 1.f : low) * d;
-        ur = u * (z > 0.f ? e * d : d);
-    } else if (ZERO && z > -80.f) {
-        const float soft = fmaxf(z, 0.f) + log1p_unit(e), root = rsqrtf(soft);
+        const float low = e * d;
+        u = z > 0.f ? d : low;
+        if (PLAIN) {
+            ur = low * d;
+        } else {
+            if (z <= 0.f) u = fast_exp(z - m) * d;
+            ur = u * (z > 0.f ? low : d);
+        }
+    } else if (PLAIN || z > 0.f) {
+        const float soft = fmaf(2.f, half_log1p(e), fmaxf(z, 0.f)), root = fast_rsqrt(soft);
         u = soft * root;
         ur = 0.5f * (z > 0.f ? d : e * d) * root;
     } else {
         // softplus(z) = e^z q
-        const float q = e > 1e-30f ? __fdividef(log1p_unit(e), e) : 1.f, root = rsqrtf(q), x = expf(0.5f * (z - m));
+        const float q = e > 1e-30f ? 2.f * half_log1p(e) * fast_rcp(e) : 1.f, root = fast_rsqrt(q);
+        const float x = fast_exp(0.5f * (z - m));
         u = q * root * x;
         ur = 0.5f * d * root * x;
     }
+}
+
+// The rare rows' scores out of line: unrolled beside the others they would double the code every
+// block first has to fetch.
+template <int SCORE>
+__device__ __noinline__ float2 balance_score_rare(float z, float m) {
+    float2 v;
+    balance_score<SCORE, false>(z, m, v.x, v.y);
+    return v;
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -172,34 +264,48 @@ __device__ __forceinline__ uint32_t expert_of(uint32_t lane, uint32_t j) {
     return (j / VEC) * (32u * VEC) + lane * VEC + j % VEC;
 }
 
+template <typename T, uint32_t NV, uint32_t VEC>
+struct BalRow {
+    BalVec<T, VEC> v[NV / VEC];
+    bool live;
+    __device__ __forceinline__ void load(const BalanceParams& p, uint32_t t) {
+        live = !p.mask || p.mask[t];
+        const T* z = static_cast<const T*>(p.logits) + (size_t)t * p.stride;
+#pragma unroll
+        for (uint32_t j = 0; j < NV; j += VEC) {
+            const uint32_t e = expert_of<VEC>(threadIdx.x & 31u, j);
+            if (e < p.E) v[j / VEC] = *reinterpret_cast<const BalVec<T, VEC>*>(z + e);
+        }
+    }
+};
+
 // One token by a warp: returns weight * d_t and writes the row's gradient.
 template <typename T, int SCORE, uint32_t NV, uint32_t VEC>
-__device__ __forceinline__ float balance_row(const BalanceParams& p, uint32_t t, const float (&f)[NV], float weight,
-                                             float up) {
+__device__ __forceinline__ float balance_row(const BalanceParams& p, const BalRow<T, NV, VEC>& row, uint32_t t,
+                                             const float (&f)[NV], float weight, float up) {
     const uint32_t lane = threadIdx.x & 31u;
-    const T* z = static_cast<const T*>(p.logits) + (size_t)t * p.stride;
     float u[NV], ur[NV];
     float m = -INFINITY;
+    bool deep = false;
 #pragma unroll
-    for (uint32_t j = 0; j < NV; j += VEC) {
-        const uint32_t e = expert_of<VEC>(lane, j);
-        if (e < p.E) {
-            const BalVec<T, VEC> v = *reinterpret_cast<const BalVec<T, VEC>*>(z + e);
-#pragma unroll
-            for (uint32_t i = 0; i < VEC; ++i) u[j + i] = bl_float(v.v[i]);
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < VEC; ++i) u[j + i] = -INFINITY;
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < VEC; ++i) m = fmaxf(m, u[j + i]);
+    for (uint32_t j = 0; j < NV; ++j) {
+        const bool in = expert_of<VEC>(lane, j) < p.E;
+        u[j] = in ? bl_float(row.v[j / VEC].v[j % VEC]) : SCORE == VLB_SCORE_SOFTMAX ? -INFINITY : -79.f;
+        if (SCORE != VLB_SCORE_SOFTMAX) deep |= !(u[j] > -80.f);
+        if (in) m = fmaxf(m, u[j]);
     }
+    // (a place past the experts passes as -79: its score, under 2^-56 of the sum, leaves it as it is)
     const bool zero = SCORE != VLB_SCORE_SOFTMAX && __any_sync(0xffffffffu, m >= 0.f);
+    const bool plain = zero && !__any_sync(0xffffffffu, deep);
     bool none = false;
-    if (zero) {
-        m = 0.f;
-    } else {
-        m = warp_max(m);
+    if (zero) m = 0.f;
+    if (!plain) {
+        if (SCORE != VLB_SCORE_SOFTMAX) {
+#pragma unroll
+            for (uint32_t j = 0; j < NV; ++j)
+                if (expert_of<VEC>(lane, j) >= p.E) u[j] = -INFINITY;
+        }
+        if (!zero) m = warp_max(m);
         if (m == -INFINITY) {
             // no expert left by the row's mask: it adds nothing and gets no gradient; but a row
             // that holds a NaN is no such row
@@ -207,15 +313,20 @@ __device__ __forceinline__ float balance_row(const BalanceParams& p, uint32_t t,
 #pragma unroll
             for (uint32_t j = 0; j < NV; ++j) nan |= u[j] != u[j];
             none = !__any_sync(0xffffffffu, nan);
+            m = 0.f;  // its scores come out as 0
         }
     }
     float total = 0.f, dot = 0.f;
 #pragma unroll
     for (uint32_t j = 0; j < NV; ++j) {
-        const float zj = u[j];
-        if (expert_of<VEC>(lane, j) >= p.E || none) u[j] = ur[j] = 0.f;
-        else if (zero) balance_score<SCORE, true>(zj, 0.f, u[j], ur[j]);
-        else balance_score<SCORE, false>(zj, m, u[j], ur[j]);
+        const float zj = u[j];  // -inf (masked) scores 0
+        if (SCORE == VLB_SCORE_SOFTMAX || plain) {
+            balance_score<SCORE, true>(zj, m, u[j], ur[j]);
+        } else {
+            const float2 v = balance_score_rare<SCORE>(zj, m);
+            u[j] = v.x;
+            ur[j] = v.y;
+        }
         total += u[j];
         dot = fmaf(u[j], f[j], dot);
     }
@@ -251,70 +362,83 @@ __device__ __forceinline__ void clear_row(const BalanceParams& p, uint32_t t) {
     }
 }
 
-// A block takes a run of tokens, sequence by sequence. ONE: one block is the whole call, with one
-// sequence, and counts for itself.
+// A block takes a run of tokens, sequence by sequence; a warp reads its next row while it works on
+// one. ONE: one block is the whole call, with one sequence, and counts for itself.
 template <typename T, int SCORE, uint32_t NV, uint32_t VEC, bool ONE>
-__global__ void __launch_bounds__(kBalThreads) balance_kernel(const BalanceParams p) {
-    __shared__ float f_s[512];
-    __shared__ uint32_t hist[512], word[2];
+__global__ void __launch_bounds__(kBalThreads, NV > 8 ? 1 : 2) balance_kernel(const BalanceParams p) {
+    __shared__ uint32_t hist[513], alive_s, offsets_s[kBalSeqs + 1];
     __shared__ double part[kBalWarps];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    if (!ONE) tc::grid_dependency_wait();
-    if (tid < 2u) word[tid] = 0;
-    if (ONE)
-        for (uint32_t e = tid; e < p.E; e += kBalThreads) hist[e] = 0;
-    __syncthreads();
-    // the sequences with a live token; ONE: the live tokens
-    uint32_t mine = 0;
-    if (ONE) {
-        uint32_t lo = 0, hi = p.T;
-        if (p.seq_offsets) lo = min(p.seq_offsets[0], p.T), hi = max(lo, min(p.seq_offsets[1], p.T));
-        mine = count_routes(p, lo, hi, hist);
-    } else {
-        for (uint32_t s = tid; s < p.S; s += kBalThreads) mine += part_sum(p, s, p.E) != 0;
-        // the counts' own output, the sequences dealt over the blocks
-        for (uint32_t s = blockIdx.x; s < p.S; s += gridDim.x)
-            for (uint32_t e = tid; e < p.E; e += kBalThreads) p.counts[(size_t)s * p.E + e] = part_sum(p, s, e);
-    }
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if (lane == 0 && mine) atomicAdd(word, mine);
-    __syncthreads();
-    const float up = p.upstream ? *p.upstream : 1.f;
-    const uint32_t alive = ONE ? word[0] != 0 : word[0];
-    const float base = alive ? p.coefficient / (float)alive : 0.f;
-    double sum = 0.0;
     const uint32_t t0 = (uint32_t)((uint64_t)p.T * blockIdx.x / gridDim.x);
     const uint32_t t1 = (uint32_t)((uint64_t)p.T * (blockIdx.x + 1u) / gridDim.x);
+    BalRow<T, NV, VEC> row;
+    if (t0 + warp < t1) row.load(p, t0 + warp);  // no kernel's output: on its way while the counts are taken
+    const uint32_t* offsets = near_offsets(p, offsets_s);
+    if (tid == 0) alive_s = 0;
+    if (ONE)
+        for (uint32_t e = tid; e <= p.E; e += kBalThreads) hist[e] = 0;
+    const float up = p.upstream ? *p.upstream : 1.f;
+    // [t, end): tokens of sequence s, or of none (held)
+    uint32_t s = 0, end = t1;
+    bool held = true;
+    const auto segment = [&](uint32_t t) {
+        if (!offsets) return;
+        s = sequence_after(offsets, p.S, t);
+        held = s < p.S && offsets[s] <= t;
+        end = held ? min(t1, offsets[s + 1]) : s < p.S ? min(t1, offsets[s]) : t1;
+    };
+    const auto fetch_counts = [&] {
+        if (held)
+            for (uint32_t e = tid; e <= p.E; e += kBalThreads) hist[e] = part_sum(p, s, e);
+    };
+    if (t0 < t1) segment(t0);
+    if (!ONE) tc::grid_dependency_wait();
+    __syncthreads();
+    if (ONE) {
+        uint32_t lo = 0, hi = p.T;
+        if (offsets) lo = min(offsets[0], p.T), hi = max(lo, min(offsets[1], p.T));
+        count_routes(p, lo, hi, hist);
+    } else {
+        uint32_t with = 0;  // sequences with a live token
+        for (uint32_t i = tid; i < p.S; i += kBalThreads) with += part_sum(p, i, p.E) != 0;
+        if (t0 < t1) fetch_counts();
+        // the counts' own output, the sequences dealt over the blocks
+        for (uint32_t i = blockIdx.x; i < p.S; i += gridDim.x)
+            for (uint32_t e = tid; e < p.E; e += kBalThreads) p.counts[(size_t)i * p.E + e] = part_sum(p, i, e);
+        with = __reduce_add_sync(0xffffffffu, with);
+        if (lane == 0 && with) atomicAdd(&alive_s, with);
+    }
+    __syncthreads();
+    const uint32_t alive = ONE ? hist[p.E] != 0 : alive_s;
+    const float base = alive ? p.coefficient / (float)alive : 0.f;
+    double sum = 0.0;
+    uint32_t mine = t0 + warp;  // this warp's next token, its logits in `row`
     for (uint32_t t = t0; t < t1;) {
-        // [t, end): tokens of sequence s, or of none
-        uint32_t s = 0, end = t1;
-        bool held = true;
-        if (p.seq_offsets) {
-            s = sequence_after(p, t);
-            if (s == p.S) held = false;
-            else if (p.seq_offsets[s] > t) held = false, end = min(t1, p.seq_offsets[s]);
-            else end = min(t1, p.seq_offsets[s + 1]);
-        }
         float weight = 0.f, f[NV];
         if (held) {
-            __syncthreads();
-            if (!ONE && tid == 0) word[1] = part_sum(p, s, p.E);
-            for (uint32_t e = tid; e < p.E; e += kBalThreads) f_s[e] = (float)(ONE ? hist[e] : part_sum(p, s, e));
-            __syncthreads();
-            const uint32_t n = ONE ? word[0] : word[1];
+            const uint32_t n = hist[p.E];
             weight = n ? base / (float)n : 0.f;
             const float scale = n ? (float)p.E / ((float)p.k * (float)n) : 0.f;
 #pragma unroll
             for (uint32_t j = 0; j < NV; ++j) {
                 const uint32_t e = expert_of<VEC>(lane, j);
-                f[j] = e < p.E ? f_s[e] * scale : 0.f;
+                f[j] = e < p.E ? (float)hist[e] * scale : 0.f;
             }
         }
-        for (uint32_t r = t + warp; r < end; r += kBalWarps) {
-            if (held && (!p.mask || p.mask[r])) sum += (double)balance_row<T, SCORE, NV, VEC>(p, r, f, weight, up);
+        while (mine < end) {
+            const uint32_t r = mine;
+            const BalRow<T, NV, VEC> now = row;
+            mine += kBalWarps;
+            if (mine < t1) row.load(p, mine);
+            if (held && now.live) sum += (double)balance_row<T, SCORE, NV, VEC>(p, now, r, f, weight, up);
             else clear_row<T, NV, VEC>(p, r);
         }
         t = end;
+        if (t >= t1) break;
+        __syncthreads();  // hist is read by all
+        segment(t);
+        if (!ONE) fetch_counts();
+        __syncthreads();
     }
     if (ONE)
         for (uint32_t e = tid; e < p.E; e += kBalThreads) p.counts[e] = hist[e];
@@ -344,25 +468,38 @@ __global__ void __launch_bounds__(kBalThreads) balance_kernel(const BalanceParam
     if (lane == 0) *p.loss = (float)v;
 }
 
+// Blocks that count a sequence, a power of two: about 128 in all, but none for less than 256 tokens.
+uint32_t balance_pieces(uint32_t T, uint32_t S) {
+    uint32_t n = 1;
+    while (n < kBalCluster * kBalParts && n * S < 128u && n * S * 256u < T) n *= 2u;
+    return n;
+}
+
 template <typename T, int SCORE, uint32_t NV, uint32_t VEC>
 cudaError_t balance_launch(const BalanceParams& p, cudaStream_t s) {
     if (p.S == 1 && p.T <= kBalOneTokens) {
         balance_kernel<T, SCORE, NV, VEC, true><<<1, kBalThreads, 0, s>>>(p);
         return cudaGetLastError();
     }
-    balance_count_kernel<<<p.S * p.parts, kBalThreads, 0, s>>>(p);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    const uint32_t want = (p.T + kBalWarps - 1u) / kBalWarps;
+    const uint32_t pieces = balance_pieces(p.T, p.S), log_pieces = (uint32_t)__builtin_ctz(pieces);
+    const uint32_t cluster = pieces < kBalCluster ? pieces : kBalCluster;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(want < 1u ? 1u : want < kBalanceBlocks ? want : kBalanceBlocks);
+    cfg.gridDim = dim3(p.S * pieces);
     cfg.blockDim = dim3(kBalThreads);
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, balance_count_kernel, p, log_pieces, cluster);
+    if (e != cudaSuccess) return e;
+    const uint32_t want = (p.T + kBalWarps - 1u) / kBalWarps;
+    attr = cudaLaunchAttribute{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(want < 1u ? 1u : want < kBalanceBlocks ? want : kBalanceBlocks);
     return cudaLaunchKernelEx(&cfg, balance_kernel<T, SCORE, NV, VEC, false>, p);
 }
 
@@ -393,11 +530,9 @@ cudaError_t balance_typed(const BalanceParams& p, cudaStream_t s) {
 
 }  // namespace
 
-// Parts a sequence's routes are counted in: enough blocks to fill the GPU when the sequences are few,
-// few enough that the second kernel's blocks sum them in little time (64: 1 us at 256 experts).
 uint32_t balance_parts(uint32_t T, uint32_t S) {
-    const uint32_t by_seqs = S >= 64u ? 1u : 64u / S, by_tokens = T / 256u + 1u;
-    return by_seqs < by_tokens ? by_seqs : by_tokens;
+    const uint32_t pieces = balance_pieces(T, S);
+    return pieces < kBalCluster ? 1u : pieces / kBalCluster;
 }
 
 cudaError_t launch_balance(const BalanceParams& p, cudaStream_t s) {

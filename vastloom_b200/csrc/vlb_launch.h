@@ -123,9 +123,9 @@ struct BalanceParams {
     int score, logits_type;
     float coefficient;
 };
-constexpr uint32_t kBalanceBlocks = 444;  // 3 blocks of 512 threads on each of 148 SMs
+constexpr uint32_t kBalanceBlocks = 296;  // 2 blocks of 512 threads on each of 148 SMs
 constexpr uint32_t kBalOneTokens = 128;   // up to here one block does the whole call
-uint32_t balance_parts(uint32_t T, uint32_t S);
+uint32_t balance_parts(uint32_t T, uint32_t S);  // parts of a sequence's counts in the workspace
 cudaError_t launch_balance(const BalanceParams& p, cudaStream_t s);
 
 }  // namespace vlb
