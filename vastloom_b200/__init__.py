@@ -148,6 +148,11 @@ class _BalanceDesc(C.Structure):
                 ("reserved0", C.c_uint32)]
 
 
+# the same descriptions packed as bytes: building a ctypes structure costs more than the call
+_INT8_LINEAR_PACK = struct.Struct("=15Q4I2ifI").pack
+_BALANCE_PACK = struct.Struct("=12Q4I2ifI").pack
+
+
 class _LayerDesc(C.Structure):
     _fields_ = [
         ("hidden", C.c_uint32),
@@ -271,11 +276,11 @@ def load_library() -> C.CDLL:
         "vlb_layer_last_hyper_split": (I, [P, P, U32, P, P, P]),
         "vlb_int8_quantize_device": (I, [P, I, P, U64, U64, P, P, F, U32, U32, P, U64, P, P]),
         "vlb_int8_workspace_bytes": (U64, [U32, U32]),
-        "vlb_int8_linear_device": (I, [P, C.POINTER(_Int8LinearDesc), P]),
+        "vlb_int8_linear_device": (I, [P, P, P]),
         "vlb_int8_status": (I, [P, P]),
         "vlb_route_plan_device": (I, [P, P, P, U32, U32, U32, P, P, P, P, P, P]),
         "vlb_balance_workspace_bytes": (U64, [U32, U32, U32]),
-        "vlb_balance_loss_device": (I, [P, C.POINTER(_BalanceDesc), P]),
+        "vlb_balance_loss_device": (I, [P, P, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -625,9 +630,9 @@ class Device:
         call and need a workspace (int8_workspace_bytes); int8 rows bring x_scale_ptr."""
         w = weights
         st = self.lib.vlb_int8_linear_device(
-            self.h, _Int8LinearDesc(x_ptr, x_stride, x_rows, row_index_ptr, up_ptr, x_scale_ptr, row_weight_ptr, w.ptr,
-                                    w.scale_ptr, w.stride, offsets_ptr, y_ptr, y_stride, ws_ptr, ws_bytes, rows,
-                                    w.cols, w.rows, w.groups, x_type, y_type, swiglu_limit, 0), stream or None)
+            self.h, _INT8_LINEAR_PACK(x_ptr, x_stride, x_rows, row_index_ptr, up_ptr, x_scale_ptr, row_weight_ptr, w.ptr,
+                                      w.scale_ptr, w.stride, offsets_ptr, y_ptr, y_stride, ws_ptr, ws_bytes, rows,
+                                      w.cols, w.rows, w.groups, x_type, y_type, swiglu_limit, 0), stream or None)
         if st:
             self._check(st)
 
@@ -682,9 +687,9 @@ class Device:
         """Load-balance loss, per-expert counts and the logits' gradient (vlb_balance_loss_device) on
         raw device pointers; a loss or gradient pointer of 0 leaves that output out."""
         st = self.lib.vlb_balance_loss_device(
-            self.h, _BalanceDesc(logits_ptr, logits_stride, idx_ptr, mask_ptr, seq_offsets_ptr, upstream_ptr, loss_ptr,
-                                 counts_ptr, dlogits_ptr, dlogits_stride, ws_ptr, ws_bytes, T, E, k, n_seqs, score,
-                                 logits_type, coefficient, 0), stream or None)
+            self.h, _BALANCE_PACK(logits_ptr, logits_stride, idx_ptr, mask_ptr, seq_offsets_ptr, upstream_ptr, loss_ptr,
+                                  counts_ptr, dlogits_ptr, dlogits_stride, ws_ptr, ws_bytes, T, E, k, n_seqs, score,
+                                  logits_type, coefficient, 0), stream or None)
         if st:
             self._check(st)
 

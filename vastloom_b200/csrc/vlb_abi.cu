@@ -1779,6 +1779,10 @@ int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void
             p.x_scale = d.x_scale;
             p.x_stride = d.x_stride;
             if (d.rows == 0) return VLB_OK;
+            if (int8_few(p) && d.x_stride % 16 == 0 && aligned(d.x, 16)) {
+                VLB_CUDA(h, launch_int8_few(p, Int8QuantParams{}, d.x_type, d.y_type, s));
+                return VLB_OK;
+            }
         } else {
             if (const char* why =
                     bad_float_rows(d.x_type, d.x, d.x_stride, d.x_rows, d.row_index, d.up, d.swiglu_limit, d.rows, d.cols))
@@ -1800,6 +1804,10 @@ int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void
             q.cols = d.cols;
             q.fill_cols = (uint32_t)int8_pitch(d.cols);
             q.limit = d.swiglu_limit;
+            if (int8_few(p)) {
+                VLB_CUDA(h, launch_int8_few(p, q, d.x_type, d.y_type, s));
+                return VLB_OK;
+            }
             VLB_CUDA(h, launch_int8_quantize(q, d.x_type, s));
             p.x = q.q;
             p.x_scale = q.scale;

@@ -359,6 +359,145 @@ __global__ void __launch_bounds__(256) int8_linear_kernel(const Int8LinearParams
     }
 }
 
+// ---- product of few rows ------------------------------------------------------------------------
+//
+// One launch from the float rows on: for a handful of rows a call is as long as its launches and the
+// latency of its loads, and the weights are its bytes. A block quantizes the rows into shared memory
+// while its warps' first weights are on their way; then a warp takes two channels at a time, a lane
+// 16 bytes of each every 512, four such pieces of both in flight, dp4a against the rows. A call with
+// groups takes one row a block and that row's matrix (rows <= 16: two rows of one group read it
+// twice, from L2).
+
+constexpr uint32_t kFewThreads = 256, kFewWarps = kFewThreads / 32u, kFewPieces = 4;
+constexpr uint32_t kFewSmem = 64u * 1024u;
+
+// 16 bytes of a weight row from byte k on, zeros past K.
+__device__ __forceinline__ uint4 few_load(const int8_t* row, uint32_t k, uint32_t cols) {
+    if (k + 16u <= cols) return __ldg(reinterpret_cast<const uint4*>(row + k));
+    if (k >= cols) return make_uint4(0u, 0u, 0u, 0u);
+    return make_uint4(load_word(row, k, cols), load_word(row, k + 4u, cols), load_word(row, k + 8u, cols),
+                      load_word(row, k + 12u, cols));
+}
+
+__device__ __forceinline__ void store_typed(void* y, size_t at, float v, int type) {
+    if (type == VLB_DTYPE_F32) static_cast<float*>(y)[at] = v;
+    else if (type == VLB_DTYPE_F16) static_cast<__half*>(y)[at] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
+}
+
+// T: the rows' type, int8_t for rows that are integers already. ROWS: rows of a block.
+template <typename T, uint32_t ROWS>
+__global__ void __launch_bounds__(kFewThreads, 2) int8_few_kernel(const Int8LinearParams l, const Int8QuantParams q, int y_type,
+                                                               uint32_t channels) {
+    extern __shared__ __align__(16) unsigned char few_smem[];
+    __shared__ uint32_t top[ROWS], group_s;
+    __shared__ float scale[ROWS];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t pitch = (l.cols + 15u) / 16u * 16u;
+    uint32_t row0 = 0, rows = l.rows, g = 0;
+    if (l.offsets) {
+        row0 = blockIdx.y;
+        rows = 1;
+        if (tid == 0) group_s = l.groups;
+        __syncthreads();
+        for (uint32_t i = tid; i < l.groups; i += kFewThreads) {
+            uint32_t lo, hi;
+            group_range(l, i, lo, hi);
+            if (row0 >= lo && row0 < hi) atomicMin(&group_s, i);
+        }
+        __syncthreads();
+        g = group_s;
+        if (g == l.groups) return;
+    }
+    const uint32_t n_end = min(l.out_cols, (blockIdx.x + 1u) * channels);
+    const int8_t* w = l.w + (size_t)g * l.out_cols * l.w_stride;
+    uint32_t n = blockIdx.x * channels + 2u * warp;
+    uint4 a[kFewPieces], b[kFewPieces];
+    const auto fetch = [&](uint32_t n, uint32_t k0) {
+        const int8_t *wa = w + (size_t)n * l.w_stride, *wb = w + (size_t)min(n + 1u, l.out_cols - 1u) * l.w_stride;
+#pragma unroll
+        for (uint32_t i = 0; i < kFewPieces; ++i) {
+            a[i] = few_load(wa, k0 + 512u * i + 16u * lane, l.cols);
+            b[i] = few_load(wb, k0 + 512u * i + 16u * lane, l.cols);
+        }
+    };
+    if (n < n_end) fetch(n, 0);
+    // the rows: warps share them out, each row's warps its columns
+    if (tid < ROWS) top[tid] = 0;
+    __syncthreads();
+    const uint32_t row_warps = kFewWarps / ROWS, m = warp / row_warps, part = (warp % row_warps) * 32u + lane;
+    const uint32_t r = row0 + m;
+    int8_t* xs = reinterpret_cast<int8_t*>(few_smem);
+    if constexpr (std::is_same<T, int8_t>::value) {
+        if (m < rows && part == 0) scale[m] = l.row_weight ? l.x_scale[r] * l.row_weight[r] : l.x_scale[r];
+        for (uint32_t c = part * 16u; c < pitch; c += row_warps * 512u)
+            *reinterpret_cast<uint4*>(xs + m * pitch + c) =
+                m < rows ? few_load(l.x + (size_t)r * l.x_stride, c, l.cols) : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+        const uint64_t src = m < rows ? q.row_index ? q.row_index[r] : r : ~0ull;
+        const bool have = src < q.x_rows;
+        const size_t base = have ? src * q.x_stride : 0;
+        const auto value = [&](uint32_t c) {
+            return q.up ? row_value<T, true>(q, base + c) : row_value<T, false>(q, base + c);
+        };
+        uint32_t most = 0;
+        if (have)
+#pragma unroll 8
+            for (uint32_t c = part; c < l.cols; c += row_warps * 32u)
+                most = max(most, __float_as_uint(value(c)) & 0x7fffffffu);
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) atomicMax(top + m, most);
+        __syncthreads();
+        const RowStep st = row_step(top[m]);
+        if (m < rows && part == 0) scale[m] = l.row_weight ? st.scale * l.row_weight[r] : st.scale;
+#pragma unroll 8
+        for (uint32_t c = part; c < pitch; c += row_warps * 32u)
+            xs[m * pitch + c] = (int8_t)(have && c < l.cols ? quant_byte(value(c), st) : 0u);
+    }
+    __syncthreads();
+    for (; n < n_end; n += 2u * kFewWarps) {
+        int32_t sum[2][ROWS] = {};
+        for (uint32_t k0 = 0; k0 < l.cols; k0 += 512u * kFewPieces) {
+            uint4 va[kFewPieces], vb[kFewPieces];
+#pragma unroll
+            for (uint32_t i = 0; i < kFewPieces; ++i) va[i] = a[i], vb[i] = b[i];
+            // the next pieces, of these channels or the next two
+            if (k0 + 512u * kFewPieces < l.cols) fetch(n, k0 + 512u * kFewPieces);
+            else if (n + 2u * kFewWarps < n_end) fetch(n + 2u * kFewWarps, 0);
+#pragma unroll
+            for (uint32_t i = 0; i < kFewPieces; ++i) {
+                const uint32_t k = k0 + 512u * i + 16u * lane;
+                if (k >= pitch) break;
+#pragma unroll
+                for (uint32_t j = 0; j < ROWS; ++j) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(xs + j * pitch + k);
+                    sum[0][j] = __dp4a((int)va[i].x, (int)x.x, sum[0][j]);
+                    sum[1][j] = __dp4a((int)vb[i].x, (int)x.x, sum[1][j]);
+                    sum[0][j] = __dp4a((int)va[i].y, (int)x.y, sum[0][j]);
+                    sum[1][j] = __dp4a((int)vb[i].y, (int)x.y, sum[1][j]);
+                    sum[0][j] = __dp4a((int)va[i].z, (int)x.z, sum[0][j]);
+                    sum[1][j] = __dp4a((int)vb[i].z, (int)x.z, sum[1][j]);
+                    sum[0][j] = __dp4a((int)va[i].w, (int)x.w, sum[0][j]);
+                    sum[1][j] = __dp4a((int)vb[i].w, (int)x.w, sum[1][j]);
+                }
+            }
+        }
+        // lane c * ROWS + j stores row j of channel c
+        int32_t mine = 0;
+#pragma unroll
+        for (uint32_t c = 0; c < 2u; ++c)
+#pragma unroll
+            for (uint32_t j = 0; j < ROWS; ++j) {
+                const int32_t v = __reduce_add_sync(0xffffffffu, sum[c][j]);
+                if (lane == c * ROWS + j) mine = v;
+            }
+        const uint32_t c = n + lane / ROWS, j = lane % ROWS;
+        if (lane < 2u * ROWS && j < rows && c < n_end)
+            store_typed(l.y, (size_t)(row0 + j) * l.y_stride + c,
+                        (float)mine * scale[j] * l.w_scale[(size_t)g * l.out_cols + c], y_type);
+    }
+}
+
 // ---- product on the tensor cores ---------------------------------------------------------------
 //
 // D[channel][token] = W X^T by tcgen05.mma kind::i8: a tile is 128 channels (the TMEM lanes) by up
@@ -453,9 +592,9 @@ __device__ __forceinline__ MmTile mm_tile(const MmShared& sh, const Int8MmaParam
     }
     const uint32_t tt = sh.first[a + 1] - sh.first[a], local = t - sh.first[a] * p.ct;
     const uint32_t c = local / tt, j = local - c * tt;
-    const uint32_t n = sh.cnt[a];  // balanced: the group's tiles differ by one row at most
-    const uint32_t from = (uint32_t)((uint64_t)n * j / tt), to = (uint32_t)((uint64_t)n * (j + 1u) / tt);
-    return MmTile{a, sh.lo[a] + from, to - from, c * p.channels};
+    // balanced: the first `more` of the group's tiles have one row more than the others
+    const uint32_t each = sh.cnt[a] / tt, more = sh.cnt[a] - each * tt;
+    return MmTile{a, sh.lo[a] + j * each + min(j, more), each + (j < more ? 1u : 0u), c * p.channels};
 }
 
 template <typename TY>
@@ -855,6 +994,7 @@ cudaError_t general_type(const Int8LinearParams& p, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+// Opts a kernel in to `bytes` of shared memory, once on each device.
 template <typename K>
 cudaError_t smem_once(K kernel, size_t bytes) {
     static std::mutex mu;
@@ -912,8 +1052,10 @@ Mm mma_plan(Int8MmaParams& p, uint32_t sms) {
     const uint32_t used = l.groups < l.rows ? l.groups : l.rows;
     const uint32_t mean = (l.rows + used - 1u) / used;
     const auto split_of = [&](uint64_t tiles) {
+        // clusters of 8 only while they are few: more of them do not fit the GPU at once (16 tiles of
+        // 2048 x 2048 x 64 rows: 14 us in eights, 9 in fours)
         uint32_t split = 1;
-        while (split < 8u && tiles * split * 2u <= sms && p.nk >= split * 2u) split *= 2u;
+        while (split < 8u && tiles * split * 2u <= (split < 4u ? sms : 64u) && p.nk >= split * 2u) split *= 2u;
         return split;
     };
     Mm mode = Mm::kOne;
@@ -1000,6 +1142,36 @@ uint32_t sm_count() {
     return n ? n : 148u;
 }
 
+// What int8_few_kernel takes: its dp4a work grows with the rows (2048 x 2048: 3.6 us for one, 6.1 for
+// 4, 9.3 for 8; 4096 x 4096: 5.7, 11.2, 21.9), the tensor cores' two launches do not (about 9 and 10).
+constexpr uint32_t kFewRows = 8, kFewGroupedRows = 16;
+constexpr uint64_t kFewWork = 1u << 24;
+
+template <typename T, uint32_t ROWS>
+cudaError_t few_launch(const Int8LinearParams& l, const Int8QuantParams& q, int y_type, uint32_t sms, cudaStream_t s) {
+    auto* kernel = int8_few_kernel<T, ROWS>;
+    const size_t smem = (size_t)ROWS * ((l.cols + 15u) / 16u * 16u);
+    if (smem > 48u * 1024u) {
+        const cudaError_t e = smem_once(kernel, kFewSmem);
+        if (e != cudaSuccess) return e;
+    }
+    // about two blocks an SM (their registers), so that their set-up overlaps
+    const uint32_t sets = l.offsets ? l.rows : 1u;
+    uint32_t channels = (uint32_t)(((uint64_t)l.out_cols * sets + 2u * sms - 1u) / (2u * sms));
+    channels = (channels + 2u * kFewWarps - 1u) / (2u * kFewWarps) * (2u * kFewWarps);
+    kernel<<<dim3((l.out_cols + channels - 1u) / channels, sets), kFewThreads, smem, s>>>(l, q, y_type, channels);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t few_rows(const Int8LinearParams& l, const Int8QuantParams& q, int y_type, cudaStream_t s) {
+    const uint32_t rows = l.offsets ? 1u : l.rows, sms = sm_count();
+    if (rows <= 1u) return few_launch<T, 1>(l, q, y_type, sms, s);
+    if (rows <= 2u) return few_launch<T, 2>(l, q, y_type, sms, s);
+    if (rows <= 4u) return few_launch<T, 4>(l, q, y_type, sms, s);
+    return few_launch<T, 8>(l, q, y_type, sms, s);
+}
+
 template <typename TY>
 cudaError_t linear_type(const Int8LinearParams& l, bool after_quantize, cudaStream_t s) {
     if (tma_rows(l.w, l.w_stride) && tma_rows(l.x, l.x_stride)) {
@@ -1024,6 +1196,23 @@ cudaError_t launch_int8_quantize(const Int8QuantParams& p, int x_type, cudaStrea
         case VLB_DTYPE_F16: return quantize_type<__half>(p, s);
         case VLB_DTYPE_BF16: return quantize_type<__nv_bfloat16>(p, s);
         default: return cudaErrorInvalidValue;
+    }
+}
+
+bool int8_few(const Int8LinearParams& l) {
+    if (l.rows > (l.offsets ? kFewGroupedRows : kFewRows) || !tma_rows(l.w, l.w_stride)) return false;
+    if (!l.offsets && l.rows > 2u && (uint64_t)l.rows * l.cols * l.out_cols > kFewWork) return false;
+    uint32_t rows = 1;
+    while (!l.offsets && rows < l.rows) rows *= 2u;
+    return (size_t)rows * ((l.cols + 15u) / 16u * 16u) <= kFewSmem;
+}
+
+cudaError_t launch_int8_few(const Int8LinearParams& l, const Int8QuantParams& q, int x_type, int y_type, cudaStream_t s) {
+    switch (x_type) {
+        case VLB_DTYPE_F32: return few_rows<float>(l, q, y_type, s);
+        case VLB_DTYPE_F16: return few_rows<__half>(l, q, y_type, s);
+        case VLB_DTYPE_BF16: return few_rows<__nv_bfloat16>(l, q, y_type, s);
+        default: return few_rows<int8_t>(l, q, y_type, s);
     }
 }
 

@@ -99,6 +99,10 @@ struct Int8LinearParams {
 };
 constexpr uint32_t kInt8MaxGroups = 1024;
 cudaError_t launch_int8_quantize(const Int8QuantParams& p, int x_type, cudaStream_t s);
+// A product of few rows in one launch, its rows quantized on the way (q: their source, x_type I8:
+// unused); int8_few: whether it takes the call.
+bool int8_few(const Int8LinearParams& l);
+cudaError_t launch_int8_few(const Int8LinearParams& l, const Int8QuantParams& q, int x_type, int y_type, cudaStream_t s);
 // after_quantize: launch_int8_quantize went before it on the stream (the product may start beside it)
 cudaError_t launch_int8_linear(const Int8LinearParams& p, int y_type, bool after_quantize, cudaStream_t s);
 // reads and clears the error bits of the products on the current device (synchronises s)
