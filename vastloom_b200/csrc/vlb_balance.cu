@@ -117,6 +117,7 @@ __device__ __forceinline__ void count_routes(const BalanceParams& p, uint32_t lo
 // distributed shared memory to one part: E counts and, behind them, the live tokens.
 __global__ void __launch_bounds__(kBalThreads) balance_count_kernel(const BalanceParams p, uint32_t log_pieces, uint32_t cluster) {
     __shared__ uint32_t hist[513], foreign, offsets_s[kBalSeqs + 1];
+    tc::grid_dependency_wait();
     tc::grid_launch_dependents();
     const uint32_t tid = threadIdx.x, s = blockIdx.x >> log_pieces;
     const uint32_t piece = blockIdx.x & ((1u << log_pieces) - 1u);
@@ -371,8 +372,10 @@ __global__ void __launch_bounds__(kBalThreads, NV > 8 ? 1 : 2) balance_kernel(co
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     const uint32_t t0 = (uint32_t)((uint64_t)p.T * blockIdx.x / gridDim.x);
     const uint32_t t1 = (uint32_t)((uint64_t)p.T * (blockIdx.x + 1u) / gridDim.x);
+    if (ONE) tc::grid_dependency_wait();
+    tc::grid_launch_dependents();
     BalRow<T, NV, VEC> row;
-    if (t0 + warp < t1) row.load(p, t0 + warp);  // no kernel's output: on its way while the counts are taken
+    if (t0 + warp < t1) row.load(p, t0 + warp);  // on its way while the counts are taken
     const uint32_t* offsets = near_offsets(p, offsets_s);
     if (tid == 0) alive_s = 0;
     if (ONE)
@@ -477,30 +480,15 @@ uint32_t balance_pieces(uint32_t T, uint32_t S) {
 
 template <typename T, int SCORE, uint32_t NV, uint32_t VEC>
 cudaError_t balance_launch(const BalanceParams& p, cudaStream_t s) {
-    if (p.S == 1 && p.T <= kBalOneTokens) {
-        balance_kernel<T, SCORE, NV, VEC, true><<<1, kBalThreads, 0, s>>>(p);
-        return cudaGetLastError();
-    }
+    if (p.S == 1 && p.T <= kBalOneTokens)
+        return launch_chained(balance_kernel<T, SCORE, NV, VEC, true>, dim3(1), kBalThreads, 0, 0, s, p);
     const uint32_t pieces = balance_pieces(p.T, p.S), log_pieces = (uint32_t)__builtin_ctz(pieces);
     const uint32_t cluster = pieces < kBalCluster ? pieces : kBalCluster;
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr{};
-    cfg.gridDim = dim3(p.S * pieces);
-    cfg.blockDim = dim3(kBalThreads);
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, balance_count_kernel, p, log_pieces, cluster);
+    const cudaError_t e = launch_chained(balance_count_kernel, dim3(p.S * pieces), kBalThreads, 0, cluster, s, p, log_pieces, cluster);
     if (e != cudaSuccess) return e;
     const uint32_t want = (p.T + kBalWarps - 1u) / kBalWarps;
-    attr = cudaLaunchAttribute{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(want < 1u ? 1u : want < kBalanceBlocks ? want : kBalanceBlocks);
-    return cudaLaunchKernelEx(&cfg, balance_kernel<T, SCORE, NV, VEC, false>, p);
+    const uint32_t blocks = want < 1u ? 1u : want < kBalanceBlocks ? want : kBalanceBlocks;
+    return launch_chained(balance_kernel<T, SCORE, NV, VEC, false>, dim3(blocks), kBalThreads, 0, 0, s, p);
 }
 
 // NV: values of a row a lane holds; VEC: neighbours it loads at once, 1 where the rows do not start

@@ -90,6 +90,7 @@ template <typename T, bool SWIGLU>
 __global__ void __launch_bounds__(256) int8_quantize_kernel(const Int8QuantParams p) {
     __shared__ uint32_t top[8];
     const uint32_t tid = threadIdx.x;
+    tc::grid_dependency_wait();
     tc::grid_launch_dependents();
     for (size_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const uint64_t src = p.row_index ? p.row_index[r] : r;
@@ -196,6 +197,7 @@ template <typename T, bool SWIGLU, uint32_t ROW, uint32_t KEEP>
 __global__ void __launch_bounds__(256) int8_quantize_vec_kernel(const Int8QuantParams p) {
     constexpr uint32_t N = RowVec<T>::kN;
     __shared__ uint32_t top[8];
+    tc::grid_dependency_wait();
     tc::grid_launch_dependents();
     const uint32_t tid = threadIdx.x % ROW;
     const uint32_t vecs = (p.cols + N - 1u) / N, all = (p.fill_cols + N - 1u) / N;  // of x; of q
@@ -317,6 +319,8 @@ __device__ __forceinline__ uint32_t load_word(const int8_t* row, uint32_t c, uin
 template <typename TY>
 __global__ void __launch_bounds__(256) int8_linear_kernel(const Int8LinearParams p) {
     __shared__ uint32_t xs[kGenTile][kGenK / 4 + 1], ws[kGenTile][kGenK / 4 + 1];
+    tc::grid_dependency_wait();
+    tc::grid_launch_dependents();
     const uint32_t tid = threadIdx.x, tr = tid / 16u, tc = tid % 16u;
     const uint32_t n0 = blockIdx.x * kGenTile;
     for (uint32_t g = blockIdx.z; g < p.groups; g += gridDim.z) {
@@ -394,6 +398,8 @@ __global__ void __launch_bounds__(kFewThreads, 2) int8_few_kernel(const Int8Line
     __shared__ float scale[ROWS];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t pitch = (l.cols + 15u) / 16u * 16u;
+    tc::grid_dependency_wait();
+    tc::grid_launch_dependents();
     uint32_t row0 = 0, rows = l.rows, g = 0;
     if (l.offsets) {
         row0 = blockIdx.y;
@@ -530,6 +536,7 @@ struct Int8MmaParams {
     uint32_t ct, nk;    // channel tiles, K chunks
     uint32_t tmem_cols, acc_cols;
     uint32_t split;
+    uint32_t early;     // the kernel ahead quantizes the tokens: weights may be loaded beside it
 };
 
 // A wait that ran out (a fault of this code: every wait's event is this CTA's own copies or
@@ -624,7 +631,9 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         sh.lo = sh.first + l.groups + 1;
         sh.cnt = sh.lo + l.groups;
     }
+    if (!p.early) tc::grid_dependency_wait();
     if (smem & 1023u) {  // the swizzle atoms need it; the same in every CTA of the launch
+        tc::grid_dependency_wait();
         if (tid == 0) atomicOr(&g_int8_error, 2u);
         return;
     }
@@ -683,6 +692,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
     bool dirty = false, pending = false;  // copies / products under way when a role gave up
     uint32_t pending_bar = 0, pending_parity = 0;
 
+    tc::grid_launch_dependents();
     // ---- roles; in SPLIT mode each returns to the common tile loop after one tile -------------
     uint32_t stage = 0, phase = 0, it = 0;
     bool waited = false;  // on the kernel ahead
@@ -930,6 +940,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
             tc::cluster_sync();
         }
     }
+    if (!waited) tc::grid_dependency_wait();  // also a CTA without a tile
     __syncthreads();
     if (warp == kMmEpiWarps && lane == 0 && dirty) {
         // after giving up: copies already issued land before the CTA's shared memory goes away
@@ -964,21 +975,18 @@ cudaError_t quantize_rows(const Int8QuantParams& p, cudaStream_t s) {
     };
     const bool vec = on(p.x, p.x_stride * sizeof(T), 16) && on(p.up, 0, 16) && on(p.q, p.q_stride, N);
     if (!vec) {
-        int8_quantize_kernel<T, SWIGLU><<<p.rows < 65535u ? p.rows : 65535u, 256, 0, s>>>(p);
-    } else if (p.cols <= 32u * 8u * N && p.rows >= 2048u) {
+        return launch_chained(int8_quantize_kernel<T, SWIGLU>, dim3(p.rows < 65535u ? p.rows : 65535u), 256, 0, 0, s, p);
+    }
+    if (p.cols <= 32u * 8u * N && p.rows >= 2048u) {
         const uint32_t grid = (p.rows + 7u) / 8u;
         if (p.cols <= 32u * 4u * N)
-            int8_quantize_vec_kernel<T, SWIGLU, 32, 4><<<grid, 256, 0, s>>>(p);
-        else
-            int8_quantize_vec_kernel<T, SWIGLU, 32, 8><<<grid, 256, 0, s>>>(p);
-    } else {
-        const uint32_t grid = p.rows < 65535u ? p.rows : 65535u;
-        if (p.cols <= 256u * 2u * N)
-            int8_quantize_vec_kernel<T, SWIGLU, 256, 2><<<grid, 256, 0, s>>>(p);
-        else
-            int8_quantize_vec_kernel<T, SWIGLU, 256, 4><<<grid, 256, 0, s>>>(p);
+            return launch_chained(int8_quantize_vec_kernel<T, SWIGLU, 32, 4>, dim3(grid), 256, 0, 0, s, p);
+        return launch_chained(int8_quantize_vec_kernel<T, SWIGLU, 32, 8>, dim3(grid), 256, 0, 0, s, p);
     }
-    return cudaGetLastError();
+    const uint32_t grid = p.rows < 65535u ? p.rows : 65535u;
+    if (p.cols <= 256u * 2u * N)
+        return launch_chained(int8_quantize_vec_kernel<T, SWIGLU, 256, 2>, dim3(grid), 256, 0, 0, s, p);
+    return launch_chained(int8_quantize_vec_kernel<T, SWIGLU, 256, 4>, dim3(grid), 256, 0, 0, s, p);
 }
 
 template <typename T>
@@ -990,8 +998,7 @@ template <typename TY>
 cudaError_t general_type(const Int8LinearParams& p, cudaStream_t s) {
     const uint32_t tiles_n = (p.out_cols + kGenTile - 1u) / kGenTile, tiles_r = (p.rows + kGenTile - 1u) / kGenTile;
     const dim3 grid(tiles_n, tiles_r < 1024u ? tiles_r : 1024u, p.groups < 1024u ? p.groups : 1024u);
-    int8_linear_kernel<TY><<<grid, 256, 0, s>>>(p);
-    return cudaGetLastError();
+    return launch_chained(int8_linear_kernel<TY>, grid, 256, 0, 0, s, p);
 }
 
 // Opts a kernel in to `bytes` of shared memory, once on each device.
@@ -1105,30 +1112,13 @@ Mm mma_plan(Int8MmaParams& p, uint32_t sms) {
 }
 
 template <typename TY, Mm MODE>
-cudaError_t mma_launch(const Int8MmaParams& p, uint32_t sms, bool after_quantize, cudaStream_t s) {
+cudaError_t mma_launch(const Int8MmaParams& p, uint32_t sms, cudaStream_t s) {
     auto* kernel = int8_mma_kernel<TY, MODE>;
     const uint32_t in_cluster = MODE == Mm::kSplit ? p.split : MODE == Mm::kPair ? 2u : 1u;
     cudaError_t e = smem_once(kernel, kMmSmemLimit);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[2];
-    cfg.gridDim = dim3(sms / in_cluster * in_cluster);
-    cfg.blockDim = dim3(kMmThreads);
-    cfg.dynamicSmemBytes = p.stages * (kMmWStage + p.x_stage) + mm_fixed_bytes(p.l.groups);
-    cfg.stream = s;
-    cfg.attrs = attr;
-    if (MODE != Mm::kOne) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attr[cfg.numAttrs].val.clusterDim.x = in_cluster;
-        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
-        ++cfg.numAttrs;
-    }
-    if (after_quantize) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-        ++cfg.numAttrs;
-    }
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    const size_t smem = p.stages * (kMmWStage + p.x_stage) + mm_fixed_bytes(p.l.groups);
+    return launch_chained(kernel, dim3(sms / in_cluster * in_cluster), kMmThreads, smem, MODE == Mm::kOne ? 0 : in_cluster, s, p);
 }
 
 uint32_t sm_count() {
@@ -1159,8 +1149,8 @@ cudaError_t few_launch(const Int8LinearParams& l, const Int8QuantParams& q, int 
     const uint32_t sets = l.offsets ? l.rows : 1u;
     uint32_t channels = (uint32_t)(((uint64_t)l.out_cols * sets + 2u * sms - 1u) / (2u * sms));
     channels = (channels + 2u * kFewWarps - 1u) / (2u * kFewWarps) * (2u * kFewWarps);
-    kernel<<<dim3((l.out_cols + channels - 1u) / channels, sets), kFewThreads, smem, s>>>(l, q, y_type, channels);
-    return cudaGetLastError();
+    return launch_chained(kernel, dim3((l.out_cols + channels - 1u) / channels, sets), kFewThreads, smem, 0, s, l, q, y_type,
+                          channels);
 }
 
 template <typename T>
@@ -1177,13 +1167,14 @@ cudaError_t linear_type(const Int8LinearParams& l, bool after_quantize, cudaStre
     if (tma_rows(l.w, l.w_stride) && tma_rows(l.x, l.x_stride)) {
         Int8MmaParams p{};
         p.l = l;
+        p.early = after_quantize;
         const uint32_t sms = sm_count();
         const Mm mode = mma_plan(p, sms);
         if (encode_rows(&p.wmap, l.w, (uint64_t)l.groups * l.out_cols, l.cols, l.w_stride, kMmChannels) &&
             encode_rows(&p.xmap, l.x, l.rows, l.cols, l.x_stride, p.box))
-            return mode == Mm::kPair    ? mma_launch<TY, Mm::kPair>(p, sms, after_quantize, s)
-                   : mode == Mm::kSplit ? mma_launch<TY, Mm::kSplit>(p, sms, after_quantize, s)
-                                        : mma_launch<TY, Mm::kOne>(p, sms, after_quantize, s);
+            return mode == Mm::kPair    ? mma_launch<TY, Mm::kPair>(p, sms, s)
+                   : mode == Mm::kSplit ? mma_launch<TY, Mm::kSplit>(p, sms, s)
+                                        : mma_launch<TY, Mm::kOne>(p, sms, s);
     }
     return general_type<TY>(l, s);
 }

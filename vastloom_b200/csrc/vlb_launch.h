@@ -73,6 +73,31 @@ bool hc_entry_fits(uint32_t m, uint32_t H);
 cudaError_t launch_rms_norm(const float* x, const float* w, uint32_t rows, uint32_t width,
                             float eps, float* out, uint32_t* xmax, double* out_d, cudaStream_t s);
 
+// Launches a kernel that may start before the kernel ahead of it on the stream has ended: its blocks
+// come up meanwhile and wait (griddepcontrol.wait) before they touch anything that kernel may write
+// or read. Every block waits before it ends, so that a kernel behind waits for all before it.
+// cluster: blocks of a cluster, 0 none.
+template <typename... P, typename... A>
+cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, uint32_t block, size_t smem, uint32_t cluster, cudaStream_t s,
+                           const A&... args) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[2];
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    if (cluster) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 // ---- products on 8-bit integers (vlb_int8.cu) ----
 struct Int8QuantParams {
     const void* x;             // rows of VLB_DTYPE_F32 / F16 / BF16
