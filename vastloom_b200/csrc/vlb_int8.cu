@@ -115,9 +115,9 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(const Int8QuantParam
     }
 }
 
-// ---- row quantizer, rows on 16-byte boundaries ---------------------------------------------------
+// ---- row quantizer, integers written in words ----------------------------------------------------
 //
-// HBM-bound: every element is read once (16 bytes a load) and kept in registers between the row's
+// HBM-bound: every element is read once (16 bytes a load where the rows allow it) and kept in registers between the row's
 // maximum and its rounding; rows longer than the registers hold are read twice, the second time
 // mostly from L2. A warp takes a row of up to 8 loads a lane (8 rows a CTA: no barrier, all loads
 // in flight at once); longer rows, and calls of too few rows to fill the GPU with warps, take a
@@ -192,9 +192,10 @@ __device__ __forceinline__ void store_bytes(int8_t* q, const float (&x)[N], cons
     else *reinterpret_cast<uint32_t*>(q) = w[0];
 }
 
-// ROW: threads of a row (32 or the CTA's 256); KEEP: vectors a thread keeps.
-template <typename T, bool SWIGLU, uint32_t ROW, uint32_t KEEP>
-__global__ void __launch_bounds__(256) int8_quantize_vec_kernel(const Int8QuantParams p) {
+// ROW: threads of a row (32 or the CTA's 256); KEEP: vectors a thread keeps; WIDE: rows start on
+// 16-byte boundaries (others load each element by itself, from lines the warp shares).
+template <typename T, bool SWIGLU, uint32_t ROW, uint32_t KEEP, bool WIDE>
+__global__ void __launch_bounds__(256, SWIGLU || KEEP > 4 ? 3 : 5) int8_quantize_vec_kernel(const Int8QuantParams p) {
     constexpr uint32_t N = RowVec<T>::kN;
     __shared__ uint32_t top[8];
     tc::grid_dependency_wait();
@@ -210,8 +211,8 @@ __global__ void __launch_bounds__(256) int8_quantize_vec_kernel(const Int8QuantP
         auto fetch = [&](const T* row, uint32_t v) {
             RowVec<T> a;
             if (v >= have) a.clear();
-            else if ((v + 1u) * N <= p.cols) a.load(row + (size_t)v * N);
-            else a.load_part(row + (size_t)v * N, p.cols - v * N);
+            else if (WIDE && (v + 1u) * N <= p.cols) a.load(row + (size_t)v * N);
+            else a.load_part(row + (size_t)v * N, min(N, p.cols - v * N));
             return a;
         };
         RowVec<T> a[KEEP];
@@ -973,20 +974,23 @@ cudaError_t quantize_rows(const Int8QuantParams& p, cudaStream_t s) {
     auto on = [](const void* at, size_t stride_bytes, size_t n) {
         return reinterpret_cast<uintptr_t>(at) % n == 0 && stride_bytes % n == 0;
     };
-    const bool vec = on(p.x, p.x_stride * sizeof(T), 16) && on(p.up, 0, 16) && on(p.q, p.q_stride, N);
-    if (!vec) {
+    const bool wide = on(p.x, p.x_stride * sizeof(T), 16) && on(p.up, 0, 16);
+    if (!on(p.q, p.q_stride, N))
         return launch_chained(int8_quantize_kernel<T, SWIGLU>, dim3(p.rows < 65535u ? p.rows : 65535u), 256, 0, 0, s, p);
-    }
-    if (p.cols <= 32u * 8u * N && p.rows >= 2048u) {
-        const uint32_t grid = (p.rows + 7u) / 8u;
-        if (p.cols <= 32u * 4u * N)
-            return launch_chained(int8_quantize_vec_kernel<T, SWIGLU, 32, 4>, dim3(grid), 256, 0, 0, s, p);
-        return launch_chained(int8_quantize_vec_kernel<T, SWIGLU, 32, 8>, dim3(grid), 256, 0, 0, s, p);
-    }
+    const auto launch = [&](auto* narrow_kernel, auto* wide_kernel, uint32_t grid) {
+        return launch_chained(wide ? wide_kernel : narrow_kernel, dim3(grid), 256, 0, 0, s, p);
+    };
+    if (p.rows >= 2048u && p.cols <= 32u * 4u * N)
+        return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 4, false>, int8_quantize_vec_kernel<T, SWIGLU, 32, 4, true>,
+                      (p.rows + 7u) / 8u);
+    if constexpr (!SWIGLU)
+        if (p.rows >= 2048u && p.cols <= 32u * 8u * N)
+            return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 8, false>, int8_quantize_vec_kernel<T, SWIGLU, 32, 8, true>,
+                          (p.rows + 7u) / 8u);
     const uint32_t grid = p.rows < 65535u ? p.rows : 65535u;
     if (p.cols <= 256u * 2u * N)
-        return launch_chained(int8_quantize_vec_kernel<T, SWIGLU, 256, 2>, dim3(grid), 256, 0, 0, s, p);
-    return launch_chained(int8_quantize_vec_kernel<T, SWIGLU, 256, 4>, dim3(grid), 256, 0, 0, s, p);
+        return launch(int8_quantize_vec_kernel<T, SWIGLU, 256, 2, false>, int8_quantize_vec_kernel<T, SWIGLU, 256, 2, true>, grid);
+    return launch(int8_quantize_vec_kernel<T, SWIGLU, 256, 4, false>, int8_quantize_vec_kernel<T, SWIGLU, 256, 4, true>, grid);
 }
 
 template <typename T>
