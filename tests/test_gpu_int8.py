@@ -350,7 +350,8 @@ def test_linear_large(dev, torch, M, N, K):
 
 
 @pytest.mark.parametrize("counts,N,K", [([700, 0, 300, 513, 1, 2000], 1100, 300), ([0, 1300, 1300], 2000, 64),
-                                        ([400] * 20, 1000, 96), ([0, 5000, 3], 700, 500)])
+                                        ([400] * 20, 1000, 96), ([0, 5000, 3], 700, 500),
+                                        ([9000, 0, 7411, 30], 300, 1037)])
 def test_large_groups(dev, torch, counts, N, K):
     rng = np.random.default_rng(N)
     G, rows, T = len(counts), sum(counts), 900
@@ -368,6 +369,24 @@ def test_large_groups(dev, torch, counts, N, K):
     for g in range(G):
         sl = slice(off[g], off[g + 1])
         check_product(out[sl], product(q[index[sl]], s[index[sl]], w[g, :, :K], sw[g], rw[sl]), "f32")
+
+
+def test_gathered_rows_that_are_not_there(dev, torch):
+    """Indices past x are rows of zeros, also where the rows are quantized apart from their copies."""
+    rng = np.random.default_rng(12)
+    T, K, N = 70, 1024, 40
+    for rows in (6, 300, 16400):
+        x, w = rng.standard_normal((T, K)).astype(np.float32), rng.integers(-127, 128, (1, N, K), dtype=np.int8)
+        index = rng.integers(0, T + 9, rows).astype(np.int32)
+        index[rows // 2] = -1
+        sw = rng.random((1, N), np.float32)
+        ic = cuda(torch, index)
+        y = run_linear(dev, torch, cuda(torch, x), cuda(torch, w), cuda(torch, sw), rows=rows, x_rows=T,
+                       row_index_ptr=ic.data_ptr()).cpu().numpy()
+        there = (index >= 0) & (index < T)
+        q, s = quantized(x)
+        src = np.where(there, index, 0)
+        check_product(y, product(q[src], s[src] * there, w[0], sw[0]), "f32")
 
 
 @pytest.mark.parametrize("offsets", [[2, 5, 9], [0, 4, 100], [0, 7, 3], [50, 60, 70], [-1, 5, 9]])

@@ -121,26 +121,27 @@ __global__ void __launch_bounds__(kBalThreads) balance_count_kernel(const Balanc
     tc::grid_launch_dependents();
     const uint32_t tid = threadIdx.x, s = blockIdx.x >> log_pieces;
     const uint32_t piece = blockIdx.x & ((1u << log_pieces) - 1u);
+    uint32_t lo = 0, hi = p.T;
+    if (p.seq_offsets) lo = min(p.seq_offsets[s], p.T), hi = max(lo, min(p.seq_offsets[s + 1], p.T));
+    const uint32_t* offsets = near_offsets(p, offsets_s);
     for (uint32_t e = tid; e <= p.E; e += kBalThreads) hist[e] = 0;
     if (tid == 0) foreign = 0;
-    __syncthreads();
-    const uint32_t* offsets = near_offsets(p, offsets_s);
-    uint32_t lo = 0, hi = p.T;
-    if (offsets) lo = min(offsets[s], p.T), hi = max(lo, min(offsets[s + 1], p.T));
+    if (blockIdx.x == 0 && tid == 0) *p.ticket = 0;
     const uint32_t from = lo + (uint32_t)(((uint64_t)(hi - lo) * piece) >> log_pieces);
     const uint32_t to = lo + (uint32_t)(((uint64_t)(hi - lo) * (piece + 1u)) >> log_pieces);
+    __syncthreads();
     if ((tid == 0 || tid == 32u) && offsets && from < to) {
         // offsets that fall: a range whose ends another sequence holds is empty
         const uint32_t t = tid ? to - 1u : from;
         if (sequence_after(offsets, p.S, t) != s || offsets[s] > t) foreign = 1;
     }
-    if (blockIdx.x == 0 && tid == 0) *p.ticket = 0;
+    count_routes(p, from, to, hist);
     __syncthreads();
-    count_routes(p, from, foreign ? from : to, hist);
+    if (foreign)
+        for (uint32_t e = tid; e <= p.E; e += kBalThreads) hist[e] = 0;
     uint32_t* out = p.part + (size_t)(blockIdx.x / cluster) * (p.E + 1u);
     if (cluster == 1u) {
-        __syncthreads();
-        for (uint32_t e = tid; e <= p.E; e += kBalThreads) out[e] = hist[e];
+        for (uint32_t e = tid; e <= p.E; e += kBalThreads) out[e] = hist[e];  // entries this thread zeroed, or summed by all
         return;
     }
     tc::cluster_sync();
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(kBalThreads, NV > 8 ? 1 : 2) balance_kernel(co
     if (ONE)
         for (uint32_t e = tid; e <= p.E; e += kBalThreads) hist[e] = 0;
     const float up = p.upstream ? *p.upstream : 1.f;
-    // [t, end): tokens of sequence s, or of none (held)
+    // [t, end): tokens of sequence s, or of none
     uint32_t s = 0, end = t1;
     bool held = true;
     const auto segment = [&](uint32_t t) {
@@ -483,7 +484,7 @@ cudaError_t balance_launch(const BalanceParams& p, cudaStream_t s) {
     if (p.S == 1 && p.T <= kBalOneTokens)
         return launch_chained(balance_kernel<T, SCORE, NV, VEC, true>, dim3(1), kBalThreads, 0, 0, s, p);
     const uint32_t pieces = balance_pieces(p.T, p.S), log_pieces = (uint32_t)__builtin_ctz(pieces);
-    const uint32_t cluster = pieces < kBalCluster ? pieces : kBalCluster;
+    const uint32_t cluster = pieces / balance_parts(p.T, p.S);
     const cudaError_t e = launch_chained(balance_count_kernel, dim3(p.S * pieces), kBalThreads, 0, cluster, s, p, log_pieces, cluster);
     if (e != cudaSuccess) return e;
     const uint32_t want = (p.T + kBalWarps - 1u) / kBalWarps;
@@ -520,7 +521,7 @@ cudaError_t balance_typed(const BalanceParams& p, cudaStream_t s) {
 
 uint32_t balance_parts(uint32_t T, uint32_t S) {
     const uint32_t pieces = balance_pieces(T, S);
-    return pieces < kBalCluster ? 1u : pieces / kBalCluster;
+    return pieces <= kBalParts ? pieces : pieces / kBalCluster;
 }
 
 cudaError_t launch_balance(const BalanceParams& p, cudaStream_t s) {

@@ -290,6 +290,29 @@ __global__ void __launch_bounds__(256, SWIGLU || KEEP > 4 ? 3 : 5) int8_quantize
     }
 }
 
+// Quantized rows by index: a warp a row, 16 bytes a lane.
+__global__ void __launch_bounds__(256) int8_gather_kernel(const Int8GatherParams p) {
+    tc::grid_dependency_wait();
+    tc::grid_launch_dependents();
+    const uint32_t lane = threadIdx.x & 31u, vecs = (uint32_t)(p.pitch / 16u);
+    for (size_t r = (size_t)blockIdx.x * 8u + (threadIdx.x >> 5); r < p.rows; r += (size_t)gridDim.x * 8u) {
+        const uint32_t src = p.row_index[r];
+        const bool have = src < p.x_rows;
+        const uint4* from = reinterpret_cast<const uint4*>(p.x + (size_t)(have ? src : 0u) * p.pitch);
+        uint4* to = reinterpret_cast<uint4*>(p.q + r * p.pitch);
+        if (lane == 0) p.scale[r] = have ? p.x_scale[src] : 0.f;
+        for (uint32_t v0 = lane; v0 < vecs; v0 += 128u) {
+            uint4 a[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i)
+                a[i] = have && v0 + 32u * i < vecs ? from[v0 + 32u * i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i)
+                if (v0 + 32u * i < vecs) to[v0 + 32u * i] = a[i];
+        }
+    }
+}
+
 // ---- groups ----------------------------------------------------------------------------------
 
 // Rows of group g, kept inside [0, rows] whatever the offsets hold.
@@ -605,12 +628,6 @@ __device__ __forceinline__ MmTile mm_tile(const MmShared& sh, const Int8MmaParam
     return MmTile{a, sh.lo[a] + j * each + min(j, more), each + (j < more ? 1u : 0u), c * p.channels};
 }
 
-template <typename TY>
-__device__ __forceinline__ void mm_store(const Int8LinearParams& l, uint32_t row, uint32_t n, int32_t acc, float s,
-                                         float t) {
-    static_cast<TY*>(l.y)[(size_t)row * l.y_stride + n] = from_float<TY>((float)acc * s * t);
-}
-
 template <typename TY, Mm MODE>
 __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_constant__ Int8MmaParams p) {
     constexpr bool SPLIT = MODE == Mm::kSplit, PAIR = MODE == Mm::kPair;
@@ -877,7 +894,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
             // role has given up
             const MmTile tile = mm_tile(sh, p, t);
             bool ok = true;
-            float cs = 0.f;
+            float cs[4] = {};
             float* ts = sh.scale;
             if (warp == kMmEpiWarps) {
                 ok = __all_sync(0xffffffffu, *sh.abort == 0) && produce(t);
@@ -894,8 +911,11 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
                 }
                 ok = __all_sync(0xffffffffu, *sh.abort == 0 && mm_wait(sh.acc_full, it & 1u, sh.abort));
                 ++it;
-                const uint32_t n = tile.channel0 + 32u * quad + lane;
-                cs = n < l.out_cols ? l.w_scale[(size_t)tile.g * l.out_cols + n] : 0.f;
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; ++i) {
+                    const uint32_t n = tile.channel0 + 4u * lane + i;
+                    cs[i] = n < l.out_cols ? l.w_scale[(size_t)tile.g * l.out_cols + n] : 0.f;
+                }
                 if (ok) {
                     tc::fence_after_sync();
                     const uint32_t src = tmem + ((32u * quad) << 16);
@@ -914,25 +934,30 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
             __syncwarp();
             tc::cluster_sync();
             if (warp < kMmEpiWarps) {
-                const uint32_t c = 32u * quad + lane, n = tile.channel0 + c;
-                // two columns at a time, so that up to 16 loads from the peers are in flight
-                const uint32_t pace = 2u * p.split;
-                for (uint32_t j = rank * 2u + half; j < tile.count; j += 2u * pace) {
-                    uint32_t v[2][8];
+                // a warp takes every split-th token, a lane four neighbouring channels: the loads of two
+                // tokens from all peers are in flight together
+                const uint32_t pace = kMmEpiWarps * p.split, c = 4u * lane, n = tile.channel0 + c;
+                for (uint32_t j = rank + p.split * warp; j < tile.count; j += 2u * pace) {
+                    uint4 v[2][8];
 #pragma unroll
                     for (uint32_t u = 0; u < 2u; ++u)
 #pragma unroll
                         for (uint32_t r = 0; r < 8u; ++r)
                             v[u][r] = r < p.split && j + u * pace < tile.count
-                                          ? tc::cluster_ld(smem + ((j + u * pace) * kMmChannels + c) * 4u, r) : 0u;
+                                          ? tc::cluster_ld16(smem + ((j + u * pace) * kMmChannels + c) * 4u, r)
+                                          : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
                     for (uint32_t u = 0; u < 2u; ++u) {
                         if (j + u * pace >= tile.count) break;
-                        uint32_t sum = 0;
+                        uint4 sum = v[u][0];
 #pragma unroll
-                        for (uint32_t r = 0; r < 8u; ++r) sum += v[u][r];
-                        const uint32_t row = tile.row0 + j + u * pace;
-                        if (n < l.out_cols) mm_store<TY>(l, row, n, (int32_t)sum, ts[j + u * pace], cs);
+                        for (uint32_t r = 1; r < 8u; ++r)
+                            sum.x += v[u][r].x, sum.y += v[u][r].y, sum.z += v[u][r].z, sum.w += v[u][r].w;
+                        const float s = ts[j + u * pace];
+                        TY* y = static_cast<TY*>(l.y) + (size_t)(tile.row0 + j + u * pace) * l.y_stride + n;
+#pragma unroll
+                        for (uint32_t i = 0; i < 4u; ++i)
+                            if (n + i < l.out_cols) y[i] = from_float<TY>((float)(int32_t)(&sum.x)[i] * s * cs[i]);
                     }
                 }
             }
@@ -1192,6 +1217,10 @@ cudaError_t launch_int8_quantize(const Int8QuantParams& p, int x_type, cudaStrea
         case VLB_DTYPE_BF16: return quantize_type<__nv_bfloat16>(p, s);
         default: return cudaErrorInvalidValue;
     }
+}
+
+cudaError_t launch_int8_gather(const Int8GatherParams& p, cudaStream_t s) {
+    return launch_chained(int8_gather_kernel, dim3((p.rows + 7u) / 8u), 256, 0, 0, s, p);
 }
 
 bool int8_few(const Int8LinearParams& l) {

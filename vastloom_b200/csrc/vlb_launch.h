@@ -111,6 +111,15 @@ struct Int8QuantParams {
     uint32_t fill_cols;        // columns written: cols, then zeros
     float limit;               // SwiGLU clamp, 0: none
 };
+struct Int8GatherParams {
+    const int8_t* x;           // [x_rows] quantized rows of `pitch` bytes (a multiple of 16)
+    const float* x_scale;
+    const uint32_t* row_index; // an index >= x_rows: a row of zeros, scale 0
+    int8_t* q;
+    float* scale;
+    size_t pitch;
+    uint32_t x_rows, rows;
+};
 struct Int8LinearParams {
     const int8_t* x;           // [rows] of x_stride
     const float* x_scale;
@@ -123,6 +132,7 @@ struct Int8LinearParams {
     uint32_t rows, cols, out_cols, groups;
 };
 constexpr uint32_t kInt8MaxGroups = 1024;
+cudaError_t launch_int8_gather(const Int8GatherParams& p, cudaStream_t s);
 cudaError_t launch_int8_quantize(const Int8QuantParams& p, int x_type, cudaStream_t s);
 // A product of few rows in one launch, its rows quantized on the way (q: their source, x_type I8:
 // unused); int8_few: whether it takes the call.

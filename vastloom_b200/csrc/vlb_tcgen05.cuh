@@ -297,6 +297,16 @@ __device__ __forceinline__ uint32_t cluster_ld(uint32_t addr, uint32_t rank) {
     return v;
 }
 
+// 16 bytes from there.
+__device__ __forceinline__ uint4 cluster_ld16(uint32_t addr, uint32_t rank) {
+    uint4 v;
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [a];\n\t}"
+        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+        : "r"(addr), "r"(rank)
+        : "memory");
+    return v;
+}
 // This block's shared-memory address `addr`, as seen in block `rank` of the cluster.
 __device__ __forceinline__ uint32_t cluster_map(uint32_t addr, uint32_t rank) {
     uint32_t a;
