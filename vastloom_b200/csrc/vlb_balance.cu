@@ -21,6 +21,7 @@
 #include <cuda_runtime.h>
 
 #include "vlb_launch.h"
+#include "vlb_math.cuh"
 #include "vlb_tcgen05.cuh"
 
 namespace vlb {
@@ -168,27 +169,8 @@ __device__ __forceinline__ uint32_t part_sum(const BalanceParams& p, uint32_t s,
     return sum;
 }
 
-// The row's arithmetic is what bounds the kernel next to HBM, so it uses the approximate reciprocal,
-// root and power of two (2 units of 2^-23 each; subnormals are 0).
-__device__ __forceinline__ float fast_rcp(float x) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ float fast_rsqrt(float x) {
-    float r;
-    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-// e^x as 2^(x log2 e). The rounding of the exponent's product, which grows with |x|, is put back:
-// 2^(t + c) = 2^t (1 + c ln 2), c the product's rest.
-__device__ __forceinline__ float fast_exp(float x) {
-    const float t = x * 1.44269504f;
-    const float c = fmaf(x, 1.44269504f, -t);
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-    return x < -1000.f ? 0.f : fmaf(e, c * 0.693147181f, e);
-}
+// e^x for any x <= 0 (-inf: 0; a NaN stays).
+__device__ __forceinline__ float exp_low(float x) { return x < -1000.f ? 0.f : fast_exp(x); }
 
 // log(1 + e) / 2 for e in [0, 1] as artanh(e / (2 + e)): the series' next term is below 2^-26 of it,
 // and small e keep their bits.
@@ -204,34 +186,33 @@ __device__ __forceinline__ float half_log1p(float e) {
 
 // u(z) / U and u(z) r(z) / U, U a power that only depends on m = min(0, largest z) (softmax: m the
 // largest z): with it taken out the sums stay normal numbers however low a row's logits are.
-// PLAIN: m is 0 and every z is above -80, as in nearly every row.
+// PLAIN: m is 0 and every z is in (-80, 900), as in nearly every row.
 template <int SCORE, bool PLAIN>
 __device__ __forceinline__ void balance_score(float z, float m, float& u, float& ur) {
     if (SCORE == VLB_SCORE_SOFTMAX) {
-        u = fast_exp(z - m);
+        u = exp_low(z - m);
         ur = u;
-        return;
-    }
-    const float e = fast_exp(-fabsf(z)), d = fast_rcp(1.f + e);
-    if (SCORE == VLB_SCORE_SIGMOID) {
-        const float low = e * d;
-        u = z > 0.f ? d : low;
-        if (PLAIN) {
-            ur = low * d;
-        } else {
-            if (z <= 0.f) u = fast_exp(z - m) * d;
-            ur = u * (z > 0.f ? low : d);
-        }
-    } else if (PLAIN || z > 0.f) {
-        const float soft = fmaf(2.f, half_log1p(e), fmaxf(z, 0.f)), root = fast_rsqrt(soft);
-        u = soft * root;
-        ur = 0.5f * (z > 0.f ? d : e * d) * root;
+    } else if (SCORE == VLB_SCORE_SIGMOID && PLAIN) {
+        const float t = fast_exp(-z);  // below e^80; r = 1 - u = t u
+        u = fast_rcp(1.f + t);
+        ur = t * u * u;
+    } else if (SCORE == VLB_SCORE_SIGMOID) {
+        const float e = exp_low(-fabsf(z)), d = fast_rcp(1.f + e);
+        u = z > 0.f ? d : exp_low(z - m) * d;
+        ur = u * (z > 0.f ? e * d : d);
     } else {
-        // softplus(z) = e^z q
-        const float q = e > 1e-30f ? 2.f * half_log1p(e) * fast_rcp(e) : 1.f, root = fast_rsqrt(q);
-        const float x = fast_exp(0.5f * (z - m));
-        u = q * root * x;
-        ur = 0.5f * d * root * x;
+        const float e = PLAIN ? fast_exp(-fabsf(z)) : exp_low(-fabsf(z)), d = fast_rcp(1.f + e);
+        if (PLAIN || z > 0.f) {
+            const float soft = fmaf(2.f, half_log1p(e), fmaxf(z, 0.f)), root = fast_rsqrt(soft);
+            u = soft * root;
+            ur = (z > 0.f ? 0.5f : 0.5f * e) * d * root;
+        } else {
+            // softplus(z) = e^z q
+            const float q = e > 1e-30f ? 2.f * half_log1p(e) * fast_rcp(e) : 1.f, root = fast_rsqrt(q);
+            const float x = exp_low(0.5f * (z - m));
+            u = q * root * x;
+            ur = 0.5f * d * root * x;
+        }
     }
 }
 
@@ -244,11 +225,6 @@ __device__ __noinline__ float2 balance_score_rare(float z, float m) {
     return v;
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -266,7 +242,7 @@ __device__ __forceinline__ uint32_t expert_of(uint32_t lane, uint32_t j) {
     return (j / VEC) * (32u * VEC) + lane * VEC + j % VEC;
 }
 
-template <typename T, uint32_t NV, uint32_t VEC>
+template <typename T, uint32_t NV, uint32_t VEC, bool FULL>
 struct BalRow {
     BalVec<T, VEC> v[NV / VEC];
     bool live;
@@ -276,14 +252,14 @@ struct BalRow {
 #pragma unroll
         for (uint32_t j = 0; j < NV; j += VEC) {
             const uint32_t e = expert_of<VEC>(threadIdx.x & 31u, j);
-            if (e < p.E) v[j / VEC] = *reinterpret_cast<const BalVec<T, VEC>*>(z + e);
+            if (FULL || e < p.E) v[j / VEC] = *reinterpret_cast<const BalVec<T, VEC>*>(z + e);
         }
     }
 };
 
 // One token by a warp: returns weight * d_t and writes the row's gradient.
-template <typename T, int SCORE, uint32_t NV, uint32_t VEC>
-__device__ __forceinline__ float balance_row(const BalanceParams& p, const BalRow<T, NV, VEC>& row, uint32_t t,
+template <typename T, int SCORE, uint32_t NV, uint32_t VEC, bool FULL>
+__device__ __forceinline__ float balance_row(const BalanceParams& p, const BalRow<T, NV, VEC, FULL>& row, uint32_t t,
                                              const float (&f)[NV], float weight, float up) {
     const uint32_t lane = threadIdx.x & 31u;
     float u[NV], ur[NV];
@@ -291,21 +267,21 @@ __device__ __forceinline__ float balance_row(const BalanceParams& p, const BalRo
     bool deep = false;
 #pragma unroll
     for (uint32_t j = 0; j < NV; ++j) {
-        const bool in = expert_of<VEC>(lane, j) < p.E;
+        const bool in = FULL || expert_of<VEC>(lane, j) < p.E;
         u[j] = in ? bl_float(row.v[j / VEC].v[j % VEC]) : SCORE == VLB_SCORE_SOFTMAX ? -INFINITY : -79.f;
-        if (SCORE != VLB_SCORE_SOFTMAX) deep |= !(u[j] > -80.f);
+        if (SCORE != VLB_SCORE_SOFTMAX) deep |= u[j] < -80.f;
         if (in) m = fmaxf(m, u[j]);
     }
     // (a place past the experts passes as -79: its score, under 2^-56 of the sum, leaves it as it is)
     const bool zero = SCORE != VLB_SCORE_SOFTMAX && __any_sync(0xffffffffu, m >= 0.f);
-    const bool plain = zero && !__any_sync(0xffffffffu, deep);
+    const bool plain = zero && !__any_sync(0xffffffffu, deep || m > 900.f);
     bool none = false;
     if (zero) m = 0.f;
     if (!plain) {
         if (SCORE != VLB_SCORE_SOFTMAX) {
 #pragma unroll
             for (uint32_t j = 0; j < NV; ++j)
-                if (expert_of<VEC>(lane, j) >= p.E) u[j] = -INFINITY;
+                if (!FULL && expert_of<VEC>(lane, j) >= p.E) u[j] = -INFINITY;
         }
         if (!zero) m = warp_max(m);
         if (m == -INFINITY) {
@@ -332,19 +308,23 @@ __device__ __forceinline__ float balance_row(const BalanceParams& p, const BalRo
         total += u[j];
         dot = fmaf(u[j], f[j], dot);
     }
-    total = warp_sum(total);
-    dot = warp_sum(dot);
-    const float inv = none ? 0.f : 1.f / total, d = dot * inv;
+    // both sums at once: the lower half of the warp goes on with one, the upper with the other
+    float half = (lane & 16u ? dot : total) + __shfl_xor_sync(0xffffffffu, lane & 16u ? total : dot, 16);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) half += __shfl_xor_sync(0xffffffffu, half, o);
+    total = __shfl_sync(0xffffffffu, half, 0);
+    dot = __shfl_sync(0xffffffffu, half, 16);
+    const float inv = none ? 0.f : fast_rcp(total), d = dot * inv;
     if (p.dlogits) {
         T* grad = static_cast<T*>(p.dlogits) + (size_t)t * p.grad_stride;
-        const float gw = up * weight * inv;
+        const float gw = up * weight * inv, gd = gw * d;
 #pragma unroll
         for (uint32_t j = 0; j < NV; j += VEC) {
             const uint32_t e = expert_of<VEC>(lane, j);
             BalVec<T, VEC> v;
 #pragma unroll
-            for (uint32_t i = 0; i < VEC; ++i) bl_set(v.v[i], gw * ur[j + i] * (f[j + i] - d));
-            if (e < p.E) *reinterpret_cast<BalVec<T, VEC>*>(grad + e) = v;
+            for (uint32_t i = 0; i < VEC; ++i) bl_set(v.v[i], ur[j + i] * fmaf(gw, f[j + i], -gd));
+            if (FULL || e < p.E) *reinterpret_cast<BalVec<T, VEC>*>(grad + e) = v;
         }
     }
     return weight * d;
@@ -366,7 +346,7 @@ __device__ __forceinline__ void clear_row(const BalanceParams& p, uint32_t t) {
 
 // A block takes a run of tokens, sequence by sequence; a warp reads its next row while it works on
 // one. ONE: one block is the whole call, with one sequence, and counts for itself.
-template <typename T, int SCORE, uint32_t NV, uint32_t VEC, bool ONE>
+template <typename T, int SCORE, uint32_t NV, uint32_t VEC, bool FULL, bool ONE>
 __global__ void __launch_bounds__(kBalThreads, NV > 8 ? 1 : 2) balance_kernel(const BalanceParams p) {
     __shared__ uint32_t hist[513], alive_s, offsets_s[kBalSeqs + 1];
     __shared__ double part[kBalWarps];
@@ -375,7 +355,7 @@ __global__ void __launch_bounds__(kBalThreads, NV > 8 ? 1 : 2) balance_kernel(co
     const uint32_t t1 = (uint32_t)((uint64_t)p.T * (blockIdx.x + 1u) / gridDim.x);
     if (ONE) tc::grid_dependency_wait();
     tc::grid_launch_dependents();
-    BalRow<T, NV, VEC> row;
+    BalRow<T, NV, VEC, FULL> row;
     if (t0 + warp < t1) row.load(p, t0 + warp);  // on its way while the counts are taken
     const uint32_t* offsets = near_offsets(p, offsets_s);
     if (tid == 0) alive_s = 0;
@@ -431,10 +411,10 @@ __global__ void __launch_bounds__(kBalThreads, NV > 8 ? 1 : 2) balance_kernel(co
         }
         while (mine < end) {
             const uint32_t r = mine;
-            const BalRow<T, NV, VEC> now = row;
+            const BalRow<T, NV, VEC, FULL> now = row;
             mine += kBalWarps;
             if (mine < t1) row.load(p, mine);
-            if (held && now.live) sum += (double)balance_row<T, SCORE, NV, VEC>(p, now, r, f, weight, up);
+            if (held && now.live) sum += (double)balance_row<T, SCORE, NV, VEC, FULL>(p, now, r, f, weight, up);
             else clear_row<T, NV, VEC>(p, r);
         }
         t = end;
@@ -479,21 +459,22 @@ uint32_t balance_pieces(uint32_t T, uint32_t S) {
     return n;
 }
 
-template <typename T, int SCORE, uint32_t NV, uint32_t VEC>
+template <typename T, int SCORE, uint32_t NV, uint32_t VEC, bool FULL>
 cudaError_t balance_launch(const BalanceParams& p, cudaStream_t s) {
     if (p.S == 1 && p.T <= kBalOneTokens)
-        return launch_chained(balance_kernel<T, SCORE, NV, VEC, true>, dim3(1), kBalThreads, 0, 0, s, p);
+        return launch_chained(balance_kernel<T, SCORE, NV, VEC, FULL, true>, dim3(1), kBalThreads, 0, 0, s, p);
     const uint32_t pieces = balance_pieces(p.T, p.S), log_pieces = (uint32_t)__builtin_ctz(pieces);
     const uint32_t cluster = pieces / balance_parts(p.T, p.S);
     const cudaError_t e = launch_chained(balance_count_kernel, dim3(p.S * pieces), kBalThreads, 0, cluster, s, p, log_pieces, cluster);
     if (e != cudaSuccess) return e;
     const uint32_t want = (p.T + kBalWarps - 1u) / kBalWarps;
     const uint32_t blocks = want < 1u ? 1u : want < kBalanceBlocks ? want : kBalanceBlocks;
-    return launch_chained(balance_kernel<T, SCORE, NV, VEC, false>, dim3(blocks), kBalThreads, 0, 0, s, p);
+    return launch_chained(balance_kernel<T, SCORE, NV, VEC, FULL, false>, dim3(blocks), kBalThreads, 0, 0, s, p);
 }
 
 // NV: values of a row a lane holds; VEC: neighbours it loads at once, 1 where the rows do not start
-// on such a boundary.
+// on such a boundary; FULL: the row fills the warp's values (64 to 512 experts by powers of two), no
+// place is checked.
 template <typename T, int SCORE>
 cudaError_t balance_scored(const BalanceParams& p, cudaStream_t s) {
     const auto fits = [&](uint32_t n) {
@@ -501,11 +482,15 @@ cudaError_t balance_scored(const BalanceParams& p, cudaStream_t s) {
         return p.E % n == 0 && p.stride % n == 0 && p.grad_stride % n == 0 && on(p.logits) && on(p.dlogits);
     };
     constexpr uint32_t V = 16u / sizeof(T);
+    if (p.E == 64u && fits(2)) return balance_launch<T, SCORE, 2, 2, true>(p, s);
+    if (p.E == 128u && fits(4)) return balance_launch<T, SCORE, 4, 4, true>(p, s);
+    if (p.E == 256u && fits(V)) return balance_launch<T, SCORE, 8, V, true>(p, s);
+    if (p.E == 512u && fits(V)) return balance_launch<T, SCORE, 16, V, true>(p, s);
     if (p.E <= 64u)
-        return fits(2) ? balance_launch<T, SCORE, 2, 2>(p, s) : balance_launch<T, SCORE, 2, 1>(p, s);
+        return fits(2) ? balance_launch<T, SCORE, 2, 2, false>(p, s) : balance_launch<T, SCORE, 2, 1, false>(p, s);
     if (p.E <= 256u)
-        return fits(V) ? balance_launch<T, SCORE, 8, V>(p, s) : balance_launch<T, SCORE, 8, 1>(p, s);
-    return fits(V) ? balance_launch<T, SCORE, 16, V>(p, s) : balance_launch<T, SCORE, 16, 1>(p, s);
+        return fits(V) ? balance_launch<T, SCORE, 8, V, false>(p, s) : balance_launch<T, SCORE, 8, 1, false>(p, s);
+    return fits(V) ? balance_launch<T, SCORE, 16, V, false>(p, s) : balance_launch<T, SCORE, 16, 1, false>(p, s);
 }
 
 template <typename T>

@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "vlb_launch.h"
+#include "vlb_math.cuh"
 #include "vlb_tcgen05.cuh"
 
 namespace vlb {
@@ -43,14 +44,14 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
 }
 
 // silu(g) * u with the clamp of the layer's experts (gate from above, up on both sides). The
-// comparisons keep a NaN, which fminf / fmaxf would drop. The quotient by the approximate
-// reciprocal is within 2 units of 2^-23; a gate below -87 gives 0 (its true value is under 1e-35).
+// comparisons keep a NaN, which fminf / fmaxf would drop. A gate below -88 gives about 0 (its true
+// value is under 1e-35).
 __device__ __forceinline__ float swiglu(float g, float u, float limit) {
     if (limit > 0.f) {
         g = g > limit ? limit : g;
         u = u > limit ? limit : (u < -limit ? -limit : u);
     }
-    return __fdividef(g, 1.f + expf(-g)) * u;
+    return g * fast_rcp(1.f + fast_exp(fminf(-g, 88.f))) * u;
 }
 
 // ---- row quantizer ---------------------------------------------------------------------------
@@ -119,8 +120,8 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(const Int8QuantParam
 //
 // HBM-bound: every element is read once (16 bytes a load where the rows allow it) and kept in registers between the row's
 // maximum and its rounding; rows longer than the registers hold are read twice, the second time
-// mostly from L2. A warp takes a row of up to 8 loads a lane (8 rows a CTA: no barrier, all loads
-// in flight at once); longer rows, and calls of too few rows to fill the GPU with warps, take a
+// mostly from L2. A warp takes a row of up to 16 loads a lane (8 rows a CTA: no barrier, all loads
+// in flight at once, and what a row costs beside its elements paid by one warp); longer rows, and calls of too few rows to fill the GPU with warps, take a
 // CTA a row.
 
 template <typename T>
@@ -152,8 +153,8 @@ struct RowVec {
     }
 };
 
-// Largest |x| of a vector, as float bits. 16-bit types compare two magnitudes an instruction; their
-// bit patterns order like their values, a NaN above infinity.
+// Largest |x| of vectors, as float bits, a NaN above all. 16-bit types compare two magnitudes an
+// instruction.
 template <typename T>
 struct RowMax {
     uint32_t m = 0;
@@ -161,7 +162,15 @@ struct RowMax {
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i) {
             const uint32_t w = (&v.raw.x)[i];
-            m = sizeof(T) == 4 ? max(m, w & 0x7fffffffu) : __vmaxu2(m, w & 0x7fff7fffu);
+            if constexpr (sizeof(T) == 4) {
+                m = max(m, w & 0x7fffffffu);
+            } else {
+                const uint32_t a = w & 0x7fff7fffu;
+                if constexpr (std::is_same<T, __half>::value)
+                    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m) : "r"(a));
+                else
+                    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(a));
+            }
         }
     }
     __device__ __forceinline__ uint32_t bits() const {
@@ -195,7 +204,7 @@ __device__ __forceinline__ void store_bytes(int8_t* q, const float (&x)[N], cons
 // ROW: threads of a row (32 or the CTA's 256); KEEP: vectors a thread keeps; WIDE: rows start on
 // 16-byte boundaries (others load each element by itself, from lines the warp shares).
 template <typename T, bool SWIGLU, uint32_t ROW, uint32_t KEEP, bool WIDE>
-__global__ void __launch_bounds__(256, SWIGLU || KEEP > 4 ? 3 : 5) int8_quantize_vec_kernel(const Int8QuantParams p) {
+__global__ void __launch_bounds__(256, KEEP > 8 ? 2 : SWIGLU || KEEP > 4 ? 3 : 5) int8_quantize_vec_kernel(const Int8QuantParams p) {
     constexpr uint32_t N = RowVec<T>::kN;
     __shared__ uint32_t top[8];
     tc::grid_dependency_wait();
@@ -1011,6 +1020,10 @@ cudaError_t quantize_rows(const Int8QuantParams& p, cudaStream_t s) {
     if constexpr (!SWIGLU)
         if (p.rows >= 2048u && p.cols <= 32u * 8u * N)
             return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 8, false>, int8_quantize_vec_kernel<T, SWIGLU, 32, 8, true>,
+                          (p.rows + 7u) / 8u);
+    if constexpr (!SWIGLU)
+        if (p.rows >= 2048u && p.cols <= 32u * 16u * N)
+            return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 16, false>, int8_quantize_vec_kernel<T, SWIGLU, 32, 16, true>,
                           (p.rows + 7u) / 8u);
     const uint32_t grid = p.rows < 65535u ? p.rows : 65535u;
     if (p.cols <= 256u * 2u * N)
