@@ -371,11 +371,14 @@ __global__ void __launch_bounds__(kBalThreads, NV > 8 ? 1 : 2) balance_kernel(co
         held = s < p.S && offsets[s] <= t;
         end = held ? min(t1, offsets[s + 1]) : s < p.S ? min(t1, offsets[s]) : t1;
     };
+    // Counts in one part (short sequences): each warp takes its tokens' from memory when it meets a
+    // new sequence. In several: the block adds them up in shared memory, a sequence at a time.
+    const bool by_warp = !ONE && p.parts == 1u;
     const auto fetch_counts = [&] {
         if (held)
             for (uint32_t e = tid; e <= p.E; e += kBalThreads) hist[e] = part_sum(p, s, e);
     };
-    if (t0 < t1) segment(t0);
+    if (t0 < t1 && !by_warp) segment(t0);
     if (!ONE) tc::grid_dependency_wait();
     __syncthreads();
     if (ONE) {
@@ -385,7 +388,7 @@ __global__ void __launch_bounds__(kBalThreads, NV > 8 ? 1 : 2) balance_kernel(co
     } else {
         uint32_t with = 0;  // sequences with a live token
         for (uint32_t i = tid; i < p.S; i += kBalThreads) with += part_sum(p, i, p.E) != 0;
-        if (t0 < t1) fetch_counts();
+        if (t0 < t1 && !by_warp) fetch_counts();
         // the counts' own output, the sequences dealt over the blocks
         for (uint32_t i = blockIdx.x; i < p.S; i += gridDim.x)
             for (uint32_t e = tid; e < p.E; e += kBalThreads) p.counts[(size_t)i * p.E + e] = part_sum(p, i, e);
@@ -397,32 +400,43 @@ __global__ void __launch_bounds__(kBalThreads, NV > 8 ? 1 : 2) balance_kernel(co
     const float base = alive ? p.coefficient / (float)alive : 0.f;
     double sum = 0.0;
     uint32_t mine = t0 + warp;  // this warp's next token, its logits in `row`
-    for (uint32_t t = t0; t < t1;) {
-        float weight = 0.f, f[NV];
-        if (held) {
-            const uint32_t n = hist[p.E];
-            weight = n ? base / (float)n : 0.f;
-            const float scale = n ? (float)p.E / ((float)p.k * (float)n) : 0.f;
+    float weight = 0.f, f[NV];
+    const auto shares = [&](const uint32_t* counts) {
+        const uint32_t n = counts[p.E];
+        weight = n ? base / (float)n : 0.f;
+        const float scale = n ? (float)p.E / ((float)p.k * (float)n) : 0.f;
 #pragma unroll
-            for (uint32_t j = 0; j < NV; ++j) {
-                const uint32_t e = expert_of<VEC>(lane, j);
-                f[j] = e < p.E ? (float)hist[e] * scale : 0.f;
-            }
+        for (uint32_t j = 0; j < NV; ++j) {
+            const uint32_t e = expert_of<VEC>(lane, j);
+            f[j] = FULL || e < p.E ? (float)counts[e] * scale : 0.f;
         }
-        while (mine < end) {
-            const uint32_t r = mine;
-            const BalRow<T, NV, VEC, FULL> now = row;
-            mine += kBalWarps;
-            if (mine < t1) row.load(p, mine);
-            if (held && now.live) sum += (double)balance_row<T, SCORE, NV, VEC, FULL>(p, now, r, f, weight, up);
-            else clear_row<T, NV, VEC>(p, r);
+    };
+    const auto next_token = [&] {
+        const uint32_t r = mine;
+        const BalRow<T, NV, VEC, FULL> now = row;
+        mine += kBalWarps;
+        if (mine < t1) row.load(p, mine);
+        if (held && now.live) sum += (double)balance_row<T, SCORE, NV, VEC, FULL>(p, now, r, f, weight, up);
+        else clear_row<T, NV, VEC>(p, r);
+    };
+    if (by_warp) {
+        for (uint32_t upto = t0; mine < t1; next_token()) {
+            if (mine < upto) continue;
+            segment(mine);
+            upto = end;
+            if (held) shares(p.part + (size_t)s * (p.E + 1u));
         }
-        t = end;
-        if (t >= t1) break;
-        __syncthreads();  // hist is read by all
-        segment(t);
-        if (!ONE) fetch_counts();
-        __syncthreads();
+    } else {
+        for (uint32_t t = t0; t < t1;) {
+            if (held) shares(hist);
+            while (mine < end) next_token();
+            t = end;
+            if (t >= t1) break;
+            __syncthreads();  // hist is read by all
+            segment(t);
+            if (!ONE) fetch_counts();
+            __syncthreads();
+        }
     }
     if (ONE)
         for (uint32_t e = tid; e < p.E; e += kBalThreads) p.counts[e] = hist[e];

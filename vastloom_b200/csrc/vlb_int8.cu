@@ -86,39 +86,73 @@ __device__ __forceinline__ float row_value(const Int8QuantParams& p, size_t at) 
     return swiglu(x, to_float(static_cast<const T*>(p.up)[at]), p.limit);
 }
 
-// One CTA a row: the row's largest |x|, then its bytes (zeros up to the row's pitch).
-template <typename T, bool SWIGLU>
+// Rows at any alignment: neighbouring lanes take neighbouring elements, a thread up to KEEP of them in
+// registers between the row's maximum and its rounding (the rest is read twice); bytes are written
+// one a lane. ROW: threads of a row (32 or the CTA's 256).
+template <typename T, bool SWIGLU, uint32_t ROW, uint32_t KEEP>
 __global__ void __launch_bounds__(256) int8_quantize_kernel(const Int8QuantParams p) {
     __shared__ uint32_t top[8];
-    const uint32_t tid = threadIdx.x;
     tc::grid_dependency_wait();
     tc::grid_launch_dependents();
-    for (size_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    const uint32_t tid = threadIdx.x % ROW;
+    for (size_t r = (size_t)blockIdx.x * (256u / ROW) + threadIdx.x / ROW; r < p.rows;
+         r += (size_t)gridDim.x * (256u / ROW)) {
         const uint64_t src = p.row_index ? p.row_index[r] : r;
-        const bool have = src < p.x_rows;
+        const uint32_t have = src < p.x_rows ? p.cols : 0u;
         const size_t base = src * p.x_stride;
+        const T* x = static_cast<const T*>(p.x) + base + tid;
+        const T* up = SWIGLU ? static_cast<const T*>(p.up) + base + tid : nullptr;
+        float v[KEEP];
         uint32_t m = 0;
-        if (have)
-            for (uint32_t c = tid; c < p.cols; c += blockDim.x)
-                m = max(m, __float_as_uint(row_value<T, SWIGLU>(p, base + c)) & 0x7fffffffu);
+        {
+            T a[KEEP], b[SWIGLU ? KEEP : 1];  // all loads first
+#pragma unroll
+            for (uint32_t i = 0; i < KEEP; ++i) {
+                a[i] = from_float<T>(0.f);
+                if (tid + i * ROW < have) a[i] = x[i * ROW];
+                if constexpr (SWIGLU) {
+                    b[i] = from_float<T>(0.f);
+                    if (tid + i * ROW < have) b[i] = up[i * ROW];
+                }
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < KEEP; ++i) {
+                v[i] = to_float(a[i]);
+                if constexpr (SWIGLU) v[i] = swiglu(v[i], to_float(b[i]), p.limit);
+                m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+            }
+        }
+#pragma unroll 4
+        for (uint32_t c = tid + KEEP * ROW; c < have; c += ROW)
+            m = max(m, __float_as_uint(row_value<T, SWIGLU>(p, base + c)) & 0x7fffffffu);
         m = __reduce_max_sync(0xffffffffu, m);
-        __syncthreads();
-        if ((tid & 31u) == 0) top[tid >> 5] = m;
-        __syncthreads();
-        m = 0;
-        for (uint32_t i = 0; i < blockDim.x / 32u; ++i) m = max(m, top[i]);
+        if constexpr (ROW == 256) {
+            __syncthreads();
+            if ((tid & 31u) == 0) top[tid >> 5] = m;
+            __syncthreads();
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) m = max(m, top[i]);
+        }
         const RowStep st = row_step(m);
         if (tid == 0) p.scale[r] = st.scale;
-        for (uint32_t c = tid; c < p.fill_cols; c += blockDim.x) {
-            const bool in = have && c < p.cols;
-            p.q[r * p.q_stride + c] = (int8_t)(in ? quant_byte(row_value<T, SWIGLU>(p, base + c), st) : 0u);
+        int8_t* q = p.q + r * p.q_stride;
+        if (st.lift != 1.f) {  // a row of zeros, of tiny values, or not finite
+#pragma unroll
+            for (uint32_t i = 0; i < KEEP; ++i) v[i] = st.inv == 0.f ? 0.f : v[i] * st.lift;
         }
+#pragma unroll
+        for (uint32_t i = 0; i < KEEP; ++i)
+            if (tid + i * ROW < p.fill_cols)
+                q[tid + i * ROW] = (int8_t)__float_as_uint(__fadd_rn(__fmul_rn(v[i], st.inv), 12582912.f));
+#pragma unroll 4
+        for (uint32_t c = tid + KEEP * ROW; c < p.fill_cols; c += ROW)
+            q[c] = (int8_t)(c < have ? quant_byte(row_value<T, SWIGLU>(p, base + c), st) : 0u);
     }
 }
 
-// ---- row quantizer, integers written in words ----------------------------------------------------
+// ---- row quantizer, rows on 16-byte boundaries ---------------------------------------------------
 //
-// HBM-bound: every element is read once (16 bytes a load where the rows allow it) and kept in registers between the row's
+// HBM-bound: every element is read once (16 bytes a load) and kept in registers between the row's
 // maximum and its rounding; rows longer than the registers hold are read twice, the second time
 // mostly from L2. A warp takes a row of up to 16 loads a lane (8 rows a CTA: no barrier, all loads
 // in flight at once, and what a row costs beside its elements paid by one warp); longer rows, and calls of too few rows to fill the GPU with warps, take a
@@ -201,9 +235,8 @@ __device__ __forceinline__ void store_bytes(int8_t* q, const float (&x)[N], cons
     else *reinterpret_cast<uint32_t*>(q) = w[0];
 }
 
-// ROW: threads of a row (32 or the CTA's 256); KEEP: vectors a thread keeps; WIDE: rows start on
-// 16-byte boundaries (others load each element by itself, from lines the warp shares).
-template <typename T, bool SWIGLU, uint32_t ROW, uint32_t KEEP, bool WIDE>
+// ROW: threads of a row (32 or the CTA's 256); KEEP: vectors a thread keeps.
+template <typename T, bool SWIGLU, uint32_t ROW, uint32_t KEEP>
 __global__ void __launch_bounds__(256, KEEP > 8 ? 2 : SWIGLU || KEEP > 4 ? 3 : 5) int8_quantize_vec_kernel(const Int8QuantParams p) {
     constexpr uint32_t N = RowVec<T>::kN;
     __shared__ uint32_t top[8];
@@ -220,8 +253,8 @@ __global__ void __launch_bounds__(256, KEEP > 8 ? 2 : SWIGLU || KEEP > 4 ? 3 : 5
         auto fetch = [&](const T* row, uint32_t v) {
             RowVec<T> a;
             if (v >= have) a.clear();
-            else if (WIDE && (v + 1u) * N <= p.cols) a.load(row + (size_t)v * N);
-            else a.load_part(row + (size_t)v * N, min(N, p.cols - v * N));
+            else if ((v + 1u) * N <= p.cols) a.load(row + (size_t)v * N);
+            else a.load_part(row + (size_t)v * N, p.cols - v * N);
             return a;
         };
         RowVec<T> a[KEEP];
@@ -1008,27 +1041,21 @@ cudaError_t quantize_rows(const Int8QuantParams& p, cudaStream_t s) {
     auto on = [](const void* at, size_t stride_bytes, size_t n) {
         return reinterpret_cast<uintptr_t>(at) % n == 0 && stride_bytes % n == 0;
     };
-    const bool wide = on(p.x, p.x_stride * sizeof(T), 16) && on(p.up, 0, 16);
-    if (!on(p.q, p.q_stride, N))
-        return launch_chained(int8_quantize_kernel<T, SWIGLU>, dim3(p.rows < 65535u ? p.rows : 65535u), 256, 0, 0, s, p);
-    const auto launch = [&](auto* narrow_kernel, auto* wide_kernel, uint32_t grid) {
-        return launch_chained(wide ? wide_kernel : narrow_kernel, dim3(grid), 256, 0, 0, s, p);
-    };
-    if (p.rows >= 2048u && p.cols <= 32u * 4u * N)
-        return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 4, false>, int8_quantize_vec_kernel<T, SWIGLU, 32, 4, true>,
-                      (p.rows + 7u) / 8u);
-    if constexpr (!SWIGLU)
-        if (p.rows >= 2048u && p.cols <= 32u * 8u * N)
-            return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 8, false>, int8_quantize_vec_kernel<T, SWIGLU, 32, 8, true>,
-                          (p.rows + 7u) / 8u);
-    if constexpr (!SWIGLU)
-        if (p.rows >= 2048u && p.cols <= 32u * 16u * N)
-            return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 16, false>, int8_quantize_vec_kernel<T, SWIGLU, 32, 16, true>,
-                          (p.rows + 7u) / 8u);
-    const uint32_t grid = p.rows < 65535u ? p.rows : 65535u;
-    if (p.cols <= 256u * 2u * N)
-        return launch(int8_quantize_vec_kernel<T, SWIGLU, 256, 2, false>, int8_quantize_vec_kernel<T, SWIGLU, 256, 2, true>, grid);
-    return launch(int8_quantize_vec_kernel<T, SWIGLU, 256, 4, false>, int8_quantize_vec_kernel<T, SWIGLU, 256, 4, true>, grid);
+    const uint32_t by_block = p.rows < 65535u ? p.rows : 65535u, by_warp = (p.rows + 7u) / 8u;
+    const auto launch = [&](auto* kernel, uint32_t grid) { return launch_chained(kernel, dim3(grid), 256, 0, 0, s, p); };
+    const bool many = p.rows >= 2048u;  // enough to fill the GPU with a warp a row
+    if (!on(p.x, p.x_stride * sizeof(T), 16) || !on(p.up, 0, 16) || !on(p.q, p.q_stride, N)) {
+        if (many && p.cols <= 32u * 16u) return launch(int8_quantize_kernel<T, SWIGLU, 32, 16>, by_warp);
+        if (p.cols <= 256u * 4u) return launch(int8_quantize_kernel<T, SWIGLU, 256, 4>, by_block);
+        return launch(int8_quantize_kernel<T, SWIGLU, 256, 16>, by_block);
+    }
+    if (many && p.cols <= 32u * 4u * N) return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 4>, by_warp);
+    if constexpr (!SWIGLU) {
+        if (many && p.cols <= 32u * 8u * N) return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 8>, by_warp);
+        if (many && p.cols <= 32u * 16u * N) return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 16>, by_warp);
+    }
+    if (p.cols <= 256u * 2u * N) return launch(int8_quantize_vec_kernel<T, SWIGLU, 256, 2>, by_block);
+    return launch(int8_quantize_vec_kernel<T, SWIGLU, 256, 4>, by_block);
 }
 
 template <typename T>
@@ -1175,8 +1202,9 @@ uint32_t sm_count() {
 }
 
 // What int8_few_kernel takes: its dp4a work grows with the rows (2048 x 2048: 3.6 us for one, 6.1 for
-// 4, 9.3 for 8; 4096 x 4096: 5.7, 11.2, 21.9), the tensor cores' two launches do not (about 9 and 10).
-constexpr uint32_t kFewRows = 8, kFewGroupedRows = 16;
+// 4, 9.3 for 8; 4096 x 4096: 5.7, 11.2, 21.9), the tensor cores' two launches do not (about 6 and 9);
+// every block quantizes all rows, which for 5 rows of 3470 takes longer than the products.
+constexpr uint32_t kFewRows = 8, kFewGroupedRows = 16, kFewElements = 8192;
 constexpr uint64_t kFewWork = 1u << 24;
 
 template <typename T, uint32_t ROWS>
@@ -1238,7 +1266,9 @@ cudaError_t launch_int8_gather(const Int8GatherParams& p, cudaStream_t s) {
 
 bool int8_few(const Int8LinearParams& l) {
     if (l.rows > (l.offsets ? kFewGroupedRows : kFewRows) || !tma_rows(l.w, l.w_stride)) return false;
-    if (!l.offsets && l.rows > 2u && (uint64_t)l.rows * l.cols * l.out_cols > kFewWork) return false;
+    if (!l.offsets && l.rows > 2u &&
+        ((uint64_t)l.rows * l.cols > kFewElements || (uint64_t)l.rows * l.cols * l.out_cols > kFewWork))
+        return false;
     uint32_t rows = 1;
     while (!l.offsets && rows < l.rows) rows *= 2u;
     return (size_t)rows * ((l.cols + 15u) / 16u * 16u) <= kFewSmem;
