@@ -576,9 +576,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) int8_few_kernel(const Int8Line
 // to 256 tokens of one group (the columns), so a lane of the epilogue holds one channel's scale and
 // a warp's stores are 32 neighbouring channels of one token; few tokens cost few columns.
 // K runs in chunks of 128 bytes (one 128-byte swizzle row) through a ring of TMA stages.
-// Roles: warps 0-7 epilogue, warp 8 TMA, warp 9 MMA; two accumulators, so a tile's epilogue runs
-// beside the next tile's products. Persistent CTAs, tiles in order, a group's token tiles
-// innermost (its weights come from HBM once).
+// Roles: warps 0-7 epilogue, warp 8 TMA, warp 9 MMA, warp 10 the tiles' places and scales for the
+// epilogue, a tile or two ahead (behind an epilogue's stores their lookup took 3,000 to 5,000 cycles
+// of a tile's 8,000); two accumulators, so a tile's epilogue runs beside the next tile's products.
+// Persistent CTAs, tiles in order, a group's token tiles innermost (its weights come from HBM once).
 // PAIR: two CTAs share a tile of 256 channels (cta_group::2): each loads its own 128 channels and half
 // the tokens, which is two thirds of the operand bytes a CTA alone takes from L2 for the same products.
 // SPLIT: a cluster shares a tile, each CTA a part of K; the partial sums are integers, so their
@@ -586,7 +587,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) int8_few_kernel(const Int8Line
 
 enum class Mm { kOne, kSplit, kPair };
 constexpr uint32_t kMmChannels = 128, kMmMaxTokens = 256, kMmKc = 128;
-constexpr uint32_t kMmEpiWarps = 8, kMmThreads = (kMmEpiWarps + 2) * 32;
+constexpr uint32_t kMmEpiWarps = 8, kMmThreads = (kMmEpiWarps + 3) * 32;
 constexpr uint32_t kMmWStage = kMmChannels * kMmKc;
 constexpr uint32_t kMmMaxStages = 12;
 constexpr uint32_t kMmSmemLimit = 227u * 1024u;
@@ -618,14 +619,17 @@ struct MmShared {
     uint32_t* lo;     // [groups] first row
     uint32_t* cnt;    // [groups] rows
     float* scale;     // [2][256] the tile's token scales
-    uint64_t *full, *empty, *acc_full, *acc_empty;
+    float* channel;   // [2][128] its channels'
+    MmTile* tile;     // [2]
+    uint64_t *full, *empty, *acc_full, *acc_empty, *tile_full, *tile_empty;
     uint32_t* tmem;
     volatile uint32_t* abort;
 };
 
 __host__ __device__ constexpr uint32_t mm_table_bytes(uint32_t groups) { return (3u * groups + 1u) * 4u; }
 __host__ __device__ constexpr uint32_t mm_fixed_bytes(uint32_t groups) {
-    return 2u * kMmMaxTokens * 4u + (2u * kMmMaxStages + 4u) * 8u + 16u + mm_table_bytes(groups) + 16u;
+    return 2u * (kMmMaxTokens + kMmChannels) * 4u + 2u * 16u + (2u * kMmMaxStages + 8u) * 8u + 16u + mm_table_bytes(groups) +
+           16u;
 }
 
 // Columns of a tile's products: the shapes' steps are 16 for one CTA, 32 for a pair.
@@ -681,11 +685,15 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
     {
         unsigned char* at = mm_smem + p.stages * stage_bytes;
         sh.scale = reinterpret_cast<float*>(at);
-        sh.full = reinterpret_cast<uint64_t*>(at + 2u * kMmMaxTokens * 4u);
+        sh.channel = sh.scale + 2u * kMmMaxTokens;
+        sh.tile = reinterpret_cast<MmTile*>(sh.channel + 2u * kMmChannels);
+        sh.full = reinterpret_cast<uint64_t*>(sh.tile + 2);
         sh.empty = sh.full + kMmMaxStages;
         sh.acc_full = sh.empty + kMmMaxStages;
         sh.acc_empty = sh.acc_full + 2;
-        sh.tmem = reinterpret_cast<uint32_t*>(sh.acc_empty + 2);
+        sh.tile_full = sh.acc_empty + 2;
+        sh.tile_empty = sh.tile_full + 2;
+        sh.tmem = reinterpret_cast<uint32_t*>(sh.tile_empty + 2);
         sh.abort = sh.tmem + 1;
         sh.first = sh.tmem + 4;
         sh.lo = sh.first + l.groups + 1;
@@ -711,6 +719,8 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         for (uint32_t i = 0; i < 2u; ++i) {
             tc::mbar_init(sh.acc_full + i, 1);
             tc::mbar_init(sh.acc_empty + i, PAIR ? 2u * kMmEpiWarps : kMmEpiWarps);
+            tc::mbar_init(sh.tile_full + i, 1);
+            tc::mbar_init(sh.tile_empty + i, kMmEpiWarps);
         }
         *sh.abort = 0;
         tc::mbar_fence_init();
@@ -854,22 +864,45 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         return true;
     };
     const uint32_t quad = warp & 3u, half = warp >> 2;
-    auto epilogue = [&](uint32_t t) -> bool {
-        const MmTile tile = mm_tile(sh, p, t);
+    // the whole warp
+    auto place = [&](uint32_t t) -> bool {
         const uint32_t buf = it & 1u, use = it >> 1;
-        float* ts = sh.scale + buf * kMmMaxTokens;
+        const MmTile tile = mm_tile(sh, p, t);
         if (!waited) {
             tc::grid_dependency_wait();
             waited = true;
         }
-        if (tid < tile.count) {
-            const uint32_t r = tile.row0 + tid;
-            ts[tid] = l.row_weight ? l.x_scale[r] * l.row_weight[r] : l.x_scale[r];
+        float ts[kMmMaxTokens / 32u], cs[kMmChannels / 32u];
+#pragma unroll
+        for (uint32_t i = 0; i < kMmMaxTokens / 32u; ++i) {
+            const uint32_t j = lane + 32u * i;
+            ts[i] = j < tile.count ? l.x_scale[tile.row0 + j] : 0.f;
+            if (l.row_weight && j < tile.count) ts[i] *= l.row_weight[tile.row0 + j];
         }
+#pragma unroll
+        for (uint32_t i = 0; i < kMmChannels / 32u; ++i) {
+            const uint32_t n = tile.channel0 + (PAIR ? rank * kMmChannels : 0u) + lane + 32u * i;
+            cs[i] = n < l.out_cols ? l.w_scale[(size_t)tile.g * l.out_cols + n] : 0.f;
+        }
+        if (!__all_sync(0xffffffffu, mm_wait(sh.tile_empty + buf, (use & 1u) ^ 1u, sh.abort))) return false;
+#pragma unroll
+        for (uint32_t i = 0; i < kMmMaxTokens / 32u; ++i) sh.scale[buf * kMmMaxTokens + lane + 32u * i] = ts[i];
+#pragma unroll
+        for (uint32_t i = 0; i < kMmChannels / 32u; ++i) sh.channel[buf * kMmChannels + lane + 32u * i] = cs[i];
+        if (lane == 0) sh.tile[buf] = tile;
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(sh.tile_full + buf);
+        ++it;
+        return true;
+    };
+    auto epilogue = [&]() -> bool {
+        const uint32_t buf = it & 1u, use = it >> 1;
+        const float* ts = sh.scale + buf * kMmMaxTokens;
+        bool ok = __all_sync(0xffffffffu, mm_wait(sh.tile_full + buf, use & 1u, sh.abort));
+        const MmTile tile = sh.tile[buf];
+        const float cs = sh.channel[buf * kMmChannels + 32u * quad + lane];
         const uint32_t n = tile.channel0 + (PAIR ? rank * kMmChannels : 0u) + 32u * quad + lane;
-        const float cs = n < l.out_cols ? l.w_scale[(size_t)tile.g * l.out_cols + n] : 0.f;
-        asm volatile("bar.sync 1, %0;" ::"n"(kMmEpiWarps * 32) : "memory");
-        const bool ok = __all_sync(0xffffffffu, mm_wait(sh.acc_full + buf, use & 1u, sh.abort));
+        ok = ok && __all_sync(0xffffffffu, mm_wait(sh.acc_full + buf, use & 1u, sh.abort));
         if (ok) {
             tc::fence_after_sync();
             const uint32_t src = tmem + buf * p.acc_cols + ((32u * quad) << 16);
@@ -902,6 +935,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
             tc::fence_before_sync();
             __syncwarp();
             if (lane == 0) {
+                tc::mbar_arrive(sh.tile_empty + buf);
                 if (PAIR) tc::mbar_arrive_cluster(tc::cluster_map(tc::smem_u32(sh.acc_empty + buf), 0));
                 else tc::mbar_arrive(sh.acc_empty + buf);
             }
@@ -912,13 +946,20 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
 
     if (!SPLIT) {
         if (warp < kMmEpiWarps) {
-            // after a role has given up the epilogue warps still walk every tile (their waits end at
-            // once), so that all of them meet at each tile's named barrier
             for (uint32_t t = begin; t < total; t += step)
-                if (!epilogue(t) && lane == 0) mm_fail(sh.abort);
+                if (!epilogue()) {
+                    if (lane == 0) mm_fail(sh.abort);
+                    break;
+                }
         } else if (warp == kMmEpiWarps) {
             for (uint32_t t = begin; t < total; t += step)
                 if (!produce(t)) {
+                    if (lane == 0) mm_fail(sh.abort);
+                    break;
+                }
+        } else if (warp == kMmEpiWarps + 2u) {
+            for (uint32_t t = begin; t < total; t += step)
+                if (!place(t)) {
                     if (lane == 0) mm_fail(sh.abort);
                     break;
                 }
@@ -942,7 +983,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
                 ok = __all_sync(0xffffffffu, *sh.abort == 0) && produce(t);
             } else if (warp == kMmEpiWarps + 1u) {
                 ok = __all_sync(0xffffffffu, *sh.abort == 0) && multiply(t);
-            } else {
+            } else if (warp < kMmEpiWarps) {
                 if (!waited) {
                     tc::grid_dependency_wait();
                     waited = true;
