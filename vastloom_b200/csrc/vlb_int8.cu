@@ -1084,7 +1084,9 @@ cudaError_t quantize_rows(const Int8QuantParams& p, cudaStream_t s) {
     };
     const uint32_t by_block = p.rows < 65535u ? p.rows : 65535u, by_warp = (p.rows + 7u) / 8u;
     const auto launch = [&](auto* kernel, uint32_t grid) { return launch_chained(kernel, dim3(grid), 256, 0, 0, s, p); };
-    const bool many = p.rows >= 2048u;  // enough to fill the GPU with a warp a row
+    // a warp a row where that fills the GPU (with a product of 16 channels, a warp / a CTA a row: 512
+    // rows of 1024 bf16 8.4 / 8.6 us, 1024 8.6 / 10.2, 4096 10.9 / 15.9)
+    const bool many = p.rows >= 1024u;
     if (!on(p.x, p.x_stride * sizeof(T), 16) || !on(p.up, 0, 16) || !on(p.q, p.q_stride, N)) {
         if (many && p.cols <= 32u * 16u) return launch(int8_quantize_kernel<T, SWIGLU, 32, 16>, by_warp);
         if (p.cols <= 256u * 4u) return launch(int8_quantize_kernel<T, SWIGLU, 256, 4>, by_block);
@@ -1164,10 +1166,7 @@ bool tma_rows(const int8_t* p, size_t stride) {
 // Tile width, split or pairs of a product on the tensor cores. Returns the mode.
 Mm mma_plan(Int8MmaParams& p, uint32_t sms) {
     const Int8LinearParams& l = p.l;
-    p.ct = (l.out_cols + kMmChannels - 1u) / kMmChannels;
     p.nk = (l.cols + kMmKc - 1u) / kMmKc;
-    const uint32_t used = l.groups < l.rows ? l.groups : l.rows;
-    const uint32_t mean = (l.rows + used - 1u) / used;
     const auto split_of = [&](uint64_t tiles) {
         // clusters of 8 only while they are few: more of them do not fit the GPU at once (16 tiles of
         // 2048 x 2048 x 64 rows: 14 us in eights, 9 in fours)
@@ -1175,40 +1174,61 @@ Mm mma_plan(Int8MmaParams& p, uint32_t sms) {
         while (split < 8u && tiles * split * 2u <= (split < 4u ? sms : 64u) && p.nk >= split * 2u) split *= 2u;
         return split;
     };
+    const auto up = [](uint32_t v, uint32_t step) { return (v + step - 1u) / step * step; };
     Mm mode = Mm::kOne;
-    if (mean > kMmMaxTokens / 2u && (uint64_t)l.rows * p.ct >= (uint64_t)kMmMaxTokens * sms / 2u) mode = Mm::kPair;
-    const uint32_t step = mode == Mm::kPair ? 32u : 16u, units = mode == Mm::kPair ? sms / 2u : sms;
-    if (mode == Mm::kPair) {
-        p.channels = 2u * kMmChannels;
-        p.ct = (l.out_cols + p.channels - 1u) / p.channels;
-    } else {
-        p.channels = kMmChannels;
-    }
-    const auto up = [&](uint32_t v) { return (v + step - 1u) / step * step; };
     if (l.groups == 1) {
-        // the width whose waves of tiles take the least time, a K chunk of a tile taking about its
-        // columns + 240 cycles (424 at 128 columns, 525 at 256: its weights' bytes and the products'
-        // issue do not shrink with the width); one tile of tokens where they fit one
+        // One CTA a tile (K split over a cluster where the tiles are few) or pairs, and the tiles'
+        // width: what takes the least cycles by what was measured - a K chunk its columns + 240 (424
+        // at 128 columns, 525 at 256; a tenth more for CTAs alone, which draw more from L2), an
+        // epilogue 1,500 and 18 a column, a split's sums 4,000 and 32 a column, a pair's start 1,500.
+        // (4096 x 4096, int8 rows, split or alone / pairs: 130 rows 9.8 / 11.2 us, 300 12.4 / 11.8,
+        // 2048 28.8 / 26.5; 1024 -> 4096: 130 rows 8.9 / 6.9, 1024 8.1 / 9.1.)
         uint64_t best = ~0ull;
-        const uint32_t most = up(l.rows < kMmMaxTokens ? l.rows : kMmMaxTokens);
-        for (uint32_t w = most; w >= 128u || w == most; w -= step) {
-            const uint64_t n = (l.rows + w - 1u) / w, tiles = n * p.ct, waves = (tiles + units - 1u) / units;
-            const uint32_t balanced = up((uint32_t)((l.rows + n - 1u) / n));
-            const uint32_t split = mode == Mm::kPair ? 1u : split_of(tiles);
-            const uint64_t cost = waves * (balanced + 240u) * ((p.nk + split - 1u) / split);
-            if (cost < best) best = cost, p.width = w, p.split = split;
-            if (w == most && l.rows <= kMmMaxTokens) break;
+        for (uint32_t pair = 0; pair < 2u; ++pair) {
+            const uint32_t step = pair ? 32u : 16u, most = up(l.rows < kMmMaxTokens ? l.rows : kMmMaxTokens, step);
+            const uint64_t ct = (l.out_cols + kMmChannels * (1u + pair) - 1u) / (kMmChannels * (1u + pair));
+            for (uint32_t w = most; w >= 64u || w == most; w -= step) {
+                const uint64_t n = (l.rows + w - 1u) / w, tiles = n * ct;
+                const uint32_t split = pair ? 1u : split_of(tiles);
+                const uint64_t units = pair ? sms / 2u : sms / split, waves = (tiles + units - 1u) / units;
+                const uint64_t columns = up((uint32_t)((l.rows + n - 1u) / n), step);
+                uint64_t main = (p.nk + split - 1u) / split * (columns + 240u), cost;
+                if (split > 1u) {
+                    cost = waves * (main + 4000u + 32u * columns);
+                } else {
+                    if (!pair) main += main / 10u;
+                    const uint64_t tail = 1500u + 18u * columns;
+                    cost = (waves - 1u) * (main > tail ? main : tail) + main + tail + (pair ? 1500u : 0u);
+                }
+                if (cost < best) {
+                    best = cost;
+                    mode = pair ? Mm::kPair : split > 1u ? Mm::kSplit : Mm::kOne;
+                    p.width = w;
+                    p.split = split;
+                }
+                if (w <= step) break;
+            }
         }
     } else {
-        // unknown rows a group: room for the usual spread around the mean, or a second tile would
-        // read the group's weights again
+        // The rows of each group are on the device only. Pairs from about 100 rows a group (64 groups
+        // of 2048 x 2048: 64 rows 55.6 us alone / 56.9 in pairs, 96 60.0 / 60.5, 128 65.2 / 61.8, 512
+        // 155 / 142); room for the usual spread around the mean, or a second tile would read the
+        // group's weights again.
+        const uint32_t used = l.groups < l.rows ? l.groups : l.rows, mean = (l.rows + used - 1u) / used;
         uint32_t spread = 1;
         while (spread * spread < mean) ++spread;
-        const uint32_t want = up(mean + 3u * spread);
+        if (mean >= 100u) mode = Mm::kPair;
+        const uint32_t want = up(mean + 3u * spread, mode == Mm::kPair ? 32u : 16u);
         p.width = want < kMmMaxTokens ? want : kMmMaxTokens;
-        p.split = mode == Mm::kPair ? 1u : split_of((uint64_t)used * ((mean + p.width - 1u) / p.width) * p.ct);
+        p.split = 1;
+        if (mode == Mm::kOne) {
+            const uint64_t ct = (l.out_cols + kMmChannels - 1u) / kMmChannels;
+            p.split = split_of((uint64_t)used * ((mean + p.width - 1u) / p.width) * ct);
+            if (p.split > 1) mode = Mm::kSplit;
+        }
     }
-    if (p.split > 1) mode = Mm::kSplit;
+    p.channels = mode == Mm::kPair ? 2u * kMmChannels : kMmChannels;
+    p.ct = (l.out_cols + p.channels - 1u) / p.channels;
     const uint32_t held = mode == Mm::kPair ? p.width / 2u : p.width;  // token rows in one CTA's stage
     p.box = held < 128u ? held : 128u;
     p.x_stage = (held + p.box - 1u) / p.box * p.box * kMmKc;
