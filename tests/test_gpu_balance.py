@@ -267,6 +267,36 @@ def test_equal_inputs_give_equal_bits(dev, torch):
         assert r[0] == runs[0][0] and np.array_equal(r[1], runs[0][1]) and torch.equal(r[3], runs[0][3])
 
 
+@pytest.mark.parametrize("T,offsets", [(60, None), (3000, None), (3000, [0, 5, 900, 3000])])
+def test_inputs_written_just_before(dev, torch, T, offsets):
+    """Logits and routes that the kernels ahead on the stream write, and rewrite once the call has been
+    enqueued; one workspace for all calls."""
+    rng = np.random.default_rng(11)
+    E, k, n, S = 96, 4, 5, 1 if offsets is None else len(offsets) - 1
+    src = torch.randn(n, T, E).cuda()
+    ids = [routes(rng, T, E, k) for _ in range(n)]
+    idc = torch.from_numpy(np.stack(ids).astype(np.int32)).cuda()
+    oc = None if offsets is None else torch.tensor(offsets, dtype=torch.int32).cuda()
+    z, idx = torch.zeros(T, E, device="cuda"), torch.zeros(T, k, dtype=torch.int32, device="cuda")
+    lo, co, gr = (torch.zeros(n, device="cuda"), torch.zeros(n, S, E, dtype=torch.int32, device="cuda"),
+                  torch.zeros(n, T, E, device="cuda"))
+    size = vb.balance_workspace_bytes(T, E, S)
+    ws = torch.full((size,), 0x5a, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    for i in range(n):
+        z.copy_(src[i])
+        idx.copy_(idc[i])
+        dev.balance_loss_device(z.data_ptr(), idx.data_ptr(), T, E, k, counts_ptr=co[i].data_ptr(), ws_ptr=ws.data_ptr(),
+                                ws_bytes=size, seq_offsets_ptr=0 if oc is None else oc.data_ptr(), n_seqs=S,
+                                loss_ptr=lo[i:].data_ptr(), dlogits_ptr=gr[i].data_ptr(), stream=1)
+        z.fill_(float("nan"))
+        idx.fill_(-1)
+    torch.cuda.synchronize()
+    for i in range(n):
+        got = (float(lo[i]), co[i].cpu().numpy(), gr[i].cpu().numpy().astype(np.float64), None)
+        check(got, plain(src[i].cpu().numpy(), ids[i], "softmax", 1.0, None, offsets), "f32")
+
+
 def test_many_sequences_and_host_form(dev, torch):
     rng = np.random.default_rng(9)
     T, E, k = 700, 20, 2

@@ -291,6 +291,49 @@ def test_another_stream(dev, torch):
     check_product(y.cpu().numpy(), product(q, sc, w[0].cpu().numpy(), sw[0].cpu().numpy()), "f32")
 
 
+@pytest.mark.parametrize("M", [1, 40, 700])
+def test_inputs_written_just_before(dev, torch, M):
+    """Weights and rows that the kernels ahead on the stream write, and rewrite as soon as the product
+    has been enqueued: launches that come up early still see this call's."""
+    K, N, n = 1024, 512, 6
+    src_w, src_x = torch.randn(n, N, K).cuda(), torch.randn(n, M, K).cuda()
+    w, sw = torch.zeros(1, N, K, dtype=torch.int8, device="cuda"), torch.zeros(1, N, device="cuda")
+    x = torch.zeros(M, K, device="cuda")
+    y = torch.zeros(n, M, N, device="cuda")
+    buf = torch.zeros(vb.int8_workspace_bytes(M, K), dtype=torch.uint8, device="cuda")
+    for i in range(n):
+        dev.int8_quantize_device(src_w[i].data_ptr(), N, K, w.data_ptr(), sw.data_ptr(), stream=LEGACY)
+        x.copy_(src_x[i])
+        run_linear(dev, torch, x, w, sw, y=y[i], ws_buf=buf)
+        x.fill_(float("nan"))
+        w.fill_(1)
+        sw.fill_(3.0)
+    for i in range(n):
+        qw, ws = quantized(src_w[i].cpu().numpy())
+        q, s = quantized(src_x[i].cpu().numpy())
+        check_product(y[i].cpu().numpy(), product(q, s, qw, ws), "f32")
+
+
+@pytest.mark.parametrize("M", [3, 100, 600])
+def test_two_streams_at_once(dev, torch, M):
+    """Two streams with workspaces of their own, their calls interleaved."""
+    K, N, n = 512, 1500, 8
+    w, sw = torch.randint(-127, 128, (1, N, K), dtype=torch.int8, device="cuda"), torch.rand(1, N, device="cuda")
+    x = [torch.randn(M, K).cuda() for _ in range(2)]
+    y = [torch.zeros(n, M, N, device="cuda") for _ in range(2)]
+    bufs = [torch.zeros(vb.int8_workspace_bytes(M, K), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(n):
+        for j in range(2):
+            run_linear(dev, torch, x[j], w, sw, y=y[j][i], ws_buf=bufs[j], stream=streams[j].cuda_stream)
+    torch.cuda.synchronize()
+    for j in range(2):
+        q, s = quantized(x[j].cpu().numpy())
+        check_product(y[j][0].cpu().numpy(), product(q, s, w[0].cpu().numpy(), sw[0].cpu().numpy()), "f32")
+        assert all(torch.equal(y[j][0], y[j][i]) for i in range(n))
+
+
 def test_captured_in_a_graph(dev, torch):
     x = torch.randn(5, 256).cuda()
     w = torch.randint(-127, 128, (1, 300, 256), dtype=torch.int8, device="cuda")
