@@ -237,7 +237,7 @@ __device__ __forceinline__ void store_bytes(int8_t* q, const float (&x)[N], cons
 
 // ROW: threads of a row (32 or the CTA's 256); KEEP: vectors a thread keeps.
 template <typename T, bool SWIGLU, uint32_t ROW, uint32_t KEEP>
-__global__ void __launch_bounds__(256, KEEP > 8 ? 2 : SWIGLU || KEEP > 4 ? 3 : 5) int8_quantize_vec_kernel(const Int8QuantParams p) {
+__global__ void __launch_bounds__(256, KEEP > (SWIGLU ? 4 : 8) ? 2 : SWIGLU || KEEP > 4 ? 3 : 5) int8_quantize_vec_kernel(const Int8QuantParams p) {
     constexpr uint32_t N = RowVec<T>::kN;
     __shared__ uint32_t top[8];
     tc::grid_dependency_wait();
@@ -257,23 +257,27 @@ __global__ void __launch_bounds__(256, KEEP > 8 ? 2 : SWIGLU || KEEP > 4 ? 3 : 5
             else a.load_part(row + (size_t)v * N, p.cols - v * N);
             return a;
         };
-        RowVec<T> a[KEEP];
+        RowVec<T> a[SWIGLU ? 1 : KEEP];
         float f[SWIGLU ? KEEP : 1][N];
         uint32_t m = 0;
         if constexpr (SWIGLU) {
-            RowVec<T> b[KEEP];
+            constexpr uint32_t kAtOnce = KEEP < 4u ? KEEP : 4u;  // loads of both operands in flight
 #pragma unroll
-            for (uint32_t i = 0; i < KEEP; ++i) {
-                a[i] = fetch(x, tid + i * ROW);
-                b[i] = fetch(up, tid + i * ROW);
-            }
+            for (uint32_t i0 = 0; i0 < KEEP; i0 += kAtOnce) {
+                RowVec<T> a[kAtOnce], b[kAtOnce];
 #pragma unroll
-            for (uint32_t i = 0; i < KEEP; ++i)
-#pragma unroll
-                for (uint32_t j = 0; j < N; ++j) {
-                    f[i][j] = swiglu(a[i].get(j), b[i].get(j), p.limit);
-                    m = max(m, __float_as_uint(f[i][j]) & 0x7fffffffu);
+                for (uint32_t i = 0; i < kAtOnce; ++i) {
+                    a[i] = fetch(x, tid + (i0 + i) * ROW);
+                    b[i] = fetch(up, tid + (i0 + i) * ROW);
                 }
+#pragma unroll
+                for (uint32_t i = 0; i < kAtOnce; ++i)
+#pragma unroll
+                    for (uint32_t j = 0; j < N; ++j) {
+                        f[i0 + i][j] = swiglu(a[i].get(j), b[i].get(j), p.limit);
+                        m = max(m, __float_as_uint(f[i0 + i][j]) & 0x7fffffffu);
+                    }
+            }
             for (uint32_t v = tid + KEEP * ROW; v < have; v += ROW) {
                 const RowVec<T> c = fetch(x, v), d = fetch(up, v);
 #pragma unroll
@@ -1093,8 +1097,8 @@ cudaError_t quantize_rows(const Int8QuantParams& p, cudaStream_t s) {
         return launch(int8_quantize_kernel<T, SWIGLU, 256, 16>, by_block);
     }
     if (many && p.cols <= 32u * 4u * N) return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 4>, by_warp);
+    if (many && p.cols <= 32u * 8u * N) return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 8>, by_warp);
     if constexpr (!SWIGLU) {
-        if (many && p.cols <= 32u * 8u * N) return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 8>, by_warp);
         if (many && p.cols <= 32u * 16u * N) return launch(int8_quantize_vec_kernel<T, SWIGLU, 32, 16>, by_warp);
     }
     if (p.cols <= 256u * 2u * N) return launch(int8_quantize_vec_kernel<T, SWIGLU, 256, 2>, by_block);
