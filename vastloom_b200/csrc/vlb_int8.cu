@@ -438,11 +438,15 @@ __global__ void __launch_bounds__(256) int8_linear_kernel(const Int8LinearParams
 // One launch from the float rows on: for a handful of rows a call is as long as its launches and the
 // latency of its loads, and the weights are its bytes. A block quantizes the rows into shared memory
 // while its warps' first weights are on their way; then a warp takes two channels at a time, a lane
-// 16 bytes of each every 512, four such pieces of both in flight, dp4a against the rows. A call with
+// 16 bytes of each every 512, two or four such pieces of both in flight, dp4a against the rows. A call with
 // groups takes one row a block and that row's matrix (rows <= 16: two rows of one group read it
 // twice, from L2).
 
-constexpr uint32_t kFewThreads = 256, kFewWarps = kFewThreads / 32u, kFewPieces = 4;
+constexpr uint32_t kFewThreads = 256, kFewWarps = kFewThreads / 32u;
+// Pieces of a channel in flight, and blocks an SM: one row has registers for twice the blocks, whose
+// set-up then overlaps (16 rows of 64 experts' 2048 x 2048: 4 pieces and 2 blocks 19.2 us, 2 and 4 14.8).
+__host__ __device__ constexpr uint32_t few_pieces(uint32_t rows) { return rows == 1u ? 2u : 4u; }
+__host__ __device__ constexpr uint32_t few_blocks(uint32_t rows) { return rows == 1u ? 4u : 2u; }
 constexpr uint32_t kFewSmem = 64u * 1024u;
 
 // 16 bytes of a weight row from byte k on, zeros past K.
@@ -461,8 +465,9 @@ __device__ __forceinline__ void store_typed(void* y, size_t at, float v, int typ
 
 // T: the rows' type, int8_t for rows that are integers already. ROWS: rows of a block.
 template <typename T, uint32_t ROWS>
-__global__ void __launch_bounds__(kFewThreads, 2) int8_few_kernel(const Int8LinearParams l, const Int8QuantParams q, int y_type,
+__global__ void __launch_bounds__(kFewThreads, few_blocks(ROWS)) int8_few_kernel(const Int8LinearParams l, const Int8QuantParams q, int y_type,
                                                                uint32_t channels) {
+    constexpr uint32_t kFewPieces = few_pieces(ROWS);
     extern __shared__ __align__(16) unsigned char few_smem[];
     __shared__ uint32_t top[ROWS], group_s;
     __shared__ float scale[ROWS];
@@ -1280,9 +1285,8 @@ cudaError_t few_launch(const Int8LinearParams& l, const Int8QuantParams& q, int 
         const cudaError_t e = smem_once(kernel, kFewSmem);
         if (e != cudaSuccess) return e;
     }
-    // about two blocks an SM (their registers), so that their set-up overlaps
-    const uint32_t sets = l.offsets ? l.rows : 1u;
-    uint32_t channels = (uint32_t)(((uint64_t)l.out_cols * sets + 2u * sms - 1u) / (2u * sms));
+    const uint32_t sets = l.offsets ? l.rows : 1u, slots = few_blocks(ROWS) * sms;
+    uint32_t channels = (uint32_t)(((uint64_t)l.out_cols * sets + slots - 1u) / slots);
     channels = (channels + 2u * kFewWarps - 1u) / (2u * kFewWarps) * (2u * kFewWarps);
     return launch_chained(kernel, dim3((l.out_cols + channels - 1u) / channels, sets), kFewThreads, smem, 0, s, l, q, y_type,
                           channels);
