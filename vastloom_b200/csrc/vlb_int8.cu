@@ -439,8 +439,7 @@ __global__ void __launch_bounds__(256) int8_linear_kernel(const Int8LinearParams
 // latency of its loads, and the weights are its bytes. A block quantizes the rows into shared memory
 // while its warps' first weights are on their way; then a warp takes two channels at a time, a lane
 // 16 bytes of each every 512, two or four such pieces of both in flight, dp4a against the rows. A call with
-// groups takes one row a block and that row's matrix (rows <= 16: two rows of one group read it
-// twice, from L2).
+// groups takes one row a block and that row's matrix (two rows of one group read it twice, from L2).
 
 constexpr uint32_t kFewThreads = 256, kFewWarps = kFewThreads / 32u;
 // Pieces of a channel in flight, and blocks an SM: one row has registers for twice the blocks, whose
@@ -1273,8 +1272,11 @@ uint32_t sm_count() {
 
 // What int8_few_kernel takes: its dp4a work grows with the rows (2048 x 2048: 3.6 us for one, 6.1 for
 // 4, 9.3 for 8; 4096 x 4096: 5.7, 11.2, 21.9), the tensor cores' two launches do not (about 6 and 9);
-// every block quantizes all rows, which for 5 rows of 3470 takes longer than the products.
-constexpr uint32_t kFewRows = 8, kFewGroupedRows = 16, kFewElements = 8192;
+// every block quantizes all rows, which for 5 rows of 3470 takes longer than the products. Grouped rows
+// read a matrix each: while they are no more than the groups, few share one (64 groups of 2048 x 2048,
+// few / tensor cores: 8 rows 8.8 / 10.7 us, 24 18.6 / 22.2, 32 25.3 / 23.6; 8 groups: 8 rows 8.2 / 10.3,
+// 16 12.9 / 10.5).
+constexpr uint32_t kFewRows = 8, kFewGroupedRows = 24, kFewElements = 8192;
 constexpr uint64_t kFewWork = 1u << 24;
 
 template <typename T, uint32_t ROWS>
@@ -1335,6 +1337,7 @@ cudaError_t launch_int8_gather(const Int8GatherParams& p, cudaStream_t s) {
 
 bool int8_few(const Int8LinearParams& l) {
     if (l.rows > (l.offsets ? kFewGroupedRows : kFewRows) || !tma_rows(l.w, l.w_stride)) return false;
+    if (l.offsets && l.rows > l.groups) return false;
     if (!l.offsets && l.rows > 2u &&
         ((uint64_t)l.rows * l.cols > kFewElements || (uint64_t)l.rows * l.cols * l.out_cols > kFewWork))
         return false;
