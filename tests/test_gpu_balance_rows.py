@@ -1,0 +1,66 @@
+"""Which rows of the logits the balance loss reads: live ones, and no others (a caller may leave the
+memory of masked tokens, and of tokens that no sequence holds, without content or without backing).
+
+The logits lie in page-locked host memory, which the GPU reads over its host link: 64 MB of rows that
+are not to be read would take 1 ms at 64 GB/s, the link's nominal rate, and the call without them
+takes some tens of microseconds. 0.4 ms is asked of the fastest of eight calls, a factor of two and
+more on either side. Every row is backed, so that a kernel that reads them is slow and no worse.
+"""
+
+import numpy as np
+import pytest
+
+import vastloom_b200 as vb
+from test_gpu_balance import KIND, SCORES, check, dev, plain, routes, torch  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+T, E, K = 65536, 256, 2
+LIMIT_MS = 0.4
+
+
+@pytest.mark.parametrize("case", ["all masked", "few live", "outside", "outside, masked"])
+def test_rows_that_are_not_live_are_not_read(dev, torch, case):  # noqa: F811
+    rng = np.random.default_rng(len(case))
+    z = torch.empty(T, E, pin_memory=True)
+    z.fill_(float("nan"))
+    mask, offsets = None, None
+    if "masked" in case or case == "few live":
+        mask = np.zeros(T, bool)
+        mask[rng.integers(0, T, 64 if case != "all masked" else 0)] = True
+    if "outside" in case:  # the first and the last tokens belong to no sequence
+        offsets = [30000, 30007, 30007, 30100]
+    live = np.ones(T, bool) if mask is None else mask
+    if offsets:
+        if mask is not None:
+            mask[30000:30100:3] = True
+        held = np.zeros(T, bool)
+        held[offsets[0]:offsets[-1]] = True
+        live = live & held
+    z[torch.from_numpy(live)] = torch.from_numpy(rng.standard_normal((int(live.sum()), E)).astype(np.float32))
+    idx = routes(rng, T, E, K) if live.any() else np.zeros((T, K), np.int64)
+    S = 1 if offsets is None else len(offsets) - 1
+    ic = torch.from_numpy(idx.astype(np.int32)).cuda()
+    mc = None if mask is None else torch.from_numpy(mask.astype(np.uint8)).cuda()
+    oc = None if offsets is None else torch.tensor(offsets, dtype=torch.int32).cuda()
+    lo, co = torch.full((1,), 9.0, device="cuda"), torch.full((S, E), 9, dtype=torch.int32, device="cuda")
+    gr = torch.full((T, E), 9.0, device="cuda")
+    n = vb.balance_workspace_bytes(T, E, S)
+    ws = torch.full((n,), 0x5a, dtype=torch.uint8, device="cuda")
+    times = []
+    for _ in range(8):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        torch.cuda.synchronize()
+        a.record()
+        dev.balance_loss_device(z.data_ptr(), ic.data_ptr(), T, E, K, counts_ptr=co.data_ptr(), ws_ptr=ws.data_ptr(),
+                                ws_bytes=n, logits_type=KIND["f32"], score=SCORES["sigmoid"],
+                                mask_ptr=0 if mc is None else mc.data_ptr(), seq_offsets_ptr=0 if oc is None else oc.data_ptr(),
+                                n_seqs=S, loss_ptr=lo.data_ptr(), dlogits_ptr=gr.data_ptr(), stream=1)
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b))
+    got = (float(lo[0]), co.cpu().numpy(), gr.cpu().numpy().astype(np.float64), None)
+    check(got, plain(np.where(live[:, None], z.numpy(), 0), idx, "sigmoid", 1.0, live if offsets is None else mask, offsets),
+          "f32")
+    assert np.all(got[2][~live] == 0)
+    assert min(times) <= LIMIT_MS, times

@@ -246,8 +246,10 @@ template <typename T, uint32_t NV, uint32_t VEC, bool FULL>
 struct BalRow {
     BalVec<T, VEC> v[NV / VEC];
     bool live;
-    __device__ __forceinline__ void load(const BalanceParams& p, uint32_t t) {
-        live = !p.mask || p.mask[t];
+    // A row that is not live is not read: its memory may not be there.
+    __device__ __forceinline__ void load(const BalanceParams& p, uint32_t t, bool is_live) {
+        live = is_live;
+        if (!live) return;
         const T* z = static_cast<const T*>(p.logits) + (size_t)t * p.stride;
 #pragma unroll
         for (uint32_t j = 0; j < NV; j += VEC) {
@@ -345,7 +347,7 @@ __device__ __forceinline__ void clear_row(const BalanceParams& p, uint32_t t) {
 }
 
 // A block takes a run of tokens, sequence by sequence; a warp reads its next row while it works on
-// one. ONE: one block is the whole call, with one sequence, and counts for itself.
+// one, if that row is live. ONE: one block is the whole call, with one sequence, and counts for itself.
 template <typename T, int SCORE, uint32_t NV, uint32_t VEC, bool FULL, bool ONE>
 __global__ void __launch_bounds__(kBalThreads, NV > 8 ? 1 : 2) balance_kernel(const BalanceParams p) {
     __shared__ uint32_t hist[513], alive_s, offsets_s[kBalSeqs + 1];
@@ -355,8 +357,15 @@ __global__ void __launch_bounds__(kBalThreads, NV > 8 ? 1 : 2) balance_kernel(co
     const uint32_t t1 = (uint32_t)((uint64_t)p.T * (blockIdx.x + 1u) / gridDim.x);
     if (ONE) tc::grid_dependency_wait();
     tc::grid_launch_dependents();
+    // A token is live when the mask has it and some sequence holds it: [first, past), as the offsets
+    // do not fall. `ahead`: whether the token after the one in `row` is, read a row early so that a
+    // row's load waits for no flag.
+    uint32_t first = 0, past = t1;
+    if (p.seq_offsets) first = p.seq_offsets[0], past = min(t1, p.seq_offsets[p.S]);
+    const auto is_live = [&](uint32_t t) { return t >= first && t < past && (!p.mask || p.mask[t]); };
     BalRow<T, NV, VEC, FULL> row;
-    if (t0 + warp < t1) row.load(p, t0 + warp);  // on its way while the counts are taken
+    row.load(p, t0 + warp, is_live(t0 + warp));  // on its way while the counts are taken
+    bool ahead = is_live(t0 + warp + kBalWarps);
     const uint32_t* offsets = near_offsets(p, offsets_s);
     if (tid == 0) alive_s = 0;
     if (ONE)
@@ -415,7 +424,8 @@ __global__ void __launch_bounds__(kBalThreads, NV > 8 ? 1 : 2) balance_kernel(co
         const uint32_t r = mine;
         const BalRow<T, NV, VEC, FULL> now = row;
         mine += kBalWarps;
-        if (mine < t1) row.load(p, mine);
+        row.load(p, mine, ahead);
+        ahead = is_live(mine + kBalWarps);
         if (held && now.live) sum += (double)balance_row<T, SCORE, NV, VEC, FULL>(p, now, r, f, weight, up);
         else clear_row<T, NV, VEC>(p, r);
     };
