@@ -447,6 +447,9 @@ constexpr uint32_t kFewThreads = 256, kFewWarps = kFewThreads / 32u;
 __host__ __device__ constexpr uint32_t few_pieces(uint32_t rows) { return rows == 1u ? 2u : 4u; }
 __host__ __device__ constexpr uint32_t few_blocks(uint32_t rows) { return rows == 1u ? 4u : 2u; }
 constexpr uint32_t kFewSmem = 64u * 1024u;
+// Dynamic shared memory a launch may ask for without an opt-in: the default 48 KB hold the kernel's
+// static arrays too (up to 1 KB as the compiler lays them out).
+constexpr uint32_t kFewDefaultSmem = 47u * 1024u;
 
 // 16 bytes of a weight row from byte k on, zeros past K.
 __device__ __forceinline__ uint4 few_load(const int8_t* row, uint32_t k, uint32_t cols) {
@@ -1283,7 +1286,7 @@ template <typename T, uint32_t ROWS>
 cudaError_t few_launch(const Int8LinearParams& l, const Int8QuantParams& q, int y_type, uint32_t sms, cudaStream_t s) {
     auto* kernel = int8_few_kernel<T, ROWS>;
     const size_t smem = (size_t)ROWS * ((l.cols + 15u) / 16u * 16u);
-    if (smem > 48u * 1024u) {
+    if (smem > kFewDefaultSmem) {
         const cudaError_t e = smem_once(kernel, kFewSmem);
         if (e != cudaSuccess) return e;
     }
