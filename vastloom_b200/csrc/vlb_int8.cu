@@ -44,14 +44,14 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
 }
 
 // silu(g) * u with the clamp of the layer's experts (gate from above, up on both sides). The
-// comparisons keep a NaN, which fminf / fmaxf would drop. A gate below -88 gives about 0 (its true
-// value is under 1e-35).
+// comparisons keep a NaN, which fminf / fmaxf would drop. The exponential takes the gate inside
+// [-88, 1000]: beyond, its reciprocal is 0 (silu's true value is under 1e-35) and 1.
 __device__ __forceinline__ float swiglu(float g, float u, float limit) {
     if (limit > 0.f) {
         g = g > limit ? limit : g;
         u = u > limit ? limit : (u < -limit ? -limit : u);
     }
-    return g * fast_rcp(1.f + fast_exp(fminf(-g, 88.f))) * u;
+    return g * fast_rcp(1.f + fast_exp(fmaxf(fminf(-g, 88.f), -1000.f))) * u;
 }
 
 // ---- row quantizer ---------------------------------------------------------------------------
