@@ -1,7 +1,7 @@
-"""Which rows of the logits the balance loss reads: live ones, and no others (a caller may leave the
-memory of masked tokens, and of tokens that no sequence holds, without content or without backing).
+"""Rows of the balance loss at their limits.
 
-The logits lie in page-locked host memory, which the GPU reads over its host link: 64 MB of rows that
+Which rows of the logits it reads: live ones, and no others (a caller may leave the memory of masked
+tokens, and of tokens that no sequence holds, without content or without backing). The logits lie in page-locked host memory, which the GPU reads over its host link: 64 MB of rows that
 are not to be read would take 1 ms at 64 GB/s, the link's nominal rate, and the call without them
 takes some tens of microseconds. 0.4 ms is asked of the fastest of eight calls, a factor of two and
 more on either side. Every row is backed, so that a kernel that reads them is slow and no worse.
@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 
 import vastloom_b200 as vb
-from test_gpu_balance import KIND, SCORES, check, dev, plain, routes, torch  # noqa: F401
+from test_gpu_balance import KIND, SCORES, check, dev, plain, routes, run, torch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +64,23 @@ def test_rows_that_are_not_live_are_not_read(dev, torch, case):  # noqa: F811
           "f32")
     assert np.all(got[2][~live] == 0)
     assert min(times) <= LIMIT_MS, times
+
+
+def test_softmax_far_below_the_row_maximum(dev, torch):  # noqa: F811
+    """Scores of logits 10 to 87 below their row's maximum (multiples of 2^-8, so that the difference is
+    exact), an expert's that no token chose: the gradient -upstream weight p d, d the share of the chosen
+    one. Bound in units of 2^-24: exponential 5, two reciprocals 4, count share 2, weight 3, the sum, d
+    and four products 7: 21, and 24 are asked. An error that grew with the distance would pass it."""
+    rng = np.random.default_rng(5)
+    n, experts = 78, 64
+    far = 10 + np.arange(n) + np.floor(256 * rng.random(n)) / 256
+    far = np.minimum(far, 87)
+    z = np.full((n, experts), 3.25, np.float32)
+    z[:, 1:] -= far[:, None].astype(np.float32)
+    idx = np.zeros((n, 1), np.int64)  # every token's maximum
+    got = run(dev, torch, torch.from_numpy(z).cuda(), idx, score="softmax", coef=1e4, up=1e4)
+    p = np.exp(-far) / (1 + (experts - 1) * np.exp(-far))
+    d = experts / (1 + (experts - 1) * np.exp(-far))
+    want = (-1e8 / n * p * d)[:, None]
+    assert np.all(np.abs(got[2][:, 1:] - want) <= 24 * 2.0 ** -24 * np.abs(want)), float(
+        np.max(np.abs(got[2][:, 1:] / want - 1)) * 2.0 ** 24)

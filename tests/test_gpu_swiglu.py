@@ -84,3 +84,17 @@ def test_product_of_the_largest_gates(dev, torch, x_type, rows):  # noqa: F811
                    up_ptr=guc.data_ptr() + K * guc.element_size())
     q, s = quantize(dev, torch, gu, K)
     check_product(y.cpu().numpy(), product(q, s, w[0], sw[0]), "f32")
+
+
+@pytest.mark.parametrize("rows,cols", [(8, 64), (8, 77), (1030, 96)])
+@pytest.mark.parametrize("x_type", ["f32", "f16", "bf16"])
+def test_rows_of_far_gates(dev, torch, x_type, rows, cols):  # noqa: F811
+    """Every gate of a row near -40, -50, ... -85: an error of the exponential that grows with the gate
+    shows in the row's scale. (Values of 1e-35 and more: normal numbers, also divided by 127.)"""
+    g = torch.Generator().manual_seed(cols)
+    far = -torch.tensor([40.0, 50.0, 60.0, 70.0, 75.0, 80.0, 83.0, 85.0])[torch.arange(rows) % 8]
+    gu = torch.empty(rows, 2 * cols)
+    gu[:, :cols] = far[:, None] + torch.rand(rows, cols, generator=g) - 0.5
+    gu[:, cols:] = 200 + 100 * torch.rand(rows, cols, generator=g)
+    gu = gu.to(dt(torch, x_type))
+    check(*quantize(dev, torch, gu, cols), exact(gu, cols))
