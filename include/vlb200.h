@@ -557,6 +557,7 @@ typedef struct vlb_int8_linear_desc {
     float swiglu_limit;
     uint32_t reserved0;
 } vlb_int8_linear_desc;
+/* Never falls as rows or cols rise. */
 uint64_t vlb_int8_workspace_bytes(uint32_t rows, uint32_t cols);
 int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void* stream);
 /* Synchronises `stream` and reports (VLB_ERR_INTERNAL_ERROR), once, whether a wait inside a product
@@ -607,6 +608,7 @@ typedef struct vlb_balance_desc {
     float coefficient;
     uint32_t reserved0;
 } vlb_balance_desc;
+/* Never falls as T, E or n_seqs rise: a workspace of the largest call serves every smaller one. */
 uint64_t vlb_balance_workspace_bytes(uint32_t T, uint32_t E, uint32_t n_seqs);
 int vlb_balance_loss_device(vlb_handle* h, const vlb_balance_desc* desc, void* stream);
 

@@ -1904,7 +1904,7 @@ int vlb_route_plan_device(vlb_handle* h, const uint32_t* idx, const float* weigh
 uint64_t vlb_balance_workspace_bytes(uint32_t T, uint32_t E, uint32_t n_seqs) {
     if (n_seqs == 0) return 0;
     // ticket | the blocks' losses | the parts' counts
-    return 256 + kBalanceBlocks * 8 + (uint64_t)n_seqs * balance_parts(T, n_seqs) * ((uint64_t)E + 1) * 4;
+    return 256 + kBalanceBlocks * 8 + balance_parts_bound(T, n_seqs) * ((uint64_t)E + 1) * 4;
 }
 
 int vlb_balance_loss_device(vlb_handle* h, const vlb_balance_desc* desc, void* stream) {

@@ -533,6 +533,16 @@ uint32_t balance_parts(uint32_t T, uint32_t S) {
     return pieces <= kBalParts ? pieces : pieces / kBalCluster;
 }
 
+// Parts of all sequences that any call of at most T tokens in at most S sequences has: it never falls
+// as T or S rise, though balance_parts does where clusters begin. With n = balance_pieces > 1 pieces a
+// sequence, half of them were too few: n / 2 * S < 128 and n / 2 * S < T / 256.
+uint64_t balance_parts_bound(uint32_t T, uint32_t S) {
+    const uint64_t tokens = ((uint64_t)T + 255u) / 256u, q = tokens < 128u ? tokens : 128u;
+    const uint64_t pieces = q > 1u ? 2u * (q - 1u) : 0u, most = (uint64_t)S * kBalParts;
+    const uint64_t split = pieces < most ? pieces : most;
+    return split > S ? split : S;
+}
+
 cudaError_t launch_balance(const BalanceParams& p, cudaStream_t s) {
     switch (p.logits_type) {
         case VLB_DTYPE_F32: return balance_typed<float>(p, s);

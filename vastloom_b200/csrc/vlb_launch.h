@@ -165,6 +165,7 @@ struct BalanceParams {
 constexpr uint32_t kBalanceBlocks = 296;  // 2 blocks of 512 threads on each of 148 SMs
 constexpr uint32_t kBalOneTokens = 128;   // up to here one block does the whole call
 uint32_t balance_parts(uint32_t T, uint32_t S);  // parts of a sequence's counts in the workspace
+uint64_t balance_parts_bound(uint32_t T, uint32_t S);  // of all sequences, of the largest call up to T and S
 cudaError_t launch_balance(const BalanceParams& p, cudaStream_t s);
 
 }  // namespace vlb
