@@ -666,7 +666,7 @@ class Device:
         bufs = [self.to_device(x), self.buffer(max(4, n * weights.rows * 4)), self.buffer(max(16, ws))]
         try:
             self.int8_linear_device(weights, bufs[0].address, n, bufs[1].address, ws_ptr=bufs[2].address, ws_bytes=ws)
-            self.synchronize()
+            self.int8_status()  # waits for the product; a wait inside it that ran out is an error
             return bufs[1].download(np.float32, n * weights.rows).reshape(n, weights.rows)
         finally:
             for b in bufs:
