@@ -560,8 +560,9 @@ typedef struct vlb_int8_linear_desc {
 /* Never falls as rows or cols rise. */
 uint64_t vlb_int8_workspace_bytes(uint32_t rows, uint32_t cols);
 int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void* stream);
-/* Synchronises `stream` and reports (VLB_ERR_INTERNAL_ERROR), once, whether a wait inside a product
- * on the handle's device has run out since the last report; its waits are bounded by two seconds. */
+/* Synchronises `stream` and reports (VLB_ERR_INTERNAL_ERROR), once, whether a wait inside one of this
+ * handle's products has run out since the last report; their waits are bounded by two seconds. A
+ * handle outlives its products and the graphs that hold them. */
 int vlb_int8_status(vlb_handle* h, void* stream);
 
 /* The plan of a grouped product from a route (idx u32 [T x k], weights f32 [T x k]): the pairs in

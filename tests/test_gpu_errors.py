@@ -1,0 +1,35 @@
+"""The report of int8 products whose waits ran out: one word a handle, in host memory, which the kernel
+sets and vlb_int8_status reads and clears. The word is set here by the host; no wait is made to run out
+on the GPU."""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import vastloom_b200 as vb
+
+pytestmark = pytest.mark.gpu
+
+
+def error_word(dev):
+    fn = dev.lib["_ZN3vlb15int8_error_wordEP10vlb_handle"]
+    fn.restype, fn.argtypes = C.POINTER(C.c_uint32), [C.c_void_p]
+    return fn(dev.h)
+
+
+def test_a_report_belongs_to_its_handle():
+    with vb.Device(0, install_codebooks=False) as a, vb.Device(0, install_codebooks=False) as b:
+        w, s = a.to_device(np.ones((4, 16), np.int8)), a.to_device(np.ones(4, np.float32))
+        weights = vb.Int8Weights(w.address, s.address, 4, 16)
+        x = np.ones((3, 16), np.float32)
+        error_word(a)[0] = 1
+        b.int8_status()
+        assert b.int8_linear(weights, x).shape == (3, 4)  # asks for b's status: a's report stays
+        with pytest.raises(vb.VlbError, match="ran out"):
+            a.int8_status()
+        a.int8_status()  # reported once
+        error_word(a)[0] = 1
+        with pytest.raises(vb.VlbError, match="ran out"):
+            a.int8_linear(weights, x)
+        assert np.array_equal(a.int8_linear(weights, x), b.int8_linear(weights, x))

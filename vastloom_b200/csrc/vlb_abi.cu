@@ -98,6 +98,9 @@ struct vlb_handle {
     uint32_t* upload_results = nullptr;
     std::vector<uint32_t> upload_slots;
     std::unordered_set<vlb_upload*> uploads;
+    // set to 1 by an int8 product of this handle whose wait ran out, until vlb_int8_status reads it:
+    // page-locked, since the kernel writes it
+    uint32_t* int8_error = nullptr;
     // a record's matrices share one allocation (a device allocation costs ~0.4 ms of host time):
     // live matrices per shared allocation, freed with the last of them
     std::unordered_map<void*, uint32_t> block_refs;
@@ -235,6 +238,11 @@ struct vlb_layer {
     cudaEvent_t ev[kMoePhases + 1] = {};
 };
 
+namespace vlb {
+// Where the int8 products of a handle report a wait that ran out, and vlb_int8_status looks.
+uint32_t* int8_error_word(vlb_handle* h) { return h->int8_error; }
+}  // namespace vlb
+
 #define VLB_LOCK(h)                                                                     \
     if (!(h)) {                                                                          \
         t_error = "null handle";                                                         \
@@ -334,6 +342,14 @@ int vlb_open(int ordinal, const vlb_governor* governor, uint64_t min_free_after,
         delete h;
         return VLB_ERR_IO_ERROR;
     }
+    e = cudaHostAlloc(reinterpret_cast<void**>(&h->int8_error), 64, cudaHostAllocPortable | cudaHostAllocMapped);
+    if (e != cudaSuccess) {
+        t_error = cuda_msg("cudaHostAlloc", e);
+        cudaStreamDestroy(h->stream);
+        delete h;
+        return VLB_ERR_RESOURCE_EXHAUSTED;
+    }
+    *h->int8_error = 0;
     *out = h;
     return VLB_OK;
 }
@@ -355,6 +371,7 @@ void vlb_close(vlb_handle* h) {
         h->allocs.clear();
         if (h->upload_stream) cudaStreamDestroy(h->upload_stream);
         if (h->upload_results) cudaFreeHost(h->upload_results);
+        cudaFreeHost(h->int8_error);
         cudaStreamDestroy(h->stream);
     }
     delete h;
@@ -1774,6 +1791,7 @@ int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void
         p.w_scale = d.w_scale;
         p.offsets = d.offsets;
         p.y = d.y;
+        p.error = vlb::int8_error_word(h);
         p.w_stride = d.w_stride;
         p.y_stride = d.y_stride;
         p.rows = d.rows;
@@ -1851,9 +1869,8 @@ int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void
 int vlb_int8_status(vlb_handle* h, void* stream) {
     VLB_GUARDED({
         VLB_LOCK(h);
-        uint32_t bits = 0;
-        VLB_CUDA(h, int8_take_error(&bits, h->pick(stream)));
-        if (bits) return h->fail(VLB_ERR_INTERNAL_ERROR, "a wait inside an int8 product ran out");
+        VLB_CUDA(h, cudaStreamSynchronize(h->pick(stream)));
+        if (__atomic_exchange_n(vlb::int8_error_word(h), 0u, __ATOMIC_ACQ_REL)) return h->fail(VLB_ERR_INTERNAL_ERROR, "a wait inside an int8 product ran out");
         return VLB_OK;
     })
 }

@@ -617,10 +617,6 @@ struct Int8MmaParams {
     uint32_t early;     // the kernel ahead quantizes the tokens: weights may be loaded beside it
 };
 
-// A wait that ran out (a fault of this code: every wait's event is this CTA's own copies or
-// products); sticky until read.
-__device__ uint32_t g_int8_error;
-
 struct MmTile {
     uint32_t g, row0, count, channel0;
 };
@@ -665,9 +661,15 @@ __device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, volatile
     }
 }
 
-__device__ __forceinline__ void mm_fail(volatile uint32_t* abort) {
+// A wait that ran out (a fault of this code: every wait's event is this CTA's own copies or
+// products) is told to the call's handle: its word in host memory holds 1 until it is read.
+__device__ __forceinline__ void mm_report(const Int8LinearParams& l) {
+    *static_cast<volatile uint32_t*>(l.error) = 1u;
+    __threadfence_system();
+}
+__device__ __forceinline__ void mm_fail(volatile uint32_t* abort, const Int8LinearParams& l) {
     *abort = 1u;
-    atomicOr(&g_int8_error, 1u);
+    mm_report(l);
 }
 
 __device__ __forceinline__ MmTile mm_tile(const MmShared& sh, const Int8MmaParams& p, uint32_t t) {
@@ -713,7 +715,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
     if (!p.early) tc::grid_dependency_wait();
     if (smem & 1023u) {  // the swizzle atoms need it; the same in every CTA of the launch
         tc::grid_dependency_wait();
-        if (tid == 0) atomicOr(&g_int8_error, 2u);
+        if (tid == 0) mm_report(l);
         return;
     }
     if (warp == kMmEpiWarps) {
@@ -959,25 +961,25 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         if (warp < kMmEpiWarps) {
             for (uint32_t t = begin; t < total; t += step)
                 if (!epilogue()) {
-                    if (lane == 0) mm_fail(sh.abort);
+                    if (lane == 0) mm_fail(sh.abort, l);
                     break;
                 }
         } else if (warp == kMmEpiWarps) {
             for (uint32_t t = begin; t < total; t += step)
                 if (!produce(t)) {
-                    if (lane == 0) mm_fail(sh.abort);
+                    if (lane == 0) mm_fail(sh.abort, l);
                     break;
                 }
         } else if (warp == kMmEpiWarps + 2u) {
             for (uint32_t t = begin; t < total; t += step)
                 if (!place(t)) {
-                    if (lane == 0) mm_fail(sh.abort);
+                    if (lane == 0) mm_fail(sh.abort, l);
                     break;
                 }
         } else if (!PAIR || rank == 0) {
             for (uint32_t t = begin; t < total; t += step)
                 if (!multiply(t)) {
-                    if (lane == 0) mm_fail(sh.abort);
+                    if (lane == 0) mm_fail(sh.abort, l);
                     break;
                 }
         }
@@ -1024,7 +1026,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
                     tc::fence_before_sync();
                 }
             }
-            if (!ok && lane == 0) mm_fail(sh.abort);
+            if (!ok && lane == 0) mm_fail(sh.abort, l);
             __syncwarp();
             tc::cluster_sync();
             if (warp < kMmEpiWarps) {
@@ -1365,14 +1367,6 @@ cudaError_t launch_int8_linear(const Int8LinearParams& p, int y_type, bool after
         case VLB_DTYPE_BF16: return linear_type<__nv_bfloat16>(p, after_quantize, s);
         default: return cudaErrorInvalidValue;
     }
-}
-
-cudaError_t int8_take_error(uint32_t* bits, cudaStream_t s) {
-    void* at = nullptr;
-    cudaError_t e = cudaGetSymbolAddress(&at, g_int8_error);
-    if (e == cudaSuccess) e = cudaMemcpyAsync(bits, at, 4, cudaMemcpyDeviceToHost, s);
-    if (e == cudaSuccess) e = cudaMemsetAsync(at, 0, 4, s);
-    return e == cudaSuccess ? cudaStreamSynchronize(s) : e;
 }
 
 }  // namespace vlb

@@ -128,6 +128,7 @@ struct Int8LinearParams {
     const float* w_scale;      // [groups x out_cols]
     const uint32_t* offsets;   // [groups + 1] or null (one group, every row)
     void* y;
+    uint32_t* error;           // the handle's word in host memory: 1 once a wait has run out
     size_t x_stride, w_stride, y_stride;
     uint32_t rows, cols, out_cols, groups;
 };
@@ -140,8 +141,6 @@ bool int8_few(const Int8LinearParams& l);
 cudaError_t launch_int8_few(const Int8LinearParams& l, const Int8QuantParams& q, int x_type, int y_type, cudaStream_t s);
 // after_quantize: launch_int8_quantize went before it on the stream (the product may start beside it)
 cudaError_t launch_int8_linear(const Int8LinearParams& p, int y_type, bool after_quantize, cudaStream_t s);
-// reads and clears the error bits of the products on the current device (synchronises s)
-cudaError_t int8_take_error(uint32_t* bits, cudaStream_t s);
 
 // ---- the router's balance loss (vlb_balance.cu) ----
 struct BalanceParams {
