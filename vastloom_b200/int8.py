@@ -69,14 +69,17 @@ class Int8Experts:
 
 class Int8MoeLayer:
     """One MoE layer on int8 experts: w1, w3 ([I, H]) and w2 ([H, I]) of every expert, optionally a
-    shared expert's three."""
+    shared expert's three. swiglu_limit clamps the routed experts' SwiGLU, shared_swiglu_limit the
+    shared one's (None: as the routed ones; 0: no clamp), as the two limits of MoeLayer."""
 
     def __init__(self, dev: Device, *, router: np.ndarray, w1: Sequence[Expert], w3: Sequence[Expert],
                  w2: Sequence[Expert], top_k: int, score: int = SCORE_SQRT_SOFTPLUS, bias: Optional[np.ndarray] = None,
                  route_scale: float = 1.0, swiglu_limit: float = 0.0,
-                 shared: Optional[tuple[Expert, Expert, Expert]] = None, max_tokens: int = 64):
+                 shared: Optional[tuple[Expert, Expert, Expert]] = None, max_tokens: int = 64,
+                 shared_swiglu_limit: Optional[float] = None):
         self.dev, self.top_k, self.score, self.route_scale = dev, top_k, score, route_scale
         self.swiglu_limit, self.max_tokens = swiglu_limit, max_tokens
+        self.shared_swiglu_limit = swiglu_limit if shared_swiglu_limit is None else shared_swiglu_limit
         router = np.ascontiguousarray(router, dtype=np.float32)
         self.E, self.H = router.shape
         if not len(w1) == len(w3) == len(w2) == self.E:
@@ -126,8 +129,8 @@ class Int8MoeLayer:
         gate_up.fill(group, self.I, w3)
         down.fill(group, 0, w2)
 
-    def _products(self, gate_up: Int8Experts, down: Int8Experts, rows: int, out, T: int, row_index: int = 0,
-                  row_weight: int = 0, offsets: int = 0) -> None:
+    def _products(self, gate_up: Int8Experts, down: Int8Experts, limit: float, rows: int, out, T: int,
+                  row_index: int = 0, row_weight: int = 0, offsets: int = 0) -> None:
         """gate/up of `rows` rows of x, SwiGLU, down into `out` (f32)."""
         b, dev = self._b, self.dev
         dev.int8_linear_device(gate_up.weights, b["x"].address, rows, b["gate_up"].address, y_type=DTYPE_BF16, x_rows=T,
@@ -135,7 +138,7 @@ class Int8MoeLayer:
                                ws_bytes=b["ws"].nbytes)
         dev.int8_linear_device(down.weights, b["gate_up"].address, rows, out.address, x_type=DTYPE_BF16,
                                x_stride=2 * self.I, up_ptr=b["gate_up"].address + 2 * self.I,
-                               swiglu_limit=self.swiglu_limit, row_weight_ptr=row_weight, offsets_ptr=offsets,
+                               swiglu_limit=limit, row_weight_ptr=row_weight, offsets_ptr=offsets,
                                ws_ptr=b["ws"].address, ws_bytes=b["ws"].nbytes)
 
     def forward(self, x: np.ndarray, logits: Optional[np.ndarray] = None) -> np.ndarray:
@@ -160,10 +163,10 @@ class Int8MoeLayer:
         dev.route_plan_device(b["idx"].address, b["weights"].address, T, k, E, b["plan_ws"].address,
                               b["row_index"].address, b["row_weight"].address, b["elem_row"].address,
                               b["offsets"].address)
-        self._products(self.gate_up, self.down, T * k, b["rows"], T, b["row_index"].address, b["row_weight"].address,
-                       b["offsets"].address)
+        self._products(self.gate_up, self.down, self.swiglu_limit, T * k, b["rows"], T, b["row_index"].address,
+                       b["row_weight"].address, b["offsets"].address)
         if self.shared:
-            self._products(*self.shared, T, b["own"], T)
+            self._products(*self.shared, self.shared_swiglu_limit, T, b["own"], T)
         dev._check(dev.lib.vlb_ep_combine_device(dev.h, b["rows"].ptr, b["elem_row"].ptr, T, k,
                                                  b["own"].ptr if self.shared else None, H, b["out"].ptr, None))
         dev.int8_status()
