@@ -33,3 +33,24 @@ def test_a_report_belongs_to_its_handle():
         with pytest.raises(vb.VlbError, match="ran out"):
             a.int8_linear(weights, x)
         assert np.array_equal(a.int8_linear(weights, x), b.int8_linear(weights, x))
+
+
+def test_handles_in_several_threads():
+    """The first products of several handles at once, one in each thread: equal to a later one."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    rng = np.random.default_rng(0)
+    w, s = rng.integers(-127, 128, (300, 512), dtype=np.int8), rng.random(300, np.float32)
+    x = rng.standard_normal((40, 512)).astype(np.float32)
+
+    def run(rows):
+        with vb.Device(0, install_codebooks=False) as dev:
+            wb, sb = dev.to_device(w), dev.to_device(s)
+            weights = vb.Int8Weights(wb.address, sb.address, 300, 512)
+            return [dev.int8_linear(weights, x[:rows]) for _ in range(10)]
+
+    with ThreadPoolExecutor(6) as pool:
+        runs = list(pool.map(run, [40, 40, 1, 3, 40, 17]))
+    whole = run(40)[0]
+    for got, rows in zip(runs, [40, 40, 1, 3, 40, 17]):
+        assert all(np.array_equal(y, whole[:rows]) for y in got)

@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 #include <utility>
@@ -1264,15 +1265,15 @@ cudaError_t mma_launch(const Int8MmaParams& p, uint32_t sms, cudaStream_t s) {
     return launch_chained(kernel, dim3(sms / in_cluster * in_cluster), kMmThreads, smem, MODE == Mm::kOne ? 0 : in_cluster, s, p);
 }
 
+// SMs of the current device; handles of several devices and threads may ask at once.
 uint32_t sm_count() {
-    static uint32_t n = 0;
-    if (n == 0) {
-        int dev = 0, v = 0;
-        if (cudaGetDevice(&dev) == cudaSuccess &&
-            cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0)
-            n = (uint32_t)v;
-    }
-    return n ? n : 148u;
+    static std::atomic<uint32_t> known[64];
+    int dev = 0, v = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 148u;
+    if (dev < 64 && (v = (int)known[dev].load(std::memory_order_relaxed)) > 0) return (uint32_t)v;
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) return 148u;
+    if (dev < 64) known[dev].store((uint32_t)v, std::memory_order_relaxed);
+    return (uint32_t)v;
 }
 
 // What int8_few_kernel takes: its dp4a work grows with the rows (2048 x 2048: 3.6 us for one, 6.1 for
