@@ -592,7 +592,8 @@ typedef struct vlb_balance_desc {
     uint64_t logits_stride;      /* elements; 0 = E */
     const uint32_t* idx;         /* [T x k] */
     const uint8_t* mask;         /* [T] or NULL */
-    const uint32_t* seq_offsets; /* [n_seqs + 1], not falling, or NULL (n_seqs == 1: every token) */
+    const uint32_t* seq_offsets; /* [n_seqs + 1], not falling, or NULL (n_seqs == 1: every token). Where they
+                                  * fall the results are undefined, but nothing outside the arrays is touched */
     const float* upstream;       /* device scalar, NULL = 1 */
     float* loss;                 /* device scalar or NULL */
     uint32_t* counts;            /* [n_seqs x E] */

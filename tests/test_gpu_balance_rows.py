@@ -84,3 +84,39 @@ def test_softmax_far_below_the_row_maximum(dev, torch):  # noqa: F811
     want = (-1e8 / n * p * d)[:, None]
     assert np.all(np.abs(got[2][:, 1:] - want) <= 24 * 2.0 ** -24 * np.abs(want)), float(
         np.max(np.abs(got[2][:, 1:] / want - 1)) * 2.0 ** 24)
+
+
+@pytest.mark.parametrize("T,offsets", [(6000, [0, 5000, 100, 6000]), (6000, [6000, 0, 3000, 10]), (9000, [9000, 4000, 0]),
+                                       (6000, [4000000000, 5, 4294967295, 7]), (20000, [0, 20000, 1, 20000, 2, 20000]),
+                                       (70, [60, 10]), (6000, [0] + [5000, 3] * 300 + [6000])])
+@pytest.mark.parametrize("score", ["softmax", "sqrt_softplus"])
+def test_offsets_that_fall_touch_nothing_outside(dev, torch, T, offsets, score):  # noqa: F811
+    """Offsets outside the contract, over many tokens, pieces and parts: the results are undefined, but
+    every output lies inside its array, no count passes the pairs there are, and the call's neighbours
+    (a right one before and after, in the same workspace) are untouched."""
+    rng = np.random.default_rng(T)
+    n, k, S = 40, 3, len(offsets) - 1
+    z, idx = rng.standard_normal((T, n)).astype(np.float32), routes(rng, T, n, k)
+    right = [0] + sorted(rng.integers(0, T + 1, S - 1).tolist()) + [T]
+    want = plain(z, idx, score, 1.0, None, right)
+    zc, ic = torch.from_numpy(z).cuda(), torch.from_numpy(idx.astype(np.int32)).cuda()
+    size, guard = vb.balance_workspace_bytes(T, n, S), 1024
+    ws = torch.full((size + 4 * guard,), 0x5a, dtype=torch.uint8, device="cuda")
+    co = torch.full((S * n + 2 * guard,), 9, dtype=torch.int32, device="cuda")
+    gr = torch.full((T * n + 2 * guard,), 9.0, device="cuda")
+    for off in (right, offsets, right):
+        oc = torch.from_numpy(np.array(off, np.uint32).view(np.int32)).cuda()
+        lo = torch.full((3,), 9.0, device="cuda")
+        co[guard:-guard] = 9
+        gr[guard:-guard] = 9
+        dev.balance_loss_device(zc.data_ptr(), ic.data_ptr(), T, n, k, counts_ptr=co[guard:].data_ptr(), ws_ptr=ws.data_ptr(),
+                                ws_bytes=size, score=SCORES[score], seq_offsets_ptr=oc.data_ptr(), n_seqs=S,
+                                loss_ptr=lo[1:].data_ptr(), dlogits_ptr=gr[guard:].data_ptr(), stream=1)
+        torch.cuda.synchronize()
+        assert float(lo[0]) == 9 and float(lo[2]) == 9 and torch.all(ws[size:] == 0x5a)
+        for a in (co, gr):
+            assert torch.all(a[:guard] == 9) and torch.all(a[-guard:] == 9)
+        counts, grad = co[guard:-guard].view(S, n).cpu().numpy(), gr[guard:-guard].view(T, n).cpu().numpy()
+        assert 0 <= counts.min() and counts.sum(axis=1).max() <= T * k
+        if off is right:
+            check((float(lo[1]), counts, grad.astype(np.float64), None), want, "f32")

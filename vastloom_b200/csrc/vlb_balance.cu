@@ -132,7 +132,8 @@ __global__ void __launch_bounds__(kBalThreads) balance_count_kernel(const Balanc
     const uint32_t to = lo + (uint32_t)(((uint64_t)(hi - lo) * (piece + 1u)) >> log_pieces);
     __syncthreads();
     if ((tid == 0 || tid == 32u) && offsets && from < to) {
-        // offsets that fall: a range whose ends another sequence holds is empty
+        // offsets that fall are outside the contract; a range whose ends another sequence holds counts
+        // as empty, so that no count passes the tokens' pairs
         const uint32_t t = tid ? to - 1u : from;
         if (sequence_after(offsets, p.S, t) != s || offsets[s] > t) foreign = 1;
     }
