@@ -711,7 +711,7 @@ class Device:
         try:
             bufs.append(self.buffer(ws))
             if mask is not None:
-                m = np.ascontiguousarray(mask).astype(np.uint8)
+                m = np.ascontiguousarray(np.asarray(mask) != 0).astype(np.uint8)
                 if m.shape != (T,):
                     raise ValueError("mask must have one entry for each token")
                 bufs.append(self.to_device(m))
