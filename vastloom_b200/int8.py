@@ -47,7 +47,7 @@ class Int8Experts:
         else:
             source = np.ascontiguousarray(source, dtype=np.float32)
             n, cols = source.shape
-        if cols != self.cols or row0 + n > self.rows or not 0 <= group < self.weights.groups:
+        if cols != self.cols or not 0 <= row0 <= self.rows - n or not 0 <= group < self.weights.groups:
             raise ValueError(f"a [{n}, {cols}] matrix does not fit rows {row0}.. of [{self.rows}, {self.cols}]")
         wide = dev.buffer(n * cols * 4, "int8-source")
         try:
