@@ -584,7 +584,10 @@ int vlb_route_plan_device(vlb_handle* h, const uint32_t* idx_dev, const float* w
  * is live when mask[t] != 0 (NULL: all) and a sequence holds it; others give nothing, their logits
  * are not read and their gradient is 0. A slot whose id is >= E was dropped: it is not counted. A
  * live token whose logits are all -inf counts in n_s, adds 0 and gets gradient 0. No live token:
- * L = 0. Sums of any order-dependent kind run in a fixed order: equal inputs give equal bits.
+ * L = 0. Sums of any order-dependent kind run in a fixed order: equal inputs give equal bits. A row's
+ * arithmetic is in 32 bits (the loss in 64), its subnormals 0. dlogits has the logits' type: in f16,
+ * elements below 3e-8 (a batch of some ten thousand tokens) round to 0 unless `upstream` carries a
+ * scale, which multiplies them before they are rounded.
  * E <= 512, k <= 64, k <= E. T = 0 is valid. The reference does not train; its routers' scores are
  * cited at VLB_SCORE_*. Enqueued on `stream`; allocates nothing and does not synchronise. */
 typedef struct vlb_balance_desc {

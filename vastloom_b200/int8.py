@@ -70,7 +70,10 @@ class Int8Experts:
 class Int8MoeLayer:
     """One MoE layer on int8 experts: w1, w3 ([I, H]) and w2 ([H, I]) of every expert, optionally a
     shared expert's three. swiglu_limit clamps the routed experts' SwiGLU, shared_swiglu_limit the
-    shared one's (None: as the routed ones; 0: no clamp), as the two limits of MoeLayer."""
+    shared one's (None: as the routed ones; 0: no clamp), as the two limits of MoeLayer. The gate and
+    up values between the two products are held in bf16 (half of f32's bytes through HBM; their
+    rounding, 2^-9, is below that of the 8-bit rows made of them). Every forward also takes the
+    balance loss and the counts."""
 
     def __init__(self, dev: Device, *, router: np.ndarray, w1: Sequence[Expert], w3: Sequence[Expert],
                  w2: Sequence[Expert], top_k: int, score: int = SCORE_SQRT_SOFTPLUS, bias: Optional[np.ndarray] = None,
