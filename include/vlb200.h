@@ -515,8 +515,8 @@ enum { VLB_DTYPE_F32 = 0, VLB_DTYPE_F16 = 1, VLB_DTYPE_BF16 = 2, VLB_DTYPE_I8 = 
  * NULL): row r is x row row_index[r]; an index >= x_rows gives a row of zeros. x_rows 0 = rows.
  * up_dev (or NULL; type and stride of x): the row is silu(min(x, L)) * clamp(up, -L, L), the
  * experts' SwiGLU (execute_expert, deepseek_v4_graph.cpp:1826-1895), L = swiglu_limit, 0 = no
- * clamp. x_type F32, F16 or BF16. Enqueued on `stream` (NULL = the handle's; 1 =
- * cudaStreamLegacy). */
+ * clamp. x_type F32, F16 or BF16. rows and cols < 2^31. Enqueued on `stream` (NULL = the handle's;
+ * 1 = cudaStreamLegacy). */
 int vlb_int8_quantize_device(vlb_handle* h, int x_type, const void* x_dev, uint64_t x_stride, uint64_t x_rows,
                              const uint32_t* row_index_dev, const void* up_dev, float swiglu_limit, uint32_t rows,
                              uint32_t cols, int8_t* q_dev, uint64_t q_stride, float* scale_dev, void* stream);

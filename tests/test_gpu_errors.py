@@ -54,3 +54,12 @@ def test_handles_in_several_threads():
     whole = run(40)[0]
     for got, rows in zip(runs, [40, 40, 1, 3, 40, 17]):
         assert all(np.array_equal(y, whole[:rows]) for y in got)
+
+
+@pytest.mark.parametrize("cols", [1 << 31, (1 << 32) - 300, (1 << 32) - 1])
+def test_quantizer_refuses_rows_past_32_bit_steps(cols):
+    """On the host, before anything is launched."""
+    with vb.Device(0, install_codebooks=False) as dev:
+        buf = dev.buffer(4096)
+        with pytest.raises(vb.VlbError, match="2\\^31 columns"):
+            dev.int8_quantize_device(buf.address, 1, cols, buf.address + 1024, buf.address + 2048)

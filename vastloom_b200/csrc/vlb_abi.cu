@@ -1736,6 +1736,8 @@ int vlb_int8_quantize_device(vlb_handle* h, int x_type, const void* x, uint64_t 
         if (q_stride == 0) q_stride = cols;
         if (cols == 0 || rows > 0x7fffffffu)
             return h->fail(VLB_ERR_INVALID_ARGUMENT, "int8 quantize: cols must be positive and rows below 2^31");
+        if (cols > 0x7fffffffu)  // the kernels step through a row in 32 bits
+            return h->fail(VLB_ERR_UNSUPPORTED, "int8 quantize: rows of 2^31 columns and more");
         if (const char* why = bad_float_rows(x_type, x, x_stride, x_rows, row_index, up, swiglu_limit, rows, cols))
             return h->fail(VLB_ERR_INVALID_ARGUMENT, std::string("int8 quantize: ") + why);
         if (rows && (!q || !scale || !aligned(scale, 4)))
