@@ -1700,9 +1700,9 @@ static size_t int8_rows_bytes(uint32_t rows, uint32_t cols) { return ((size_t)ro
 static size_t int8_block_bytes(uint32_t rows, uint32_t cols) {
     return int8_rows_bytes(rows, cols) + ((size_t)rows * 4 + 255) / 256 * 256;
 }
-// Rows used more than once on average are quantized once and then copied: from 16 M elements on that
-// beats quantizing each copy (32,768 rows of 2048 bf16 from 4096: 23 us against 33); below, the launch
-// outweighs it.
+// Rows used twice or more on average, in a call of 16 M elements or more, are quantized once and then
+// copied instead of quantized for each use (32,768 rows of 2048 bf16 from 4096: 23 us against 33); in
+// smaller calls the second launch outweighs it.
 static bool int8_gather_apart(uint64_t x_rows, uint32_t rows, uint32_t cols) {
     return x_rows * 2 <= rows && (uint64_t)rows * cols >= (1u << 24);
 }

@@ -1276,12 +1276,13 @@ uint32_t sm_count() {
     return (uint32_t)v;
 }
 
-// What int8_few_kernel takes: its dp4a work grows with the rows (2048 x 2048: 3.6 us for one, 6.1 for
-// 4, 9.3 for 8; 4096 x 4096: 5.7, 11.2, 21.9), the tensor cores' two launches do not (about 6 and 9);
-// every block quantizes all rows, which for 5 rows of 3470 takes longer than the products. Grouped rows
-// read a matrix each: while they are no more than the groups, few share one (64 groups of 2048 x 2048,
-// few / tensor cores: 8 rows 8.8 / 10.7 us, 24 18.6 / 22.2, 32 25.3 / 23.6; 8 groups: 8 rows 8.2 / 10.3,
-// 16 12.9 / 10.5).
+// What int8_few_kernel takes. Dense: up to kFewRows rows, from 3 on no more than kFewElements elements
+// and kFewWork products; its dp4a work grows with the rows while the tensor cores' two launches do not
+// (2048 x 2048: 3.6 us for one row, 6.1 for 4, 9.3 for 8, against about 6; 4096 x 4096: 5.7, 11.2, 21.9,
+// against about 9), and every block quantizes all rows (5 rows of 3470: longer than the products).
+// Grouped: up to kFewGroupedRows rows and no more than the groups, as each row reads its matrix and few
+// then share one (2048 x 2048, few / tensor cores: 8, 24, 32 rows of 64 groups 8.8 / 10.7, 18.6 / 22.2,
+// 25.3 / 23.6 us; 8, 16 rows of 8 groups 8.2 / 10.3, 12.9 / 10.5). Measured at these widths only.
 constexpr uint32_t kFewRows = 8, kFewGroupedRows = 24, kFewElements = 8192;
 constexpr uint64_t kFewWork = 1u << 24;
 
