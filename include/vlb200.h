@@ -617,6 +617,171 @@ typedef struct vlb_balance_desc {
 uint64_t vlb_balance_workspace_bytes(uint32_t T, uint32_t E, uint32_t n_seqs);
 int vlb_balance_loss_device(vlb_handle* h, const vlb_balance_desc* desc, void* stream);
 
+/* ---- the residual's addition and RMS norm ---------------------------------------------------
+ * For each row r of x (`type` F32, F16 or BF16) and residual (`residual_type`: F32, or x's type):
+ *     h = x + residual,   s = 1 / sqrt(mean_c h_c^2 + eps),   y_c = h_c s weight_c
+ * in 32 bits; residual_out = h rounded to residual_type, y = the norm of h (not of its rounding)
+ * rounded to x's type, and q, q_scale = y as vlb_int8_quantize_device makes int8 rows (of y before it
+ * is rounded): the rows an int8 product or vlb_sort_tokens_device takes next. Any of residual_out, y
+ * and the pair q, q_scale may be NULL, not all. residual NULL: h = x. weight NULL: 1. Rows whose h
+ * passes 1.8e19 (its square has no 32-bit value) are scaled on the way. A row whose h holds a NaN is NaN
+ * throughout, one with an infinity is NaN there and 0 elsewhere; both have q = 0 and scale NaN.
+ * An output may be an input's own memory (same address, type and stride): the stream updated in place;
+ * else nothing may overlap. Strides in elements, 0 = cols; any alignment of the elements' own size
+ * works, rows on 16-byte boundaries are faster. cols < 2^31; eps in [1e-30, inf). vlb_rms_norm_device
+ * is the reference's norm (f64 chains, bit for bit); this one is the form for blocks around the int8
+ * products. Enqueued on `stream` (NULL = the handle's; 1 = cudaStreamLegacy); allocates nothing and
+ * does not synchronise. */
+typedef struct vlb_add_rms_norm_desc {
+    const void* x;               /* [rows] rows of type */
+    uint64_t x_stride;
+    const void* residual;        /* [rows] rows of residual_type or NULL */
+    uint64_t residual_stride;
+    const float* weight;         /* [cols] or NULL */
+    void* residual_out;          /* [rows] rows of residual_type or NULL */
+    uint64_t residual_out_stride;
+    void* y;                     /* [rows] rows of type or NULL */
+    uint64_t y_stride;
+    int8_t* q;                   /* [rows] rows, with q_scale, or NULL */
+    uint64_t q_stride;
+    float* q_scale;              /* [rows] */
+    uint32_t rows;
+    uint32_t cols;
+    int32_t type;
+    int32_t residual_type;
+    float eps;
+    uint32_t reserved0;
+} vlb_add_rms_norm_desc;
+int vlb_add_rms_norm_device(vlb_handle* h, const vlb_add_rms_norm_desc* desc, void* stream);
+
+/* The gradient of it, with h as the forward pass left it (residual_out; x itself where there was no
+ * residual) and s computed again from it. n = h s, g = dy weight:
+ *     d = s (g - n mean_c(g n)) + dh,    dx = d,  dresidual = d,    dweight_c = sum_r dy n
+ * dy is the gradient of y, dh (or NULL) what reaches residual_out from further on. dx (x's type) and
+ * dresidual (residual_type) are the same numbers, each rounded once; of one type, one of them is
+ * enough. Any of dx, dresidual and dweight may be NULL, not all; dx may be dy's memory and dresidual
+ * dh's. Sums over rows run in a fixed order: equal inputs give equal bits. rows = 0 gives a dweight of
+ * zeros. ws: vlb_add_rms_norm_grad_workspace_bytes(rows, cols), 16-byte aligned, for dweight alone. */
+typedef struct vlb_add_rms_norm_grad_desc {
+    const void* dy;              /* [rows] rows of type */
+    uint64_t dy_stride;
+    const void* h;               /* [rows] rows of residual_type */
+    uint64_t h_stride;
+    const float* weight;         /* [cols] or NULL */
+    const void* dh;              /* [rows] rows of residual_type or NULL */
+    uint64_t dh_stride;
+    void* dx;                    /* [rows] rows of type or NULL */
+    uint64_t dx_stride;
+    void* dresidual;             /* [rows] rows of residual_type or NULL */
+    uint64_t dresidual_stride;
+    float* dweight;              /* [cols] or NULL */
+    void* ws;
+    uint64_t ws_bytes;
+    uint32_t rows;
+    uint32_t cols;
+    int32_t type;
+    int32_t residual_type;
+    float eps;
+    uint32_t reserved0;
+} vlb_add_rms_norm_grad_desc;
+/* Never falls as rows or cols rise. */
+uint64_t vlb_add_rms_norm_grad_workspace_bytes(uint32_t rows, uint32_t cols);
+int vlb_add_rms_norm_grad_device(vlb_handle* h, const vlb_add_rms_norm_grad_desc* desc, void* stream);
+
+/* ---- tokens sorted by expert and back ----------------------------------------------------------
+ * The pairs (token t, slot s) of a route idx [T x k] in the dispatch's stable order (expert, then
+ * token, then slot), without a host synchronisation. A pair is live when mask[t] != 0 (NULL: all) and
+ * its id is < E; others were dropped and get no row. With n live pairs, pair p of them in order:
+ *     rows[p] = x[t],  row_scale[p] = x_scale[t],  row_index[p] = t,  row_weight[p] = weights[t][s],
+ *     elem_row[t][s] = p (VLB_NO_ROW where dropped),  offsets[e] = the first pair of expert e,
+ *     offsets[E] = n
+ * What lies behind row n of the outputs is left as it was. rows, row_scale, row_index and row_weight
+ * may be NULL (rows NULL: the order alone, x unused). A token may name an expert twice: two rows. type
+ * F32, F16, BF16 or I8: rows are copied bit by bit; offsets, row_index, row_weight and int8 rows with
+ * row_scale are what vlb_int8_linear_device takes. The gradient of rows with respect to x is
+ * vlb_combine_device of their gradient with the same elem_row and no weights; that of row_weight is
+ * row_weight's gradient at elem_row. E <= 1024, k <= 64, T x k < 2^31. T = 0 is valid. Strides in
+ * elements, 0 = H; any alignment of the elements' own size works, rows on 16-byte boundaries are
+ * faster. Nothing may overlap. Enqueued on `stream`; allocates nothing and does not synchronise. */
+#define VLB_NO_ROW 0xffffffffu
+typedef struct vlb_sort_tokens_desc {
+    const uint32_t* idx;         /* [T x k] */
+    const float* weights;        /* [T x k], with row_weight, or NULL */
+    const uint8_t* mask;         /* [T] or NULL */
+    const void* x;               /* [T] rows of type, with rows, or NULL */
+    uint64_t x_stride;
+    const float* x_scale;        /* [T], with row_scale, or NULL */
+    void* rows;                  /* [T x k] rows of type or NULL */
+    uint64_t rows_stride;
+    float* row_scale;            /* [T x k] or NULL */
+    uint32_t* row_index;         /* [T x k] or NULL */
+    float* row_weight;           /* [T x k] or NULL */
+    uint32_t* elem_row;          /* [T x k] */
+    uint32_t* offsets;           /* [E + 1] */
+    void* ws;                    /* vlb_sort_tokens_workspace_bytes(T, k, E), 16-byte aligned */
+    uint64_t ws_bytes;
+    uint32_t T;
+    uint32_t k;
+    uint32_t E;
+    uint32_t H;                  /* columns of x; unused without rows */
+    int32_t type;
+    uint32_t reserved0;
+} vlb_sort_tokens_desc;
+/* Never falls as T, k or E rise. */
+uint64_t vlb_sort_tokens_workspace_bytes(uint32_t T, uint32_t k, uint32_t E);
+int vlb_sort_tokens_device(vlb_handle* h, const vlb_sort_tokens_desc* desc, void* stream);
+
+/* Rows back to their tokens:
+ *     out[t] = sum_s weights[t][s] rows[elem_row[t][s]] + residual[t]
+ * in 32 bits, slots in order, the residual last, rounded once to `out_type`. An elem_row >= n_rows
+ * (VLB_NO_ROW) adds nothing, whatever its weight. weights NULL: 1; residual NULL: 0. rows of `type`,
+ * residual and out of out_type (F32, F16 or BF16 each); out may be the residual's own memory (same
+ * address and stride), else nothing may overlap. T = 0 is valid, also n_rows = 0. Enqueued on
+ * `stream`; allocates nothing and does not synchronise. */
+typedef struct vlb_combine_desc {
+    const void* rows;            /* [n_rows] rows of type */
+    uint64_t rows_stride;        /* elements; 0 = H */
+    const uint32_t* elem_row;    /* [T x k] */
+    const float* weights;        /* [T x k] or NULL */
+    const void* residual;        /* [T] rows of out_type or NULL */
+    uint64_t residual_stride;
+    void* out;                   /* [T] rows of out_type */
+    uint64_t out_stride;
+    uint32_t T;
+    uint32_t k;
+    uint32_t H;
+    uint32_t n_rows;
+    int32_t type;
+    int32_t out_type;
+} vlb_combine_desc;
+int vlb_combine_device(vlb_handle* h, const vlb_combine_desc* desc, void* stream);
+
+/* The gradient of it (the residual's is dout itself):
+ *     drows[elem_row[t][s]] = weights[t][s] dout[t],   dweights[t][s] = sum_c dout[t]_c rows[elem_row[t][s]]_c
+ * dweights is 0 where elem_row >= n_rows; rows of drows that no pair names are left as they were. Each
+ * row is named once at most, as vlb_sort_tokens_device leaves it (of a row named twice, drows holds
+ * either pair's). rows (for dweights alone) and drows of `type`, dout of out_type; drows may be the
+ * rows' own memory (same address and stride). drows or dweights may be NULL, not both. Sums run in a
+ * fixed order. */
+typedef struct vlb_combine_grad_desc {
+    const void* dout;            /* [T] rows of out_type */
+    uint64_t dout_stride;        /* elements; 0 = H */
+    const void* rows;            /* [n_rows] rows of type; unused without dweights */
+    uint64_t rows_stride;
+    const uint32_t* elem_row;    /* [T x k] */
+    const float* weights;        /* [T x k] or NULL */
+    void* drows;                 /* [n_rows] rows of type or NULL */
+    uint64_t drows_stride;
+    float* dweights;             /* [T x k] or NULL */
+    uint32_t T;
+    uint32_t k;
+    uint32_t H;
+    uint32_t n_rows;
+    int32_t type;
+    int32_t out_type;
+} vlb_combine_grad_desc;
+int vlb_combine_grad_device(vlb_handle* h, const vlb_combine_grad_desc* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

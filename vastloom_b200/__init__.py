@@ -49,6 +49,8 @@ DTYPE_F16 = 1
 DTYPE_BF16 = 2
 DTYPE_I8 = 3
 
+NO_ROW = 0xFFFFFFFF  # elem_row of a dropped pair
+
 SCORE_SQRT_SOFTPLUS = 0
 SCORE_SIGMOID = 1
 SCORE_SOFTMAX = 2
@@ -148,9 +150,54 @@ class _BalanceDesc(C.Structure):
                 ("reserved0", C.c_uint32)]
 
 
+class _AddRmsNormDesc(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_uint64), ("residual", C.c_void_p), ("residual_stride", C.c_uint64),
+                ("weight", C.c_void_p), ("residual_out", C.c_void_p), ("residual_out_stride", C.c_uint64),
+                ("y", C.c_void_p), ("y_stride", C.c_uint64), ("q", C.c_void_p), ("q_stride", C.c_uint64),
+                ("q_scale", C.c_void_p), ("rows", C.c_uint32), ("cols", C.c_uint32), ("type", C.c_int32),
+                ("residual_type", C.c_int32), ("eps", C.c_float), ("reserved0", C.c_uint32)]
+
+
+class _AddRmsNormGradDesc(C.Structure):
+    _fields_ = [("dy", C.c_void_p), ("dy_stride", C.c_uint64), ("h", C.c_void_p), ("h_stride", C.c_uint64),
+                ("weight", C.c_void_p), ("dh", C.c_void_p), ("dh_stride", C.c_uint64), ("dx", C.c_void_p),
+                ("dx_stride", C.c_uint64), ("dresidual", C.c_void_p), ("dresidual_stride", C.c_uint64),
+                ("dweight", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_uint64), ("rows", C.c_uint32),
+                ("cols", C.c_uint32), ("type", C.c_int32), ("residual_type", C.c_int32), ("eps", C.c_float),
+                ("reserved0", C.c_uint32)]
+
+
+class _SortTokensDesc(C.Structure):
+    _fields_ = [("idx", C.c_void_p), ("weights", C.c_void_p), ("mask", C.c_void_p), ("x", C.c_void_p),
+                ("x_stride", C.c_uint64), ("x_scale", C.c_void_p), ("rows", C.c_void_p), ("rows_stride", C.c_uint64),
+                ("row_scale", C.c_void_p), ("row_index", C.c_void_p), ("row_weight", C.c_void_p),
+                ("elem_row", C.c_void_p), ("offsets", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_uint64),
+                ("T", C.c_uint32), ("k", C.c_uint32), ("E", C.c_uint32), ("H", C.c_uint32), ("type", C.c_int32),
+                ("reserved0", C.c_uint32)]
+
+
+class _CombineDesc(C.Structure):
+    _fields_ = [("rows", C.c_void_p), ("rows_stride", C.c_uint64), ("elem_row", C.c_void_p), ("weights", C.c_void_p),
+                ("residual", C.c_void_p), ("residual_stride", C.c_uint64), ("out", C.c_void_p),
+                ("out_stride", C.c_uint64), ("T", C.c_uint32), ("k", C.c_uint32), ("H", C.c_uint32),
+                ("n_rows", C.c_uint32), ("type", C.c_int32), ("out_type", C.c_int32)]
+
+
+class _CombineGradDesc(C.Structure):
+    _fields_ = [("dout", C.c_void_p), ("dout_stride", C.c_uint64), ("rows", C.c_void_p), ("rows_stride", C.c_uint64),
+                ("elem_row", C.c_void_p), ("weights", C.c_void_p), ("drows", C.c_void_p), ("drows_stride", C.c_uint64),
+                ("dweights", C.c_void_p), ("T", C.c_uint32), ("k", C.c_uint32), ("H", C.c_uint32),
+                ("n_rows", C.c_uint32), ("type", C.c_int32), ("out_type", C.c_int32)]
+
+
 # the same descriptions packed as bytes: building a ctypes structure costs more than the call
 _INT8_LINEAR_PACK = struct.Struct("=15Q4I2ifI").pack
 _BALANCE_PACK = struct.Struct("=12Q4I2ifI").pack
+_ADD_RMS_NORM_PACK = struct.Struct("=12Q2I2ifI").pack
+_ADD_RMS_NORM_GRAD_PACK = struct.Struct("=14Q2I2ifI").pack
+_SORT_TOKENS_PACK = struct.Struct("=15Q4IiI").pack
+_COMBINE_PACK = struct.Struct("=8Q4I2i").pack
+_COMBINE_GRAD_PACK = struct.Struct("=9Q4I2i").pack
 
 
 class _LayerDesc(C.Structure):
@@ -196,7 +243,9 @@ EXPORTS = (
     "vlb_upload_record_async vlb_upload_query vlb_upload_finish vlb_host_alloc vlb_host_free "
     "vlb_layer_set_hyper_connection vlb_layer_last_hyper_split "
     "vlb_int8_quantize_device vlb_int8_workspace_bytes vlb_int8_linear_device vlb_int8_status vlb_route_plan_device "
-    "vlb_balance_workspace_bytes vlb_balance_loss_device"
+    "vlb_balance_workspace_bytes vlb_balance_loss_device "
+    "vlb_add_rms_norm_device vlb_add_rms_norm_grad_workspace_bytes vlb_add_rms_norm_grad_device "
+    "vlb_sort_tokens_workspace_bytes vlb_sort_tokens_device vlb_combine_device vlb_combine_grad_device"
 ).split()
 
 
@@ -281,6 +330,13 @@ def load_library() -> C.CDLL:
         "vlb_route_plan_device": (I, [P, P, P, U32, U32, U32, P, P, P, P, P, P]),
         "vlb_balance_workspace_bytes": (U64, [U32, U32, U32]),
         "vlb_balance_loss_device": (I, [P, P, P]),
+        "vlb_add_rms_norm_device": (I, [P, P, P]),
+        "vlb_add_rms_norm_grad_workspace_bytes": (U64, [U32, U32]),
+        "vlb_add_rms_norm_grad_device": (I, [P, P, P]),
+        "vlb_sort_tokens_workspace_bytes": (U64, [U32, U32, U32]),
+        "vlb_sort_tokens_device": (I, [P, P, P]),
+        "vlb_combine_device": (I, [P, P, P]),
+        "vlb_combine_grad_device": (I, [P, P, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -350,6 +406,16 @@ def int8_workspace_bytes(rows: int, cols: int) -> int:
 def balance_workspace_bytes(T: int, E: int, n_seqs: int = 1) -> int:
     """Workspace of one balance-loss call."""
     return int(load_library().vlb_balance_workspace_bytes(T, E, n_seqs))
+
+
+def add_rms_norm_grad_workspace_bytes(rows: int, cols: int) -> int:
+    """Workspace of one norm gradient with the weight's."""
+    return int(load_library().vlb_add_rms_norm_grad_workspace_bytes(rows, cols))
+
+
+def sort_tokens_workspace_bytes(T: int, k: int, E: int) -> int:
+    """Workspace of one sort of tokens by expert."""
+    return int(load_library().vlb_sort_tokens_workspace_bytes(T, k, E))
 
 
 class DeviceBuffer:
@@ -729,6 +795,103 @@ class Device:
         finally:
             for b in bufs:
                 b.free()
+
+
+    # -- the residual's addition and RMS norm --
+    def add_rms_norm_device(self, x_ptr: int, rows: int, cols: int, *, x_type: int = DTYPE_F32,
+                            residual_type: int = DTYPE_F32, x_stride: int = 0, residual_ptr: int = 0,
+                            residual_stride: int = 0, weight_ptr: int = 0, eps: float = 1e-6, residual_out_ptr: int = 0,
+                            residual_out_stride: int = 0, y_ptr: int = 0, y_stride: int = 0, q_ptr: int = 0,
+                            q_stride: int = 0, q_scale_ptr: int = 0, stream: int = 0) -> None:
+        """h = x + residual and its RMS norm, in x's type and as int8 rows (vlb_add_rms_norm_device), on
+        raw device pointers; an output pointer of 0 leaves that output out."""
+        st = self.lib.vlb_add_rms_norm_device(
+            self.h, _ADD_RMS_NORM_PACK(x_ptr, x_stride, residual_ptr, residual_stride, weight_ptr, residual_out_ptr,
+                                       residual_out_stride, y_ptr, y_stride, q_ptr, q_stride, q_scale_ptr, rows, cols,
+                                       x_type, residual_type, eps, 0), stream or None)
+        if st:
+            self._check(st)
+
+    def add_rms_norm_grad_device(self, dy_ptr: int, h_ptr: int, rows: int, cols: int, *, x_type: int = DTYPE_F32,
+                                 residual_type: int = DTYPE_F32, dy_stride: int = 0, h_stride: int = 0,
+                                 weight_ptr: int = 0, eps: float = 1e-6, dh_ptr: int = 0, dh_stride: int = 0,
+                                 dx_ptr: int = 0, dx_stride: int = 0, dresidual_ptr: int = 0, dresidual_stride: int = 0,
+                                 dweight_ptr: int = 0, ws_ptr: int = 0, ws_bytes: int = 0, stream: int = 0) -> None:
+        """The gradient of add_rms_norm_device's sum and weight (vlb_add_rms_norm_grad_device), on raw
+        device pointers; dweight needs a workspace (add_rms_norm_grad_workspace_bytes)."""
+        st = self.lib.vlb_add_rms_norm_grad_device(
+            self.h, _ADD_RMS_NORM_GRAD_PACK(dy_ptr, dy_stride, h_ptr, h_stride, weight_ptr, dh_ptr, dh_stride, dx_ptr,
+                                            dx_stride, dresidual_ptr, dresidual_stride, dweight_ptr, ws_ptr, ws_bytes,
+                                            rows, cols, x_type, residual_type, eps, 0), stream or None)
+        if st:
+            self._check(st)
+
+    def add_rms_norm(self, x: np.ndarray, weight: np.ndarray, eps: float = 1e-6,
+                     residual: Optional[np.ndarray] = None):
+        """Host form on f32 or f16 rows and residual: (h, norm of h, q int8, q_scale)."""
+        x = np.ascontiguousarray(x)
+        if x.dtype not in (np.float32, np.float16) or x.ndim != 2 or np.shape(weight) != (x.shape[1],):
+            raise ValueError("x must be a float32 or float16 matrix, weight one value for each of its columns")
+        r = x if residual is None else np.ascontiguousarray(residual)
+        if r.shape != x.shape or r.dtype not in (np.float32, x.dtype):
+            raise ValueError("residual must have x's shape, in float32 or x's type")
+        kind = {np.dtype(np.float32): DTYPE_F32, np.dtype(np.float16): DTYPE_F16}
+        rows, cols = x.shape
+        bufs = [self.to_device(x), self.to_device(r), self.to_device(np.ascontiguousarray(weight, np.float32)),
+                self.buffer(max(4, r.nbytes)), self.buffer(max(4, x.nbytes)), self.buffer(max(4, x.size)),
+                self.buffer(max(4, rows * 4))]
+        try:
+            a = [b.address for b in bufs]
+            self.add_rms_norm_device(a[0], rows, cols, x_type=kind[x.dtype], residual_type=kind[r.dtype],
+                                     residual_ptr=0 if residual is None else a[1], weight_ptr=a[2], eps=eps,
+                                     residual_out_ptr=a[3], y_ptr=a[4], q_ptr=a[5], q_scale_ptr=a[6])
+            self.synchronize()
+            return (bufs[3].download(r.dtype, r.size).reshape(r.shape), bufs[4].download(x.dtype, x.size).reshape(x.shape),
+                    bufs[5].download(np.int8, x.size).reshape(x.shape), bufs[6].download(np.float32, rows))
+        finally:
+            for b in bufs:
+                b.free()
+
+    # -- tokens sorted by expert and back --
+    def sort_tokens_device(self, idx_ptr: int, T: int, k: int, E: int, *, elem_row_ptr: int, offsets_ptr: int,
+                           ws_ptr: int, ws_bytes: int, x_ptr: int = 0, H: int = 0, x_type: int = DTYPE_F32,
+                           x_stride: int = 0, x_scale_ptr: int = 0, weights_ptr: int = 0, mask_ptr: int = 0,
+                           rows_ptr: int = 0, rows_stride: int = 0, row_scale_ptr: int = 0, row_index_ptr: int = 0,
+                           row_weight_ptr: int = 0, stream: int = 0) -> None:
+        """The pairs of a route in the experts' order with each pair's row (vlb_sort_tokens_device), on
+        raw device pointers; an output pointer of 0 leaves that output out."""
+        st = self.lib.vlb_sort_tokens_device(
+            self.h, _SORT_TOKENS_PACK(idx_ptr, weights_ptr, mask_ptr, x_ptr, x_stride, x_scale_ptr, rows_ptr, rows_stride,
+                                      row_scale_ptr, row_index_ptr, row_weight_ptr, elem_row_ptr, offsets_ptr, ws_ptr,
+                                      ws_bytes, T, k, E, H, x_type, 0), stream or None)
+        if st:
+            self._check(st)
+
+    def combine_device(self, rows_ptr: int, elem_row_ptr: int, T: int, k: int, H: int, out_ptr: int, *,
+                       n_rows: Optional[int] = None, x_type: int = DTYPE_F32, y_type: int = DTYPE_F32,
+                       rows_stride: int = 0, weights_ptr: int = 0, residual_ptr: int = 0, residual_stride: int = 0,
+                       out_stride: int = 0, stream: int = 0) -> None:
+        """Rows back to their tokens, weighted, on top of a residual (vlb_combine_device), on raw device
+        pointers. n_rows: T * k unless given. x_type: the rows' type, y_type: residual's and out's."""
+        st = self.lib.vlb_combine_device(
+            self.h, _COMBINE_PACK(rows_ptr, rows_stride, elem_row_ptr, weights_ptr, residual_ptr, residual_stride, out_ptr,
+                                  out_stride, T, k, H, T * k if n_rows is None else n_rows, x_type, y_type),
+            stream or None)
+        if st:
+            self._check(st)
+
+    def combine_grad_device(self, dout_ptr: int, elem_row_ptr: int, T: int, k: int, H: int, *,
+                            n_rows: Optional[int] = None, x_type: int = DTYPE_F32, y_type: int = DTYPE_F32,
+                            dout_stride: int = 0, rows_ptr: int = 0, rows_stride: int = 0, weights_ptr: int = 0,
+                            drows_ptr: int = 0, drows_stride: int = 0, dweights_ptr: int = 0, stream: int = 0) -> None:
+        """The gradient of combine_device's rows and weights (vlb_combine_grad_device), on raw device
+        pointers; an output pointer of 0 leaves that output out."""
+        st = self.lib.vlb_combine_grad_device(
+            self.h, _COMBINE_GRAD_PACK(dout_ptr, dout_stride, rows_ptr, rows_stride, elem_row_ptr, weights_ptr, drows_ptr,
+                                       drows_stride, dweights_ptr, T, k, H, T * k if n_rows is None else n_rows, x_type,
+                                       y_type), stream or None)
+        if st:
+            self._check(st)
 
 
 class MoeLayer:

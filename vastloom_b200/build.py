@@ -24,7 +24,7 @@ DATA = PKG / "data"
 GRIDS = DATA / "iq_grids.bin"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 SOURCES = ["vlb_kernels.cu", "vlb_decode.cu", "vlb_prefill.cu", "vlb_ep.cu", "vlb_abi.cu", "vlb_noalloc.cu", "vlb_ep_driver.cu",
-           "vlb_int8.cu", "vlb_balance.cu"]
+           "vlb_int8.cu", "vlb_balance.cu", "vlb_norm.cu", "vlb_tokens.cu"]
 
 
 def reference_root() -> Path:

@@ -1978,4 +1978,251 @@ int vlb_balance_loss_device(vlb_handle* h, const vlb_balance_desc* desc, void* s
     })
 }
 
+// ---- the residual's addition and RMS norm; tokens sorted by expert and back -------------------------
+
+constexpr uint64_t kMaxRowStride = 1ull << 38;  // elements: no row's offset passes 64 bits
+
+// The types of a norm: the residual's is f32 or the rows' own. Null, or what is wrong.
+static const char* bad_norm(int type, int residual_type, uint32_t rows, uint32_t cols, float eps, const float* weight) {
+    if (!float_type(type)) return "type must be F32, F16 or BF16";
+    if (residual_type != type && residual_type != VLB_DTYPE_F32) return "residual_type must be F32 or the rows' type";
+    if (cols == 0 || cols > 0x7fffffffu || rows > 0x7fffffffu) return "cols must be positive, rows and cols below 2^31";
+    if (!(eps >= 1e-30f) || !std::isfinite(eps)) return "eps must be in [1e-30, inf)";
+    if (!aligned(weight, 4)) return "weight is not aligned to its elements";
+    return nullptr;
+}
+// Rows at p of elements of `size` bytes, `stride` (0: made cols) apart; a null p has none.
+static bool bad_rows(const void* p, uint64_t& stride, uint32_t cols, size_t size) {
+    if (stride == 0) stride = cols;
+    return p && (!aligned(p, size) || stride < cols || stride > kMaxRowStride);
+}
+
+int vlb_add_rms_norm_device(vlb_handle* h, const vlb_add_rms_norm_desc* desc, void* stream) {
+    VLB_GUARDED({
+        VLB_LOCK(h);
+        if (!desc) return h->fail(VLB_ERR_INVALID_ARGUMENT, "add rms norm: null description");
+        vlb_add_rms_norm_desc d = *desc;
+        auto bad = [&](const char* why) { return h->fail(VLB_ERR_INVALID_ARGUMENT, std::string("add rms norm: ") + why); };
+        if (const char* why = bad_norm(d.type, d.residual_type, d.rows, d.cols, d.eps, d.weight)) return bad(why);
+        const size_t es = dtype_size(d.type), rs = dtype_size(d.residual_type);
+        if (bad_rows(d.x, d.x_stride, d.cols, es) || bad_rows(d.residual, d.residual_stride, d.cols, rs) ||
+            bad_rows(d.residual_out, d.residual_out_stride, d.cols, rs) || bad_rows(d.y, d.y_stride, d.cols, es) ||
+            bad_rows(d.q, d.q_stride, d.cols, 1))
+            return bad("rows are not aligned to their elements, or a stride is out of range");
+        if (!d.q != !d.q_scale || !aligned(d.q_scale, 4)) return bad("q and q_scale go together, q_scale aligned to 4 bytes");
+        if (!d.residual_out && !d.y && !d.q) return bad("no output");
+        if (d.rows && !d.x) return bad("x is null");
+        if (d.rows == 0) return VLB_OK;
+        NormParams p{};
+        p.x = d.x;
+        p.residual = d.residual;
+        p.weight = d.weight;
+        p.h = d.residual_out;
+        p.y = d.y;
+        p.q = d.q;
+        p.scale = d.q_scale;
+        p.x_stride = d.x_stride;
+        p.residual_stride = d.residual_stride;
+        p.h_stride = d.residual_out_stride;
+        p.y_stride = d.y_stride;
+        p.q_stride = d.q_stride;
+        p.rows = d.rows;
+        p.cols = d.cols;
+        p.eps = d.eps;
+        VLB_CUDA(h, launch_add_norm(p, d.type, d.residual_type, h->pick(stream)));
+        return VLB_OK;
+    })
+}
+
+// the parts of the weight's gradient | the rows' statistics
+static uint64_t norm_parts_bytes(uint32_t rows, uint32_t cols) {
+    const uint64_t parts = rows < kNormParts ? rows : kNormParts;
+    return (parts * cols * 4 + 255) / 256 * 256;
+}
+uint64_t vlb_add_rms_norm_grad_workspace_bytes(uint32_t rows, uint32_t cols) {
+    return norm_parts_bytes(rows, cols) + (uint64_t)rows * 16;
+}
+
+int vlb_add_rms_norm_grad_device(vlb_handle* h, const vlb_add_rms_norm_grad_desc* desc, void* stream) {
+    VLB_GUARDED({
+        VLB_LOCK(h);
+        if (!desc) return h->fail(VLB_ERR_INVALID_ARGUMENT, "add rms norm gradient: null description");
+        vlb_add_rms_norm_grad_desc d = *desc;
+        auto bad = [&](const char* why) {
+            return h->fail(VLB_ERR_INVALID_ARGUMENT, std::string("add rms norm gradient: ") + why);
+        };
+        if (const char* why = bad_norm(d.type, d.residual_type, d.rows, d.cols, d.eps, d.weight)) return bad(why);
+        const size_t es = dtype_size(d.type), rs = dtype_size(d.residual_type);
+        if (bad_rows(d.dy, d.dy_stride, d.cols, es) || bad_rows(d.h, d.h_stride, d.cols, rs) ||
+            bad_rows(d.dh, d.dh_stride, d.cols, rs) || bad_rows(d.dx, d.dx_stride, d.cols, es) ||
+            bad_rows(d.dresidual, d.dresidual_stride, d.cols, rs))
+            return bad("rows are not aligned to their elements, or a stride is out of range");
+        if (!d.dx && !d.dresidual && !d.dweight) return bad("no output");
+        if (!aligned(d.dweight, 4)) return bad("dweight is not aligned to its elements");
+        if (d.rows && (!d.dy || !d.h)) return bad("dy or h is null");
+        cudaStream_t s = h->pick(stream);
+        if (d.rows == 0) {
+            if (d.dweight) VLB_CUDA(h, cudaMemsetAsync(d.dweight, 0, (size_t)d.cols * 4, s));
+            return VLB_OK;
+        }
+        if (d.dweight && (!d.ws || !aligned(d.ws, 16) || d.ws_bytes < vlb_add_rms_norm_grad_workspace_bytes(d.rows, d.cols)))
+            return bad("the workspace is null, not 16-byte aligned or below vlb_add_rms_norm_grad_workspace_bytes");
+        NormGradParams p{};
+        p.dy = d.dy;
+        p.h = d.h;
+        p.weight = d.weight;
+        p.dh = d.dh;
+        p.dx = d.dx;
+        p.dres = d.dresidual;
+        p.dw = d.dweight;
+        if (d.dweight) {
+            p.part = static_cast<float*>(d.ws);
+            p.row = reinterpret_cast<float4*>(static_cast<char*>(d.ws) + norm_parts_bytes(d.rows, d.cols));
+        }
+        p.dy_stride = d.dy_stride;
+        p.h_stride = d.h_stride;
+        p.dh_stride = d.dh_stride;
+        p.dx_stride = d.dx_stride;
+        p.dres_stride = d.dresidual_stride;
+        p.rows = d.rows;
+        p.cols = d.cols;
+        p.eps = d.eps;
+        VLB_CUDA(h, launch_add_norm_grad(p, d.type, d.residual_type, s));
+        return VLB_OK;
+    })
+}
+
+uint64_t vlb_sort_tokens_workspace_bytes(uint32_t T, uint32_t k, uint32_t E) {
+    return 256 + (uint64_t)sort_blocks((uint64_t)T * k) * E * 4;
+}
+
+int vlb_sort_tokens_device(vlb_handle* h, const vlb_sort_tokens_desc* desc, void* stream) {
+    VLB_GUARDED({
+        VLB_LOCK(h);
+        if (!desc) return h->fail(VLB_ERR_INVALID_ARGUMENT, "sort tokens: null description");
+        vlb_sort_tokens_desc d = *desc;
+        auto bad = [&](const char* why) { return h->fail(VLB_ERR_INVALID_ARGUMENT, std::string("sort tokens: ") + why); };
+        if (d.E == 0 || d.k == 0) return bad("E and k must be positive");
+        if (d.E > kSortMaxExperts || d.k > 64 || (uint64_t)d.T * d.k > 0x7fffffffull)
+            return h->fail(VLB_ERR_UNSUPPORTED, "sort tokens: E > 1024, k > 64 or T x k >= 2^31");
+        if (!d.offsets || (d.T && (!d.idx || !d.elem_row))) return bad("idx, elem_row or offsets is null");
+        if (!aligned(d.idx, 4) || !aligned(d.weights, 4) || !aligned(d.x_scale, 4) || !aligned(d.row_scale, 4) ||
+            !aligned(d.row_index, 4) || !aligned(d.row_weight, 4) || !aligned(d.elem_row, 4) || !aligned(d.offsets, 4))
+            return bad("a pointer is not aligned to its elements");
+        if (d.T && ((d.row_weight && !d.weights) || (d.row_scale && !d.x_scale)))
+            return bad("row_weight needs weights, row_scale x_scale");
+        const size_t es = dtype_size(d.type);
+        if (d.rows) {
+            if (!es) return bad("type must be F32, F16, BF16 or I8");
+            if (d.H == 0 || (d.T && !d.x)) return bad("rows need x and H");
+            if (bad_rows(d.x, d.x_stride, d.H, es) || bad_rows(d.rows, d.rows_stride, d.H, es))
+                return bad("rows are not aligned to their elements, or a stride is out of range");
+        }
+        cudaStream_t s = h->pick(stream);
+        if (d.T == 0) {
+            VLB_CUDA(h, cudaMemsetAsync(d.offsets, 0, ((size_t)d.E + 1) * 4, s));
+            return VLB_OK;
+        }
+        if (!d.ws || !aligned(d.ws, 16) || d.ws_bytes < vlb_sort_tokens_workspace_bytes(d.T, d.k, d.E))
+            return bad("the workspace is null, not 16-byte aligned or below vlb_sort_tokens_workspace_bytes");
+        SortParams p{};
+        p.idx = d.idx;
+        p.weights = d.weights;
+        p.mask = d.mask;
+        p.x_scale = d.x_scale;
+        p.row_scale = d.row_scale;
+        p.row_weight = d.row_weight;
+        p.row_index = d.row_index;
+        p.elem_row = d.elem_row;
+        p.offsets = d.offsets;
+        p.counts = static_cast<uint32_t*>(d.ws);
+        p.T = d.T;
+        p.k = d.k;
+        p.E = d.E;
+        if (d.rows) {
+            p.x = static_cast<const char*>(d.x);
+            p.rows = static_cast<char*>(d.rows);
+            p.x_stride = d.x_stride * es;
+            p.rows_stride = d.rows_stride * es;
+            p.row_bytes = d.H * es;
+            p.elem = (uint32_t)es;
+        }
+        VLB_CUDA(h, launch_sort_tokens(p, s));
+        return VLB_OK;
+    })
+}
+
+int vlb_combine_device(vlb_handle* h, const vlb_combine_desc* desc, void* stream) {
+    VLB_GUARDED({
+        VLB_LOCK(h);
+        if (!desc) return h->fail(VLB_ERR_INVALID_ARGUMENT, "combine: null description");
+        vlb_combine_desc d = *desc;
+        auto bad = [&](const char* why) { return h->fail(VLB_ERR_INVALID_ARGUMENT, std::string("combine: ") + why); };
+        if (!float_type(d.type) || !float_type(d.out_type)) return bad("type and out_type must be F32, F16 or BF16");
+        if (d.k == 0 || d.H == 0 || d.H > 0x7fffffffu) return bad("k and H must be positive, H below 2^31");
+        if (d.k > 64 || (uint64_t)d.T * d.k > 0x7fffffffull)
+            return h->fail(VLB_ERR_UNSUPPORTED, "combine: k > 64 or T x k >= 2^31");
+        const size_t es = dtype_size(d.type), os = dtype_size(d.out_type);
+        if (bad_rows(d.rows, d.rows_stride, d.H, es) || bad_rows(d.residual, d.residual_stride, d.H, os) ||
+            bad_rows(d.out, d.out_stride, d.H, os))
+            return bad("rows are not aligned to their elements, or a stride is out of range");
+        if (!aligned(d.elem_row, 4) || !aligned(d.weights, 4)) return bad("a pointer is not aligned to its elements");
+        if (d.T && (!d.elem_row || !d.out || (d.n_rows && !d.rows))) return bad("rows, elem_row or out is null");
+        if (d.T == 0) return VLB_OK;
+        CombineParams p{};
+        p.rows = d.rows;
+        p.elem_row = d.elem_row;
+        p.weights = d.weights;
+        p.residual = d.residual;
+        p.out = d.out;
+        p.rows_stride = d.rows_stride;
+        p.residual_stride = d.residual_stride;
+        p.out_stride = d.out_stride;
+        p.T = d.T;
+        p.k = d.k;
+        p.H = d.H;
+        p.n_rows = d.n_rows;
+        VLB_CUDA(h, launch_combine(p, d.type, d.out_type, h->pick(stream)));
+        return VLB_OK;
+    })
+}
+
+int vlb_combine_grad_device(vlb_handle* h, const vlb_combine_grad_desc* desc, void* stream) {
+    VLB_GUARDED({
+        VLB_LOCK(h);
+        if (!desc) return h->fail(VLB_ERR_INVALID_ARGUMENT, "combine gradient: null description");
+        vlb_combine_grad_desc d = *desc;
+        auto bad = [&](const char* why) { return h->fail(VLB_ERR_INVALID_ARGUMENT, std::string("combine gradient: ") + why); };
+        if (!float_type(d.type) || !float_type(d.out_type)) return bad("type and out_type must be F32, F16 or BF16");
+        if (d.k == 0 || d.H == 0 || d.H > 0x7fffffffu) return bad("k and H must be positive, H below 2^31");
+        if (d.k > 64 || (uint64_t)d.T * d.k > 0x7fffffffull)
+            return h->fail(VLB_ERR_UNSUPPORTED, "combine gradient: k > 64 or T x k >= 2^31");
+        const size_t es = dtype_size(d.type), os = dtype_size(d.out_type);
+        if (bad_rows(d.dout, d.dout_stride, d.H, os) || bad_rows(d.rows, d.rows_stride, d.H, es) ||
+            bad_rows(d.drows, d.drows_stride, d.H, es))
+            return bad("rows are not aligned to their elements, or a stride is out of range");
+        if (!aligned(d.elem_row, 4) || !aligned(d.weights, 4) || !aligned(d.dweights, 4))
+            return bad("a pointer is not aligned to its elements");
+        if (!d.drows && !d.dweights) return bad("no output");
+        if (d.T && (!d.elem_row || !d.dout || (d.dweights && d.n_rows && !d.rows))) return bad("dout, rows or elem_row is null");
+        if (d.T == 0) return VLB_OK;
+        CombineGradParams p{};
+        p.dout = d.dout;
+        p.rows = d.rows;
+        p.elem_row = d.elem_row;
+        p.weights = d.weights;
+        p.drows = d.drows;
+        p.dweights = d.dweights;
+        p.dout_stride = d.dout_stride;
+        p.rows_stride = d.rows_stride;
+        p.drows_stride = d.drows_stride;
+        p.T = d.T;
+        p.k = d.k;
+        p.H = d.H;
+        p.n_rows = d.n_rows;
+        VLB_CUDA(h, launch_combine_grad(p, d.type, d.out_type, h->pick(stream)));
+        return VLB_OK;
+    })
+}
+
 }  // extern "C"

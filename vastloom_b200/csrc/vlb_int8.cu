@@ -19,30 +19,11 @@
 
 #include "vlb_launch.h"
 #include "vlb_math.cuh"
+#include "vlb_rows.cuh"
 #include "vlb_tcgen05.cuh"
 
 namespace vlb {
 namespace {
-
-// ---- elements --------------------------------------------------------------------------------
-
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_float(float v);
-template <>
-__device__ __forceinline__ float from_float<float>(float v) {
-    return v;
-}
-template <>
-__device__ __forceinline__ __half from_float<__half>(float v) {
-    return __float2half_rn(v);
-}
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
-    return __float2bfloat16_rn(v);
-}
 
 // silu(g) * u with the clamp of the layer's experts (gate from above, up on both sides). The
 // comparisons keep a NaN, which fminf / fmaxf would drop. The exponential takes the gate inside
@@ -56,29 +37,6 @@ __device__ __forceinline__ float swiglu(float g, float u, float limit) {
 }
 
 // ---- row quantizer ---------------------------------------------------------------------------
-
-// What a row's largest |x| (as float bits, so that a NaN is the largest of all) makes of the row:
-// its scale, and the factor that brings it to [-127, 127]. Rows below 2^-100 are first lifted by
-// 2^100 (exact), or 127 / a would overflow. A row that is not finite keeps q = 0 and the scale
-// NaN, so the products' rows that come from it are NaN and no others.
-struct RowStep {
-    float lift, inv, scale;
-};
-__device__ __forceinline__ RowStep row_step(uint32_t amax_bits) {
-    const float a = __uint_as_float(amax_bits);
-    if (amax_bits == 0u) return RowStep{0.f, 0.f, 0.f};
-    if (amax_bits >= 0x7f800000u) return RowStep{0.f, 0.f, __uint_as_float(0x7fc00000u)};
-    const float lift = a < 0x1p-100f ? 0x1p100f : 1.f;
-    return RowStep{lift, __fdiv_rn(127.f, a * lift), __fdiv_rn(a, 127.f)};
-}
-
-// rint(x * inv) as the low byte of an integer: adding 1.5 * 2^23 leaves the rounded integer in
-// the mantissa's low bits. The product rounds to 32 bits first (the operator's definition), so it
-// must not be contracted into the addition.
-__device__ __forceinline__ uint32_t quant_byte(float x, const RowStep& st) {
-    if (st.inv == 0.f) return 0u;
-    return __float_as_uint(__fadd_rn(__fmul_rn(x * st.lift, st.inv), 12582912.f)) & 0xffu;
-}
 
 template <typename T, bool SWIGLU>
 __device__ __forceinline__ float row_value(const Int8QuantParams& p, size_t at) {
@@ -216,25 +174,6 @@ struct RowMax {
         return top << 16;
     }
 };
-
-// A vector's bytes at q; `n` of them (N but at a row's end).
-template <uint32_t N>
-__device__ __forceinline__ void store_bytes(int8_t* q, const float (&x)[N], const RowStep& st, uint32_t n) {
-    uint32_t w[N / 4];
-#pragma unroll
-    for (uint32_t i = 0; i < N; i += 4u) {
-        uint32_t b[4];
-#pragma unroll
-        for (uint32_t j = 0; j < 4u; ++j) b[j] = __float_as_uint(__fadd_rn(__fmul_rn(x[i + j], st.inv), 12582912.f));
-        w[i / 4u] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-    }
-    if (n < N) {
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i)
-            if (i < n) q[i] = (int8_t)(w[i / 4u] >> (8u * (i % 4u)));
-    } else if constexpr (N == 8) *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint32_t*>(q) = w[0];
-}
 
 // ROW: threads of a row (32 or the CTA's 256); KEEP: vectors a thread keeps.
 template <typename T, bool SWIGLU, uint32_t ROW, uint32_t KEEP>

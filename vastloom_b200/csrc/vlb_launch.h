@@ -167,4 +167,77 @@ uint32_t balance_parts(uint32_t T, uint32_t S);  // parts of a sequence's counts
 uint64_t balance_parts_bound(uint32_t T, uint32_t S);  // of all sequences, of the largest call up to T and S
 cudaError_t launch_balance(const BalanceParams& p, cudaStream_t s);
 
+// ---- the residual's addition and RMS norm (vlb_norm.cu) ----
+struct NormParams {
+    const void* x;
+    const void* residual;      // or null
+    const float* weight;       // or null: 1
+    void* h;                   // residual_out, or null
+    void* y;                   // or null
+    int8_t* q;                 // or null
+    float* scale;
+    size_t x_stride, residual_stride, h_stride, y_stride, q_stride;
+    uint32_t rows, cols;
+    float eps;
+};
+struct NormGradParams {
+    const void* dy;
+    const void* h;
+    const float* weight;       // or null: 1
+    const void* dh;            // or null
+    void* dx;                  // or null
+    void* dres;                // or null
+    float* dw;                 // or null
+    float* part;               // workspace, for dw: [kNormParts at most][cols] sums of parts of the rows
+    float4* row;               // workspace, for dw: the rows' (lift, s, mean(g n))
+    size_t dy_stride, h_stride, dh_stride, dx_stride, dres_stride;
+    uint32_t rows, cols;
+    float eps;
+};
+constexpr uint32_t kNormParts = 444;
+cudaError_t launch_add_norm(const NormParams& p, int type, int residual_type, cudaStream_t s);
+cudaError_t launch_add_norm_grad(const NormGradParams& p, int type, int residual_type, cudaStream_t s);
+
+// ---- tokens sorted by expert and back (vlb_tokens.cu) ----
+struct SortParams {
+    const uint32_t* idx;
+    const float* weights;
+    const uint8_t* mask;       // or null
+    const char* x;             // rows of H elements of `elem` bytes, or null
+    const float* x_scale;
+    char* rows;                // or null
+    float *row_scale, *row_weight;  // or null
+    uint32_t* row_index;       // or null
+    uint32_t* elem_row;
+    uint32_t* offsets;         // [E + 1]
+    uint32_t* counts;          // workspace: [blocks][E] the blocks' pairs of each expert
+    size_t x_stride, rows_stride;  // bytes
+    size_t row_bytes;
+    uint32_t T, k, E, elem;
+};
+constexpr uint32_t kSortMaxExperts = 1024;
+uint32_t sort_blocks(uint64_t pairs);
+cudaError_t launch_sort_tokens(const SortParams& p, cudaStream_t s);
+struct CombineParams {
+    const void* rows;
+    const uint32_t* elem_row;
+    const float* weights;      // or null: 1
+    const void* residual;      // or null
+    void* out;
+    size_t rows_stride, residual_stride, out_stride;
+    uint32_t T, k, H, n_rows;
+};
+cudaError_t launch_combine(const CombineParams& p, int type, int out_type, cudaStream_t s);
+struct CombineGradParams {
+    const void* dout;
+    const void* rows;          // with dweights
+    const uint32_t* elem_row;
+    const float* weights;      // or null: 1
+    void* drows;               // or null
+    float* dweights;           // or null
+    size_t dout_stride, rows_stride, drows_stride;
+    uint32_t T, k, H, n_rows;
+};
+cudaError_t launch_combine_grad(const CombineGradParams& p, int type, int out_type, cudaStream_t s);
+
 }  // namespace vlb
