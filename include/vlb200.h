@@ -565,6 +565,35 @@ int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void
  * handle outlives its products and the graphs that hold them. */
 int vlb_int8_status(vlb_handle* h, void* stream);
 
+/* The same product with bias, activation, route weight and residual in its epilogue:
+ *     z = (sum_k q[r][k] w[g][n][k]) * x_scale[r] * w_scale[g][n] + bias[g][n]
+ *     y[r][n] = row_weight[r] * act(z) + residual[r][n]
+ * act NONE, RELU, SILU (z sigmoid(z)), GELU (z Phi(z)), GELU_TANH (its tanh form) or SWIGLU: channels go in
+ * pairs, gate 2i and up 2i + 1 (rows of w so laid out, out_cols even), y and residual have out_cols / 2
+ * columns, y[r][i] = row_weight[r] * silu(min(gate, L)) * clamp(up, -L, L) + residual[r][i], L = act_limit,
+ * 0 = no clamp (the description's own swiglu_limit belongs to `up`). Everything after the integer sum is in
+ * 32 bits, rounded once to y_type; GELU is within 2^-20 |z|. residual (y_type, any stride of the elements'
+ * alignment, 0 = y's columns) may be y's own memory (same address and stride). y_stride 0 = y's columns. Rows
+ * outside every group are left as they are, their residual unread. All else as vlb_int8_linear_device, which
+ * is this call without an epilogue. */
+enum {
+    VLB_ACT_NONE = 0,
+    VLB_ACT_RELU = 1,
+    VLB_ACT_SILU = 2,
+    VLB_ACT_GELU = 3,
+    VLB_ACT_GELU_TANH = 4,
+    VLB_ACT_SWIGLU = 5
+};
+typedef struct vlb_int8_epilogue {
+    const float* bias;         /* [groups x out_cols] or NULL */
+    const void* residual;      /* [rows] rows of y_type or NULL */
+    uint64_t residual_stride;
+    int32_t act;
+    float act_limit;
+} vlb_int8_epilogue;
+int vlb_int8_linear_act_device(vlb_handle* h, const vlb_int8_linear_desc* desc, const vlb_int8_epilogue* epilogue,
+                               void* stream);
+
 /* The plan of a grouped product from a route (idx u32 [T x k], weights f32 [T x k]): the pairs in
  * the dispatch's stable order (expert, then token, then slot): row_index_dev [T*k] = the pair's
  * token, row_weight_dev [T*k] = its weight, elem_row_dev [T*k] = the row of element t * k + slot,

@@ -14,6 +14,7 @@ def test_packed_descriptions_have_the_structures_layout():
     assert bytes(vb._SortTokensDesc(*n, 31, 32, 33, 34, 2, 0)) == vb._SORT_TOKENS_PACK(*n, 31, 32, 33, 34, 2, 0)
     assert bytes(vb._CombineDesc(*n[:8], 31, 32, 33, 34, 2, 1)) == vb._COMBINE_PACK(*n[:8], 31, 32, 33, 34, 2, 1)
     assert bytes(vb._CombineGradDesc(*n[:9], 31, 32, 33, 34, 2, 1)) == vb._COMBINE_GRAD_PACK(*n[:9], 31, 32, 33, 34, 2, 1)
+    assert bytes(vb._Int8Epilogue(*n[:3], 5, 0.5)) == vb._INT8_EPILOGUE_PACK(*n[:3], 5, 0.5)
 
 
 SIZES = [0, 1, 2, 7, 31, 64, 100, 147, 148, 149, 295, 296, 300, 443, 444, 445, 1000, 1411, 4095, 4096, 4097, 65536, 1 << 20]
@@ -40,3 +41,9 @@ def test_sort_workspace_never_falls():
                                   "vlb_combine_device", "vlb_combine_grad_device"])
 def test_null_handles_are_errors(name):
     assert getattr(vb.load_library(), name)(None, None, None) == 1
+
+
+def test_int8_epilogue_of_a_null_handle_is_an_error():
+    lib = vb.load_library()
+    assert lib.vlb_int8_linear_act_device(None, None, None, None) == 1
+    assert lib.vlb_int8_linear_act_device(None, None, vb._INT8_EPILOGUE_PACK(0, 0, 0, 0, 0.0), None) == 1

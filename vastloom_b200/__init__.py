@@ -49,6 +49,14 @@ DTYPE_F16 = 1
 DTYPE_BF16 = 2
 DTYPE_I8 = 3
 
+# activations of int8_linear_act_device
+ACT_NONE = 0
+ACT_RELU = 1
+ACT_SILU = 2
+ACT_GELU = 3       # z Phi(z)
+ACT_GELU_TANH = 4
+ACT_SWIGLU = 5     # of channel pairs (gate 2i, up 2i + 1)
+
 NO_ROW = 0xFFFFFFFF  # elem_row of a dropped pair
 
 SCORE_SQRT_SOFTPLUS = 0
@@ -141,6 +149,11 @@ class _Int8LinearDesc(C.Structure):
                 ("y_type", C.c_int32), ("swiglu_limit", C.c_float), ("reserved0", C.c_uint32)]
 
 
+class _Int8Epilogue(C.Structure):
+    _fields_ = [("bias", C.c_void_p), ("residual", C.c_void_p), ("residual_stride", C.c_uint64), ("act", C.c_int32),
+                ("act_limit", C.c_float)]
+
+
 class _BalanceDesc(C.Structure):
     _fields_ = [("logits", C.c_void_p), ("logits_stride", C.c_uint64), ("idx", C.c_void_p), ("mask", C.c_void_p),
                 ("seq_offsets", C.c_void_p), ("upstream", C.c_void_p), ("loss", C.c_void_p), ("counts", C.c_void_p),
@@ -193,6 +206,7 @@ class _CombineGradDesc(C.Structure):
 # the same descriptions packed as bytes: building a ctypes structure costs more than the call
 _INT8_LINEAR_PACK = struct.Struct("=15Q4I2ifI").pack
 _BALANCE_PACK = struct.Struct("=12Q4I2ifI").pack
+_INT8_EPILOGUE_PACK = struct.Struct("=3Qif").pack
 _ADD_RMS_NORM_PACK = struct.Struct("=12Q2I2ifI").pack
 _ADD_RMS_NORM_GRAD_PACK = struct.Struct("=14Q2I2ifI").pack
 _SORT_TOKENS_PACK = struct.Struct("=15Q4IiI").pack
@@ -243,7 +257,7 @@ EXPORTS = (
     "vlb_upload_record_async vlb_upload_query vlb_upload_finish vlb_host_alloc vlb_host_free "
     "vlb_layer_set_hyper_connection vlb_layer_last_hyper_split "
     "vlb_int8_quantize_device vlb_int8_workspace_bytes vlb_int8_linear_device vlb_int8_status vlb_route_plan_device "
-    "vlb_balance_workspace_bytes vlb_balance_loss_device "
+    "vlb_balance_workspace_bytes vlb_balance_loss_device vlb_int8_linear_act_device "
     "vlb_add_rms_norm_device vlb_add_rms_norm_grad_workspace_bytes vlb_add_rms_norm_grad_device "
     "vlb_sort_tokens_workspace_bytes vlb_sort_tokens_device vlb_combine_device vlb_combine_grad_device"
 ).split()
@@ -326,6 +340,7 @@ def load_library() -> C.CDLL:
         "vlb_int8_quantize_device": (I, [P, I, P, U64, U64, P, P, F, U32, U32, P, U64, P, P]),
         "vlb_int8_workspace_bytes": (U64, [U32, U32]),
         "vlb_int8_linear_device": (I, [P, P, P]),
+        "vlb_int8_linear_act_device": (I, [P, P, P, P]),
         "vlb_int8_status": (I, [P, P]),
         "vlb_route_plan_device": (I, [P, P, P, U32, U32, U32, P, P, P, P, P, P]),
         "vlb_balance_workspace_bytes": (U64, [U32, U32, U32]),
@@ -699,6 +714,23 @@ class Device:
             self.h, _INT8_LINEAR_PACK(x_ptr, x_stride, x_rows, row_index_ptr, up_ptr, x_scale_ptr, row_weight_ptr, w.ptr,
                                       w.scale_ptr, w.stride, offsets_ptr, y_ptr, y_stride, ws_ptr, ws_bytes, rows,
                                       w.cols, w.rows, w.groups, x_type, y_type, swiglu_limit, 0), stream or None)
+        if st:
+            self._check(st)
+
+    def int8_linear_act_device(self, weights: Int8Weights, x_ptr: int, rows: int, y_ptr: int, *, act: int = ACT_NONE,
+                               act_limit: float = 0.0, bias_ptr: int = 0, residual_ptr: int = 0, residual_stride: int = 0,
+                               x_type: int = DTYPE_F32, y_type: int = DTYPE_F32, x_stride: int = 0, x_rows: int = 0,
+                               row_index_ptr: int = 0, up_ptr: int = 0, swiglu_limit: float = 0.0, x_scale_ptr: int = 0,
+                               row_weight_ptr: int = 0, offsets_ptr: int = 0, y_stride: int = 0, ws_ptr: int = 0,
+                               ws_bytes: int = 0, stream: int = 0) -> None:
+        """y = row_weight * act(x W^T + bias) + residual on 8-bit integers (vlb_int8_linear_act_device);
+        all else as int8_linear_device. ACT_SWIGLU halves y's columns."""
+        w = weights
+        st = self.lib.vlb_int8_linear_act_device(
+            self.h, _INT8_LINEAR_PACK(x_ptr, x_stride, x_rows, row_index_ptr, up_ptr, x_scale_ptr, row_weight_ptr, w.ptr,
+                                      w.scale_ptr, w.stride, offsets_ptr, y_ptr, y_stride, ws_ptr, ws_bytes, rows,
+                                      w.cols, w.rows, w.groups, x_type, y_type, swiglu_limit, 0),
+            _INT8_EPILOGUE_PACK(bias_ptr, residual_ptr, residual_stride, act, act_limit), stream or None)
         if st:
             self._check(st)
 

@@ -1763,14 +1763,16 @@ int vlb_int8_quantize_device(vlb_handle* h, int x_type, const void* x, uint64_t 
     })
 }
 
-int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void* stream) {
+// e: the epilogue, or null.
+static int int8_linear(vlb_handle* h, const vlb_int8_linear_desc* desc, const vlb_int8_epilogue* e, void* stream) {
     VLB_GUARDED({
         VLB_LOCK(h);
         if (!desc) return h->fail(VLB_ERR_INVALID_ARGUMENT, "int8 linear: null description");
         vlb_int8_linear_desc d = *desc;
         if (d.x_stride == 0) d.x_stride = d.cols;
         if (d.w_stride == 0) d.w_stride = d.cols;
-        if (d.y_stride == 0) d.y_stride = d.out_cols;
+        const uint32_t y_cols = e && e->act == VLB_ACT_SWIGLU ? d.out_cols / 2 : d.out_cols;
+        if (d.y_stride == 0) d.y_stride = y_cols;
         if (d.x_rows == 0) d.x_rows = d.rows;
         auto bad = [&](const char* why) { return h->fail(VLB_ERR_INVALID_ARGUMENT, std::string("int8 linear: ") + why); };
         if (d.cols == 0 || d.out_cols == 0 || d.groups == 0) return bad("cols, out_cols and groups must be positive");
@@ -1785,7 +1787,7 @@ int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void
         if (!aligned(d.w_scale, 4) || !aligned(d.x_scale, 4) || !aligned(d.row_weight, 4) || !aligned(d.offsets, 4) ||
             !aligned(d.y, dtype_size(d.y_type)))
             return bad("a pointer is not aligned to its elements");
-        if (d.w_stride < d.cols || d.y_stride < d.out_cols || d.w_stride > (1ull << 38) || d.y_stride > (1ull << 38))
+        if (d.w_stride < d.cols || d.y_stride < y_cols || d.w_stride > (1ull << 38) || d.y_stride > (1ull << 38))
             return bad("a stride is out of range");
         Int8LinearParams p{};
         p.row_weight = d.row_weight;
@@ -1800,6 +1802,21 @@ int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void
         p.cols = d.cols;
         p.out_cols = d.out_cols;
         p.groups = d.groups;
+        p.act = kInt8NoEpilogue;
+        if (e) {
+            if (e->act < VLB_ACT_NONE || e->act > VLB_ACT_SWIGLU) return bad("unknown activation");
+            if (e->act == VLB_ACT_SWIGLU && d.out_cols % 2) return bad("SWIGLU takes channels in pairs: out_cols must be even");
+            if (!(e->act_limit >= 0.f) || !std::isfinite(e->act_limit)) return bad("act_limit must be finite and not negative");
+            p.residual_stride = e->residual_stride ? e->residual_stride : y_cols;
+            if (!aligned(e->bias, 4) || !aligned(e->residual, dtype_size(d.y_type)))
+                return bad("a pointer is not aligned to its elements");
+            if (e->residual && (p.residual_stride < y_cols || p.residual_stride > (1ull << 38)))
+                return bad("a stride is out of range");
+            p.bias = e->bias;
+            p.residual = e->residual;
+            p.act = e->act;
+            p.act_limit = e->act_limit;
+        }
         cudaStream_t s = h->pick(stream);
         if (d.x_type == VLB_DTYPE_I8) {
             if (d.row_index || d.up) return bad("int8 rows take neither row_index nor up");
@@ -1866,6 +1883,21 @@ int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void
         VLB_CUDA(h, launch_int8_linear(p, d.y_type, d.x_type != VLB_DTYPE_I8, s));
         return VLB_OK;
     })
+}
+
+int vlb_int8_linear_device(vlb_handle* h, const vlb_int8_linear_desc* desc, void* stream) {
+    return int8_linear(h, desc, nullptr, stream);
+}
+
+int vlb_int8_linear_act_device(vlb_handle* h, const vlb_int8_linear_desc* desc, const vlb_int8_epilogue* epilogue,
+                               void* stream) {
+    if (!epilogue) {
+        VLB_GUARDED({
+            VLB_LOCK(h);
+            return h->fail(VLB_ERR_INVALID_ARGUMENT, "int8 linear: null epilogue");
+        })
+    }
+    return int8_linear(h, desc, epilogue, stream);
 }
 
 int vlb_int8_status(vlb_handle* h, void* stream) {

@@ -4,7 +4,8 @@
 //                a = max_c |x_rc|,  s_r = a / 127,  q_rc = rint(x_rc * (127 / a))
 //   linear     y_rn = (sum_k q_rk w_nk) * s_r * t_n, the sum exact in 32-bit integers
 //              (cols <= 131,071: 128 * 128 * cols < 2^31), for one matrix or grouped: row r uses
-//              the matrix of the group whose range [offsets[g], offsets[g + 1]) holds it.
+//              the matrix of the group whose range [offsets[g], offsets[g + 1]) holds it;
+//              with an epilogue y_rn = rw_r act(y_rn + b_n) + residual_rn, act also SwiGLU of channel pairs.
 //
 // The reference has no 8-bit integer path; the row scheme follows from the formulas above.
 #include <cuda_bf16.h>
@@ -34,6 +35,43 @@ __device__ __forceinline__ float swiglu(float g, float u, float limit) {
         u = u > limit ? limit : (u < -limit ? -limit : u);
     }
     return g * fast_rcp(1.f + fast_exp(fmaxf(fminf(-g, 88.f), -1000.f))) * u;
+}
+
+// ---- the products' epilogue ------------------------------------------------------------------
+//
+// z = sum * x_scale * w_scale + bias, y = row_weight * act(z) + residual, the same operations in the same
+// order in every form of the product.
+
+__device__ __forceinline__ float epi_sum(int32_t sum, float x_scale, float w_scale, float bias) {
+    return fmaf((float)sum * x_scale, w_scale, bias);
+}
+
+// z Phi(z) with erfc by Abramowitz and Stegun's 7.1.26 (|error| <= 1.5e-7): erfc(x) = (a1 t + .. + a5 t^5)
+// e^(-x^2), t = 1 / (1 + p x), x = |z| / sqrt(2) >= 0. In 32 bits the polynomial adds up to 10 units of 2^-24
+// (its terms' magnitudes sum to 4.5): z Phi(z) within 2^-20 |z|. CUDA's erfcf takes five times the
+// instructions, which a tile's epilogue does not have.
+__device__ __forceinline__ float gelu(float z) {
+    const float x = fabsf(z) * 0.707106781f;
+    const float t = fast_rcp(fmaf(0.3275911f, x, 1.f));
+    float c = fmaf(t, 1.061405429f, -1.453152027f);
+    c = fmaf(t, c, 1.421413741f);
+    c = fmaf(t, c, -0.284496736f);
+    c = fmaf(t, c, 0.254829592f);
+    const float tail = 0.5f * (c * t) * fast_exp(fmaxf(-x * x, -1000.f));  // Phi(-|z|)
+    return z * (z > 0.f ? 1.f - tail : tail);
+}
+
+// sigmoid(v): of SiLU, and of GELU's tanh form, (1 + tanh(u)) / 2 = sigmoid(2 u).
+__device__ __forceinline__ float sigmoid_of(float v) { return fast_rcp(1.f + fast_exp(fmaxf(fminf(-v, 88.f), -1000.f))); }
+
+__device__ __forceinline__ float activate(float z, int act) {
+    switch (act) {
+        case VLB_ACT_RELU: return z < 0.f ? 0.f : z;  // keeps a NaN
+        case VLB_ACT_SILU: return z * sigmoid_of(z);
+        case VLB_ACT_GELU: return gelu(z);
+        case VLB_ACT_GELU_TANH: return z * sigmoid_of(1.59576912f * fmaf(0.044715f * z * z, z, z));  // 2 sqrt(2 / pi)
+        default: return z;
+    }
 }
 
 // ---- row quantizer ---------------------------------------------------------------------------
@@ -326,7 +364,7 @@ __device__ __forceinline__ uint32_t load_word(const int8_t* row, uint32_t c, uin
     return v;
 }
 
-template <typename TY>
+template <typename TY, bool EPI>
 __global__ void __launch_bounds__(256) int8_linear_kernel(const Int8LinearParams p) {
     __shared__ uint32_t xs[kGenTile][kGenK / 4 + 1], ws[kGenTile][kGenK / 4 + 1];
     tc::grid_dependency_wait();
@@ -359,6 +397,26 @@ __global__ void __launch_bounds__(256) int8_linear_kernel(const Int8LinearParams
 #pragma unroll
             for (uint32_t i = 0; i < 4u; ++i) {
                 const uint32_t r = r0 + tr + 16u * i;
+                if constexpr (EPI) {
+                    const bool pairs = p.act == VLB_ACT_SWIGLU, have = r < hi;
+                    const float s = have ? p.x_scale[r] : 0.f, rw = have && p.row_weight ? p.row_weight[r] : 1.f;
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; ++j) {
+                        const uint32_t n = n0 + tc + 16u * j;
+                        const size_t at = (size_t)g * p.out_cols + n;
+                        const bool in = n < p.out_cols;
+                        const float z = epi_sum(acc[i][j], s, in ? p.w_scale[at] : 0.f, in && p.bias ? p.bias[at] : 0.f);
+                        const float up = __shfl_xor_sync(0xffffffffu, z, 1);  // of a pair's gate: channel n + 1
+                        if (!have || !in || (pairs && (n & 1u))) continue;
+                        const uint32_t c = pairs ? n / 2u : n;
+                        const float a = pairs ? swiglu(z, up, p.act_limit) : activate(z, p.act);
+                        const float res = p.residual
+                                              ? to_float(static_cast<const TY*>(p.residual)[(size_t)r * p.residual_stride + c])
+                                              : 0.f;
+                        static_cast<TY*>(p.y)[(size_t)r * p.y_stride + c] = from_float<TY>(fmaf(rw, a, res));
+                    }
+                    continue;
+                }
                 if (r >= hi) continue;
                 const float s = p.row_weight ? p.x_scale[r] * p.row_weight[r] : p.x_scale[r];
 #pragma unroll
@@ -399,6 +457,11 @@ __device__ __forceinline__ uint4 few_load(const int8_t* row, uint32_t k, uint32_
                       load_word(row, k + 12u, cols));
 }
 
+__device__ __forceinline__ float load_typed(const void* y, size_t at, int type) {
+    if (type == VLB_DTYPE_F32) return static_cast<const float*>(y)[at];
+    if (type == VLB_DTYPE_F16) return __half2float(static_cast<const __half*>(y)[at]);
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(y)[at]);
+}
 __device__ __forceinline__ void store_typed(void* y, size_t at, float v, int type) {
     if (type == VLB_DTYPE_F32) static_cast<float*>(y)[at] = v;
     else if (type == VLB_DTYPE_F16) static_cast<__half*>(y)[at] = __float2half_rn(v);
@@ -406,7 +469,7 @@ __device__ __forceinline__ void store_typed(void* y, size_t at, float v, int typ
 }
 
 // T: the rows' type, int8_t for rows that are integers already. ROWS: rows of a block.
-template <typename T, uint32_t ROWS>
+template <typename T, uint32_t ROWS, bool EPI>
 __global__ void __launch_bounds__(kFewThreads, few_blocks(ROWS)) int8_few_kernel(const Int8LinearParams l, const Int8QuantParams q, int y_type,
                                                                uint32_t channels) {
     constexpr uint32_t kFewPieces = few_pieces(ROWS);
@@ -452,7 +515,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(ROWS)) int8_few_kernel
     const uint32_t r = row0 + m;
     int8_t* xs = reinterpret_cast<int8_t*>(few_smem);
     if constexpr (std::is_same<T, int8_t>::value) {
-        if (m < rows && part == 0) scale[m] = l.row_weight ? l.x_scale[r] * l.row_weight[r] : l.x_scale[r];
+        if (m < rows && part == 0) scale[m] = !EPI && l.row_weight ? l.x_scale[r] * l.row_weight[r] : l.x_scale[r];
         for (uint32_t c = part * 16u; c < pitch; c += row_warps * 512u)
             *reinterpret_cast<uint4*>(xs + m * pitch + c) =
                 m < rows ? few_load(l.x + (size_t)r * l.x_stride, c, l.cols) : make_uint4(0u, 0u, 0u, 0u);
@@ -472,7 +535,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(ROWS)) int8_few_kernel
         if (lane == 0) atomicMax(top + m, most);
         __syncthreads();
         const RowStep st = row_step(top[m]);
-        if (m < rows && part == 0) scale[m] = l.row_weight ? st.scale * l.row_weight[r] : st.scale;
+        if (m < rows && part == 0) scale[m] = !EPI && l.row_weight ? st.scale * l.row_weight[r] : st.scale;
 #pragma unroll 8
         for (uint32_t c = part; c < pitch; c += row_warps * 32u)
             xs[m * pitch + c] = (int8_t)(have && c < l.cols ? quant_byte(value(c), st) : 0u);
@@ -505,16 +568,32 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(ROWS)) int8_few_kernel
                 }
             }
         }
-        // lane c * ROWS + j stores row j of channel c
-        int32_t mine = 0;
+        // lane c * ROWS + j stores row j of channel c; of a SwiGLU pair, lane j
+        int32_t mine = 0, second = 0;
 #pragma unroll
         for (uint32_t c = 0; c < 2u; ++c)
 #pragma unroll
             for (uint32_t j = 0; j < ROWS; ++j) {
                 const int32_t v = __reduce_add_sync(0xffffffffu, sum[c][j]);
                 if (lane == c * ROWS + j) mine = v;
+                if (EPI && c == 1u && lane == j) second = v;
             }
         const uint32_t c = n + lane / ROWS, j = lane % ROWS;
+        if constexpr (EPI) {
+            const bool pairs = l.act == VLB_ACT_SWIGLU;
+            if (lane < (pairs ? 1u : 2u) * ROWS && j < rows && c < n_end) {
+                const size_t at = (size_t)g * l.out_cols + c, r = row0 + j;
+                float a = epi_sum(mine, scale[j], l.w_scale[at], l.bias ? l.bias[at] : 0.f);
+                if (pairs)
+                    a = swiglu(a, epi_sum(second, scale[j], l.w_scale[at + 1u], l.bias ? l.bias[at + 1u] : 0.f), l.act_limit);
+                else
+                    a = activate(a, l.act);
+                const uint32_t to = pairs ? c / 2u : c;
+                const float res = l.residual ? load_typed(l.residual, r * l.residual_stride + to, y_type) : 0.f;
+                store_typed(l.y, r * l.y_stride + to, fmaf(l.row_weight ? l.row_weight[r] : 1.f, a, res), y_type);
+            }
+            continue;
+        }
         if (lane < 2u * ROWS && j < rows && c < n_end)
             store_typed(l.y, (size_t)(row0 + j) * l.y_stride + c,
                         (float)mine * scale[j] * l.w_scale[(size_t)g * l.out_cols + c], y_type);
@@ -567,6 +646,8 @@ struct MmShared {
     uint32_t* cnt;    // [groups] rows
     float* scale;     // [2][256] the tile's token scales
     float* channel;   // [2][128] its channels'
+    float* weight;    // with an epilogue: [2][256] the tokens' row weights,
+    float* bias;      // [2][128] the channels' biases
     MmTile* tile;     // [2]
     uint64_t *full, *empty, *acc_full, *acc_empty, *tile_full, *tile_empty;
     uint32_t* tmem;
@@ -574,8 +655,8 @@ struct MmShared {
 };
 
 __host__ __device__ constexpr uint32_t mm_table_bytes(uint32_t groups) { return (3u * groups + 1u) * 4u; }
-__host__ __device__ constexpr uint32_t mm_fixed_bytes(uint32_t groups) {
-    return 2u * (kMmMaxTokens + kMmChannels) * 4u + 2u * 16u + (2u * kMmMaxStages + 8u) * 8u + 16u + mm_table_bytes(groups) +
+__host__ __device__ constexpr uint32_t mm_fixed_bytes(uint32_t groups, bool epi) {
+    return (epi ? 4u : 2u) * (kMmMaxTokens + kMmChannels) * 4u + 2u * 16u + (2u * kMmMaxStages + 8u) * 8u + 16u + mm_table_bytes(groups) +
            16u;
 }
 
@@ -627,7 +708,7 @@ __device__ __forceinline__ MmTile mm_tile(const MmShared& sh, const Int8MmaParam
     return MmTile{a, sh.lo[a] + j * each + min(j, more), each + (j < more ? 1u : 0u), c * p.channels};
 }
 
-template <typename TY, Mm MODE>
+template <typename TY, Mm MODE, bool EPI>
 __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_constant__ Int8MmaParams p) {
     constexpr bool SPLIT = MODE == Mm::kSplit, PAIR = MODE == Mm::kPair;
     extern __shared__ __align__(1024) unsigned char mm_smem[];
@@ -639,7 +720,9 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         unsigned char* at = mm_smem + p.stages * stage_bytes;
         sh.scale = reinterpret_cast<float*>(at);
         sh.channel = sh.scale + 2u * kMmMaxTokens;
-        sh.tile = reinterpret_cast<MmTile*>(sh.channel + 2u * kMmChannels);
+        sh.weight = sh.channel + 2u * kMmChannels;
+        sh.bias = sh.weight + 2u * kMmMaxTokens;
+        sh.tile = reinterpret_cast<MmTile*>(EPI ? sh.bias + 2u * kMmChannels : sh.weight);
         sh.full = reinterpret_cast<uint64_t*>(sh.tile + 2);
         sh.empty = sh.full + kMmMaxStages;
         sh.acc_full = sh.empty + kMmMaxStages;
@@ -825,28 +908,78 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
             tc::grid_dependency_wait();
             waited = true;
         }
-        float ts[kMmMaxTokens / 32u], cs[kMmChannels / 32u];
+        float ts[kMmMaxTokens / 32u], cs[kMmChannels / 32u], rw[EPI ? kMmMaxTokens / 32u : 1u], bs[EPI ? kMmChannels / 32u : 1u];
 #pragma unroll
         for (uint32_t i = 0; i < kMmMaxTokens / 32u; ++i) {
             const uint32_t j = lane + 32u * i;
             ts[i] = j < tile.count ? l.x_scale[tile.row0 + j] : 0.f;
-            if (l.row_weight && j < tile.count) ts[i] *= l.row_weight[tile.row0 + j];
+            if constexpr (EPI) rw[i] = l.row_weight && j < tile.count ? l.row_weight[tile.row0 + j] : 1.f;
+            else if (l.row_weight && j < tile.count) ts[i] *= l.row_weight[tile.row0 + j];
         }
 #pragma unroll
         for (uint32_t i = 0; i < kMmChannels / 32u; ++i) {
             const uint32_t n = tile.channel0 + (PAIR ? rank * kMmChannels : 0u) + lane + 32u * i;
             cs[i] = n < l.out_cols ? l.w_scale[(size_t)tile.g * l.out_cols + n] : 0.f;
+            if constexpr (EPI) bs[i] = l.bias && n < l.out_cols ? l.bias[(size_t)tile.g * l.out_cols + n] : 0.f;
         }
         if (!__all_sync(0xffffffffu, mm_wait(sh.tile_empty + buf, (use & 1u) ^ 1u, sh.abort))) return false;
 #pragma unroll
         for (uint32_t i = 0; i < kMmMaxTokens / 32u; ++i) sh.scale[buf * kMmMaxTokens + lane + 32u * i] = ts[i];
 #pragma unroll
         for (uint32_t i = 0; i < kMmChannels / 32u; ++i) sh.channel[buf * kMmChannels + lane + 32u * i] = cs[i];
+        if constexpr (EPI) {
+#pragma unroll
+            for (uint32_t i = 0; i < kMmMaxTokens / 32u; ++i) sh.weight[buf * kMmMaxTokens + lane + 32u * i] = rw[i];
+#pragma unroll
+            for (uint32_t i = 0; i < kMmChannels / 32u; ++i) sh.bias[buf * kMmChannels + lane + 32u * i] = bs[i];
+        }
         if (lane == 0) sh.tile[buf] = tile;
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(sh.tile_full + buf);
         ++it;
         return true;
+    };
+    // 32 tokens from c on of channel n, with an epilogue; the whole warp. Of SwiGLU's pairs (neighbouring
+    // lanes) the even lane takes the even tokens, the odd lane the odd ones, against one exchange for two.
+    [[maybe_unused]] auto finish = [&](const uint32_t (&v)[32], const MmTile& tile, uint32_t c, uint32_t n, const float* ts,
+                                       const float* rw, float cs, float bias) {
+        const TY* from = static_cast<const TY*>(l.residual);
+        TY* y = static_cast<TY*>(l.y);
+        if (l.act == VLB_ACT_SWIGLU) {
+            const uint32_t odd = lane & 1u;
+            const bool in = n < l.out_cols;
+            TY res[16];
+#pragma unroll
+            for (uint32_t i = 0; i < 16u; ++i) {
+                const uint32_t j = c + 2u * i + odd;
+                res[i] = from_float<TY>(0.f);
+                if (from && in && j < tile.count) res[i] = from[(size_t)(tile.row0 + j) * l.residual_stride + n / 2u];
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 16u; ++i) {
+                const uint32_t j = c + 2u * i;
+                const float z0 = epi_sum((int32_t)v[2 * i], ts[j], cs, bias);
+                const float z1 = epi_sum((int32_t)v[2 * i + 1], ts[j + 1u], cs, bias);
+                const float other = __shfl_xor_sync(0xffffffffu, odd ? z0 : z1, 1);
+                const float a = odd ? swiglu(other, z1, l.act_limit) : swiglu(z0, other, l.act_limit);
+                if (in && j + odd < tile.count)
+                    y[(size_t)(tile.row0 + j + odd) * l.y_stride + n / 2u] = from_float<TY>(fmaf(rw[j + odd], a, to_float(res[i])));
+            }
+            return;
+        }
+        if (n >= l.out_cols) return;
+        TY res[32];
+#pragma unroll
+        for (uint32_t i = 0; i < 32u; ++i) {
+            res[i] = from_float<TY>(0.f);
+            if (from && c + i < tile.count) res[i] = from[(size_t)(tile.row0 + c + i) * l.residual_stride + n];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 32u; ++i) {
+            const float a = activate(epi_sum((int32_t)v[i], ts[c + i], cs, bias), l.act);
+            if (c + i < tile.count)
+                y[(size_t)(tile.row0 + c + i) * l.y_stride + n] = from_float<TY>(fmaf(rw[c + i], a, to_float(res[i])));
+        }
     };
     auto epilogue = [&]() -> bool {
         const uint32_t buf = it & 1u, use = it >> 1;
@@ -866,7 +999,9 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
                 tc::tmem_wait_ld();
                 TY* y = static_cast<TY*>(l.y) + (size_t)(tile.row0 + c) * l.y_stride + n;
                 const float4* t4 = reinterpret_cast<const float4*>(ts + c);
-                if (tile.count - c >= 32u && n - lane + 32u <= l.out_cols) {
+                if constexpr (EPI) {
+                    finish(v, tile, c, n, ts, sh.weight + buf * kMmMaxTokens, cs, sh.bias[buf * kMmChannels + 32u * quad + lane]);
+                } else if (tile.count - c >= 32u && n - lane + 32u <= l.out_cols) {
 #pragma unroll
                     for (uint32_t i = 0; i < 32u; i += 4u) {
                         const float4 t = t4[i / 4u];
@@ -930,7 +1065,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
             // role has given up
             const MmTile tile = mm_tile(sh, p, t);
             bool ok = true;
-            float cs[4] = {};
+            float cs[4] = {}, bs[4] = {};
             float* ts = sh.scale;
             if (warp == kMmEpiWarps) {
                 ok = __all_sync(0xffffffffu, *sh.abort == 0) && produce(t);
@@ -943,7 +1078,8 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
                 }
                 if (tid < tile.count) {
                     const uint32_t r = tile.row0 + tid;
-                    ts[tid] = l.row_weight ? l.x_scale[r] * l.row_weight[r] : l.x_scale[r];
+                    ts[tid] = !EPI && l.row_weight ? l.x_scale[r] * l.row_weight[r] : l.x_scale[r];
+                    if constexpr (EPI) sh.weight[tid] = l.row_weight ? l.row_weight[r] : 1.f;
                 }
                 ok = __all_sync(0xffffffffu, *sh.abort == 0 && mm_wait(sh.acc_full, it & 1u, sh.abort));
                 ++it;
@@ -951,6 +1087,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
                 for (uint32_t i = 0; i < 4u; ++i) {
                     const uint32_t n = tile.channel0 + 4u * lane + i;
                     cs[i] = n < l.out_cols ? l.w_scale[(size_t)tile.g * l.out_cols + n] : 0.f;
+                    if (EPI && l.bias && n < l.out_cols) bs[i] = l.bias[(size_t)tile.g * l.out_cols + n];
                 }
                 if (ok) {
                     tc::fence_after_sync();
@@ -990,6 +1127,24 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
                         for (uint32_t r = 1; r < 8u; ++r)
                             sum.x += v[u][r].x, sum.y += v[u][r].y, sum.z += v[u][r].z, sum.w += v[u][r].w;
                         const float s = ts[j + u * pace];
+                        if constexpr (EPI) {
+                            const bool pairs = l.act == VLB_ACT_SWIGLU;
+                            const size_t r = tile.row0 + j + u * pace;
+                            const float rw = sh.weight[j + u * pace];
+                            const TY* from = static_cast<const TY*>(l.residual);
+                            float z[4];
+#pragma unroll
+                            for (uint32_t i = 0; i < 4u; ++i) z[i] = epi_sum((int32_t)(&sum.x)[i], s, cs[i], bs[i]);
+#pragma unroll
+                            for (uint32_t i = 0; i < 4u; ++i) {
+                                if (n + i >= l.out_cols || (pairs && (i & 1u))) continue;
+                                const uint32_t to = pairs ? (n + i) / 2u : n + i;
+                                const float a = pairs ? swiglu(z[i], z[i | 1u], l.act_limit) : activate(z[i], l.act);
+                                const float res = from ? to_float(from[r * l.residual_stride + to]) : 0.f;
+                                static_cast<TY*>(l.y)[r * l.y_stride + to] = from_float<TY>(fmaf(rw, a, res));
+                            }
+                            continue;
+                        }
                         TY* y = static_cast<TY*>(l.y) + (size_t)(tile.row0 + j + u * pace) * l.y_stride + n;
 #pragma unroll
                         for (uint32_t i = 0; i < 4u; ++i)
@@ -1059,11 +1214,11 @@ cudaError_t quantize_type(const Int8QuantParams& p, cudaStream_t s) {
     return p.up ? quantize_rows<T, true>(p, s) : quantize_rows<T, false>(p, s);
 }
 
-template <typename TY>
+template <typename TY, bool EPI>
 cudaError_t general_type(const Int8LinearParams& p, cudaStream_t s) {
     const uint32_t tiles_n = (p.out_cols + kGenTile - 1u) / kGenTile, tiles_r = (p.rows + kGenTile - 1u) / kGenTile;
     const dim3 grid(tiles_n, tiles_r < 1024u ? tiles_r : 1024u, p.groups < 1024u ? p.groups : 1024u);
-    return launch_chained(int8_linear_kernel<TY>, grid, 256, 0, 0, s, p);
+    return launch_chained(int8_linear_kernel<TY, EPI>, grid, 256, 0, 0, s, p);
 }
 
 // Opts a kernel in to `bytes` of shared memory, once on each device.
@@ -1188,19 +1343,19 @@ Mm mma_plan(Int8MmaParams& p, uint32_t sms) {
     p.acc_cols = p.width < 32u ? 32u : p.width;
     p.tmem_cols = 32;
     while (p.tmem_cols < (mode == Mm::kSplit ? 1u : 2u) * p.acc_cols) p.tmem_cols *= 2u;
-    const uint32_t room = kMmSmemLimit - 1024u - mm_fixed_bytes(l.groups);
+    const uint32_t room = kMmSmemLimit - 1024u - mm_fixed_bytes(l.groups, l.act != kInt8NoEpilogue);
     p.stages = room / (kMmWStage + p.x_stage);
     if (p.stages > kMmMaxStages) p.stages = kMmMaxStages;
     return mode;
 }
 
-template <typename TY, Mm MODE>
+template <typename TY, Mm MODE, bool EPI>
 cudaError_t mma_launch(const Int8MmaParams& p, uint32_t sms, cudaStream_t s) {
-    auto* kernel = int8_mma_kernel<TY, MODE>;
+    auto* kernel = int8_mma_kernel<TY, MODE, EPI>;
     const uint32_t in_cluster = MODE == Mm::kSplit ? p.split : MODE == Mm::kPair ? 2u : 1u;
     cudaError_t e = smem_once(kernel, kMmSmemLimit);
     if (e != cudaSuccess) return e;
-    const size_t smem = p.stages * (kMmWStage + p.x_stage) + mm_fixed_bytes(p.l.groups);
+    const size_t smem = p.stages * (kMmWStage + p.x_stage) + mm_fixed_bytes(p.l.groups, EPI);
     return launch_chained(kernel, dim3(sms / in_cluster * in_cluster), kMmThreads, smem, MODE == Mm::kOne ? 0 : in_cluster, s, p);
 }
 
@@ -1225,9 +1380,9 @@ uint32_t sm_count() {
 constexpr uint32_t kFewRows = 8, kFewGroupedRows = 24, kFewElements = 8192;
 constexpr uint64_t kFewWork = 1u << 24;
 
-template <typename T, uint32_t ROWS>
+template <typename T, uint32_t ROWS, bool EPI>
 cudaError_t few_launch(const Int8LinearParams& l, const Int8QuantParams& q, int y_type, uint32_t sms, cudaStream_t s) {
-    auto* kernel = int8_few_kernel<T, ROWS>;
+    auto* kernel = int8_few_kernel<T, ROWS, EPI>;
     const size_t smem = (size_t)ROWS * ((l.cols + 15u) / 16u * 16u);
     if (smem > kFewDefaultSmem) {
         const cudaError_t e = smem_once(kernel, kFewSmem);
@@ -1240,16 +1395,16 @@ cudaError_t few_launch(const Int8LinearParams& l, const Int8QuantParams& q, int 
                           channels);
 }
 
-template <typename T>
+template <typename T, bool EPI>
 cudaError_t few_rows(const Int8LinearParams& l, const Int8QuantParams& q, int y_type, cudaStream_t s) {
     const uint32_t rows = l.offsets ? 1u : l.rows, sms = sm_count();
-    if (rows <= 1u) return few_launch<T, 1>(l, q, y_type, sms, s);
-    if (rows <= 2u) return few_launch<T, 2>(l, q, y_type, sms, s);
-    if (rows <= 4u) return few_launch<T, 4>(l, q, y_type, sms, s);
-    return few_launch<T, 8>(l, q, y_type, sms, s);
+    if (rows <= 1u) return few_launch<T, 1, EPI>(l, q, y_type, sms, s);
+    if (rows <= 2u) return few_launch<T, 2, EPI>(l, q, y_type, sms, s);
+    if (rows <= 4u) return few_launch<T, 4, EPI>(l, q, y_type, sms, s);
+    return few_launch<T, 8, EPI>(l, q, y_type, sms, s);
 }
 
-template <typename TY>
+template <typename TY, bool EPI>
 cudaError_t linear_type(const Int8LinearParams& l, bool after_quantize, cudaStream_t s) {
     if (tma_rows(l.w, l.w_stride) && tma_rows(l.x, l.x_stride)) {
         Int8MmaParams p{};
@@ -1259,11 +1414,11 @@ cudaError_t linear_type(const Int8LinearParams& l, bool after_quantize, cudaStre
         const Mm mode = mma_plan(p, sms);
         if (encode_rows(&p.wmap, l.w, (uint64_t)l.groups * l.out_cols, l.cols, l.w_stride, kMmChannels) &&
             encode_rows(&p.xmap, l.x, l.rows, l.cols, l.x_stride, p.box))
-            return mode == Mm::kPair    ? mma_launch<TY, Mm::kPair>(p, sms, s)
-                   : mode == Mm::kSplit ? mma_launch<TY, Mm::kSplit>(p, sms, s)
-                                        : mma_launch<TY, Mm::kOne>(p, sms, s);
+            return mode == Mm::kPair    ? mma_launch<TY, Mm::kPair, EPI>(p, sms, s)
+                   : mode == Mm::kSplit ? mma_launch<TY, Mm::kSplit, EPI>(p, sms, s)
+                                        : mma_launch<TY, Mm::kOne, EPI>(p, sms, s);
     }
-    return general_type<TY>(l, s);
+    return general_type<TY, EPI>(l, s);
 }
 
 }  // namespace
@@ -1292,22 +1447,31 @@ bool int8_few(const Int8LinearParams& l) {
     return (size_t)rows * ((l.cols + 15u) / 16u * 16u) <= kFewSmem;
 }
 
-cudaError_t launch_int8_few(const Int8LinearParams& l, const Int8QuantParams& q, int x_type, int y_type, cudaStream_t s) {
+template <bool EPI>
+static cudaError_t few_typed(const Int8LinearParams& l, const Int8QuantParams& q, int x_type, int y_type, cudaStream_t s) {
     switch (x_type) {
-        case VLB_DTYPE_F32: return few_rows<float>(l, q, y_type, s);
-        case VLB_DTYPE_F16: return few_rows<__half>(l, q, y_type, s);
-        case VLB_DTYPE_BF16: return few_rows<__nv_bfloat16>(l, q, y_type, s);
-        default: return few_rows<int8_t>(l, q, y_type, s);
+        case VLB_DTYPE_F32: return few_rows<float, EPI>(l, q, y_type, s);
+        case VLB_DTYPE_F16: return few_rows<__half, EPI>(l, q, y_type, s);
+        case VLB_DTYPE_BF16: return few_rows<__nv_bfloat16, EPI>(l, q, y_type, s);
+        default: return few_rows<int8_t, EPI>(l, q, y_type, s);
     }
 }
+cudaError_t launch_int8_few(const Int8LinearParams& l, const Int8QuantParams& q, int x_type, int y_type, cudaStream_t s) {
+    return l.act == kInt8NoEpilogue ? few_typed<false>(l, q, x_type, y_type, s) : few_typed<true>(l, q, x_type, y_type, s);
+}
 
-cudaError_t launch_int8_linear(const Int8LinearParams& p, int y_type, bool after_quantize, cudaStream_t s) {
+template <bool EPI>
+static cudaError_t linear_typed(const Int8LinearParams& p, int y_type, bool after_quantize, cudaStream_t s) {
     switch (y_type) {
-        case VLB_DTYPE_F32: return linear_type<float>(p, after_quantize, s);
-        case VLB_DTYPE_F16: return linear_type<__half>(p, after_quantize, s);
-        case VLB_DTYPE_BF16: return linear_type<__nv_bfloat16>(p, after_quantize, s);
+        case VLB_DTYPE_F32: return linear_type<float, EPI>(p, after_quantize, s);
+        case VLB_DTYPE_F16: return linear_type<__half, EPI>(p, after_quantize, s);
+        case VLB_DTYPE_BF16: return linear_type<__nv_bfloat16, EPI>(p, after_quantize, s);
         default: return cudaErrorInvalidValue;
     }
+}
+cudaError_t launch_int8_linear(const Int8LinearParams& p, int y_type, bool after_quantize, cudaStream_t s) {
+    return p.act == kInt8NoEpilogue ? linear_typed<false>(p, y_type, after_quantize, s)
+                                    : linear_typed<true>(p, y_type, after_quantize, s);
 }
 
 }  // namespace vlb

@@ -131,7 +131,14 @@ struct Int8LinearParams {
     uint32_t* error;           // the handle's word in host memory: 1 once a wait has run out
     size_t x_stride, w_stride, y_stride;
     uint32_t rows, cols, out_cols, groups;
+    // the epilogue of vlb_int8_linear_act_device; act < 0: none of it
+    const float* bias;         // [groups x out_cols] or null
+    const void* residual;      // rows of y's type or null
+    size_t residual_stride;
+    int act;
+    float act_limit;
 };
+constexpr int kInt8NoEpilogue = -1;
 constexpr uint32_t kInt8MaxGroups = 1024;
 cudaError_t launch_int8_gather(const Int8GatherParams& p, cudaStream_t s);
 cudaError_t launch_int8_quantize(const Int8QuantParams& p, int x_type, cudaStream_t s);
