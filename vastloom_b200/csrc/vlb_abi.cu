@@ -2061,6 +2061,7 @@ int vlb_add_rms_norm_device(vlb_handle* h, const vlb_add_rms_norm_desc* desc, vo
         p.rows = d.rows;
         p.cols = d.cols;
         p.eps = d.eps;
+        p.share = 1.f / (float)d.cols;
         VLB_CUDA(h, launch_add_norm(p, d.type, d.residual_type, h->pick(stream)));
         return VLB_OK;
     })
@@ -2119,6 +2120,7 @@ int vlb_add_rms_norm_grad_device(vlb_handle* h, const vlb_add_rms_norm_grad_desc
         p.rows = d.rows;
         p.cols = d.cols;
         p.eps = d.eps;
+        p.share = 1.f / (float)d.cols;
         VLB_CUDA(h, launch_add_norm_grad(p, d.type, d.residual_type, s));
         return VLB_OK;
     })

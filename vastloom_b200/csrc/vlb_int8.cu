@@ -12,11 +12,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <atomic>
 #include <mutex>
 #include <type_traits>
-#include <utility>
-#include <vector>
 
 #include "vlb_launch.h"
 #include "vlb_math.cuh"
@@ -1221,22 +1218,6 @@ cudaError_t general_type(const Int8LinearParams& p, cudaStream_t s) {
     return launch_chained(int8_linear_kernel<TY, EPI>, grid, 256, 0, 0, s, p);
 }
 
-// Opts a kernel in to `bytes` of shared memory, once on each device.
-template <typename K>
-cudaError_t smem_once(K kernel, size_t bytes) {
-    static std::mutex mu;
-    static std::vector<std::pair<int, const void*>> done;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    std::lock_guard<std::mutex> lock(mu);
-    for (auto& d : done)
-        if (d.first == dev && d.second == (const void*)kernel) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess) done.emplace_back(dev, (const void*)kernel);
-    return e;
-}
-
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -1357,17 +1338,6 @@ cudaError_t mma_launch(const Int8MmaParams& p, uint32_t sms, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const size_t smem = p.stages * (kMmWStage + p.x_stage) + mm_fixed_bytes(p.l.groups, EPI);
     return launch_chained(kernel, dim3(sms / in_cluster * in_cluster), kMmThreads, smem, MODE == Mm::kOne ? 0 : in_cluster, s, p);
-}
-
-// SMs of the current device; handles of several devices and threads may ask at once.
-uint32_t sm_count() {
-    static std::atomic<uint32_t> known[64];
-    int dev = 0, v = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 148u;
-    if (dev < 64 && (v = (int)known[dev].load(std::memory_order_relaxed)) > 0) return (uint32_t)v;
-    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) return 148u;
-    if (dev < 64) known[dev].store((uint32_t)v, std::memory_order_relaxed);
-    return (uint32_t)v;
 }
 
 // What int8_few_kernel takes. Dense: up to kFewRows rows, from 3 on no more than kFewElements elements

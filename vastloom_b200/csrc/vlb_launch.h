@@ -3,6 +3,11 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
+#include <mutex>
+#include <utility>
+#include <vector>
+
 #include "vlb_internal.cuh"
 
 namespace vlb {
@@ -98,6 +103,33 @@ cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, uint32_t block, size
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
+// Opts a kernel in to `bytes` of shared memory, once on each device.
+template <typename K>
+inline cudaError_t smem_once(K kernel, size_t bytes) {
+    static std::mutex mu;
+    static std::vector<std::pair<int, const void*>> done;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mu);
+    for (auto& d : done)
+        if (d.first == dev && d.second == (const void*)kernel) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done.emplace_back(dev, (const void*)kernel);
+    return e;
+}
+
+// SMs of the current device; handles of several devices and threads may ask at once.
+inline uint32_t sm_count() {
+    static std::atomic<uint32_t> known[64];
+    int dev = 0, v = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 148u;
+    if (dev < 64 && (v = (int)known[dev].load(std::memory_order_relaxed)) > 0) return (uint32_t)v;
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) return 148u;
+    if (dev < 64) known[dev].store((uint32_t)v, std::memory_order_relaxed);
+    return (uint32_t)v;
+}
+
 // ---- products on 8-bit integers (vlb_int8.cu) ----
 struct Int8QuantParams {
     const void* x;             // rows of VLB_DTYPE_F32 / F16 / BF16
@@ -185,7 +217,7 @@ struct NormParams {
     float* scale;
     size_t x_stride, residual_stride, h_stride, y_stride, q_stride;
     uint32_t rows, cols;
-    float eps;
+    float eps, share;          // share: 1 / cols
 };
 struct NormGradParams {
     const void* dy;
@@ -199,7 +231,7 @@ struct NormGradParams {
     float4* row;               // workspace, for dw: the rows' (lift, s, mean(g n))
     size_t dy_stride, h_stride, dh_stride, dx_stride, dres_stride;
     uint32_t rows, cols;
-    float eps;
+    float eps, share;          // share: 1 / cols
 };
 constexpr uint32_t kNormParts = 444;
 cudaError_t launch_add_norm(const NormParams& p, int type, int residual_type, cudaStream_t s);

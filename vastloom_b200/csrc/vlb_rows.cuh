@@ -5,6 +5,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace vlb {
 
 // ---- elements --------------------------------------------------------------------------------
@@ -44,12 +46,46 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p, uint32_t n) {
     }
     return a;
 }
+// Two elements an instruction, or a shift and a mask, where they come in pairs.
+template <uint32_t V, typename T>
+__device__ __forceinline__ void unpack(const Pack<T, V>& a, float (&f)[V]) {
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < V; i += 2) {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(&a)[i / 2];
+            if constexpr (std::is_same<T, __half>::value) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+                f[i] = v.x, f[i + 1] = v.y;
+            } else {
+                f[i] = __uint_as_float(w << 16), f[i + 1] = __uint_as_float(w & 0xffff0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) f[i] = to_float(a.v[i]);
+    }
+}
+template <typename T, uint32_t V>
+__device__ __forceinline__ Pack<T, V> pack(const float (&f)[V]) {
+    Pack<T, V> a;
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < V; i += 2) {
+            if constexpr (std::is_same<T, __half>::value)
+                *reinterpret_cast<__half2*>(&a.v[i]) = __floats2half2_rn(f[i], f[i + 1]);
+            else
+                *reinterpret_cast<__nv_bfloat162*>(&a.v[i]) = __floats2bfloat162_rn(f[i], f[i + 1]);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) a.v[i] = from_float<T>(f[i]);
+    }
+    return a;
+}
 // Rounds V values to the first n elements at p.
 template <uint32_t V, typename T>
 __device__ __forceinline__ void store_pack(T* p, const float (&f)[V], uint32_t n) {
-    Pack<T, V> a;
-#pragma unroll
-    for (uint32_t i = 0; i < V; ++i) a.v[i] = from_float<T>(f[i]);
+    const Pack<T, V> a = pack<T>(f);
     if (n >= V) {
         *reinterpret_cast<Pack<T, V>*>(p) = a;
     } else {
@@ -59,18 +95,24 @@ __device__ __forceinline__ void store_pack(T* p, const float (&f)[V], uint32_t n
     }
 }
 
-// Sum and largest over the ROW threads of a row (a warp, or the whole CTA), the same in each of them
-// and in a fixed order. at: two sets of ROW / 32 words that take turns, so that one barrier is enough.
-template <uint32_t ROW>
+// Sum and largest over the ROW threads of a row (a warp, or neighbouring warps), the same in each of them and
+// in a fixed order. at: two sets of ROW / 32 words of the row's own that take turns, so that one barrier is
+// enough; barrier: its number, where a CTA of THREADS holds several rows.
+template <uint32_t ROW, uint32_t THREADS = ROW>
 struct RowReduce {
     float (*at)[ROW / 32u];
     uint32_t turn = 0;
+    __device__ __forceinline__ void sync() const {
+        if constexpr (ROW == THREADS) __syncthreads();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1u + threadIdx.x / ROW), "n"(ROW) : "memory");
+    }
+    __device__ __forceinline__ static uint32_t warp() { return threadIdx.x % ROW >> 5; }
     __device__ __forceinline__ float sum(float v) {
 #pragma unroll
         for (uint32_t d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
         if constexpr (ROW > 32u) {
-            if ((threadIdx.x & 31u) == 0) at[turn][threadIdx.x >> 5] = v;
-            __syncthreads();
+            if ((threadIdx.x & 31u) == 0) at[turn][warp()] = v;
+            sync();
             v = 0.f;
 #pragma unroll
             for (uint32_t i = 0; i < ROW / 32u; ++i) v += at[turn][i];
@@ -81,8 +123,8 @@ struct RowReduce {
     __device__ __forceinline__ uint32_t most(uint32_t v) {
         v = __reduce_max_sync(0xffffffffu, v);
         if constexpr (ROW > 32u) {
-            if ((threadIdx.x & 31u) == 0) at[turn][threadIdx.x >> 5] = __uint_as_float(v);
-            __syncthreads();
+            if ((threadIdx.x & 31u) == 0) at[turn][warp()] = __uint_as_float(v);
+            sync();
 #pragma unroll
             for (uint32_t i = 0; i < ROW / 32u; ++i) v = max(v, __float_as_uint(at[turn][i]));
             turn ^= 1u;
@@ -90,6 +132,25 @@ struct RowReduce {
         return v;
     }
 };
+// Two sums behind one barrier.
+template <uint32_t ROW, uint32_t THREADS>
+__device__ __forceinline__ void reduce_two(RowReduce<ROW, THREADS>& first, RowReduce<ROW, THREADS>& second, float& a, float& b) {
+#pragma unroll
+    for (uint32_t d = 16; d; d >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, d);
+        b += __shfl_xor_sync(0xffffffffu, b, d);
+    }
+    if constexpr (ROW > 32u) {
+        float *x = first.at[first.turn], *y = second.at[second.turn];
+        if ((threadIdx.x & 31u) == 0) x[first.warp()] = a, y[first.warp()] = b;
+        first.sync();
+        a = b = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < ROW / 32u; ++i) a += x[i], b += y[i];
+        first.turn ^= 1u;
+        second.turn ^= 1u;
+    }
+}
 
 // What a row's largest |x| (as float bits, so that a NaN is the largest of all) makes of the row:
 // its scale, and the factor that brings it to [-127, 127]. Rows below 2^-100 are first lifted by
