@@ -657,7 +657,7 @@ int vlb_balance_loss_device(vlb_handle* h, const vlb_balance_desc* desc, void* s
  * throughout, one with an infinity is NaN there and 0 elsewhere; both have q = 0 and scale NaN.
  * An output may be an input's own memory (same address, type and stride): the stream updated in place;
  * else nothing may overlap. Strides in elements, 0 = cols; any alignment of the elements' own size
- * works, rows on 16-byte boundaries are faster. cols < 2^31; eps in [1e-30, inf). vlb_rms_norm_device
+ * works, rows on 16-byte boundaries are faster. cols < 2^30; eps in [1e-30, inf). vlb_rms_norm_device
  * is the reference's norm (f64 chains, bit for bit); this one is the form for blocks around the int8
  * products. Enqueued on `stream` (NULL = the handle's; 1 = cudaStreamLegacy); allocates nothing and
  * does not synchronise. */

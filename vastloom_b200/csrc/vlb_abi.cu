@@ -2018,7 +2018,7 @@ constexpr uint64_t kMaxRowStride = 1ull << 38;  // elements: no row's offset pas
 static const char* bad_norm(int type, int residual_type, uint32_t rows, uint32_t cols, float eps, const float* weight) {
     if (!float_type(type)) return "type must be F32, F16 or BF16";
     if (residual_type != type && residual_type != VLB_DTYPE_F32) return "residual_type must be F32 or the rows' type";
-    if (cols == 0 || cols > 0x7fffffffu || rows > 0x7fffffffu) return "cols must be positive, rows and cols below 2^31";
+    if (cols == 0 || cols >= (1u << 30) || rows > 0x7fffffffu) return "cols must be in [1, 2^30), rows below 2^31";
     if (!(eps >= 1e-30f) || !std::isfinite(eps)) return "eps must be in [1e-30, inf)";
     if (!aligned(weight, 4)) return "weight is not aligned to its elements";
     return nullptr;
@@ -2073,7 +2073,7 @@ static uint64_t norm_parts_bytes(uint32_t rows, uint32_t cols) {
     return (parts * cols * 4 + 255) / 256 * 256;
 }
 uint64_t vlb_add_rms_norm_grad_workspace_bytes(uint32_t rows, uint32_t cols) {
-    return norm_parts_bytes(rows, cols) + (uint64_t)rows * 16;
+    return norm_parts_bytes(rows, cols) + (uint64_t)rows * 8;
 }
 
 int vlb_add_rms_norm_grad_device(vlb_handle* h, const vlb_add_rms_norm_grad_desc* desc, void* stream) {
@@ -2110,7 +2110,7 @@ int vlb_add_rms_norm_grad_device(vlb_handle* h, const vlb_add_rms_norm_grad_desc
         p.dw = d.dweight;
         if (d.dweight) {
             p.part = static_cast<float*>(d.ws);
-            p.row = reinterpret_cast<float4*>(static_cast<char*>(d.ws) + norm_parts_bytes(d.rows, d.cols));
+            p.row = reinterpret_cast<float2*>(static_cast<char*>(d.ws) + norm_parts_bytes(d.rows, d.cols));
         }
         p.dy_stride = d.dy_stride;
         p.h_stride = d.h_stride;

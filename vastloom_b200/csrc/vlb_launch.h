@@ -227,8 +227,8 @@ struct NormGradParams {
     void* dx;                  // or null
     void* dres;                // or null
     float* dw;                 // or null
-    float* part;               // workspace, for dw: [kNormParts at most][cols] sums of parts of the rows
-    float4* row;               // workspace, for dw: the rows' (lift, s, mean(g n))
+    float* part;               // workspace: [kNormParts at most][cols] sums of parts of the rows, for dw
+    float2* row;               // workspace: the rows' (s, mean(g n)), for rows too long for registers
     size_t dy_stride, h_stride, dh_stride, dx_stride, dres_stride;
     uint32_t rows, cols;
     float eps, share;          // share: 1 / cols

@@ -4,8 +4,13 @@
 //              q = rint(y * (127 / a)), scale = a / 127
 //   gradient   n = h s,  g = dy w,  d = s (g - n mean(g n)) + dh,  dw = sum over rows of dy n
 //
-// Both move every element once and do a handful of operations on it: HBM bounds them. The sums are in
-// 32 bits. Where the squares pass them (h above 1.8e19) the row is taken again with h lifted by 2^-70.
+// Both move every element once and do a dozen operations on it: HBM bounds them. The sums are in 32 bits.
+// Where the squares pass them (h above 1.8e19) the row is taken again with h lifted by 2^-70.
+//
+// Rows come as pieces of V neighbouring elements (16 bytes of the wider type), ROW threads a row, KEEP pieces
+// a thread. A matrix whose stride is no multiple of V has its rows at V different offsets from a 16-byte
+// boundary: pieces then start on the boundary before the row, and a thread takes only rows of one offset,
+// so that its columns, their weights and their sums stay its own.
 //
 // The reference's norm is deepseek_v4_rms_norm (deepseek_v4_reference.cpp:170-206), without residual,
 // other types or gradient; the formulas above are this file's own.
@@ -21,12 +26,16 @@ namespace vlb {
 namespace {
 
 constexpr float kNormLift = 0x1p-70f;
-// Rows from which a ring pays, the threads and CTAs an SM of its kernels, and its depth: as many rows as a CTA's
-// share of the shared memory holds, 16-byte pieces for each thread, at most 6.
-constexpr uint32_t kRingRows = 1024, kRingSmem = 216u * 1024u, kNormThreads = 256, kGradThreads = 512;
-__host__ __device__ constexpr uint32_t norm_ctas(uint32_t keep) { return keep > 2u ? 2u : 4u; }
-__host__ __device__ constexpr uint32_t ring_depth(uint32_t pieces, uint32_t threads, uint32_t ctas) {
-    return kRingSmem / ctas / (pieces * threads * 16u) < 6u ? kRingSmem / ctas / (pieces * threads * 16u) : 6u;
+
+// The rings' shared memory an SM, threads and CTAs an SM, and depth: as many rows as a CTA's share holds of
+// `bytes` a thread, at most 6.
+constexpr uint32_t kRingSmem = 216u * 1024u, kGradThreads = 512;
+__host__ __device__ constexpr uint32_t norm_threads(uint32_t row) { return row > 256u ? row : 256u; }
+__host__ __device__ constexpr uint32_t norm_ctas(uint32_t row, uint32_t elements, bool shifted) {
+    return (elements > 16u ? 512u : shifted ? 768u : 1024u) / norm_threads(row);
+}
+__host__ __device__ constexpr uint32_t ring_depth(uint32_t bytes, uint32_t threads, uint32_t ctas) {
+    return kRingSmem / ctas / (bytes * threads) < 6u ? kRingSmem / ctas / (bytes * threads) : 6u;
 }
 
 // 1 / sqrt(mean + eps) of a row's sum of lifted squares; share: 1 / cols.
@@ -34,32 +43,100 @@ __device__ __forceinline__ float norm_step(float sum, float share, float eps, fl
     return __frsqrt_rn(fmaf(sum, share, eps * lift * lift));
 }
 
-// Bytes of y: V of them from column c on, n inside the row.
-template <uint32_t V>
-__device__ __forceinline__ void store_row_bytes(int8_t* q, const float (&y)[V], const RowStep& st, uint32_t n) {
-    if constexpr (V == 1) {
-        if (n) q[0] = (int8_t)quant_byte(y[0], st);
-    } else {
-        float v[V];
+// A ring of rows in shared memory, filled by cp.async: thread by thread, each reading back what it asked for
+// itself, so that waiting for its own copies is all the synchronisation there is. BYTES of a row a thread,
+// DEPTH rows; `before`: the bytes a thread has of the operands in front.
+template <uint32_t THREADS, uint32_t BYTES, uint32_t DEPTH>
+struct RowRing {
+    static_assert(DEPTH >= 1u, "a row has to fit");
+    char* at;
+    uint32_t stage = 0;
+    template <uint32_t SIZE>
+    __device__ __forceinline__ char* slot(uint32_t st, uint32_t before, uint32_t piece) const {
+        return at + (st * BYTES + before) * THREADS + (piece * THREADS + threadIdx.x) * SIZE;
+    }
+    // piece `piece` at p, columns c .. c + V - 1 of cols: zeros behind the row, what lies before it as it is
+    template <uint32_t V, typename E>
+    __device__ __forceinline__ void ask(uint32_t st, uint32_t before, uint32_t piece, const E* p, int32_t c, uint32_t cols) const {
+        constexpr uint32_t kSize = V * sizeof(E);
+        const int32_t left = (int32_t)cols - c;
+        const uint32_t have = left <= 0 ? 0u : min((uint32_t)left, V) * (uint32_t)sizeof(E);
+        char* to = slot<kSize>(st, before, piece);
+        if (have == 0) {  // no address of this row's
+            if constexpr (kSize == 16) *reinterpret_cast<uint4*>(to) = make_uint4(0u, 0u, 0u, 0u);
+            else *reinterpret_cast<uint2*>(to) = make_uint2(0u, 0u);
+        } else if constexpr (kSize == 16) {
+            tc::cp_async16(to, p, have);
+        } else {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(tc::smem_u32(to)), "l"(p), "r"(have) : "memory");
+        }
+    }
+    template <uint32_t V, typename E>
+    __device__ __forceinline__ Pack<E, V> get(uint32_t before, uint32_t piece) const {
+        return *reinterpret_cast<const Pack<E, V>*>(slot<V * sizeof(E)>(stage, before, piece));
+    }
+    __device__ __forceinline__ uint32_t behind() const { return stage ? stage - 1u : DEPTH - 1u; }
+    __device__ __forceinline__ void next() {
+        if (++stage == DEPTH) stage = 0;
+    }
+    __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory"); }
+};
+
+// The weights of a thread's columns from c0 on (zeros outside the row), the same in every row it takes.
+template <uint32_t V, uint32_t ROW, uint32_t KEEP>
+__device__ __forceinline__ void row_weights(const float* weight, int32_t c0, uint32_t cols, float (&w)[KEEP][V]) {
+    const bool wide = V % 4 == 0 && weight && reinterpret_cast<uintptr_t>(weight + c0) % 16u == 0;
 #pragma unroll
-        for (uint32_t i = 0; i < V; ++i) v[i] = st.inv == 0.f ? 0.f : y[i] * st.lift;
-        store_bytes<V>(q, v, st, n);
+    for (uint32_t i = 0; i < KEEP; ++i) {
+        const int32_t c = c0 + (int32_t)(i * ROW * V);
+        if (wide && inside(c, V, cols)) {
+            unpack(*reinterpret_cast<const Pack<float, V>*>(weight + c), w[i]);
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < V; ++j)
+                w[i][j] = (uint32_t)(c + (int32_t)j) >= cols ? 0.f : weight ? __ldg(weight + c + (int32_t)j) : 1.f;
+        }
     }
 }
 
-// What is done with row r once its pieces h are in registers: KEEP of V elements a thread, the first of them
-// at column `first`, ROW * V apart. LONG: the row may go on behind them; that is read again in each step.
+// Bytes of y: V of them from column c on, where they are inside [0, cols).
+template <uint32_t V>
+__device__ __forceinline__ void store_row_bytes(int8_t* q, float (&y)[V], const RowStep& st, int32_t c, uint32_t cols) {
+    if (st.lift != 1.f) {  // a row of zeros, of tiny values, or not finite
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) y[i] = st.inv == 0.f ? 0.f : y[i] * st.lift;
+    }
+    if constexpr (V % 4 == 0) {
+        if (inside(c, V, cols)) {
+            store_bytes<V>(q, y, st, V);
+            return;
+        }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < V; ++i)
+        if ((uint32_t)(c + (int32_t)i) < cols)
+            q[i] = (int8_t)__float_as_uint(__fadd_rn(__fmul_rn(y[i], st.inv), 12582912.f));
+}
+
+// ---- forward ---------------------------------------------------------------------------------
+
+// What is done with row r once its pieces h are in registers (zeros outside the row), the thread's first from
+// column c0 on, the others ROW * V apart. LONG: the row goes on behind them; that is read again in each step.
 // Every element is read and written by one thread: outputs may lie over inputs.
-template <typename T, typename R, uint32_t V, uint32_t ROW, uint32_t KEEP, bool LONG, typename REDUCE>
-__device__ __forceinline__ void norm_row(const NormParams& p, size_t r, float (&h)[KEEP][V], REDUCE& reduce) {
-    constexpr uint32_t kStep = ROW * V;
-    const uint32_t first = threadIdx.x % ROW * V, end = LONG ? p.cols : 0u;
-    const auto left = [&](uint32_t c) { return c < p.cols ? p.cols - c : 0u; };
-    const auto again = [&](uint32_t c, float (&f)[V]) {
-        unpack(load_pack<V>(static_cast<const T*>(p.x) + r * p.x_stride + c, left(c)), f);
+// weight multiplies piece i by its columns' weights.
+template <typename T, typename R, uint32_t V, uint32_t ROW, uint32_t KEEP, bool LONG, typename W, typename REDUCE>
+__device__ __forceinline__ void norm_row(const NormParams& p, size_t r, int32_t c0, float (&h)[KEEP][V], W&& weight,
+                                         REDUCE& reduce) {
+    constexpr int32_t kStep = ROW * V;
+    const int32_t rest = c0 + (int32_t)KEEP * kStep, end = LONG ? (int32_t)p.cols : rest;
+    R* to_h = static_cast<R*>(p.h) + r * p.h_stride;
+    T* to_y = static_cast<T*>(p.y) + r * p.y_stride;
+    int8_t* to_q = p.q + r * p.q_stride;
+    const auto again = [&](int32_t c, float (&f)[V]) {
+        unpack(load_piece<V>(static_cast<const T*>(p.x) + r * p.x_stride + c, c, p.cols), f);
         if (!p.residual) return;
         float more[V];
-        unpack(load_pack<V>(static_cast<const R*>(p.residual) + r * p.residual_stride + c, left(c)), more);
+        unpack(load_piece<V>(static_cast<const R*>(p.residual) + r * p.residual_stride + c, c, p.cols), more);
 #pragma unroll
         for (uint32_t j = 0; j < V; ++j) f[j] += more[j];
     };
@@ -69,7 +146,7 @@ __device__ __forceinline__ void norm_row(const NormParams& p, size_t r, float (&
         for (uint32_t i = 0; i < KEEP; ++i)
 #pragma unroll
             for (uint32_t j = 0; j < V; ++j) sum = fmaf(h[i][j] * lift, h[i][j] * lift, sum);
-        for (uint32_t c = first + KEEP * kStep; c < end; c += kStep) {
+        for (int32_t c = rest; c < end; c += kStep) {
             float f[V];
             again(c, f);
 #pragma unroll
@@ -80,75 +157,76 @@ __device__ __forceinline__ void norm_row(const NormParams& p, size_t r, float (&
     float lift = 1.f, sum = squares(1.f);
     if (!(sum < INFINITY)) sum = squares(lift = kNormLift);
     const float s = norm_step(sum, p.share, p.eps, lift) * lift;
-    // h to y, from column c on
-    const auto norm = [&](float (&f)[V], uint32_t c) {
+    const auto norm = [&](int32_t c, float (&f)[V]) {  // of the columns behind the pieces
+        float more[1][V];
+        row_weights<V, ROW, 1>(p.weight, c, p.cols, more);
 #pragma unroll
-        for (uint32_t j = 0; j < V; ++j) f[j] *= s;
-        if (!p.weight) return;
-        const Pack<float, V> w = load_pack<V>(p.weight + c, left(c));
-#pragma unroll
-        for (uint32_t j = 0; j < V; ++j) f[j] *= w.v[j];
+        for (uint32_t j = 0; j < V; ++j) f[j] = f[j] * s * more[0][j];
     };
 #pragma unroll
     for (uint32_t i = 0; i < KEEP; ++i) {
-        const uint32_t c = first + i * kStep;
-        if (p.h) store_pack<V>(static_cast<R*>(p.h) + r * p.h_stride + c, h[i], left(c));
-        norm(h[i], c);
-        if (p.y) store_pack<V>(static_cast<T*>(p.y) + r * p.y_stride + c, h[i], left(c));
+        const int32_t c = c0 + (int32_t)i * kStep;
+        if (p.h) store_piece<V>(to_h + c, h[i], c, p.cols);
+#pragma unroll
+        for (uint32_t j = 0; j < V; ++j) h[i][j] *= s;
+        weight(i, h[i]);
+        if (p.y) store_piece<V>(to_y + c, h[i], c, p.cols);
     }
     RowStep st{};
     if (p.q) {
         uint32_t most = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < KEEP; ++i)  // zeros behind the row's end, also where the row is NaN
+        for (uint32_t i = 0; i < KEEP; ++i)  // outside the row 0, or NaN where the row is
 #pragma unroll
-            for (uint32_t j = 0; j < V; ++j)
-                if (first + i * kStep + j < p.cols) most = max(most, __float_as_uint(h[i][j]) & 0x7fffffffu);
-        for (uint32_t c = first + KEEP * kStep; c < end; c += kStep) {
+            for (uint32_t j = 0; j < V; ++j) most = max(most, __float_as_uint(h[i][j]) & 0x7fffffffu);
+        for (int32_t c = rest; c < end; c += kStep) {
             float f[V];
             again(c, f);
-            norm(f, c);
+            norm(c, f);
 #pragma unroll
-            for (uint32_t j = 0; j < V; ++j)
-                if (c + j < p.cols) most = max(most, __float_as_uint(f[j]) & 0x7fffffffu);
+            for (uint32_t j = 0; j < V; ++j) most = max(most, __float_as_uint(f[j]) & 0x7fffffffu);
         }
         st = row_step(reduce.most(most));
         if (threadIdx.x % ROW == 0) p.scale[r] = st.scale;
 #pragma unroll
-        for (uint32_t i = 0; i < KEEP; ++i)
-            store_row_bytes<V>(p.q + r * p.q_stride + first + i * kStep, h[i], st, min(V, left(first + i * kStep)));
+        for (uint32_t i = 0; i < KEEP; ++i) {
+            const int32_t c = c0 + (int32_t)i * kStep;
+            store_row_bytes<V>(to_q + c, h[i], st, c, p.cols);
+        }
     }
-    for (uint32_t c = first + KEEP * kStep; c < end; c += kStep) {
+    for (int32_t c = rest; c < end; c += kStep) {
         float f[V];
         again(c, f);
-        if (p.h) store_pack<V>(static_cast<R*>(p.h) + r * p.h_stride + c, f, left(c));
-        norm(f, c);
-        if (p.y) store_pack<V>(static_cast<T*>(p.y) + r * p.y_stride + c, f, left(c));
-        if (p.q) store_row_bytes<V>(p.q + r * p.q_stride + c, f, st, min(V, left(c)));
+        if (p.h) store_piece<V>(to_h + c, f, c, p.cols);
+        norm(c, f);
+        if (p.y) store_piece<V>(to_y + c, f, c, p.cols);
+        if (p.q) store_row_bytes<V>(to_q + c, f, st, c, p.cols);
     }
 }
 
-// Few rows, rows at any alignment (V 1), rows longer than the pieces: a CTA a row, loads straight to registers.
+// Few rows, rows whose operands lie at different offsets (V 1), rows longer than the pieces: a CTA a row, loads
+// straight to registers.
 template <typename T, typename R, uint32_t V, uint32_t ROW, uint32_t KEEP, bool LONG>
 __global__ void __launch_bounds__(ROW) add_norm_kernel(const NormParams p) {
     constexpr uint32_t kStep = ROW * V;
     __shared__ float scratch[2][ROW / 32u];
+    const int32_t c0 = threadIdx.x * V;
+    float w[KEEP][V];
     tc::grid_dependency_wait();
     tc::grid_launch_dependents();
     RowReduce<ROW> reduce{scratch};
-    const uint32_t first = threadIdx.x * V;
     for (size_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        const auto left = [&](uint32_t c) { return c < p.cols ? p.cols - c : 0u; };
-        const T* x = static_cast<const T*>(p.x) + r * p.x_stride;
+        const T* x = static_cast<const T*>(p.x) + r * p.x_stride + c0;
         Pack<T, V> a[KEEP];  // all loads first
         Pack<R, V> b[KEEP];
 #pragma unroll
-        for (uint32_t i = 0; i < KEEP; ++i) a[i] = load_pack<V>(x + first + i * kStep, left(first + i * kStep));
+        for (uint32_t i = 0; i < KEEP; ++i) a[i] = load_piece<V>(x + i * kStep, c0 + (int32_t)(i * kStep), p.cols);
         if (p.residual) {
-            const R* res = static_cast<const R*>(p.residual) + r * p.residual_stride;
+            const R* res = static_cast<const R*>(p.residual) + r * p.residual_stride + c0;
 #pragma unroll
-            for (uint32_t i = 0; i < KEEP; ++i) b[i] = load_pack<V>(res + first + i * kStep, left(first + i * kStep));
+            for (uint32_t i = 0; i < KEEP; ++i) b[i] = load_piece<V>(res + i * kStep, c0 + (int32_t)(i * kStep), p.cols);
         }
+        if (r == blockIdx.x) row_weights<V, ROW, KEEP>(p.weight, c0, p.cols, w);
         float h[KEEP][V];
 #pragma unroll
         for (uint32_t i = 0; i < KEEP; ++i) {
@@ -159,180 +237,90 @@ __global__ void __launch_bounds__(ROW) add_norm_kernel(const NormParams p) {
 #pragma unroll
             for (uint32_t j = 0; j < V; ++j) h[i][j] += more[j];
         }
-        norm_row<T, R, V, ROW, KEEP, LONG>(p, r, h, reduce);
+        norm_row<T, R, V, ROW, KEEP, LONG>(p, r, c0, h, [&](uint32_t i, float (&f)[V]) {
+#pragma unroll
+            for (uint32_t j = 0; j < V; ++j) f[j] *= w[i][j];
+        }, reduce);
     }
 }
 
-// A ring of rows in shared memory, filled by cp.async: thread by thread, each reading back what it asked for
-// itself, so that waiting for its own copies is all the synchronisation there is. PIECES 16-byte pieces of a
-// row a thread, DEPTH rows.
-template <uint32_t THREADS, uint32_t PIECES, uint32_t DEPTH>
-struct RowRing {
-    uint4* at;  // [DEPTH][PIECES][THREADS]
-    uint32_t stage = 0;
-    __device__ __forceinline__ uint4* slot(uint32_t st, uint32_t piece) { return at + (st * PIECES + piece) * THREADS + threadIdx.x; }
-    // V elements from p on, `left` of them inside the row (zeros behind), as pieces `piece` on of stage st
-    template <uint32_t V, typename E>
-    __device__ __forceinline__ void ask(uint32_t st, uint32_t piece, const E* p, uint32_t left) {
-        constexpr uint32_t kPer = 16u / sizeof(E);
-#pragma unroll
-        for (uint32_t i = 0; i < V / kPer; ++i) {
-            const uint32_t have = left > i * kPer ? min(left - i * kPer, kPer) : 0u;
-            tc::cp_async16(slot(st, piece + i), have ? p + i * kPer : p, have * (uint32_t)sizeof(E));
-        }
-    }
-    template <uint32_t V, typename E>
-    __device__ __forceinline__ Pack<E, V> get(uint32_t piece) {
-        constexpr uint32_t kPer = 16u / sizeof(E);
-        Pack<E, V> a;
-#pragma unroll
-        for (uint32_t i = 0; i < V / kPer; ++i) reinterpret_cast<uint4*>(&a)[i] = *slot(stage, piece + i);
-        return a;
-    }
-    __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory"); }
-};
-
-// Many rows: persistent CTAs, DEPTH rows ahead on their way to shared memory, since the registers that h
-// takes leave too few threads to hold enough loads in flight themselves.
-template <typename T, typename R, uint32_t ROW, uint32_t KEEP, uint32_t DEPTH>
-__global__ void __launch_bounds__(kNormThreads, norm_ctas(KEEP)) add_norm_ring_kernel(const NormParams p) {
-    constexpr uint32_t V = 16u / sizeof(T), kThreads = kNormThreads, kRows = kThreads / ROW, kStep = ROW * V, kRes = sizeof(R) / sizeof(T);
-    constexpr uint32_t kPieces = KEEP * (1u + kRes);
-    static_assert(DEPTH >= 1u, "a row has to fit");
+// Many rows: persistent CTAs, DEPTH rows ahead on their way to shared memory, since the registers that h and w
+// take leave too few threads to hold enough loads in flight themselves. 16,384 x 4096 bf16, h and y written:
+// a CTA a row from registers 126 us, rings 85 (6.3 TB/s).
+template <typename T, typename R, uint32_t ROW, uint32_t KEEP, uint32_t DEPTH, bool SHIFTED>
+__global__ void __launch_bounds__(norm_threads(ROW), norm_ctas(ROW, KEEP * 16u / sizeof(R), SHIFTED)) add_norm_ring_kernel(const NormParams p) {
+    constexpr uint32_t V = 16u / sizeof(R), kThreads = norm_threads(ROW), kRows = kThreads / ROW, kStep = ROW * V;
+    constexpr uint32_t kX = KEEP * V * sizeof(T);
     extern __shared__ uint4 ring_smem[];
     __shared__ float scratch[kRows][2][ROW / 32u];
     tc::grid_dependency_wait();
     tc::grid_launch_dependents();
     RowReduce<ROW, kThreads> reduce{scratch[threadIdx.x / ROW]};
-    RowRing<kThreads, kPieces, DEPTH> ring{ring_smem};
-    const uint32_t first = threadIdx.x % ROW * V;
-    const size_t step = (size_t)gridDim.x * kRows;
-    size_t ahead = (size_t)blockIdx.x * kRows + threadIdx.x / ROW;
+    RowRing<kThreads, kX + KEEP * 16u, DEPTH> ring{reinterpret_cast<char*>(ring_smem)};
+    const size_t step = (size_t)gridDim.x * kRows, row0 = (size_t)blockIdx.x * kRows + threadIdx.x / ROW;
+    const int32_t c0 = (int32_t)(threadIdx.x % ROW * V) - (int32_t)(row0 * p.x_stride % V);  // of every row: V divides step
+    const T* x = static_cast<const T*>(p.x) + row0 * p.x_stride + c0;
+    const R* res = static_cast<const R*>(p.residual) + row0 * p.residual_stride + c0;
+    size_t ahead = row0;
     const auto ask = [&](uint32_t st) {
         if (ahead < p.rows) {
-            const T* x = static_cast<const T*>(p.x) + ahead * p.x_stride;
-            const R* res = static_cast<const R*>(p.residual) + ahead * p.residual_stride;
 #pragma unroll
             for (uint32_t i = 0; i < KEEP; ++i) {
-                const uint32_t c = first + i * kStep, left = c < p.cols ? p.cols - c : 0u;
-                ring.template ask<V>(st, i, x + (left ? c : 0u), left);
-                if (p.residual) ring.template ask<V>(st, KEEP + i * kRes, res + (left ? c : 0u), left);
+                const int32_t c = c0 + (int32_t)(i * kStep);
+                ring.template ask<V>(st, 0, i, x + i * kStep, c, p.cols);
+                if (p.residual) ring.template ask<V>(st, kX, i, res + i * kStep, c, p.cols);
             }
         }
         tc::cp_async_commit();
         ahead += step;
+        x += step * p.x_stride;
+        res += step * p.residual_stride;
     };
-    size_t r = ahead;
 #pragma unroll
     for (uint32_t i = 0; i + 1u < DEPTH; ++i) ask(i);
-    for (; r < p.rows; r += step) {
-        ask(ring.stage ? ring.stage - 1u : DEPTH - 1u);
+    // SHIFTED, the weights do not lie on 16 bytes: they stay in registers. Else they are loaded again, from L1, and
+    // the registers they would take hold a CTA more (16,384 x 4096 bf16: 99 us in registers, 86 from L1)
+    float w[SHIFTED ? KEEP : 1u][V];
+    if constexpr (SHIFTED) row_weights<V, ROW, KEEP>(p.weight, c0, p.cols, w);
+    for (size_t r = row0; r < p.rows; r += step) {
+        ask(ring.behind());
         ring.wait();
         float h[KEEP][V];
 #pragma unroll
         for (uint32_t i = 0; i < KEEP; ++i) {
-            unpack(ring.template get<V, T>(i), h[i]);
-            if (!p.residual) continue;
-            float more[V];
-            unpack(ring.template get<V, R>(KEEP + i * kRes), more);
+            unpack(ring.template get<V, T>(0, i), h[i]);
+            if (p.residual) {
+                float more[V];
+                unpack(ring.template get<V, R>(kX, i), more);
 #pragma unroll
-            for (uint32_t j = 0; j < V; ++j) h[i][j] += more[j];
+                for (uint32_t j = 0; j < V; ++j) h[i][j] += more[j];
+            }
+            if constexpr (SHIFTED) clip(h[i], c0 + (int32_t)(i * kStep), p.cols);
         }
-        norm_row<T, R, V, ROW, KEEP, false>(p, r, h, reduce);
-        if (++ring.stage == DEPTH) ring.stage = 0;
+        norm_row<T, R, V, ROW, KEEP, false>(p, r, c0, h, [&](uint32_t i, float (&f)[V]) {
+            if constexpr (SHIFTED) {
+#pragma unroll
+                for (uint32_t j = 0; j < V; ++j) f[j] *= w[i][j];
+            } else if (p.weight) {
+                const int32_t c = c0 + (int32_t)(i * kStep);
+                const Pack<float, V> v = load_piece<V>(p.weight + c, c, p.cols);
+#pragma unroll
+                for (uint32_t j = 0; j < V; ++j) f[j] *= v.v[j];
+            }
+        }, reduce);
+        ring.next();
     }
     tc::cp_async_wait_all();
 }
 
-// A row's dx and dresidual; with dw only its lift, step and mean(g n), for the kernel below.
-template <typename T, typename R, uint32_t ROW>
-__global__ void __launch_bounds__(256) norm_grad_rows_kernel(const NormGradParams p) {
-    __shared__ float scratch[2][ROW / 32u];
-    tc::grid_dependency_wait();
-    tc::grid_launch_dependents();
-    RowReduce<ROW> reduce{scratch};
-    const uint32_t tid = threadIdx.x % ROW;
-    for (size_t r = (size_t)blockIdx.x * (256u / ROW) + threadIdx.x / ROW; r < p.rows;
-         r += (size_t)gridDim.x * (256u / ROW)) {
-        const T* dy = static_cast<const T*>(p.dy) + r * p.dy_stride;
-        const R* h = static_cast<const R*>(p.h) + r * p.h_stride;
-        const R* dh = p.dh ? static_cast<const R*>(p.dh) + r * p.dh_stride : nullptr;
-        const auto grad = [&](uint32_t c) { return to_float(dy[c]) * (p.weight ? p.weight[c] : 1.f); };
-        float lift = 1.f, sum = 0.f, along = 0.f;
-        const auto sums = [&] {
-            sum = along = 0.f;
-            for (uint32_t c = tid; c < p.cols; c += ROW) {
-                const float v = to_float(h[c]) * lift;
-                sum += v * v;
-                along += grad(c) * v;
-            }
-            sum = reduce.sum(sum);
-            along = reduce.sum(along);
-        };
-        sums();
-        if (!(sum < INFINITY)) {
-            lift = kNormLift;
-            sums();
-        }
-        const float s = norm_step(sum, p.share, p.eps, lift);
-        const float mean = along * s * p.share;
-        if (p.dw) {
-            if (tid == 0) p.row[r] = make_float4(lift, s, mean, 0.f);
-            continue;
-        }
-        for (uint32_t c = tid; c < p.cols; c += ROW) {
-            const float n = to_float(h[c]) * lift * s;
-            const float d = (grad(c) - n * mean) * s * lift + (dh ? to_float(dh[c]) : 0.f);
-            if (p.dx) static_cast<T*>(p.dx)[r * p.dx_stride + c] = from_float<T>(d);
-            if (p.dres) static_cast<R*>(p.dres)[r * p.dres_stride + c] = from_float<R>(d);
-        }
-    }
-}
-
-// dx, dresidual, and part[y][c] = sum of dy n over the rows of part y. A thread a column.
-template <typename T, typename R>
-__global__ void __launch_bounds__(256) norm_grad_cols_kernel(const NormGradParams p, uint32_t rows_each) {
-    tc::grid_dependency_wait();
-    tc::grid_launch_dependents();
-    const uint32_t c = blockIdx.x * 256u + threadIdx.x;
-    if (c >= p.cols) return;
-    const uint32_t lo = blockIdx.y * rows_each, hi = min(p.rows, lo + rows_each);
-    const float w = p.weight ? p.weight[c] : 1.f;
-    float acc = 0.f;
-    for (size_t r = lo; r < hi; ++r) {
-        const float4 row = p.row[r];
-        const float dy = to_float(static_cast<const T*>(p.dy)[r * p.dy_stride + c]);
-        const float n = to_float(static_cast<const R*>(p.h)[r * p.h_stride + c]) * row.x * row.y;
-        const float d = (dy * w - n * row.z) * row.y * row.x +
-                        (p.dh ? to_float(static_cast<const R*>(p.dh)[r * p.dh_stride + c]) : 0.f);
-        if (p.dx) static_cast<T*>(p.dx)[r * p.dx_stride + c] = from_float<T>(d);
-        if (p.dres) static_cast<R*>(p.dres)[r * p.dres_stride + c] = from_float<R>(d);
-        acc += dy * n;
-    }
-    p.part[(size_t)blockIdx.y * p.cols + c] = acc;
-}
-
-// The weights of a thread's columns (zeros behind the row's end), the same in every row.
-template <uint32_t V, uint32_t ROW, uint32_t KEEP>
-__device__ __forceinline__ void row_weights(const float* weight, uint32_t cols, float (&w)[KEEP][V]) {
-#pragma unroll
-    for (uint32_t i = 0; i < KEEP; ++i) {
-        const uint32_t c = threadIdx.x % ROW * V + i * ROW * V, left = c < cols ? cols - c : 0u;
-        Pack<float, V> a;
-        if (weight) a = load_pack<V>(weight + (left ? c : 0u), left);
-#pragma unroll
-        for (uint32_t j = 0; j < V; ++j) w[i][j] = weight ? a.v[j] : 1.f;
-    }
-}
+// ---- gradient --------------------------------------------------------------------------------
 
 // Row r; adds dy n to acc. dy, h and dh give piece i (from registers, or again from shared memory: holding all
 // three beside the weights and the sums would take more registers than there are).
-template <typename T, typename R, uint32_t V, uint32_t ROW, uint32_t KEEP, typename DY, typename H, typename DH, typename REDUCE>
-__device__ __forceinline__ void norm_grad_row(const NormGradParams& p, size_t r, DY&& dy, H&& h, DH&& dh,
+template <typename T, typename R, uint32_t V, uint32_t ROW, uint32_t KEEP, bool SHIFTED, typename DY, typename H, typename DH, typename REDUCE>
+__device__ __forceinline__ void norm_grad_row(const NormGradParams& p, size_t r, int32_t c0, DY&& dy, H&& h, DH&& dh,
                                               const float (&w)[KEEP][V], float (&acc)[KEEP][V], REDUCE& reduce, REDUCE& reduce2) {
-    constexpr uint32_t kStep = ROW * V;
-    const uint32_t first = threadIdx.x % ROW * V;
-    const auto left = [&](uint32_t c) { return c < p.cols ? p.cols - c : 0u; };
+    constexpr int32_t kStep = ROW * V;
     float sum, along;
     const auto sums = [&](float lift) {
         sum = along = 0.f;
@@ -341,6 +329,10 @@ __device__ __forceinline__ void norm_grad_row(const NormGradParams& p, size_t r,
             float g[V], v[V];
             unpack(dy(i), g);
             unpack(h(i), v);
+            if constexpr (SHIFTED) {
+                clip(v, c0 + (int32_t)i * kStep, p.cols);
+                clip(g, c0 + (int32_t)i * kStep, p.cols);
+            }
 #pragma unroll
             for (uint32_t j = 0; j < V; ++j) {
                 const float n = v[j] * lift;
@@ -357,7 +349,7 @@ __device__ __forceinline__ void norm_grad_row(const NormGradParams& p, size_t r,
     const float mean = along * step * p.share;
 #pragma unroll
     for (uint32_t i = 0; i < KEEP; ++i) {
-        const uint32_t c = first + i * kStep;
+        const int32_t c = c0 + (int32_t)i * kStep;
         float g[V], v[V], d[V];
         unpack(dy(i), g);
         unpack(h(i), v);
@@ -365,124 +357,206 @@ __device__ __forceinline__ void norm_grad_row(const NormGradParams& p, size_t r,
         for (uint32_t j = 0; j < V; ++j) {
             const float n = v[j] * s;
             d[j] = fmaf(-n, mean, g[j] * w[i][j]) * s;
-            acc[i][j] = fmaf(g[j], n, acc[i][j]);
+            acc[i][j] = fmaf(g[j], n, acc[i][j]);  // outside the row: of columns that are not stored
         }
         if (p.dh) {
             unpack(dh(i), v);
 #pragma unroll
             for (uint32_t j = 0; j < V; ++j) d[j] += v[j];
         }
-        if (p.dx) store_pack<V>(static_cast<T*>(p.dx) + r * p.dx_stride + c, d, left(c));
-        if (p.dres) store_pack<V>(static_cast<R*>(p.dres) + r * p.dres_stride + c, d, left(c));
+        if (p.dx) store_piece<V>(static_cast<T*>(p.dx) + r * p.dx_stride + c, d, c, p.cols);
+        if (p.dres) store_piece<V>(static_cast<R*>(p.dres) + r * p.dres_stride + c, d, c, p.cols);
     }
 }
 
-// The CTA's part of the weight's gradient. all: where it holds several rows, room for a piece of each.
-template <uint32_t V, uint32_t ROW, uint32_t KEEP, uint32_t THREADS>
-__device__ __forceinline__ void norm_grad_part(const NormGradParams& p, const float (&acc)[KEEP][V], float* all) {
+// The CTA's part of the weight's gradient: its rows' sums added in order in shared memory, column by column (rows
+// at different offsets have a column in different threads). all: room for a row of floats and a 32nd.
+template <uint32_t V, uint32_t ROW, uint32_t KEEP, uint32_t THREADS, bool SHIFTED>
+__device__ __forceinline__ void norm_grad_part(const NormGradParams& p, int32_t c0, const float (&acc)[KEEP][V], float* all) {
     constexpr uint32_t kRows = THREADS / ROW, kStep = ROW * V;
-    const uint32_t first = threadIdx.x % ROW * V;
     float* part = p.part + (size_t)blockIdx.x * p.cols;
-    if constexpr (kRows > 1u) {  // the rows' sums, in order
-#pragma unroll
-        for (uint32_t i = 0; i < KEEP; ++i) {
-            __syncthreads();
-#pragma unroll
-            for (uint32_t j = 0; j < V; ++j) all[threadIdx.x / ROW * kStep + first + j] = acc[i][j];
-            __syncthreads();
-            for (uint32_t c = threadIdx.x; c < kStep && i * kStep + c < p.cols; c += THREADS) {
-                float v = all[c];
-#pragma unroll
-                for (uint32_t k = 1; k < kRows; ++k) v += all[k * kStep + c];
-                part[i * kStep + c] = v;
-            }
-        }
-    } else {
+    const auto each = [&](auto&& f) {
 #pragma unroll
         for (uint32_t i = 0; i < KEEP; ++i)
 #pragma unroll
-            for (uint32_t j = 0; j < V; ++j)
-                if (first + i * kStep + j < p.cols) part[first + i * kStep + j] = acc[i][j];
+            for (uint32_t j = 0; j < V; ++j) {
+                const uint32_t c = (uint32_t)(c0 + (int32_t)(i * kStep + j));
+                if (c < p.cols) f(c, acc[i][j]);
+            }
+    };
+    if constexpr (kRows == 1u) {
+        each([&](uint32_t c, float v) { part[c] = v; });
+    } else {
+        [[maybe_unused]] const auto place = [](uint32_t c) { return c + c / 32u; };  // lanes V columns apart on banks of their own
+        for (uint32_t k = 0; k < kRows; ++k) {
+            __syncthreads();
+            if (threadIdx.x / ROW != k) continue;
+            if constexpr (SHIFTED) {
+                if (k == 0) each([&](uint32_t c, float v) { all[place(c)] = v; });
+                else each([&](uint32_t c, float v) { all[place(c)] += v; });
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < KEEP; ++i) {
+                    float4* to = reinterpret_cast<float4*>(all + c0 + i * kStep);
+#pragma unroll
+                    for (uint32_t j = 0; j < V; j += 4u) {
+                        float4 v = k ? to[j / 4u] : make_float4(0.f, 0.f, 0.f, 0.f);
+                        v.x += acc[i][j], v.y += acc[i][j + 1u], v.z += acc[i][j + 2u], v.w += acc[i][j + 3u];
+                        to[j / 4u] = v;
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        for (uint32_t c = threadIdx.x; c < p.cols; c += THREADS) part[c] = all[SHIFTED ? place(c) : c];
     }
 }
 
-// Rows that registers hold whole, in one pass: a CTA takes every gridDim.x-th row and adds up dy n of its rows
-// in registers, a column always in the same thread; it leaves one part.
+// Few rows, rows whose operands lie at different offsets (V 1): a CTA takes every gridDim.x-th row and adds up
+// dy n of its rows in registers; it leaves one part.
 template <typename T, typename R, uint32_t V, uint32_t ROW, uint32_t KEEP>
 __global__ void __launch_bounds__(ROW) norm_grad_kernel(const NormGradParams p) {
     constexpr uint32_t kStep = ROW * V;
     __shared__ float scratch[2][2][ROW / 32u];
+    const int32_t c0 = threadIdx.x * V;
+    float acc[KEEP][V] = {}, w[KEEP][V];
     tc::grid_dependency_wait();
     tc::grid_launch_dependents();
     RowReduce<ROW> reduce{scratch[0]}, reduce2{scratch[1]};
-    const uint32_t first = threadIdx.x % ROW * V;
-    const auto left = [&](uint32_t c) { return c < p.cols ? p.cols - c : 0u; };
-    float acc[KEEP][V] = {}, w[KEEP][V];
-    row_weights<V, ROW, KEEP>(p.weight, p.cols, w);
     for (size_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         Pack<T, V> dy[KEEP];
         Pack<R, V> h[KEEP], dh[KEEP];
 #pragma unroll
         for (uint32_t i = 0; i < KEEP; ++i) {
-            const uint32_t c = first + i * kStep;
-            dy[i] = load_pack<V>(static_cast<const T*>(p.dy) + r * p.dy_stride + c, left(c));
-            h[i] = load_pack<V>(static_cast<const R*>(p.h) + r * p.h_stride + c, left(c));
-            if (p.dh) dh[i] = load_pack<V>(static_cast<const R*>(p.dh) + r * p.dh_stride + c, left(c));
+            const int32_t c = c0 + (int32_t)(i * kStep);
+            dy[i] = load_piece<V>(static_cast<const T*>(p.dy) + r * p.dy_stride + c, c, p.cols);
+            h[i] = load_piece<V>(static_cast<const R*>(p.h) + r * p.h_stride + c, c, p.cols);
+            if (p.dh) dh[i] = load_piece<V>(static_cast<const R*>(p.dh) + r * p.dh_stride + c, c, p.cols);
         }
-        norm_grad_row<T, R, V, ROW, KEEP>(
-            p, r, [&](uint32_t i) { return dy[i]; }, [&](uint32_t i) { return h[i]; }, [&](uint32_t i) { return dh[i]; }, w,
+        if (r == blockIdx.x) row_weights<V, ROW, KEEP>(p.weight, c0, p.cols, w);
+        norm_grad_row<T, R, V, ROW, KEEP, false>(
+            p, r, c0, [&](uint32_t i) { return dy[i]; }, [&](uint32_t i) { return h[i]; }, [&](uint32_t i) { return dh[i]; }, w,
             acc, reduce, reduce2);
     }
-    if (p.dw) norm_grad_part<V, ROW, KEEP, ROW>(p, acc, nullptr);
+    if (p.dw) norm_grad_part<V, ROW, KEEP, ROW, false>(p, c0, acc, nullptr);
 }
 
-// The same with rows ahead on their way to shared memory, as add_norm_ring_kernel.
-template <typename T, typename R, uint32_t ROW, uint32_t KEEP, uint32_t DEPTH>
+// Many rows, as add_norm_ring_kernel; a CTA an SM, so that few parts are left. 8192 x 4096 bf16 with dh and dw:
+// from registers 156 us, rings 49 with the sum of the parts (5.5 TB/s).
+template <typename T, typename R, uint32_t ROW, uint32_t KEEP, uint32_t DEPTH, bool SHIFTED>
 __global__ void __launch_bounds__(kGradThreads, 1) norm_grad_ring_kernel(const NormGradParams p) {
-    constexpr uint32_t V = 16u / sizeof(T), kThreads = kGradThreads, kRows = kThreads / ROW, kStep = ROW * V, kRes = sizeof(R) / sizeof(T);
-    constexpr uint32_t kH = KEEP, kDh = KEEP * (1u + kRes), kPieces = KEEP * (1u + 2u * kRes);
-    static_assert(DEPTH >= 1u, "a row has to fit");
+    constexpr uint32_t V = 16u / sizeof(R), kThreads = kGradThreads, kRows = kThreads / ROW, kStep = ROW * V;
+    constexpr uint32_t kH = KEEP * V * sizeof(T), kDh = kH + KEEP * 16u;
     extern __shared__ uint4 ring_smem[];
     __shared__ float scratch[2][kRows][2][ROW / 32u];
     tc::grid_dependency_wait();
     tc::grid_launch_dependents();
     RowReduce<ROW, kThreads> reduce{scratch[0][threadIdx.x / ROW]}, reduce2{scratch[1][threadIdx.x / ROW]};
-    RowRing<kThreads, kPieces, DEPTH> ring{ring_smem};
-    const uint32_t first = threadIdx.x % ROW * V;
-    const size_t step = (size_t)gridDim.x * kRows;
-    size_t ahead = (size_t)blockIdx.x * kRows + threadIdx.x / ROW;
+    RowRing<kThreads, kDh + KEEP * 16u, DEPTH> ring{reinterpret_cast<char*>(ring_smem)};
+    const size_t step = (size_t)gridDim.x * kRows, row0 = (size_t)blockIdx.x * kRows + threadIdx.x / ROW;
+    const int32_t c0 = (int32_t)(threadIdx.x % ROW * V) - (int32_t)(row0 * p.dy_stride % V);  // of every row: V divides step
+    const T* dy = static_cast<const T*>(p.dy) + row0 * p.dy_stride + c0;
+    const R* h = static_cast<const R*>(p.h) + row0 * p.h_stride + c0;
+    const R* dh = static_cast<const R*>(p.dh) + row0 * p.dh_stride + c0;
+    size_t ahead = row0;
     const auto ask = [&](uint32_t st) {
         if (ahead < p.rows) {
-            const T* dy = static_cast<const T*>(p.dy) + ahead * p.dy_stride;
-            const R* h = static_cast<const R*>(p.h) + ahead * p.h_stride;
-            const R* dh = static_cast<const R*>(p.dh) + ahead * p.dh_stride;
 #pragma unroll
             for (uint32_t i = 0; i < KEEP; ++i) {
-                const uint32_t c = first + i * kStep, left = c < p.cols ? p.cols - c : 0u, at = left ? c : 0u;
-                ring.template ask<V>(st, i, dy + at, left);
-                ring.template ask<V>(st, kH + i * kRes, h + at, left);
-                if (p.dh) ring.template ask<V>(st, kDh + i * kRes, dh + at, left);
+                const int32_t c = c0 + (int32_t)(i * kStep);
+                ring.template ask<V>(st, 0, i, dy + i * kStep, c, p.cols);
+                ring.template ask<V>(st, kH, i, h + i * kStep, c, p.cols);
+                if (p.dh) ring.template ask<V>(st, kDh, i, dh + i * kStep, c, p.cols);
             }
         }
         tc::cp_async_commit();
         ahead += step;
+        dy += step * p.dy_stride;
+        h += step * p.h_stride;
+        dh += step * p.dh_stride;
     };
-    size_t r = ahead;
 #pragma unroll
     for (uint32_t i = 0; i + 1u < DEPTH; ++i) ask(i);
     float acc[KEEP][V] = {}, w[KEEP][V];
-    row_weights<V, ROW, KEEP>(p.weight, p.cols, w);
-    for (; r < p.rows; r += step) {
-        ask(ring.stage ? ring.stage - 1u : DEPTH - 1u);
+    row_weights<V, ROW, KEEP>(p.weight, c0, p.cols, w);
+    for (size_t r = row0; r < p.rows; r += step) {
+        ask(ring.behind());
         ring.wait();
-        norm_grad_row<T, R, V, ROW, KEEP>(
-            p, r, [&](uint32_t i) { return ring.template get<V, T>(i); },
-            [&](uint32_t i) { return ring.template get<V, R>(kH + i * kRes); },
-            [&](uint32_t i) { return ring.template get<V, R>(kDh + i * kRes); }, w, acc, reduce, reduce2);
-        if (++ring.stage == DEPTH) ring.stage = 0;
+        norm_grad_row<T, R, V, ROW, KEEP, SHIFTED>(
+            p, r, c0, [&](uint32_t i) { return ring.template get<V, T>(0, i); },
+            [&](uint32_t i) { return ring.template get<V, R>(kH, i); },
+            [&](uint32_t i) { return ring.template get<V, R>(kDh, i); }, w, acc, reduce, reduce2);
+        ring.next();
     }
     tc::cp_async_wait_all();
-    if (p.dw) norm_grad_part<V, ROW, KEEP, kThreads>(p, acc, reinterpret_cast<float*>(ring_smem));
+    if (p.dw) norm_grad_part<V, ROW, KEEP, kThreads, SHIFTED>(p, c0, acc, reinterpret_cast<float*>(ring_smem));
+}
+
+// Rows too long for registers, read again for dx and dresidual; with dw only a row's s and mean(g n), and the next
+// kernel does the rest.
+template <typename T, typename R, uint32_t ROW>
+__global__ void __launch_bounds__(ROW) norm_grad_rows_kernel(const NormGradParams p) {
+    __shared__ float scratch[2][2][ROW / 32u];
+    tc::grid_dependency_wait();
+    tc::grid_launch_dependents();
+    RowReduce<ROW> reduce{scratch[0]}, reduce2{scratch[1]};
+    for (size_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const T* dy = static_cast<const T*>(p.dy) + r * p.dy_stride;
+        const R* h = static_cast<const R*>(p.h) + r * p.h_stride;
+        float lift = 1.f, sum, along;
+        const auto sums = [&] {
+            sum = along = 0.f;
+#pragma unroll 4
+            for (uint32_t c = threadIdx.x; c < p.cols; c += ROW) {
+                const float v = to_float(h[c]) * lift;
+                sum = fmaf(v, v, sum);
+                along = fmaf(to_float(dy[c]) * (p.weight ? p.weight[c] : 1.f), v, along);
+            }
+            reduce_two(reduce, reduce2, sum, along);
+        };
+        sums();
+        if (!(sum < INFINITY)) {
+            lift = kNormLift;
+            sums();
+        }
+        const float step = norm_step(sum, p.share, p.eps, lift);
+        const float s = step * lift, mean = along * step * p.share;
+        if (p.dw) {
+            if (threadIdx.x == 0) p.row[r] = make_float2(s, mean);
+            continue;
+        }
+        const R* dh = p.dh ? static_cast<const R*>(p.dh) + r * p.dh_stride : nullptr;
+#pragma unroll 4
+        for (uint32_t c = threadIdx.x; c < p.cols; c += ROW) {
+            const float d = fmaf(-to_float(h[c]) * s, mean, to_float(dy[c]) * (p.weight ? p.weight[c] : 1.f)) * s +
+                            (dh ? to_float(dh[c]) : 0.f);
+            if (p.dx) static_cast<T*>(p.dx)[r * p.dx_stride + c] = from_float<T>(d);
+            if (p.dres) static_cast<R*>(p.dres)[r * p.dres_stride + c] = from_float<R>(d);
+        }
+    }
+}
+
+// A thread a column of the rows of part blockIdx.y.
+template <typename T, typename R>
+__global__ void __launch_bounds__(256) norm_grad_cols_kernel(const NormGradParams p, uint32_t rows_each) {
+    tc::grid_dependency_wait();
+    tc::grid_launch_dependents();
+    const uint32_t c = blockIdx.x * 256u + threadIdx.x;
+    if (c >= p.cols) return;
+    const uint32_t lo = blockIdx.y * rows_each, hi = min(p.rows, lo + rows_each);
+    const float w = p.weight ? p.weight[c] : 1.f;
+    float acc = 0.f;
+    for (size_t r = lo; r < hi; ++r) {
+        const float2 row = p.row[r];
+        const float dy = to_float(static_cast<const T*>(p.dy)[r * p.dy_stride + c]);
+        const float n = to_float(static_cast<const R*>(p.h)[r * p.h_stride + c]) * row.x;
+        const float d = fmaf(-n, row.y, dy * w) * row.x +
+                        (p.dh ? to_float(static_cast<const R*>(p.dh)[r * p.dh_stride + c]) : 0.f);
+        if (p.dx) static_cast<T*>(p.dx)[r * p.dx_stride + c] = from_float<T>(d);
+        if (p.dres) static_cast<R*>(p.dres)[r * p.dres_stride + c] = from_float<R>(d);
+        acc = fmaf(dy, n, acc);
+    }
+    p.part[(size_t)blockIdx.y * p.cols + c] = acc;
 }
 
 // dw[c] = sum of the parts, in order: 32 columns by 32 shares of the parts a CTA.
@@ -503,32 +577,44 @@ __global__ void __launch_bounds__(1024) norm_grad_sum_kernel(const NormGradParam
     p.dw[c] = acc;
 }
 
-bool on16(const void* p, size_t stride_bytes) { return reinterpret_cast<uintptr_t>(p) % 16u == 0 && stride_bytes % 16u == 0; }
+// ---- hosts -----------------------------------------------------------------------------------
 
-// Calls f with the pieces a thread takes of a row, as types: of V elements, ROW threads, KEEP pieces.
-template <uint32_t V_, uint32_t ROW_, uint32_t KEEP_>
-struct Shape {
-    static constexpr uint32_t V = V_, ROW = ROW_, KEEP = KEEP_;
+// Whether the operands' rows all lie at one offset from a boundary of V elements, `stride` giving it: every
+// base on a boundary, every stride the same modulo V. A null operand has none.
+struct Offsets {
+    uint64_t stride;
+    uint32_t v;
+    bool fit;
+    void add(const void* p, uint64_t s, size_t size) {
+        if (p && (reinterpret_cast<uintptr_t>(p) % (v * size) || s % v != stride % v)) fit = false;
+    }
+    bool shifted() const { return stride % v != 0; }
 };
 
-constexpr uint32_t ring_depth(uint32_t pieces, uint32_t ctas) {
-    return kRingSmem / ctas / (pieces * 256u * 16u) < 6u ? kRingSmem / ctas / (pieces * 256u * 16u) : 6u;
-}
-uint32_t ring_blocks(uint32_t ctas, uint32_t rows) {
-    const uint32_t all = ctas * sm_count();
-    return rows < all ? rows : all;
+// Persistent CTAs of `rows_each` rows: at most `most`, and rows at several offsets taken V at a time.
+uint32_t ring_blocks(uint32_t most, uint32_t rows, uint32_t rows_each, uint32_t v, bool shifted) {
+    const uint32_t need = (rows + rows_each - 1u) / rows_each, blocks = need < most ? need : most;
+    const uint32_t whole = shifted && v > rows_each ? v / rows_each : 1u;
+    return blocks / whole * whole;
 }
 template <typename K, typename P>
-cudaError_t launch_ring(K* kernel, uint32_t pieces, uint32_t threads, uint32_t blocks, cudaStream_t s, const P& p) {
-    const size_t smem = (size_t)pieces * threads * 16u;
+cudaError_t launch_ring(K* kernel, size_t smem, uint32_t threads, uint32_t blocks, cudaStream_t s, const P& p) {
     const cudaError_t e = smem_once(kernel, smem);
     if (e != cudaSuccess) return e;
     return launch_chained(kernel, dim3(blocks), threads, smem, 0, s, p);
 }
 
+template <uint32_t V_, uint32_t ROW_, uint32_t KEEP_>
+struct Shape {
+    static constexpr uint32_t V = V_, ROW = ROW_, KEEP = KEEP_;
+};
+
+// Rows from which a ring pays: below, a CTA of more threads a row is over sooner.
+constexpr uint32_t kNormRingRows = 64, kGradRingRows = 64;
+
 template <typename T, typename R>
 cudaError_t norm_typed(const NormParams& p, cudaStream_t s) {
-    constexpr uint32_t N = 16u / sizeof(T);
+    constexpr uint32_t V = 16u / sizeof(R);
     const auto run = [&](auto shape) {
         using S = decltype(shape);
         const bool whole = p.cols <= S::V * S::ROW * S::KEEP;
@@ -536,38 +622,53 @@ cudaError_t norm_typed(const NormParams& p, cudaStream_t s) {
                                     : add_norm_kernel<T, R, S::V, S::ROW, S::KEEP, true>,
                               dim3(p.rows < 65535u ? p.rows : 65535u), S::ROW, 0, 0, s, p);
     };
+    Offsets at{p.x_stride, V, true};
+    at.add(p.x, p.x_stride, sizeof(T));
+    at.add(p.residual, p.residual_stride, sizeof(R));
+    at.add(p.h, p.h_stride, sizeof(R));
+    at.add(p.y, p.y_stride, sizeof(T));
+    at.add(p.q, p.q_stride, 1);
     const auto run_ring = [&](auto shape) {
         using S = decltype(shape);
-        constexpr uint32_t kPieces = S::KEEP * (1u + sizeof(R) / sizeof(T)), kCtas = norm_ctas(S::KEEP), kRows = kNormThreads / S::ROW;
-        constexpr uint32_t kDepth = ring_depth(kPieces, kNormThreads, kCtas);
-        return launch_ring(add_norm_ring_kernel<T, R, S::ROW, S::KEEP, kDepth>, kPieces * kDepth, kNormThreads,
-                           ring_blocks(kCtas, (p.rows + kRows - 1u) / kRows), s, p);
+        constexpr uint32_t kBytes = S::KEEP * V * (sizeof(T) + sizeof(R)), kThreads = norm_threads(S::ROW);
+        const auto launch = [&](auto shifted) {
+            constexpr bool kShifted = decltype(shifted)::value;
+            constexpr uint32_t kCtas = norm_ctas(S::ROW, S::KEEP * V, kShifted), kDepth = ring_depth(kBytes, kThreads, kCtas);
+            return launch_ring(add_norm_ring_kernel<T, R, S::ROW, S::KEEP, kDepth, kShifted>, kBytes * kDepth * kThreads,
+                               kThreads, ring_blocks(kCtas * sm_count(), p.rows, kThreads / S::ROW, V, kShifted), s, p);
+        };
+        // int8 rows from 16-bit ones: with the second reduction the rows ahead count for more than a CTA (16,384 x
+        // 4096 bf16 86 us with the weights from L1, 77 in registers; f32 142 and 157)
+        const bool apart = at.shifted() || reinterpret_cast<uintptr_t>(p.weight) % 16u || (p.q && sizeof(R) == 2u);
+        return apart ? launch(std::true_type{}) : launch(std::false_type{});
     };
-    const bool vec = on16(p.x, p.x_stride * sizeof(T)) && on16(p.residual, p.residual_stride * sizeof(R)) &&
-                     on16(p.h, p.h_stride * sizeof(R)) && on16(p.y, p.y_stride * sizeof(T)) && on16(p.weight, 0) &&
-                     reinterpret_cast<uintptr_t>(p.q) % N == 0 && p.q_stride % N == 0;
-    if (!vec) {
-        if (p.cols <= 256u * 4u) return run(Shape<1, 256, 4>{});
-        return run(Shape<1, 512, 8>{});
+    // pieces of a row, one more where it may begin inside one
+    const uint32_t pieces = (p.cols + V - 1u) / V + (at.shifted() ? 1u : 0u);
+    if (at.fit && p.rows >= kNormRingRows) {
+        if (pieces <= 32u) return run_ring(Shape<V, 32, 1>{});
+        if (pieces <= 64u) return run_ring(Shape<V, 32, 2>{});
+        if (pieces <= 128u) return run_ring(Shape<V, 64, 2>{});
+        if (pieces <= 256u) return run_ring(Shape<V, 128, 2>{});
+        if (pieces <= 512u) return run_ring(Shape<V, 256, 2>{});
+        if (pieces <= 1024u) return run_ring(Shape<V, 256, 4>{});
+        if (pieces <= 2048u) return run_ring(Shape<V, 512, 4>{});
+        if constexpr (V == 4u) {
+            if (pieces <= 4096u) return run_ring(Shape<V, 512, 8>{});
+        }
     }
-    const uint32_t packs = (p.cols + N - 1u) / N;
-    if (p.rows >= kRingRows) {
-        if (packs <= 32u) return run_ring(Shape<N, 32, 1>{});
-        if (packs <= 64u) return run_ring(Shape<N, 32, 2>{});
-        if (packs <= 128u) return run_ring(Shape<N, 64, 2>{});
-        if (packs <= 256u) return run_ring(Shape<N, 128, 2>{});
-        if (packs <= 512u) return run_ring(Shape<N, 256, 2>{});
-        if (packs <= 1024u) return run_ring(Shape<N, 256, 4>{});
+    if (at.fit && !at.shifted()) {
+        if (pieces <= 256u) return run(Shape<V, 256, 1>{});
+        if (pieces <= 512u) return run(Shape<V, 512, 1>{});
+        if (pieces <= 1024u) return run(Shape<V, 512, 2>{});
+        return run(Shape<V, 512, 4>{});
     }
-    if (packs <= 256u) return run(Shape<N, 256, 1>{});
-    if (packs <= 512u) return run(Shape<N, 512, 1>{});
-    if (packs <= 1024u) return run(Shape<N, 512, 2>{});
-    return run(Shape<N, 512, 4>{});
+    if (p.cols <= 256u * 4u) return run(Shape<1, 256, 4>{});
+    return run(Shape<1, 512, 8>{});
 }
 
 template <typename T, typename R>
 cudaError_t grad_typed(const NormGradParams& p, cudaStream_t s) {
-    constexpr uint32_t N = 16u / sizeof(T);
+    constexpr uint32_t V = 16u / sizeof(R);
     const auto sum = [&](uint32_t parts) {
         return launch_chained(norm_grad_sum_kernel, dim3((p.cols + 31u) / 32u), 1024, 0, 0, s, p, parts);
     };
@@ -577,37 +678,44 @@ cudaError_t grad_typed(const NormGradParams& p, cudaStream_t s) {
         const cudaError_t e = launch_chained(norm_grad_kernel<T, R, S::V, S::ROW, S::KEEP>, dim3(blocks), S::ROW, 0, 0, s, p);
         return e != cudaSuccess || !p.dw ? e : sum(blocks);
     };
-    const bool vec = on16(p.dy, p.dy_stride * sizeof(T)) && on16(p.h, p.h_stride * sizeof(R)) &&
-                     on16(p.dh, p.dh_stride * sizeof(R)) && on16(p.dx, p.dx_stride * sizeof(T)) &&
-                     on16(p.dres, p.dres_stride * sizeof(R)) && on16(p.weight, 0);
+    Offsets at{p.dy_stride, V, true};
+    at.add(p.dy, p.dy_stride, sizeof(T));
+    at.add(p.h, p.h_stride, sizeof(R));
+    at.add(p.dh, p.dh_stride, sizeof(R));
+    at.add(p.dx, p.dx_stride, sizeof(T));
+    at.add(p.dres, p.dres_stride, sizeof(R));
     const auto run_ring = [&](auto shape) {
         using S = decltype(shape);
-        constexpr uint32_t kPieces = S::KEEP * (1u + 2u * sizeof(R) / sizeof(T)), kRows = kGradThreads / S::ROW;
-        constexpr uint32_t kDepth = ring_depth(kPieces, kGradThreads, 1);
-        const uint32_t all = ring_blocks(1, (p.rows + kRows - 1u) / kRows), blocks = all < kNormParts ? all : kNormParts;
-        const cudaError_t e =
-            launch_ring(norm_grad_ring_kernel<T, R, S::ROW, S::KEEP, kDepth>, kPieces * kDepth, kGradThreads, blocks, s, p);
+        constexpr uint32_t kBytes = S::KEEP * V * (sizeof(T) + 2u * sizeof(R)), kDepth = ring_depth(kBytes, kGradThreads, 1);
+        const uint32_t most = sm_count() < kNormParts ? sm_count() : kNormParts;  // a part each
+        const uint32_t blocks = ring_blocks(most, p.rows, kGradThreads / S::ROW, V, at.shifted());
+        const cudaError_t e = launch_ring(at.shifted() ? norm_grad_ring_kernel<T, R, S::ROW, S::KEEP, kDepth, true>
+                                                       : norm_grad_ring_kernel<T, R, S::ROW, S::KEEP, kDepth, false>,
+                                          kBytes * kDepth * kGradThreads, kGradThreads, blocks, s, p);
         return e != cudaSuccess || !p.dw ? e : sum(blocks);
     };
-    if (vec) {
-        const uint32_t packs = (p.cols + N - 1u) / N;
-        if (p.rows >= kRingRows) {
-            if (packs <= 32u) return run_ring(Shape<N, 32, 1>{});
-            if (packs <= 64u) return run_ring(Shape<N, 32, 2>{});
-            if (packs <= 128u) return run_ring(Shape<N, 64, 2>{});
-            if (packs <= 256u) return run_ring(Shape<N, 128, 2>{});
-            if (packs <= 512u) return run_ring(Shape<N, 128, 4>{});
-            if (packs <= 1024u) return run_ring(Shape<N, 256, 4>{});
+    const uint32_t pieces = (p.cols + V - 1u) / V + (at.shifted() ? 1u : 0u);
+    if (at.fit && p.rows >= kGradRingRows) {
+        if (pieces <= 32u) return run_ring(Shape<V, 32, 1>{});
+        if (pieces <= 64u) return run_ring(Shape<V, 32, 2>{});
+        if (pieces <= 128u) return run_ring(Shape<V, 64, 2>{});
+        if (pieces <= 256u) return run_ring(Shape<V, 128, 2>{});
+        if (pieces <= 512u) return run_ring(Shape<V, 128, 4>{});
+        if (pieces <= 1024u) return run_ring(Shape<V, 256, 4>{});
+        if (pieces <= 2048u) return run_ring(Shape<V, 512, 4>{});
+        if constexpr (V == 4u) {
+            if (pieces <= 4096u) return run_ring(Shape<V, 512, 8>{});
         }
-        if (packs <= 256u) return run(Shape<N, 256, 1>{});
-        if (packs <= 512u) return run(Shape<N, 256, 2>{});
-        if (packs <= 1024u) return run(Shape<N, 512, 2>{});
-        if (packs <= 2048u) return run(Shape<N, 1024, 2>{});
+    }
+    if (at.fit && !at.shifted()) {
+        if (pieces <= 256u) return run(Shape<V, 256, 1>{});
+        if (pieces <= 512u) return run(Shape<V, 256, 2>{});
+        if (pieces <= 1024u) return run(Shape<V, 512, 2>{});
     } else {
         if (p.cols <= 256u * 4u) return run(Shape<1, 256, 4>{});
         if (p.cols <= 512u * 8u) return run(Shape<1, 512, 8>{});
     }
-    cudaError_t e = launch_chained(norm_grad_rows_kernel<T, R, 256>, dim3(p.rows < 65535u ? p.rows : 65535u), 256, 0, 0, s, p);
+    cudaError_t e = launch_chained(norm_grad_rows_kernel<T, R, 512>, dim3(p.rows < 65535u ? p.rows : 65535u), 512, 0, 0, s, p);
     if (e != cudaSuccess || !p.dw) return e;
     const uint32_t each = (p.rows + kNormParts - 1u) / kNormParts, parts = (p.rows + each - 1u) / each;
     e = launch_chained(norm_grad_cols_kernel<T, R>, dim3((p.cols + 255u) / 256u, parts), 256, 0, 0, s, p, each);

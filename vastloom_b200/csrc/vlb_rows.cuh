@@ -34,18 +34,29 @@ template <typename T, uint32_t V>
 struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
     T v[V];
 };
-// The first n of the pack at p (V or more: all of it), zeros behind them.
+// The columns c .. c + V - 1 of a row, p at column c: those inside [0, cols), zeros for the others. A piece that
+// is inside lies on its own alignment.
+__device__ __forceinline__ bool inside(int32_t c, uint32_t n, uint32_t cols) { return c >= 0 && (uint32_t)c + n <= cols; }
 template <uint32_t V, typename T>
-__device__ __forceinline__ Pack<T, V> load_pack(const T* p, uint32_t n) {
+__device__ __forceinline__ Pack<T, V> load_piece(const T* p, int32_t c, uint32_t cols) {
     Pack<T, V> a;
-    if (n >= V) {
+    if (inside(c, V, cols)) {
         a = *reinterpret_cast<const Pack<T, V>*>(p);
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < V; ++i) a.v[i] = i < n ? p[i] : from_float<T>(0.f);
+        for (uint32_t i = 0; i < V; ++i) a.v[i] = (uint32_t)(c + (int32_t)i) < cols ? p[i] : from_float<T>(0.f);
     }
     return a;
 }
+// Zeros outside [0, cols).
+template <uint32_t V>
+__device__ __forceinline__ void clip(float (&f)[V], int32_t c, uint32_t cols) {
+    if (inside(c, V, cols)) return;
+#pragma unroll
+    for (uint32_t i = 0; i < V; ++i)
+        if ((uint32_t)(c + (int32_t)i) >= cols) f[i] = 0.f;
+}
+
 // Two elements an instruction, or a shift and a mask, where they come in pairs.
 template <uint32_t V, typename T>
 __device__ __forceinline__ void unpack(const Pack<T, V>& a, float (&f)[V]) {
@@ -82,16 +93,16 @@ __device__ __forceinline__ Pack<T, V> pack(const float (&f)[V]) {
     }
     return a;
 }
-// Rounds V values to the first n elements at p.
+// V values rounded to the columns c .. c + V - 1, p at column c, where they are inside [0, cols).
 template <uint32_t V, typename T>
-__device__ __forceinline__ void store_pack(T* p, const float (&f)[V], uint32_t n) {
+__device__ __forceinline__ void store_piece(T* p, const float (&f)[V], int32_t c, uint32_t cols) {
     const Pack<T, V> a = pack<T>(f);
-    if (n >= V) {
+    if (inside(c, V, cols)) {
         *reinterpret_cast<Pack<T, V>*>(p) = a;
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < V; ++i)
-            if (i < n) p[i] = a.v[i];
+            if ((uint32_t)(c + (int32_t)i) < cols) p[i] = a.v[i];
     }
 }
 
