@@ -729,7 +729,7 @@ int vlb_add_rms_norm_grad_device(vlb_handle* h, const vlb_add_rms_norm_grad_desc
  * F32, F16, BF16 or I8: rows are copied bit by bit; offsets, row_index, row_weight and int8 rows with
  * row_scale are what vlb_int8_linear_device takes. The gradient of rows with respect to x is
  * vlb_combine_device of their gradient with the same elem_row and no weights; that of row_weight is
- * row_weight's gradient at elem_row. E <= 1024, k <= 64, T x k < 2^31. T = 0 is valid. Strides in
+ * row_weight's gradient at elem_row. E <= 1024, k <= 64, T x k < 2^31, H < 2^30. T = 0 is valid. Strides in
  * elements, 0 = H; any alignment of the elements' own size works, rows on 16-byte boundaries are
  * faster. Nothing may overlap. Enqueued on `stream`; allocates nothing and does not synchronise. */
 #define VLB_NO_ROW 0xffffffffu
@@ -765,7 +765,7 @@ int vlb_sort_tokens_device(vlb_handle* h, const vlb_sort_tokens_desc* desc, void
  * in 32 bits, slots in order, the residual last, rounded once to `out_type`. An elem_row >= n_rows
  * (VLB_NO_ROW) adds nothing, whatever its weight. weights NULL: 1; residual NULL: 0. rows of `type`,
  * residual and out of out_type (F32, F16 or BF16 each); out may be the residual's own memory (same
- * address and stride), else nothing may overlap. T = 0 is valid, also n_rows = 0. Enqueued on
+ * address and stride), else nothing may overlap. k <= 64, T x k < 2^31, H < 2^30. T = 0 is valid, also n_rows = 0. Enqueued on
  * `stream`; allocates nothing and does not synchronise. */
 typedef struct vlb_combine_desc {
     const void* rows;            /* [n_rows] rows of type */

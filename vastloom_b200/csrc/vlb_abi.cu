@@ -2127,7 +2127,7 @@ int vlb_add_rms_norm_grad_device(vlb_handle* h, const vlb_add_rms_norm_grad_desc
 }
 
 uint64_t vlb_sort_tokens_workspace_bytes(uint32_t T, uint32_t k, uint32_t E) {
-    return 256 + (uint64_t)sort_blocks((uint64_t)T * k) * E * 4;
+    return 256 + (uint64_t)sort_blocks_bound((uint64_t)T * k) * E * 4;
 }
 
 int vlb_sort_tokens_device(vlb_handle* h, const vlb_sort_tokens_desc* desc, void* stream) {
@@ -2148,7 +2148,7 @@ int vlb_sort_tokens_device(vlb_handle* h, const vlb_sort_tokens_desc* desc, void
         const size_t es = dtype_size(d.type);
         if (d.rows) {
             if (!es) return bad("type must be F32, F16, BF16 or I8");
-            if (d.H == 0 || (d.T && !d.x)) return bad("rows need x and H");
+            if (d.H == 0 || d.H >= (1u << 30) || (d.T && !d.x)) return bad("rows need x, and H in [1, 2^30)");
             if (bad_rows(d.x, d.x_stride, d.H, es) || bad_rows(d.rows, d.rows_stride, d.H, es))
                 return bad("rows are not aligned to their elements, or a stride is out of range");
         }
@@ -2193,7 +2193,7 @@ int vlb_combine_device(vlb_handle* h, const vlb_combine_desc* desc, void* stream
         vlb_combine_desc d = *desc;
         auto bad = [&](const char* why) { return h->fail(VLB_ERR_INVALID_ARGUMENT, std::string("combine: ") + why); };
         if (!float_type(d.type) || !float_type(d.out_type)) return bad("type and out_type must be F32, F16 or BF16");
-        if (d.k == 0 || d.H == 0 || d.H > 0x7fffffffu) return bad("k and H must be positive, H below 2^31");
+        if (d.k == 0 || d.H == 0 || d.H >= (1u << 30)) return bad("k and H must be positive, H below 2^30");
         if (d.k > 64 || (uint64_t)d.T * d.k > 0x7fffffffull)
             return h->fail(VLB_ERR_UNSUPPORTED, "combine: k > 64 or T x k >= 2^31");
         const size_t es = dtype_size(d.type), os = dtype_size(d.out_type);
@@ -2228,7 +2228,7 @@ int vlb_combine_grad_device(vlb_handle* h, const vlb_combine_grad_desc* desc, vo
         vlb_combine_grad_desc d = *desc;
         auto bad = [&](const char* why) { return h->fail(VLB_ERR_INVALID_ARGUMENT, std::string("combine gradient: ") + why); };
         if (!float_type(d.type) || !float_type(d.out_type)) return bad("type and out_type must be F32, F16 or BF16");
-        if (d.k == 0 || d.H == 0 || d.H > 0x7fffffffu) return bad("k and H must be positive, H below 2^31");
+        if (d.k == 0 || d.H == 0 || d.H >= (1u << 30)) return bad("k and H must be positive, H below 2^30");
         if (d.k > 64 || (uint64_t)d.T * d.k > 0x7fffffffull)
             return h->fail(VLB_ERR_UNSUPPORTED, "combine gradient: k > 64 or T x k >= 2^31");
         const size_t es = dtype_size(d.type), os = dtype_size(d.out_type);

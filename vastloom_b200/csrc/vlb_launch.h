@@ -256,6 +256,7 @@ struct SortParams {
 };
 constexpr uint32_t kSortMaxExperts = 1024;
 uint32_t sort_blocks(uint64_t pairs);
+uint32_t sort_blocks_bound(uint64_t pairs);  // of the largest call up to so many pairs
 cudaError_t launch_sort_tokens(const SortParams& p, cudaStream_t s);
 struct CombineParams {
     const void* rows;
