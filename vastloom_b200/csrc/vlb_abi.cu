@@ -2127,7 +2127,7 @@ int vlb_add_rms_norm_grad_device(vlb_handle* h, const vlb_add_rms_norm_grad_desc
 }
 
 uint64_t vlb_sort_tokens_workspace_bytes(uint32_t T, uint32_t k, uint32_t E) {
-    return 256 + (uint64_t)sort_blocks_bound((uint64_t)T * k) * E * 4;
+    return 256 + ((uint64_t)sort_blocks_bound((uint64_t)T * k) + 1) * E * 4;
 }
 
 int vlb_sort_tokens_device(vlb_handle* h, const vlb_sort_tokens_desc* desc, void* stream) {
@@ -2169,7 +2169,8 @@ int vlb_sort_tokens_device(vlb_handle* h, const vlb_sort_tokens_desc* desc, void
         p.row_index = d.row_index;
         p.elem_row = d.elem_row;
         p.offsets = d.offsets;
-        p.counts = static_cast<uint32_t*>(d.ws);
+        p.totals = static_cast<uint32_t*>(d.ws);
+        p.counts = p.totals + d.E;
         p.T = d.T;
         p.k = d.k;
         p.E = d.E;

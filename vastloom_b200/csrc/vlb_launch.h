@@ -249,6 +249,7 @@ struct SortParams {
     uint32_t* row_index;       // or null
     uint32_t* elem_row;
     uint32_t* offsets;         // [E + 1]
+    uint32_t* totals;          // workspace: [E] the pairs of each expert
     uint32_t* counts;          // workspace: [blocks][E] the blocks' pairs of each expert
     size_t x_stride, rows_stride;  // bytes
     size_t row_bytes;

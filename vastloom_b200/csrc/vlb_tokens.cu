@@ -106,6 +106,8 @@ __device__ __forceinline__ int32_t row_offset(const E* row) {
 
 // ---- the order -------------------------------------------------------------------------------------
 
+constexpr uint32_t kSortBlocks = 256;    // counting blocks at most
+constexpr uint32_t kSelfPairs = 16384;  // up to here the counts cost more as a launch than again in every block
 constexpr uint32_t kSortThreads = 512, kSortWarps = kSortThreads / 32u;
 
 // The expert of pair i; E where it was dropped.
@@ -156,8 +158,40 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortPara
     for (uint32_t e = threadIdx.x; e < p.E; e += kSortThreads) p.counts[(size_t)blockIdx.x * p.E + e] = hist[e];
 }
 
-// Every pair's place and what goes there of it. Shared: base[E] the block's next place on each expert,
-// by_warp[kSortWarps][E] the warps' pairs of each expert in a round of kSortThreads.
+// counts[b][e] becomes the pairs on expert e of the blocks before b, totals[e] those of all. 32 experts a block, a warp
+// a 32nd of the counting blocks.
+__global__ void __launch_bounds__(1024) sort_prefix_kernel(const SortParams p, uint32_t blocks) {
+    constexpr uint32_t kEach = kSortBlocks / 32u;
+    __shared__ uint32_t sums[32][33];
+    tc::grid_dependency_wait();
+    tc::grid_launch_dependents();
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, e = blockIdx.x * 32u + lane, b0 = warp * kEach;
+    uint32_t v[kEach], sum = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) v[i] = e < p.E && b0 + i < blocks ? p.counts[(size_t)(b0 + i) * p.E + e] : 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) sum += v[i];
+    sums[warp][lane] = sum;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < 32u; ++w) {
+        if (w < warp) before += sums[w][lane];
+        all += sums[w][lane];
+    }
+    if (e >= p.E) return;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+        if (b0 + i < blocks) p.counts[(size_t)(b0 + i) * p.E + e] = before;
+        before += v[i];
+    }
+    if (warp == 0) p.totals[e] = all;
+}
+
+// Every pair's place and what goes there of it. SELF: without the counts, every block goes through all pairs. Shared:
+// base[E] the block's next place on each expert, by_warp[kSortWarps][E] the warps' pairs of each expert in a round of
+// kSortThreads.
+template <bool SELF>
 __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const SortParams p, uint32_t each) {
     extern __shared__ uint32_t sort_smem[];
     __shared__ uint32_t warps[32];
@@ -167,22 +201,20 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const SortPara
     for (uint32_t q = tid; q < kSortWarps * p.E; q += kSortThreads) by_warp[q] = 0;
     tc::grid_dependency_wait();
     tc::grid_launch_dependents();
-    // all blocks' pairs on an expert, and those of the blocks before this one: shares of the blocks for the
-    // experts that the threads do not fill
     __syncthreads();
-    const uint32_t shares = p.E < kSortThreads ? kSortThreads / p.E : 1u;
-    for (uint32_t e0 = 0; e0 < p.E; e0 += kSortThreads) {
-        const uint32_t e = e0 + (shares > 1u ? tid % p.E : tid), share = shares > 1u ? tid / p.E : 0u;
-        if (e < p.E && share < shares) {
-            uint32_t all = 0, before = 0;
-#pragma unroll 8
-            for (uint32_t b = share; b < gridDim.x; b += shares) {
-                const uint32_t v = p.counts[(size_t)b * p.E + e];
-                all += v;
-                before += b < blockIdx.x ? v : 0u;
-            }
-            atomicAdd(by_warp + e, all);            // whole numbers: in any order the same
-            atomicAdd(by_warp + p.E + e, before);
+    // by_warp[0]: all pairs on an expert; [1]: those of the blocks before this one
+    if constexpr (SELF) {
+#pragma unroll 4
+        for (uint32_t i = tid; i < n; i += kSortThreads) {
+            const uint32_t e = pair_expert(p, i);
+            if (e >= p.E) continue;
+            atomicAdd(by_warp + e, 1u);
+            if (i < lo) atomicAdd(by_warp + p.E + e, 1u);
+        }
+    } else {
+        for (uint32_t e = tid; e < p.E; e += kSortThreads) {
+            by_warp[e] = p.totals[e];
+            by_warp[p.E + e] = p.counts[(size_t)blockIdx.x * p.E + e];
         }
     }
     __syncthreads();
@@ -323,7 +355,7 @@ __global__ void __launch_bounds__(256) sort_rows_shifted_kernel(const SortParams
 // Every block holds all pairs' experts, a warp finds a pair's place by counting the pairs before it (of smaller
 // experts, and of its own with a smaller number), and the block moves its tokens' rows; the last block takes the
 // offsets. Shared: [n] experts. E: a type of the elements' size, where SHIFTED.
-constexpr uint32_t kFewPairs = 4096, kFewWork = 1u << 20;
+constexpr uint32_t kFewPairs = 4096, kFewWork = 1u << 19;
 template <typename E, bool SHIFTED>
 __global__ void __launch_bounds__(256) sort_few_kernel(const SortParams p, uint32_t segments) {
     extern __shared__ uint32_t sort_smem[];
@@ -595,7 +627,6 @@ cudaError_t by_type(int type, F&& f) {
 }
 
 // Pairs of a block in the order's kernels: a round of kSortThreads, or as many rounds as leave kSortBlocks blocks.
-constexpr uint32_t kSortBlocks = 256;
 uint32_t sort_each(uint64_t pairs) {
     const uint64_t rounds = (pairs + kSortThreads * kSortBlocks - 1u) / (kSortThreads * kSortBlocks);
     return (uint32_t)((rounds ? rounds : 1u) * kSortThreads);
@@ -701,10 +732,16 @@ cudaError_t launch_sort_tokens(const SortParams& p, cudaStream_t s) {
     // every token's block goes through all pairs: 256 tokens of 8 5.9 us, 512 13.1, 4000 of one 24 (else 13 to 14)
     if (n <= kFewPairs && (uint64_t)p.T * n <= kFewWork) return sort_rows(p, true, s);
     const uint32_t each = sort_each(n), blocks = sort_blocks(n);
-    cudaError_t e = launch_chained(sort_count_kernel, dim3(blocks), kSortThreads, 0, 0, s, p, each);
-    if (e != cudaSuccess) return e;
-    if ((e = smem_once(sort_place_kernel, (kSortWarps + 1u) * kSortMaxExperts * 4u)) != cudaSuccess) return e;
-    e = launch_chained(sort_place_kernel, dim3(blocks), kSortThreads, (size_t)(kSortWarps + 1u) * p.E * 4u, 0, s, p, each);
+    const bool self = n <= kSelfPairs;
+    cudaError_t e = cudaSuccess;
+    if (!self) {
+        if ((e = launch_chained(sort_count_kernel, dim3(blocks), kSortThreads, 0, 0, s, p, each)) != cudaSuccess) return e;
+        e = launch_chained(sort_prefix_kernel, dim3((p.E + 31u) / 32u), 1024, 0, 0, s, p, blocks);
+        if (e != cudaSuccess) return e;
+    }
+    const auto kernel = self ? sort_place_kernel<true> : sort_place_kernel<false>;
+    if ((e = smem_once(kernel, (kSortWarps + 1u) * kSortMaxExperts * 4u)) != cudaSuccess) return e;
+    e = launch_chained(kernel, dim3(blocks), kSortThreads, (size_t)(kSortWarps + 1u) * p.E * 4u, 0, s, p, each);
     return e != cudaSuccess || !p.rows ? e : sort_rows(p, false, s);
 }
 
