@@ -61,12 +61,21 @@ __device__ __forceinline__ float gelu(float z) {
 // sigmoid(v): of SiLU, and of GELU's tanh form, (1 + tanh(u)) / 2 = sigmoid(2 u).
 __device__ __forceinline__ float sigmoid_of(float v) { return fast_rcp(1.f + fast_exp(fmaxf(fminf(-v, 88.f), -1000.f))); }
 
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if constexpr (ACT == VLB_ACT_RELU) return z < 0.f ? 0.f : z;  // keeps a NaN
+    else if constexpr (ACT == VLB_ACT_SILU) return z * sigmoid_of(z);
+    else if constexpr (ACT == VLB_ACT_GELU) return gelu(z);
+    else if constexpr (ACT == VLB_ACT_GELU_TANH)
+        return z * sigmoid_of(1.59576912f * fmaf(0.044715f * z * z, z, z));  // 2 sqrt(2 / pi)
+    else return z;
+}
 __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {
-        case VLB_ACT_RELU: return z < 0.f ? 0.f : z;  // keeps a NaN
-        case VLB_ACT_SILU: return z * sigmoid_of(z);
-        case VLB_ACT_GELU: return gelu(z);
-        case VLB_ACT_GELU_TANH: return z * sigmoid_of(1.59576912f * fmaf(0.044715f * z * z, z, z));  // 2 sqrt(2 / pi)
+        case VLB_ACT_RELU: return activate<VLB_ACT_RELU>(z);
+        case VLB_ACT_SILU: return activate<VLB_ACT_SILU>(z);
+        case VLB_ACT_GELU: return activate<VLB_ACT_GELU>(z);
+        case VLB_ACT_GELU_TANH: return activate<VLB_ACT_GELU_TANH>(z);
         default: return z;
     }
 }
@@ -614,7 +623,10 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(ROWS)) int8_few_kernel
 
 enum class Mm { kOne, kSplit, kPair };
 constexpr uint32_t kMmChannels = 128, kMmMaxTokens = 256, kMmKc = 128;
-constexpr uint32_t kMmEpiWarps = 8, kMmThreads = (kMmEpiWarps + 3) * 32;
+// Warps that take the sums to memory: twice as many where an epilogue's operations come on top (4096 x 4096 x 4096 f16
+// with GELU 96 us with 8, 75 with 16; what 8 warps hold in flight does not cover their latency).
+__host__ __device__ constexpr uint32_t mm_epi_warps(Mm mode, bool epi) { return epi && mode != Mm::kSplit ? 12u : 8u; }
+__host__ __device__ constexpr uint32_t mm_threads(Mm mode, bool epi) { return (mm_epi_warps(mode, epi) + 3u) * 32u; }
 constexpr uint32_t kMmWStage = kMmChannels * kMmKc;
 constexpr uint32_t kMmMaxStages = 12;
 constexpr uint32_t kMmSmemLimit = 227u * 1024u;
@@ -630,6 +642,7 @@ struct Int8MmaParams {
     uint32_t ct, nk;    // channel tiles, K chunks
     uint32_t tmem_cols, acc_cols;
     uint32_t split;
+    uint32_t wide;      // rows of y and of the residual lie on 16-byte boundaries
     uint32_t early;     // the kernel ahead quantizes the tokens: weights may be loaded beside it
 };
 
@@ -645,6 +658,7 @@ struct MmShared {
     float* channel;   // [2][128] its channels'
     float* weight;    // with an epilogue: [2][256] the tokens' row weights,
     float* bias;      // [2][128] the channels' biases
+    float* out;       // [turns of four warps][16][128] act(z) on its way to rows of y
     MmTile* tile;     // [2]
     uint64_t *full, *empty, *acc_full, *acc_empty, *tile_full, *tile_empty;
     uint32_t* tmem;
@@ -652,8 +666,11 @@ struct MmShared {
 };
 
 __host__ __device__ constexpr uint32_t mm_table_bytes(uint32_t groups) { return (3u * groups + 1u) * 4u; }
-__host__ __device__ constexpr uint32_t mm_fixed_bytes(uint32_t groups, bool epi) {
-    return (epi ? 4u : 2u) * (kMmMaxTokens + kMmChannels) * 4u + 2u * 16u + (2u * kMmMaxStages + 8u) * 8u + 16u + mm_table_bytes(groups) +
+__host__ __device__ constexpr uint32_t mm_out_bytes(Mm mode, bool epi) {
+    return epi && mode != Mm::kSplit ? mm_epi_warps(mode, epi) / 4u * 16u * kMmChannels * 4u : 0u;
+}
+__host__ __device__ constexpr uint32_t mm_fixed_bytes(uint32_t groups, Mm mode, bool epi) {
+    return mm_out_bytes(mode, epi) + (epi ? 4u : 2u) * (kMmMaxTokens + kMmChannels) * 4u + 2u * 16u + (2u * kMmMaxStages + 8u) * 8u + 16u + mm_table_bytes(groups) +
            16u;
 }
 
@@ -706,8 +723,9 @@ __device__ __forceinline__ MmTile mm_tile(const MmShared& sh, const Int8MmaParam
 }
 
 template <typename TY, Mm MODE, bool EPI>
-__global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_constant__ Int8MmaParams p) {
+__global__ void __launch_bounds__(mm_threads(MODE, EPI), 1) int8_mma_kernel(const __grid_constant__ Int8MmaParams p) {
     constexpr bool SPLIT = MODE == Mm::kSplit, PAIR = MODE == Mm::kPair;
+    constexpr uint32_t kEpi = mm_epi_warps(MODE, EPI);
     extern __shared__ __align__(1024) unsigned char mm_smem[];
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
     const uint32_t smem = tc::smem_u32(mm_smem), stage_bytes = kMmWStage + p.x_stage;
@@ -715,7 +733,8 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
     MmShared sh;
     {
         unsigned char* at = mm_smem + p.stages * stage_bytes;
-        sh.scale = reinterpret_cast<float*>(at);
+        sh.out = reinterpret_cast<float*>(at);
+        sh.scale = sh.out + mm_out_bytes(MODE, EPI) / 4u;
         sh.channel = sh.scale + 2u * kMmMaxTokens;
         sh.weight = sh.channel + 2u * kMmChannels;
         sh.bias = sh.weight + 2u * kMmMaxTokens;
@@ -738,11 +757,11 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         if (tid == 0) mm_report(l);
         return;
     }
-    if (warp == kMmEpiWarps) {
+    if (warp == kEpi) {
         if (PAIR) tc::tmem_alloc_pair(sh.tmem, p.tmem_cols);
         else tc::tmem_alloc(sh.tmem, p.tmem_cols);
     }
-    if (warp == kMmEpiWarps + 1u && lane < 2u)
+    if (warp == kEpi + 1u && lane < 2u)
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane ? &p.xmap : &p.wmap)) : "memory");
     if (tid == 0) {
         for (uint32_t i = 0; i < p.stages; ++i) {
@@ -751,21 +770,21 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         }
         for (uint32_t i = 0; i < 2u; ++i) {
             tc::mbar_init(sh.acc_full + i, 1);
-            tc::mbar_init(sh.acc_empty + i, PAIR ? 2u * kMmEpiWarps : kMmEpiWarps);
+            tc::mbar_init(sh.acc_empty + i, PAIR ? 2u * kEpi : kEpi);
             tc::mbar_init(sh.tile_full + i, 1);
-            tc::mbar_init(sh.tile_empty + i, kMmEpiWarps);
+            tc::mbar_init(sh.tile_empty + i, kEpi);
         }
         *sh.abort = 0;
         tc::mbar_fence_init();
     }
-    for (uint32_t g = tid; g < l.groups; g += kMmThreads) {
+    for (uint32_t g = tid; g < l.groups; g += mm_threads(MODE, EPI)) {
         uint32_t lo, hi;
         group_range(l, g, lo, hi);
         sh.lo[g] = lo;
         sh.cnt[g] = hi - lo;
     }
     __syncthreads();
-    if (warp == kMmEpiWarps + 1u) {
+    if (warp == kEpi + 1u) {
         // token tiles before each group, 32 groups a step
         uint32_t run = 0;
         for (uint32_t g0 = 0; g0 < l.groups; g0 += 32u) {
@@ -936,46 +955,111 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         ++it;
         return true;
     };
-    // 32 tokens from c on of channel n, with an epilogue; the whole warp. Of SwiGLU's pairs (neighbouring
-    // lanes) the even lane takes the even tokens, the odd lane the odd ones, against one exchange for two.
-    [[maybe_unused]] auto finish = [&](const uint32_t (&v)[32], const MmTile& tile, uint32_t c, uint32_t n, const float* ts,
-                                       const float* rw, float cs, float bias) {
-        const TY* from = static_cast<const TY*>(l.residual);
-        TY* y = static_cast<TY*>(l.y);
-        if (l.act == VLB_ACT_SWIGLU) {
-            const uint32_t odd = lane & 1u;
-            const bool in = n < l.out_cols;
-            TY res[16];
+    // Whether `ok` holds in the four warps of a turn; each of them comes here once a tile, its waits behind it.
+    [[maybe_unused]] auto all_of_turn = [&](bool ok) -> bool {
+        uint32_t all;
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t"
+            "setp.ne.u32 q, %1, 0;\n\t"
+            "barrier.cta.red.and.pred p, %2, 128, q;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t}"
+            : "=r"(all)
+            : "r"(ok ? 1u : 0u), "r"(1u + (warp >> 2))
+            : "memory");
+        return all != 0;
+    };
+    // 16 tokens from c on of the CTA's 128 channels (64 columns of y for SwiGLU), with an epilogue: the four warps of a
+    // turn. act(z) goes to shared memory, and comes back in rows of y: 16 bytes a thread of neighbouring columns, with
+    // the residual's loaded before. (Stored from where the sums are, a channel a lane, the tokens' rows are 64 bytes a
+    // store: 4096 x 4096 x 4096 f16 with GELU and a residual 88 us.)
+    [[maybe_unused]] auto finish = [&](const float (&v)[16], const MmTile& tile, uint32_t c, const float* ts, const float* rw,
+                                       float cs, float bias) {
+        constexpr uint32_t E = 16u / sizeof(TY);
+        const uint32_t turn = warp >> 2, t = tid & 127u, count = min(tile.count - c, 16u);
+        const auto put = [&](auto act) {
+            constexpr int ACT = decltype(act)::value;
+            constexpr bool PAIRS = ACT == VLB_ACT_SWIGLU;
+            constexpr uint32_t kCols = PAIRS ? 64u : 128u, kPitch = PAIRS ? 80u : 128u;  // the pitch keeps pairs off each other's banks
+            constexpr uint32_t kAcross = kCols / E, kRows = 128u / kAcross, kPasses = 16u / kRows;
+            float* at = sh.out + turn * (16u * kMmChannels);
+            const uint32_t y_cols = PAIRS ? l.out_cols / 2u : l.out_cols;
+            const uint32_t col = (tile.channel0 + (PAIR ? rank * kMmChannels : 0u)) / (PAIRS ? 2u : 1u) + t % kAcross * E;
+            const uint32_t wide = p.wide && col + E <= y_cols ? E : 0u, n_cols = col < y_cols ? min(E, y_cols - col) : 0u;
+            const size_t r0 = tile.row0 + c + t / kAcross;
+            Pack<TY, E> res[kPasses];
+            if (l.residual) {
 #pragma unroll
-            for (uint32_t i = 0; i < 16u; ++i) {
-                const uint32_t j = c + 2u * i + odd;
-                res[i] = from_float<TY>(0.f);
-                if (from && in && j < tile.count) res[i] = from[(size_t)(tile.row0 + j) * l.residual_stride + n / 2u];
+                for (uint32_t i = 0; i < kPasses; ++i) {
+                    const TY* from = static_cast<const TY*>(l.residual) + (r0 + i * kRows) * l.residual_stride + col;
+                    if (t / kAcross + i * kRows >= count) continue;
+                    if (wide) {
+                        res[i] = *reinterpret_cast<const Pack<TY, E>*>(from);
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < E; ++j)
+                            if (j < n_cols) res[i].v[j] = from[j];
+                    }
+                }
             }
+            const float4* t4 = reinterpret_cast<const float4*>(ts + c);
+            const uint32_t odd = lane & 1u;  // of a pair's lanes the even one takes the even tokens
 #pragma unroll
-            for (uint32_t i = 0; i < 16u; ++i) {
-                const uint32_t j = c + 2u * i;
-                const float z0 = epi_sum((int32_t)v[2 * i], ts[j], cs, bias);
-                const float z1 = epi_sum((int32_t)v[2 * i + 1], ts[j + 1u], cs, bias);
-                const float other = __shfl_xor_sync(0xffffffffu, odd ? z0 : z1, 1);
-                const float a = odd ? swiglu(other, z1, l.act_limit) : swiglu(z0, other, l.act_limit);
-                if (in && j + odd < tile.count)
-                    y[(size_t)(tile.row0 + j + odd) * l.y_stride + n / 2u] = from_float<TY>(fmaf(rw[j + odd], a, to_float(res[i])));
+            for (uint32_t i0 = 0; i0 < 16u; i0 += 4u) {
+                const float4 s4 = t4[i0 / 4u];
+                float z[4];
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; ++j) z[j] = epi_sum(__float_as_int(v[i0 + j]), (&s4.x)[j], cs, bias);
+                if constexpr (PAIRS) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; j += 2u) {  // one exchange for two tokens
+                        const float other = __shfl_xor_sync(0xffffffffu, odd ? z[j] : z[j + 1u], 1);
+                        at[(i0 + j + odd) * kPitch + 16u * quad + lane / 2u] =
+                            swiglu(odd ? other : z[j], odd ? z[j + 1u] : other, l.act_limit);
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; ++j) at[(i0 + j) * kPitch + 32u * quad + lane] = activate<ACT>(z[j]);
+                }
             }
-            return;
-        }
-        if (n >= l.out_cols) return;
-        TY res[32];
+            asm volatile("bar.sync %0, 128;" ::"r"(1u + turn) : "memory");
 #pragma unroll
-        for (uint32_t i = 0; i < 32u; ++i) {
-            res[i] = from_float<TY>(0.f);
-            if (from && c + i < tile.count) res[i] = from[(size_t)(tile.row0 + c + i) * l.residual_stride + n];
-        }
+            for (uint32_t i = 0; i < kPasses; ++i) {
+                const uint32_t row = t / kAcross + i * kRows;
+                float f[E];
 #pragma unroll
-        for (uint32_t i = 0; i < 32u; ++i) {
-            const float a = activate(epi_sum((int32_t)v[i], ts[c + i], cs, bias), l.act);
-            if (c + i < tile.count)
-                y[(size_t)(tile.row0 + c + i) * l.y_stride + n] = from_float<TY>(fmaf(rw[c + i], a, to_float(res[i])));
+                for (uint32_t j = 0; j < E; j += 4u)
+                    *reinterpret_cast<float4*>(f + j) = *reinterpret_cast<const float4*>(at + row * kPitch + t % kAcross * E + j);
+                const float w = rw[c + row];
+                if (l.residual) {
+                    float g[E];
+                    unpack(res[i], g);
+#pragma unroll
+                    for (uint32_t j = 0; j < E; ++j) f[j] = fmaf(w, f[j], g[j]);
+                } else {
+#pragma unroll
+                    for (uint32_t j = 0; j < E; ++j) f[j] *= w;
+                }
+                const Pack<TY, E> out = pack<TY>(f);
+                if (row >= count) continue;
+                TY* y = static_cast<TY*>(l.y) + (r0 + i * kRows) * l.y_stride + col;
+                if (wide) {
+                    *reinterpret_cast<Pack<TY, E>*>(y) = out;
+                } else {
+#pragma unroll
+                    for (uint32_t j = 0; j < E; ++j)
+                        if (j < n_cols) y[j] = out.v[j];
+                }
+            }
+            asm volatile("bar.sync %0, 128;" ::"r"(1u + turn) : "memory");
+        };
+        // one branch for all of them, whose chains then run side by side
+        switch (l.act) {
+            case VLB_ACT_RELU: return put(std::integral_constant<int, VLB_ACT_RELU>{});
+            case VLB_ACT_SILU: return put(std::integral_constant<int, VLB_ACT_SILU>{});
+            case VLB_ACT_GELU: return put(std::integral_constant<int, VLB_ACT_GELU>{});
+            case VLB_ACT_GELU_TANH: return put(std::integral_constant<int, VLB_ACT_GELU_TANH>{});
+            case VLB_ACT_SWIGLU: return put(std::integral_constant<int, VLB_ACT_SWIGLU>{});
+            default: return put(std::integral_constant<int, VLB_ACT_NONE>{});
         }
     };
     auto epilogue = [&]() -> bool {
@@ -986,19 +1070,27 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         const float cs = sh.channel[buf * kMmChannels + 32u * quad + lane];
         const uint32_t n = tile.channel0 + (PAIR ? rank * kMmChannels : 0u) + 32u * quad + lane;
         ok = ok && __all_sync(0xffffffffu, mm_wait(sh.acc_full + buf, use & 1u, sh.abort));
+        if constexpr (EPI) ok = all_of_turn(ok);  // the four warps go on to their barriers, or give up, together
         if (ok) {
             tc::fence_after_sync();
             const uint32_t src = tmem + buf * p.acc_cols + ((32u * quad) << 16);
+            if constexpr (EPI) {
+                const float bias = sh.bias[buf * kMmChannels + 32u * quad + lane];
+                for (uint32_t c = 16u * half; c < tile.count; c += 4u * kEpi) {
+                    float v[16];
+                    tc::tmem_ld16(src + c, v);
+                    tc::tmem_wait_ld();
+                    finish(v, tile, c, ts, sh.weight + buf * kMmMaxTokens, cs, bias);
+                }
+            }
             // 32 columns (tokens) at a time, the warps of a lane quarter taking turns
-            for (uint32_t c = 32u * half; c < tile.count; c += 64u) {
+            for (uint32_t c = 32u * half; !EPI && c < tile.count; c += 64u) {
                 uint32_t v[32];
                 tc::tmem_ld32(src + c, v);
                 tc::tmem_wait_ld();
                 TY* y = static_cast<TY*>(l.y) + (size_t)(tile.row0 + c) * l.y_stride + n;
                 const float4* t4 = reinterpret_cast<const float4*>(ts + c);
-                if constexpr (EPI) {
-                    finish(v, tile, c, n, ts, sh.weight + buf * kMmMaxTokens, cs, sh.bias[buf * kMmChannels + 32u * quad + lane]);
-                } else if (tile.count - c >= 32u && n - lane + 32u <= l.out_cols) {
+                if (tile.count - c >= 32u && n - lane + 32u <= l.out_cols) {
 #pragma unroll
                     for (uint32_t i = 0; i < 32u; i += 4u) {
                         const float4 t = t4[i / 4u];
@@ -1030,19 +1122,19 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
     };
 
     if (!SPLIT) {
-        if (warp < kMmEpiWarps) {
+        if (warp < kEpi) {
             for (uint32_t t = begin; t < total; t += step)
                 if (!epilogue()) {
                     if (lane == 0) mm_fail(sh.abort, l);
                     break;
                 }
-        } else if (warp == kMmEpiWarps) {
+        } else if (warp == kEpi) {
             for (uint32_t t = begin; t < total; t += step)
                 if (!produce(t)) {
                     if (lane == 0) mm_fail(sh.abort, l);
                     break;
                 }
-        } else if (warp == kMmEpiWarps + 2u) {
+        } else if (warp == kEpi + 2u) {
             for (uint32_t t = begin; t < total; t += step)
                 if (!place(t)) {
                     if (lane == 0) mm_fail(sh.abort, l);
@@ -1064,11 +1156,11 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
             bool ok = true;
             float cs[4] = {}, bs[4] = {};
             float* ts = sh.scale;
-            if (warp == kMmEpiWarps) {
+            if (warp == kEpi) {
                 ok = __all_sync(0xffffffffu, *sh.abort == 0) && produce(t);
-            } else if (warp == kMmEpiWarps + 1u) {
+            } else if (warp == kEpi + 1u) {
                 ok = __all_sync(0xffffffffu, *sh.abort == 0) && multiply(t);
-            } else if (warp < kMmEpiWarps) {
+            } else if (warp < kEpi) {
                 if (!waited) {
                     tc::grid_dependency_wait();
                     waited = true;
@@ -1103,10 +1195,10 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
             if (!ok && lane == 0) mm_fail(sh.abort, l);
             __syncwarp();
             tc::cluster_sync();
-            if (warp < kMmEpiWarps) {
+            if (warp < kEpi) {
                 // a warp takes every split-th token, a lane four neighbouring channels: the loads of two
                 // tokens from all peers are in flight together
-                const uint32_t pace = kMmEpiWarps * p.split, c = 4u * lane, n = tile.channel0 + c;
+                const uint32_t pace = kEpi * p.split, c = 4u * lane, n = tile.channel0 + c;
                 for (uint32_t j = rank + p.split * warp; j < tile.count; j += 2u * pace) {
                     uint4 v[2][8];
 #pragma unroll
@@ -1156,13 +1248,13 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
     }
     if (!waited) tc::grid_dependency_wait();  // also a CTA without a tile
     __syncthreads();
-    if (warp == kMmEpiWarps && lane == 0 && dirty) {
+    if (warp == kEpi && lane == 0 && dirty) {
         // after giving up: copies already issued land before the CTA's shared memory goes away
         const uint64_t t0 = tc::global_ns();
         while (tc::global_ns() - t0 < 1000000ull) {
         }
     }
-    if (warp == kMmEpiWarps + 1u && pending && tc::elect_lane()) {
+    if (warp == kEpi + 1u && pending && tc::elect_lane()) {
         commit(sh.acc_full + pending_bar);
         const uint64_t t0 = tc::global_ns();
         while (!tc::mbar_try(sh.acc_full + pending_bar, pending_parity) && tc::global_ns() - t0 < kMmWaitNs) {
@@ -1174,7 +1266,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) int8_mma_kernel(const __grid_co
         tc::fence_before_sync();
         tc::cluster_sync();
     }
-    if (warp == kMmEpiWarps) {
+    if (warp == kEpi) {
         tc::fence_after_sync();
         if (PAIR) tc::tmem_dealloc_pair(tmem, p.tmem_cols);
         else tc::tmem_dealloc(tmem, p.tmem_cols);
@@ -1324,7 +1416,7 @@ Mm mma_plan(Int8MmaParams& p, uint32_t sms) {
     p.acc_cols = p.width < 32u ? 32u : p.width;
     p.tmem_cols = 32;
     while (p.tmem_cols < (mode == Mm::kSplit ? 1u : 2u) * p.acc_cols) p.tmem_cols *= 2u;
-    const uint32_t room = kMmSmemLimit - 1024u - mm_fixed_bytes(l.groups, l.act != kInt8NoEpilogue);
+    const uint32_t room = kMmSmemLimit - 1024u - mm_fixed_bytes(l.groups, mode, l.act != kInt8NoEpilogue);
     p.stages = room / (kMmWStage + p.x_stage);
     if (p.stages > kMmMaxStages) p.stages = kMmMaxStages;
     return mode;
@@ -1336,8 +1428,8 @@ cudaError_t mma_launch(const Int8MmaParams& p, uint32_t sms, cudaStream_t s) {
     const uint32_t in_cluster = MODE == Mm::kSplit ? p.split : MODE == Mm::kPair ? 2u : 1u;
     cudaError_t e = smem_once(kernel, kMmSmemLimit);
     if (e != cudaSuccess) return e;
-    const size_t smem = p.stages * (kMmWStage + p.x_stage) + mm_fixed_bytes(p.l.groups, EPI);
-    return launch_chained(kernel, dim3(sms / in_cluster * in_cluster), kMmThreads, smem, MODE == Mm::kOne ? 0 : in_cluster, s, p);
+    const size_t smem = p.stages * (kMmWStage + p.x_stage) + mm_fixed_bytes(p.l.groups, MODE, EPI);
+    return launch_chained(kernel, dim3(sms / in_cluster * in_cluster), mm_threads(MODE, EPI), smem, MODE == Mm::kOne ? 0 : in_cluster, s, p);
 }
 
 // What int8_few_kernel takes. Dense: up to kFewRows rows, from 3 on no more than kFewElements elements
@@ -1380,6 +1472,10 @@ cudaError_t linear_type(const Int8LinearParams& l, bool after_quantize, cudaStre
         Int8MmaParams p{};
         p.l = l;
         p.early = after_quantize;
+        const auto on16 = [](const void* at, size_t stride) {
+            return reinterpret_cast<uintptr_t>(at) % 16u == 0 && stride * sizeof(TY) % 16u == 0;
+        };
+        p.wide = EPI && on16(l.y, l.y_stride) && (!l.residual || on16(l.residual, l.residual_stride));
         const uint32_t sms = sm_count();
         const Mm mode = mma_plan(p, sms);
         if (encode_rows(&p.wmap, l.w, (uint64_t)l.groups * l.out_cols, l.cols, l.w_stride, kMmChannels) &&
