@@ -514,6 +514,21 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(ROWS)) int8_few_kernel
         }
     };
     if (n < n_end) fetch(n, 0);
+    // with an epilogue the channels' scales and biases come beside their weights too (lane j those of channel n + j / ROWS,
+    // of a SwiGLU pair both), not after the sums
+    [[maybe_unused]] float ws[2] = {}, bs[2] = {};
+    [[maybe_unused]] const auto fetch_scales = [&](uint32_t n) {
+        const bool pairs = l.act == VLB_ACT_SWIGLU;
+        const uint32_t c = n + (pairs ? 0u : lane / ROWS);
+        const size_t at = (size_t)g * l.out_cols + c;
+#pragma unroll
+        for (uint32_t i = 0; i < 2u; ++i) {
+            if (lane >= 2u * ROWS || c + i >= l.out_cols || (i && !pairs)) continue;
+            ws[i] = l.w_scale[at + i];
+            if (l.bias) bs[i] = l.bias[at + i];
+        }
+    };
+    if (EPI && n < n_end) fetch_scales(n);
     // the rows: warps share them out, each row's warps its columns
     if (tid < ROWS) top[tid] = 0;
     __syncthreads();
@@ -532,18 +547,48 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(ROWS)) int8_few_kernel
         const auto value = [&](uint32_t c) {
             return q.up ? row_value<T, true>(q, base + c) : row_value<T, false>(q, base + c);
         };
+        // a lane's first kFewKeep elements stay in registers between the row's maximum and its rounding
+        constexpr uint32_t kFewKeep = 16;
+        float kept[kFewKeep];
+        const uint32_t step = row_warps * 32u;
         uint32_t most = 0;
+        {
+            T a[kFewKeep];  // all loads first
+#pragma unroll
+            for (uint32_t i = 0; i < kFewKeep; ++i) {
+                a[i] = from_float<T>(0.f);
+                if (have && part + i * step < l.cols) a[i] = static_cast<const T*>(q.x)[base + part + i * step];
+            }
+            if (q.up) {
+                T b[kFewKeep];
+#pragma unroll
+                for (uint32_t i = 0; i < kFewKeep; ++i) {
+                    b[i] = from_float<T>(0.f);
+                    if (have && part + i * step < l.cols) b[i] = static_cast<const T*>(q.up)[base + part + i * step];
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < kFewKeep; ++i) kept[i] = swiglu(to_float(a[i]), to_float(b[i]), q.limit);
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < kFewKeep; ++i) kept[i] = to_float(a[i]);
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kFewKeep; ++i) most = max(most, __float_as_uint(kept[i]) & 0x7fffffffu);
         if (have)
 #pragma unroll 8
-            for (uint32_t c = part; c < l.cols; c += row_warps * 32u)
+            for (uint32_t c = part + kFewKeep * step; c < l.cols; c += step)
                 most = max(most, __float_as_uint(value(c)) & 0x7fffffffu);
         most = __reduce_max_sync(0xffffffffu, most);
         if (lane == 0) atomicMax(top + m, most);
         __syncthreads();
         const RowStep st = row_step(top[m]);
         if (m < rows && part == 0) scale[m] = !EPI && l.row_weight ? st.scale * l.row_weight[r] : st.scale;
+#pragma unroll
+        for (uint32_t i = 0; i < kFewKeep; ++i)
+            if (part + i * step < pitch) xs[m * pitch + part + i * step] = (int8_t)quant_byte(kept[i], st);
 #pragma unroll 8
-        for (uint32_t c = part; c < pitch; c += row_warps * 32u)
+        for (uint32_t c = part + kFewKeep * step; c < pitch; c += step)
             xs[m * pitch + c] = (int8_t)(have && c < l.cols ? quant_byte(value(c), st) : 0u);
     }
     __syncthreads();
@@ -588,16 +633,17 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(ROWS)) int8_few_kernel
         if constexpr (EPI) {
             const bool pairs = l.act == VLB_ACT_SWIGLU;
             if (lane < (pairs ? 1u : 2u) * ROWS && j < rows && c < n_end) {
-                const size_t at = (size_t)g * l.out_cols + c, r = row0 + j;
-                float a = epi_sum(mine, scale[j], l.w_scale[at], l.bias ? l.bias[at] : 0.f);
+                const size_t r = row0 + j;
+                float a = epi_sum(mine, scale[j], ws[0], bs[0]);
                 if (pairs)
-                    a = swiglu(a, epi_sum(second, scale[j], l.w_scale[at + 1u], l.bias ? l.bias[at + 1u] : 0.f), l.act_limit);
+                    a = swiglu(a, epi_sum(second, scale[j], ws[1], bs[1]), l.act_limit);
                 else
                     a = activate(a, l.act);
                 const uint32_t to = pairs ? c / 2u : c;
                 const float res = l.residual ? load_typed(l.residual, r * l.residual_stride + to, y_type) : 0.f;
                 store_typed(l.y, r * l.y_stride + to, fmaf(l.row_weight ? l.row_weight[r] : 1.f, a, res), y_type);
             }
+            if (n + 2u * kFewWarps < n_end) fetch_scales(n + 2u * kFewWarps);
             continue;
         }
         if (lane < 2u * ROWS && j < rows && c < n_end)
@@ -642,7 +688,6 @@ struct Int8MmaParams {
     uint32_t ct, nk;    // channel tiles, K chunks
     uint32_t tmem_cols, acc_cols;
     uint32_t split;
-    uint32_t wide;      // rows of y and of the residual lie on 16-byte boundaries
     uint32_t early;     // the kernel ahead quantizes the tokens: weights may be loaded beside it
 };
 
@@ -722,7 +767,9 @@ __device__ __forceinline__ MmTile mm_tile(const MmShared& sh, const Int8MmaParam
     return MmTile{a, sh.lo[a] + j * each + min(j, more), each + (j < more ? 1u : 0u), c * p.channels};
 }
 
-template <typename TY, Mm MODE, bool EPI>
+// WIDE_Y: with an epilogue, rows of y and of the residual lie on 16-byte boundaries (a kernel of its own: the other form's
+// registers would spill into it).
+template <typename TY, Mm MODE, bool EPI, bool WIDE_Y>
 __global__ void __launch_bounds__(mm_threads(MODE, EPI), 1) int8_mma_kernel(const __grid_constant__ Int8MmaParams p) {
     constexpr bool SPLIT = MODE == Mm::kSplit, PAIR = MODE == Mm::kPair;
     constexpr uint32_t kEpi = mm_epi_warps(MODE, EPI);
@@ -976,29 +1023,34 @@ __global__ void __launch_bounds__(mm_threads(MODE, EPI), 1) int8_mma_kernel(cons
                                        float cs, float bias) {
         constexpr uint32_t E = 16u / sizeof(TY);
         const uint32_t turn = warp >> 2, t = tid & 127u, count = min(tile.count - c, 16u);
-        const auto put = [&](auto act) {
+        const auto put = [&](auto act, auto whole) {
             constexpr int ACT = decltype(act)::value;
-            constexpr bool PAIRS = ACT == VLB_ACT_SWIGLU;
-            constexpr uint32_t kCols = PAIRS ? 64u : 128u, kPitch = PAIRS ? 80u : 128u;  // the pitch keeps pairs off each other's banks
-            constexpr uint32_t kAcross = kCols / E, kRows = 128u / kAcross, kPasses = 16u / kRows;
+            // WIDE: 16 bytes a thread; rows of y at any offset: neighbouring lanes on neighbouring columns
+            constexpr bool PAIRS = ACT == VLB_ACT_SWIGLU, WIDE = decltype(whole)::value;
+            constexpr uint32_t kEach = WIDE ? E : 1u, kCols = PAIRS ? 64u : 128u;
+            constexpr uint32_t kPitch = PAIRS ? 80u : 128u;  // the pitch keeps pairs off each other's banks
+            constexpr uint32_t kAcross = kCols / kEach, kRows = 128u / kAcross, kPasses = 16u / kRows;
             float* at = sh.out + turn * (16u * kMmChannels);
             const uint32_t y_cols = PAIRS ? l.out_cols / 2u : l.out_cols;
-            const uint32_t col = (tile.channel0 + (PAIR ? rank * kMmChannels : 0u)) / (PAIRS ? 2u : 1u) + t % kAcross * E;
-            const uint32_t wide = p.wide && col + E <= y_cols ? E : 0u, n_cols = col < y_cols ? min(E, y_cols - col) : 0u;
-            const size_t r0 = tile.row0 + c + t / kAcross;
-            Pack<TY, E> res[kPasses];
+            const uint32_t col = (tile.channel0 + (PAIR ? rank * kMmChannels : 0u)) / (PAIRS ? 2u : 1u) + t % kAcross * kEach;
+            const uint32_t n_cols = col < y_cols ? min(kEach, y_cols - col) : 0u;
+            const uint32_t row0 = t / kAcross, rows = n_cols ? count : 0u;  // of this thread: row0, row0 + kRows, ..
+            const size_t r0 = tile.row0 + c + row0;
+            Pack<TY, kEach> res[kPasses];
             if (l.residual) {
+                const TY* from = static_cast<const TY*>(l.residual) + r0 * l.residual_stride + col;
 #pragma unroll
                 for (uint32_t i = 0; i < kPasses; ++i) {
-                    const TY* from = static_cast<const TY*>(l.residual) + (r0 + i * kRows) * l.residual_stride + col;
-                    if (t / kAcross + i * kRows >= count) continue;
-                    if (wide) {
-                        res[i] = *reinterpret_cast<const Pack<TY, E>*>(from);
-                    } else {
+                    if (row0 + i * kRows < rows) {
+                        if (n_cols == kEach) {
+                            res[i] = *reinterpret_cast<const Pack<TY, kEach>*>(from);
+                        } else {
 #pragma unroll
-                        for (uint32_t j = 0; j < E; ++j)
-                            if (j < n_cols) res[i].v[j] = from[j];
+                            for (uint32_t j = 0; j < kEach; ++j)
+                                if (j < n_cols) res[i].v[j] = from[j];
+                        }
                     }
+                    from += kRows * l.residual_stride;
                 }
             }
             const float4* t4 = reinterpret_cast<const float4*>(ts + c);
@@ -1022,45 +1074,49 @@ __global__ void __launch_bounds__(mm_threads(MODE, EPI), 1) int8_mma_kernel(cons
                 }
             }
             asm volatile("bar.sync %0, 128;" ::"r"(1u + turn) : "memory");
+            TY* y = static_cast<TY*>(l.y) + r0 * l.y_stride + col;
 #pragma unroll
             for (uint32_t i = 0; i < kPasses; ++i) {
-                const uint32_t row = t / kAcross + i * kRows;
-                float f[E];
-#pragma unroll
-                for (uint32_t j = 0; j < E; j += 4u)
-                    *reinterpret_cast<float4*>(f + j) = *reinterpret_cast<const float4*>(at + row * kPitch + t % kAcross * E + j);
+                const uint32_t row = row0 + i * kRows;
+                float f[kEach];
+                const Pack<float, kEach> sums = *reinterpret_cast<const Pack<float, kEach>*>(at + row * kPitch + t % kAcross * kEach);
+                unpack(sums, f);
                 const float w = rw[c + row];
                 if (l.residual) {
-                    float g[E];
+                    float g[kEach];
                     unpack(res[i], g);
 #pragma unroll
-                    for (uint32_t j = 0; j < E; ++j) f[j] = fmaf(w, f[j], g[j]);
+                    for (uint32_t j = 0; j < kEach; ++j) f[j] = fmaf(w, f[j], g[j]);
                 } else {
 #pragma unroll
-                    for (uint32_t j = 0; j < E; ++j) f[j] *= w;
+                    for (uint32_t j = 0; j < kEach; ++j) f[j] *= w;
                 }
-                const Pack<TY, E> out = pack<TY>(f);
-                if (row >= count) continue;
-                TY* y = static_cast<TY*>(l.y) + (r0 + i * kRows) * l.y_stride + col;
-                if (wide) {
-                    *reinterpret_cast<Pack<TY, E>*>(y) = out;
-                } else {
+                const Pack<TY, kEach> out = pack<TY>(f);
+                if (row < rows) {
+                    if (n_cols == kEach) {
+                        *reinterpret_cast<Pack<TY, kEach>*>(y) = out;
+                    } else {
 #pragma unroll
-                    for (uint32_t j = 0; j < E; ++j)
-                        if (j < n_cols) y[j] = out.v[j];
+                        for (uint32_t j = 0; j < kEach; ++j)
+                            if (j < n_cols) y[j] = out.v[j];
+                    }
                 }
+                y += kRows * l.y_stride;
             }
             asm volatile("bar.sync %0, 128;" ::"r"(1u + turn) : "memory");
         };
         // one branch for all of them, whose chains then run side by side
-        switch (l.act) {
-            case VLB_ACT_RELU: return put(std::integral_constant<int, VLB_ACT_RELU>{});
-            case VLB_ACT_SILU: return put(std::integral_constant<int, VLB_ACT_SILU>{});
-            case VLB_ACT_GELU: return put(std::integral_constant<int, VLB_ACT_GELU>{});
-            case VLB_ACT_GELU_TANH: return put(std::integral_constant<int, VLB_ACT_GELU_TANH>{});
-            case VLB_ACT_SWIGLU: return put(std::integral_constant<int, VLB_ACT_SWIGLU>{});
-            default: return put(std::integral_constant<int, VLB_ACT_NONE>{});
-        }
+        const auto by_act = [&](auto whole) {
+            switch (l.act) {
+                case VLB_ACT_RELU: return put(std::integral_constant<int, VLB_ACT_RELU>{}, whole);
+                case VLB_ACT_SILU: return put(std::integral_constant<int, VLB_ACT_SILU>{}, whole);
+                case VLB_ACT_GELU: return put(std::integral_constant<int, VLB_ACT_GELU>{}, whole);
+                case VLB_ACT_GELU_TANH: return put(std::integral_constant<int, VLB_ACT_GELU_TANH>{}, whole);
+                case VLB_ACT_SWIGLU: return put(std::integral_constant<int, VLB_ACT_SWIGLU>{}, whole);
+                default: return put(std::integral_constant<int, VLB_ACT_NONE>{}, whole);
+            }
+        };
+        by_act(std::integral_constant<bool, WIDE_Y>{});
     };
     auto epilogue = [&]() -> bool {
         const uint32_t buf = it & 1u, use = it >> 1;
@@ -1423,8 +1479,9 @@ Mm mma_plan(Int8MmaParams& p, uint32_t sms) {
 }
 
 template <typename TY, Mm MODE, bool EPI>
-cudaError_t mma_launch(const Int8MmaParams& p, uint32_t sms, cudaStream_t s) {
-    auto* kernel = int8_mma_kernel<TY, MODE, EPI>;
+cudaError_t mma_launch(const Int8MmaParams& p, uint32_t sms, bool wide, cudaStream_t s) {
+    constexpr bool kForms = EPI && MODE != Mm::kSplit;  // a split's sums take another way out
+    auto* kernel = wide && kForms ? int8_mma_kernel<TY, MODE, EPI, kForms> : int8_mma_kernel<TY, MODE, EPI, false>;
     const uint32_t in_cluster = MODE == Mm::kSplit ? p.split : MODE == Mm::kPair ? 2u : 1u;
     cudaError_t e = smem_once(kernel, kMmSmemLimit);
     if (e != cudaSuccess) return e;
@@ -1475,14 +1532,14 @@ cudaError_t linear_type(const Int8LinearParams& l, bool after_quantize, cudaStre
         const auto on16 = [](const void* at, size_t stride) {
             return reinterpret_cast<uintptr_t>(at) % 16u == 0 && stride * sizeof(TY) % 16u == 0;
         };
-        p.wide = EPI && on16(l.y, l.y_stride) && (!l.residual || on16(l.residual, l.residual_stride));
+        const bool wide = EPI && on16(l.y, l.y_stride) && (!l.residual || on16(l.residual, l.residual_stride));
         const uint32_t sms = sm_count();
         const Mm mode = mma_plan(p, sms);
         if (encode_rows(&p.wmap, l.w, (uint64_t)l.groups * l.out_cols, l.cols, l.w_stride, kMmChannels) &&
             encode_rows(&p.xmap, l.x, l.rows, l.cols, l.x_stride, p.box))
-            return mode == Mm::kPair    ? mma_launch<TY, Mm::kPair, EPI>(p, sms, s)
-                   : mode == Mm::kSplit ? mma_launch<TY, Mm::kSplit, EPI>(p, sms, s)
-                                        : mma_launch<TY, Mm::kOne, EPI>(p, sms, s);
+            return mode == Mm::kPair    ? mma_launch<TY, Mm::kPair, EPI>(p, sms, wide, s)
+                   : mode == Mm::kSplit ? mma_launch<TY, Mm::kSplit, EPI>(p, sms, wide, s)
+                                        : mma_launch<TY, Mm::kOne, EPI>(p, sms, wide, s);
     }
     return general_type<TY, EPI>(l, s);
 }

@@ -90,7 +90,8 @@ __device__ __forceinline__ void row_weights(const float* weight, int32_t c0, uin
     for (uint32_t i = 0; i < KEEP; ++i) {
         const int32_t c = c0 + (int32_t)(i * ROW * V);
         if (wide && inside(c, V, cols)) {
-            unpack(*reinterpret_cast<const Pack<float, V>*>(weight + c), w[i]);
+            const Pack<float, V> a = *reinterpret_cast<const Pack<float, V>*>(weight + c);
+            unpack(a, w[i]);
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < V; ++j)
@@ -369,46 +370,33 @@ __device__ __forceinline__ void norm_grad_row(const NormGradParams& p, size_t r,
     }
 }
 
-// The CTA's part of the weight's gradient: its rows' sums added in order in shared memory, column by column (rows
-// at different offsets have a column in different threads). all: room for a row of floats and a 32nd.
-template <uint32_t V, uint32_t ROW, uint32_t KEEP, uint32_t THREADS, bool SHIFTED>
+// The CTA's part of the weight's gradient: its rows' sums side by side in shared memory, added in order column by
+// column (rows at different offsets have a column in different threads). all: for each row room for its columns and
+// a 32nd, less than the ring holds of a row.
+template <uint32_t V, uint32_t ROW, uint32_t KEEP, uint32_t THREADS>
 __device__ __forceinline__ void norm_grad_part(const NormGradParams& p, int32_t c0, const float (&acc)[KEEP][V], float* all) {
     constexpr uint32_t kRows = THREADS / ROW, kStep = ROW * V;
     float* part = p.part + (size_t)blockIdx.x * p.cols;
-    const auto each = [&](auto&& f) {
+    const auto place = [](uint32_t c) { return c + c / 32u; };  // lanes V columns apart on banks of their own
+    const uint32_t pitch = place(p.cols) + 1u;
+    if constexpr (kRows > 1u) __syncthreads();  // the ring is read
 #pragma unroll
-        for (uint32_t i = 0; i < KEEP; ++i)
+    for (uint32_t i = 0; i < KEEP; ++i)
 #pragma unroll
-            for (uint32_t j = 0; j < V; ++j) {
-                const uint32_t c = (uint32_t)(c0 + (int32_t)(i * kStep + j));
-                if (c < p.cols) f(c, acc[i][j]);
-            }
-    };
-    if constexpr (kRows == 1u) {
-        each([&](uint32_t c, float v) { part[c] = v; });
-    } else {
-        [[maybe_unused]] const auto place = [](uint32_t c) { return c + c / 32u; };  // lanes V columns apart on banks of their own
-        for (uint32_t k = 0; k < kRows; ++k) {
-            __syncthreads();
-            if (threadIdx.x / ROW != k) continue;
-            if constexpr (SHIFTED) {
-                if (k == 0) each([&](uint32_t c, float v) { all[place(c)] = v; });
-                else each([&](uint32_t c, float v) { all[place(c)] += v; });
-            } else {
-#pragma unroll
-                for (uint32_t i = 0; i < KEEP; ++i) {
-                    float4* to = reinterpret_cast<float4*>(all + c0 + i * kStep);
-#pragma unroll
-                    for (uint32_t j = 0; j < V; j += 4u) {
-                        float4 v = k ? to[j / 4u] : make_float4(0.f, 0.f, 0.f, 0.f);
-                        v.x += acc[i][j], v.y += acc[i][j + 1u], v.z += acc[i][j + 2u], v.w += acc[i][j + 3u];
-                        to[j / 4u] = v;
-                    }
-                }
-            }
+        for (uint32_t j = 0; j < V; ++j) {
+            const uint32_t c = (uint32_t)(c0 + (int32_t)(i * kStep + j));
+            if (c >= p.cols) continue;
+            if constexpr (kRows == 1u) part[c] = acc[i][j];
+            else all[threadIdx.x / ROW * pitch + place(c)] = acc[i][j];
         }
+    if constexpr (kRows > 1u) {
         __syncthreads();
-        for (uint32_t c = threadIdx.x; c < p.cols; c += THREADS) part[c] = all[SHIFTED ? place(c) : c];
+        for (uint32_t c = threadIdx.x; c < p.cols; c += THREADS) {
+            float v = all[place(c)];
+#pragma unroll
+            for (uint32_t k = 1; k < kRows; ++k) v += all[k * pitch + place(c)];
+            part[c] = v;
+        }
     }
 }
 
@@ -438,7 +426,7 @@ __global__ void __launch_bounds__(ROW) norm_grad_kernel(const NormGradParams p) 
             p, r, c0, [&](uint32_t i) { return dy[i]; }, [&](uint32_t i) { return h[i]; }, [&](uint32_t i) { return dh[i]; }, w,
             acc, reduce, reduce2);
     }
-    if (p.dw) norm_grad_part<V, ROW, KEEP, ROW, false>(p, c0, acc, nullptr);
+    if (p.dw) norm_grad_part<V, ROW, KEEP, ROW>(p, c0, acc, nullptr);
 }
 
 // Many rows, as add_norm_ring_kernel; a CTA an SM, so that few parts are left. 8192 x 4096 bf16 with dh and dw:
@@ -489,7 +477,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) norm_grad_ring_kernel(const N
         ring.next();
     }
     tc::cp_async_wait_all();
-    if (p.dw) norm_grad_part<V, ROW, KEEP, kThreads, SHIFTED>(p, c0, acc, reinterpret_cast<float*>(ring_smem));
+    if (p.dw) norm_grad_part<V, ROW, KEEP, kThreads>(p, c0, acc, reinterpret_cast<float*>(ring_smem));
 }
 
 // Rows too long for registers, read again for dx and dresidual; with dw only a row's s and mean(g n), and the next

@@ -57,7 +57,8 @@ __device__ __forceinline__ void clip(float (&f)[V], int32_t c, uint32_t cols) {
         if ((uint32_t)(c + (int32_t)i) >= cols) f[i] = 0.f;
 }
 
-// Two elements an instruction, or a shift and a mask, where they come in pairs.
+// Two elements an instruction, or a shift and a mask, where they come in pairs. a lies in registers: of one in memory
+// a copy is made first, or it is read element by element.
 template <uint32_t V, typename T>
 __device__ __forceinline__ void unpack(const Pack<T, V>& a, float (&f)[V]) {
     if constexpr (sizeof(T) == 2 && V % 2 == 0) {

@@ -310,9 +310,14 @@ __device__ __forceinline__ void copy_shifted(const SortParams& p, uint32_t pair,
     const int32_t c0 = (int32_t)((segment * LANES * kSegment + lane) * V) - row_offset<V>(to);
     const uint32_t shift = Raw<V, true, E>::shift_of(x, c0);
     if (!inside_rows<V, true, E>(t, p.T, p.x_stride / sizeof(E), H)) {  // the first and the last row
-        for (uint32_t i = 0; i < kSegment * V; ++i) {
-            const uint32_t c = (uint32_t)(c0 + (int32_t)(i / V * LANES * V + i % V));
-            if (c < H) to[c] = x[c];
+        for (uint32_t i = 0; i < kSegment; ++i) {
+            const int32_t c = c0 + (int32_t)(LANES * i * V);
+            E v[V];
+#pragma unroll
+            for (uint32_t j = 0; j < V; ++j) v[j] = (uint32_t)(c + (int32_t)j) < H ? x[c + (int32_t)j] : E();
+#pragma unroll
+            for (uint32_t j = 0; j < V; ++j)
+                if ((uint32_t)(c + (int32_t)j) < H) to[c + (int32_t)j] = v[j];
         }
         return;
     }
@@ -355,7 +360,7 @@ __global__ void __launch_bounds__(256) sort_rows_shifted_kernel(const SortParams
 // Every block holds all pairs' experts, a warp finds a pair's place by counting the pairs before it (of smaller
 // experts, and of its own with a smaller number), and the block moves its tokens' rows; the last block takes the
 // offsets. Shared: [n] experts. E: a type of the elements' size, where SHIFTED.
-constexpr uint32_t kFewPairs = 4096, kFewWork = 1u << 19;
+constexpr uint32_t kFewPairs = 4096, kFewWork = 1u << 19, kFewBytes = 64u * 1024u;
 template <typename E, bool SHIFTED>
 __global__ void __launch_bounds__(256) sort_few_kernel(const SortParams p, uint32_t segments) {
     extern __shared__ uint32_t sort_smem[];
@@ -591,7 +596,8 @@ __global__ void __launch_bounds__(256, SHIFTED ? 2 : 3) combine_grad_kernel(cons
                     }
                 }
             }
-            for (uint32_t c = tid; !whole && c < p.H; c += ROW) {  // the first and the last row
+#pragma unroll 4
+            for (uint32_t c = tid; c < (whole ? 0u : p.H); c += ROW) {  // the first and the last row
                 const float g = to_float(dout[c]);
                 if (p.dweights) acc = fmaf(g, to_float(from[c]), acc);
                 if (p.drows) to[c] = from_float<T>(w * g);
@@ -729,8 +735,15 @@ uint32_t sort_blocks_bound(uint64_t pairs) {
 
 cudaError_t launch_sort_tokens(const SortParams& p, cudaStream_t s) {
     const uint32_t n = p.T * p.k;
-    // every token's block goes through all pairs: 256 tokens of 8 5.9 us, 512 13.1, 4000 of one 24 (else 13 to 14)
-    if (n <= kFewPairs && (uint64_t)p.T * n <= kFewWork) return sort_rows(p, true, s);
+    // Every token's block goes through all pairs: 256 tokens of 8 5.9 us, 512 13.1, 4000 of one 24 (else 13 to 14). Long
+    // rows are moved by a launch of their own: a token's block would take its pairs' one after another.
+    if (n <= kFewPairs && (uint64_t)p.T * n <= kFewWork) {
+        if (!p.rows || p.k * p.row_bytes <= kFewBytes) return sort_rows(p, true, s);
+        SortParams order = p;
+        order.rows = nullptr;
+        const cudaError_t e = sort_rows(order, true, s);
+        return e != cudaSuccess ? e : sort_rows(p, false, s);
+    }
     const uint32_t each = sort_each(n), blocks = sort_blocks(n);
     const bool self = n <= kSelfPairs;
     cudaError_t e = cudaSuccess;
