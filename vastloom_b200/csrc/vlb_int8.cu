@@ -443,13 +443,14 @@ __global__ void __launch_bounds__(256) int8_linear_kernel(const Int8LinearParams
 // latency of its loads, and the weights are its bytes. A block quantizes the rows into shared memory
 // while its warps' first weights are on their way; then a warp takes two channels at a time, a lane
 // 16 bytes of each every 512, two or four such pieces of both in flight, dp4a against the rows. A call with
-// groups takes one row a block and that row's matrix (two rows of one group read it twice, from L2).
+// groups (GROUPED) takes one row a block and that row's matrix (two rows of one group read it twice, from L2).
 
 constexpr uint32_t kFewThreads = 256, kFewWarps = kFewThreads / 32u;
-// Pieces of a channel in flight, and blocks an SM: one row has registers for twice the blocks, whose
-// set-up then overlaps (16 rows of 64 experts' 2048 x 2048: 4 pieces and 2 blocks 19.2 us, 2 and 4 14.8).
-__host__ __device__ constexpr uint32_t few_pieces(uint32_t rows) { return rows == 1u ? 2u : 4u; }
-__host__ __device__ constexpr uint32_t few_blocks(uint32_t rows) { return rows == 1u ? 4u : 2u; }
+// Pieces of a channel in flight, and blocks an SM. A group's row has registers for twice the blocks, whose set-up then
+// overlaps (16 rows of 64 experts' 2048 x 2048: 4 pieces and 2 blocks 19.2 us, 2 and 4 14.8); one row of one matrix fills
+// no more than two an SM (4096 x 4096: 2 pieces and 4 blocks 6.8 us, 4 and 2 6.2).
+__host__ __device__ constexpr uint32_t few_pieces(bool grouped) { return grouped ? 2u : 4u; }
+__host__ __device__ constexpr uint32_t few_blocks(bool grouped) { return grouped ? 4u : 2u; }
 constexpr uint32_t kFewSmem = 64u * 1024u;
 // Dynamic shared memory a launch may ask for without an opt-in: the default 48 KB hold the kernel's
 // static arrays too (up to 1 KB as the compiler lays them out).
@@ -475,10 +476,10 @@ __device__ __forceinline__ void store_typed(void* y, size_t at, float v, int typ
 }
 
 // T: the rows' type, int8_t for rows that are integers already. ROWS: rows of a block.
-template <typename T, uint32_t ROWS, bool EPI>
-__global__ void __launch_bounds__(kFewThreads, few_blocks(ROWS)) int8_few_kernel(const Int8LinearParams l, const Int8QuantParams q, int y_type,
+template <typename T, uint32_t ROWS, bool EPI, bool GROUPED>
+__global__ void __launch_bounds__(kFewThreads, few_blocks(GROUPED)) int8_few_kernel(const Int8LinearParams l, const Int8QuantParams q, int y_type,
                                                                uint32_t channels) {
-    constexpr uint32_t kFewPieces = few_pieces(ROWS);
+    constexpr uint32_t kFewPieces = few_pieces(GROUPED);
     extern __shared__ __align__(16) unsigned char few_smem[];
     __shared__ uint32_t top[ROWS], group_s;
     __shared__ float scale[ROWS];
@@ -487,7 +488,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(ROWS)) int8_few_kernel
     tc::grid_dependency_wait();
     tc::grid_launch_dependents();
     uint32_t row0 = 0, rows = l.rows, g = 0;
-    if (l.offsets) {
+    if constexpr (GROUPED) {
         row0 = blockIdx.y;
         rows = 1;
         if (tid == 0) group_s = l.groups;
@@ -1499,15 +1500,15 @@ cudaError_t mma_launch(const Int8MmaParams& p, uint32_t sms, bool wide, cudaStre
 constexpr uint32_t kFewRows = 8, kFewGroupedRows = 24, kFewElements = 8192;
 constexpr uint64_t kFewWork = 1u << 24;
 
-template <typename T, uint32_t ROWS, bool EPI>
+template <typename T, uint32_t ROWS, bool EPI, bool GROUPED = false>
 cudaError_t few_launch(const Int8LinearParams& l, const Int8QuantParams& q, int y_type, uint32_t sms, cudaStream_t s) {
-    auto* kernel = int8_few_kernel<T, ROWS, EPI>;
+    auto* kernel = int8_few_kernel<T, ROWS, EPI, GROUPED>;
     const size_t smem = (size_t)ROWS * ((l.cols + 15u) / 16u * 16u);
     if (smem > kFewDefaultSmem) {
         const cudaError_t e = smem_once(kernel, kFewSmem);
         if (e != cudaSuccess) return e;
     }
-    const uint32_t sets = l.offsets ? l.rows : 1u, slots = few_blocks(ROWS) * sms;
+    const uint32_t sets = GROUPED ? l.rows : 1u, slots = few_blocks(GROUPED) * sms;
     uint32_t channels = (uint32_t)(((uint64_t)l.out_cols * sets + slots - 1u) / slots);
     channels = (channels + 2u * kFewWarps - 1u) / (2u * kFewWarps) * (2u * kFewWarps);
     return launch_chained(kernel, dim3((l.out_cols + channels - 1u) / channels, sets), kFewThreads, smem, 0, s, l, q, y_type,
@@ -1516,7 +1517,8 @@ cudaError_t few_launch(const Int8LinearParams& l, const Int8QuantParams& q, int 
 
 template <typename T, bool EPI>
 cudaError_t few_rows(const Int8LinearParams& l, const Int8QuantParams& q, int y_type, cudaStream_t s) {
-    const uint32_t rows = l.offsets ? 1u : l.rows, sms = sm_count();
+    const uint32_t rows = l.rows, sms = sm_count();
+    if (l.offsets) return few_launch<T, 1, EPI, true>(l, q, y_type, sms, s);
     if (rows <= 1u) return few_launch<T, 1, EPI>(l, q, y_type, sms, s);
     if (rows <= 2u) return few_launch<T, 2, EPI>(l, q, y_type, sms, s);
     if (rows <= 4u) return few_launch<T, 4, EPI>(l, q, y_type, sms, s);
