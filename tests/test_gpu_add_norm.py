@@ -128,6 +128,38 @@ def test_norm_matches_the_formula(dev, torch, rows, cols, xt, rt, pad, shift):
         assert torch.equal(now[off], old[off])
 
 
+@pytest.mark.parametrize("rows,cols,q_pad,q_shift", [(300, 1095, 9, 0), (300, 1095, 0, 3), (90, 2048, 5, 1), (3, 520, 1, 0)])
+@pytest.mark.parametrize("xt,rt", [("bf16", "bf16"), ("f16", "f32"), ("f32", "f32")])
+def test_int8_rows_at_an_offset_of_their_own(dev, torch, rows, cols, q_pad, q_shift, xt, rt):
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x, r = rows_of(torch, g, rows, cols, xt), rows_of(torch, g, rows, cols, rt)
+    flat = torch.full((rows * (cols + q_pad) + q_shift,), 77, device="cuda", dtype=torch.int8)
+    q = flat[q_shift:].as_strided((rows, cols), (cols + q_pad, 1))
+    s, h = torch.zeros(rows, device="cuda"), torch.zeros_like(r)
+    forward(dev, torch, x, r, None, xt=xt, rt=rt, h=h, q=q, scale=s)
+    want_h, want = exact_norm(x, r, None, EPS)
+    check(h, want_h, U * np.abs(want_h), rt)
+    check_int8(q, s, want, cols)
+    between = flat[q_shift: q_shift + (rows - 1) * (cols + q_pad)].view(rows - 1, cols + q_pad)[:, cols:]
+    assert bool((between == 77).all()) and bool((flat[:q_shift] == 77).all())
+
+
+def test_norm_of_more_elements_than_32_bits(dev, torch):
+    """Offsets past 2^31 elements: the last rows of a large call, forward and gradient."""
+    rows, cols = 530000, 4099
+    x = torch.empty(rows, cols, device="cuda", dtype=torch.bfloat16).normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    y = torch.zeros_like(x)
+    forward(dev, torch, x, None, None, xt="bf16", rt="bf16", y=y)
+    dx = torch.zeros_like(x)
+    backward(dev, torch, x, x, None, None, xt="bf16", rt="bf16", dx=dx)
+    n = additions(cols) / 2 + 8
+    for at in (slice(0, 3), slice(rows // 2, rows // 2 + 2), slice(rows - 3, rows)):
+        _, want = exact_norm(x[at], None, None, EPS)
+        check(y[at], want, n * U * np.abs(want), "bf16")
+        d, bound, _, _ = exact_grad(x[at], x[at], None, None, EPS)
+        check(dx[at], d, bound, "bf16")
+
+
 @pytest.mark.parametrize("xt,rt", PAIRS)
 def test_norm_outputs_one_by_one(dev, torch, xt, rt):
     g = torch.Generator(device="cuda").manual_seed(5)

@@ -137,7 +137,9 @@ def test_order(dev, torch, T, k, E, how):
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16", "i8"])
 @pytest.mark.parametrize("T,k,E,H,how", [(1, 8, 64, 4096, "distinct"), (5, 3, 4, 1, "dropped"), (64, 8, 256, 2048, "distinct"),
                                          (77, 6, 16, 1411, "dropped"), (300, 2, 8, 33, "skewed"), (1500, 8, 32, 520, "dropped"),
-                                         (3000, 8, 64, 16, "even"), (9, 64, 40, 9000, "dropped"), (40, 8, 8, 24, "none")])
+                                         (3000, 8, 64, 16, "even"), (9, 64, 40, 9000, "dropped"), (40, 8, 8, 24, "none"),
+                                         (150, 8, 16, 6525, "even"), (2, 3, 4, 6234, "even"), (5000, 3, 9, 253, "dropped"),
+                                         (1, 1, 1, 5, "even"), (33, 20, 7, 7, "even")])
 @pytest.mark.parametrize("pad,shift", [(0, 0), (16, 0), (3, 1)])
 def test_rows(dev, torch, T, k, E, H, how, kind, pad, shift):
     rng = np.random.default_rng(T * 7 + H)
@@ -309,6 +311,37 @@ def test_gradients_match_differences(dev, torch):
         assert abs((F(a, w) - F(b, w)) / (2 * e) - np.sum(f64(dx) * (f64(a) - f64(b)) / (2 * e))) <= noise
         a, b = w + e * u, w - e * u
         assert abs((F(x, a) - F(x, b)) / (2 * e) - np.sum(f64(dw) * (f64(a) - f64(b)) / (2 * e))) <= noise * (H / 32 + 24)
+
+
+@pytest.mark.parametrize("H", [8192, 8195])
+def test_more_elements_than_32_bits(dev, torch, H):
+    """Rows past 2^31 elements: sorted, summed and their gradient, at the first, middle and last tokens."""
+    T, k, E = 34000, 8, 64
+    rng = np.random.default_rng(H)
+    idx, _ = route(rng, T, k, E, "even")
+    x = torch.empty(T, H, device="cuda", dtype=torch.bfloat16).normal_(generator=torch.Generator(device="cuda").manual_seed(3))
+    rows = torch.zeros(T * k, H, device="cuda", dtype=torch.bfloat16)
+    got = sort(dev, torch, idx, None, E, x=x, rows=rows, kind="bf16")
+    elem_row, _, order = order_of(idx, None, E)
+    assert np.array_equal(got["elem_row"].cpu().numpy().reshape(T, k), elem_row)
+    for p in (0, 1, T * k // 2, T * k - 2, T * k - 1):
+        assert torch.equal(rows[p], x[int(order[p]) // k])
+    w = torch.rand(T, k, device="cuda")
+    out, dw, drows = torch.zeros(T, H, device="cuda"), torch.zeros(T, k, device="cuda"), torch.zeros_like(rows)
+    where = got["elem_row"]
+    dev.combine_device(rows.data_ptr(), where.data_ptr(), T, k, H, out.data_ptr(), x_type=KIND["bf16"],
+                       weights_ptr=w.data_ptr(), stream=LEGACY)
+    dev.combine_grad_device(out.data_ptr(), where.data_ptr(), T, k, H, x_type=KIND["bf16"], rows_ptr=rows.data_ptr(),
+                            weights_ptr=w.data_ptr(), drows_ptr=drows.data_ptr(), dweights_ptr=dw.data_ptr(), stream=LEGACY)
+    torch.cuda.synchronize()
+    for t in (0, 1, T // 2, T - 2, T - 1):
+        v = f64(x[t])[None, :] * f64(w[t])[:, None]
+        assert np.all(np.abs(f64(out[t]) - v.sum(0)) <= (k + 2) * U * np.abs(v).sum(0))
+        prod = f64(out[t]) * f64(x[t])
+        assert np.all(np.abs(f64(dw[t]) - prod.sum()) <= (H / 32 + 24) * U * np.abs(prod).sum())
+        for s in range(k):
+            want = f64(out[t]) * f64(w[t, s])
+            assert np.all(np.abs(f64(drows[elem_row[t, s]]) - want) <= (U + UNIT["bf16"] * 1.01) * np.abs(want) + 2.0 ** -126)
 
 
 def test_no_tokens(dev, torch):

@@ -100,7 +100,7 @@ __device__ __forceinline__ void row_weights(const float* weight, int32_t c0, uin
     }
 }
 
-// Bytes of y: V of them from column c on, where they are inside [0, cols).
+// Bytes of y: V of them from column c on, where they are inside [0, cols), in one store where they lie on V bytes.
 template <uint32_t V>
 __device__ __forceinline__ void store_row_bytes(int8_t* q, float (&y)[V], const RowStep& st, int32_t c, uint32_t cols) {
     if (st.lift != 1.f) {  // a row of zeros, of tiny values, or not finite
@@ -108,7 +108,7 @@ __device__ __forceinline__ void store_row_bytes(int8_t* q, float (&y)[V], const 
         for (uint32_t i = 0; i < V; ++i) y[i] = st.inv == 0.f ? 0.f : y[i] * st.lift;
     }
     if constexpr (V % 4 == 0) {
-        if (inside(c, V, cols)) {
+        if (inside(c, V, cols) && reinterpret_cast<uintptr_t>(q) % V == 0) {
             store_bytes<V>(q, y, st, V);
             return;
         }
@@ -615,7 +615,6 @@ cudaError_t norm_typed(const NormParams& p, cudaStream_t s) {
     at.add(p.residual, p.residual_stride, sizeof(R));
     at.add(p.h, p.h_stride, sizeof(R));
     at.add(p.y, p.y_stride, sizeof(T));
-    at.add(p.q, p.q_stride, 1);
     const auto run_ring = [&](auto shape) {
         using S = decltype(shape);
         constexpr uint32_t kBytes = S::KEEP * V * (sizeof(T) + sizeof(R)), kThreads = norm_threads(S::ROW);
