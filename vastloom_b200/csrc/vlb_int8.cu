@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(GROUPED)) int8_few_ker
 // to 256 tokens of one group (the columns), so a lane of the epilogue holds one channel's scale and
 // a warp's stores are 32 neighbouring channels of one token; few tokens cost few columns.
 // K runs in chunks of 128 bytes (one 128-byte swizzle row) through a ring of TMA stages.
-// Roles: warps 0-7 epilogue, warp 8 TMA, warp 9 MMA, warp 10 the tiles' places and scales for the
+// Roles: warps 0-7 (with an epilogue 12 or 16 of them) the sums to memory, the next three TMA, MMA, and the tiles' places and scales for the
 // epilogue, a tile or two ahead (behind an epilogue's stores their lookup took 3,000 to 5,000 cycles
 // of a tile's 8,000); two accumulators, so a tile's epilogue runs beside the next tile's products.
 // Persistent CTAs, tiles in order, a group's token tiles innermost (its weights come from HBM once).
@@ -670,10 +670,15 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(GROUPED)) int8_few_ker
 
 enum class Mm { kOne, kSplit, kPair };
 constexpr uint32_t kMmChannels = 128, kMmMaxTokens = 256, kMmKc = 128;
-// Warps that take the sums to memory: twice as many where an epilogue's operations come on top (4096 x 4096 x 4096 f16
-// with GELU 96 us with 8, 75 with 16; what 8 warps hold in flight does not cover their latency).
-__host__ __device__ constexpr uint32_t mm_epi_warps(Mm mode, bool epi) { return epi && mode != Mm::kSplit ? 12u : 8u; }
-__host__ __device__ constexpr uint32_t mm_threads(Mm mode, bool epi) { return (mm_epi_warps(mode, epi) + 3u) * 32u; }
+// Warps that take the sums to memory: more where an epilogue's operations come on top, as many as registers are for
+// (elements of 2 bytes 16, of 4 12; what 8 warps hold in flight does not cover the operations' latency: 4096 x 4096 x 4096
+// f16 with GELU 96 us with 8, 67 with 16).
+__host__ __device__ constexpr uint32_t mm_epi_warps(Mm mode, bool epi, size_t element) {
+    return !epi || mode == Mm::kSplit ? 8u : element == 2u ? 16u : 12u;
+}
+__host__ __device__ constexpr uint32_t mm_threads(Mm mode, bool epi, size_t element) {
+    return (mm_epi_warps(mode, epi, element) + 3u) * 32u;
+}
 constexpr uint32_t kMmWStage = kMmChannels * kMmKc;
 constexpr uint32_t kMmMaxStages = 12;
 constexpr uint32_t kMmSmemLimit = 227u * 1024u;
@@ -712,11 +717,11 @@ struct MmShared {
 };
 
 __host__ __device__ constexpr uint32_t mm_table_bytes(uint32_t groups) { return (3u * groups + 1u) * 4u; }
-__host__ __device__ constexpr uint32_t mm_out_bytes(Mm mode, bool epi) {
-    return epi && mode != Mm::kSplit ? mm_epi_warps(mode, epi) / 4u * 16u * kMmChannels * 4u : 0u;
+__host__ __device__ constexpr uint32_t mm_out_bytes(Mm mode, bool epi, size_t element) {
+    return epi && mode != Mm::kSplit ? mm_epi_warps(mode, epi, element) / 4u * 16u * kMmChannels * 4u : 0u;
 }
-__host__ __device__ constexpr uint32_t mm_fixed_bytes(uint32_t groups, Mm mode, bool epi) {
-    return mm_out_bytes(mode, epi) + (epi ? 4u : 2u) * (kMmMaxTokens + kMmChannels) * 4u + 2u * 16u + (2u * kMmMaxStages + 8u) * 8u + 16u + mm_table_bytes(groups) +
+__host__ __device__ constexpr uint32_t mm_fixed_bytes(uint32_t groups, Mm mode, bool epi, size_t element) {
+    return mm_out_bytes(mode, epi, element) + (epi ? 4u : 2u) * (kMmMaxTokens + kMmChannels) * 4u + 2u * 16u + (2u * kMmMaxStages + 8u) * 8u + 16u + mm_table_bytes(groups) +
            16u;
 }
 
@@ -771,9 +776,9 @@ __device__ __forceinline__ MmTile mm_tile(const MmShared& sh, const Int8MmaParam
 // WIDE_Y: with an epilogue, rows of y and of the residual lie on 16-byte boundaries (a kernel of its own: the other form's
 // registers would spill into it).
 template <typename TY, Mm MODE, bool EPI, bool WIDE_Y>
-__global__ void __launch_bounds__(mm_threads(MODE, EPI), 1) int8_mma_kernel(const __grid_constant__ Int8MmaParams p) {
+__global__ void __launch_bounds__(mm_threads(MODE, EPI, sizeof(TY)), 1) int8_mma_kernel(const __grid_constant__ Int8MmaParams p) {
     constexpr bool SPLIT = MODE == Mm::kSplit, PAIR = MODE == Mm::kPair;
-    constexpr uint32_t kEpi = mm_epi_warps(MODE, EPI);
+    constexpr uint32_t kEpi = mm_epi_warps(MODE, EPI, sizeof(TY));
     extern __shared__ __align__(1024) unsigned char mm_smem[];
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
     const uint32_t smem = tc::smem_u32(mm_smem), stage_bytes = kMmWStage + p.x_stage;
@@ -782,7 +787,7 @@ __global__ void __launch_bounds__(mm_threads(MODE, EPI), 1) int8_mma_kernel(cons
     {
         unsigned char* at = mm_smem + p.stages * stage_bytes;
         sh.out = reinterpret_cast<float*>(at);
-        sh.scale = sh.out + mm_out_bytes(MODE, EPI) / 4u;
+        sh.scale = sh.out + mm_out_bytes(MODE, EPI, sizeof(TY)) / 4u;
         sh.channel = sh.scale + 2u * kMmMaxTokens;
         sh.weight = sh.channel + 2u * kMmChannels;
         sh.bias = sh.weight + 2u * kMmMaxTokens;
@@ -825,7 +830,7 @@ __global__ void __launch_bounds__(mm_threads(MODE, EPI), 1) int8_mma_kernel(cons
         *sh.abort = 0;
         tc::mbar_fence_init();
     }
-    for (uint32_t g = tid; g < l.groups; g += mm_threads(MODE, EPI)) {
+    for (uint32_t g = tid; g < l.groups; g += mm_threads(MODE, EPI, sizeof(TY))) {
         uint32_t lo, hi;
         group_range(l, g, lo, hi);
         sh.lo[g] = lo;
@@ -1402,7 +1407,7 @@ bool tma_rows(const int8_t* p, size_t stride) {
 }
 
 // Tile width, split or pairs of a product on the tensor cores. Returns the mode.
-Mm mma_plan(Int8MmaParams& p, uint32_t sms) {
+Mm mma_plan(Int8MmaParams& p, uint32_t sms, size_t y_size) {
     const Int8LinearParams& l = p.l;
     p.nk = (l.cols + kMmKc - 1u) / kMmKc;
     const auto split_of = [&](uint64_t tiles) {
@@ -1473,7 +1478,7 @@ Mm mma_plan(Int8MmaParams& p, uint32_t sms) {
     p.acc_cols = p.width < 32u ? 32u : p.width;
     p.tmem_cols = 32;
     while (p.tmem_cols < (mode == Mm::kSplit ? 1u : 2u) * p.acc_cols) p.tmem_cols *= 2u;
-    const uint32_t room = kMmSmemLimit - 1024u - mm_fixed_bytes(l.groups, mode, l.act != kInt8NoEpilogue);
+    const uint32_t room = kMmSmemLimit - 1024u - mm_fixed_bytes(l.groups, mode, l.act != kInt8NoEpilogue, y_size);
     p.stages = room / (kMmWStage + p.x_stage);
     if (p.stages > kMmMaxStages) p.stages = kMmMaxStages;
     return mode;
@@ -1486,8 +1491,8 @@ cudaError_t mma_launch(const Int8MmaParams& p, uint32_t sms, bool wide, cudaStre
     const uint32_t in_cluster = MODE == Mm::kSplit ? p.split : MODE == Mm::kPair ? 2u : 1u;
     cudaError_t e = smem_once(kernel, kMmSmemLimit);
     if (e != cudaSuccess) return e;
-    const size_t smem = p.stages * (kMmWStage + p.x_stage) + mm_fixed_bytes(p.l.groups, MODE, EPI);
-    return launch_chained(kernel, dim3(sms / in_cluster * in_cluster), mm_threads(MODE, EPI), smem, MODE == Mm::kOne ? 0 : in_cluster, s, p);
+    const size_t smem = p.stages * (kMmWStage + p.x_stage) + mm_fixed_bytes(p.l.groups, MODE, EPI, sizeof(TY));
+    return launch_chained(kernel, dim3(sms / in_cluster * in_cluster), mm_threads(MODE, EPI, sizeof(TY)), smem, MODE == Mm::kOne ? 0 : in_cluster, s, p);
 }
 
 // What int8_few_kernel takes. Dense: up to kFewRows rows, from 3 on no more than kFewElements elements
@@ -1536,7 +1541,7 @@ cudaError_t linear_type(const Int8LinearParams& l, bool after_quantize, cudaStre
         };
         const bool wide = EPI && on16(l.y, l.y_stride) && (!l.residual || on16(l.residual, l.residual_stride));
         const uint32_t sms = sm_count();
-        const Mm mode = mma_plan(p, sms);
+        const Mm mode = mma_plan(p, sms, sizeof(TY));
         if (encode_rows(&p.wmap, l.w, (uint64_t)l.groups * l.out_cols, l.cols, l.w_stride, kMmChannels) &&
             encode_rows(&p.xmap, l.x, l.rows, l.cols, l.x_stride, p.box))
             return mode == Mm::kPair    ? mma_launch<TY, Mm::kPair, EPI>(p, sms, wide, s)
