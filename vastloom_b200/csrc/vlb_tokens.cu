@@ -710,8 +710,9 @@ cudaError_t combine_grad_typed(const CombineGradParams& p, cudaStream_t s) {
     const uint64_t pairs = (uint64_t)p.T * p.k;
     const auto run = [&](auto shifted) {
         constexpr bool kShifted = decltype(shifted)::value;
-        // a CTA a pair while warps would leave SMs idle
-        if (pairs < 4096u && p.H >= 64u * V)
+        // A CTA a pair while warps would leave SMs idle, longer for long rows (bf16, CTA / warp: 512 pairs of 1024 3.4 / 2.5
+        // us, of 4096 4.0 / 5.3; 2048 pairs of 2048 11.3 / 6.3).
+        if (pairs < (p.H >= 256u * V ? 1024u : 256u) && p.H >= 64u * V)
             return launch_chained(combine_grad_kernel<T, O, 256, kShifted>, dim3((uint32_t)pairs), 256, 0, 0, s, p);
         if (p.H <= 32u * V)
             return launch_chained(combine_grad_kernel<T, O, 8, kShifted>, dim3(item_blocks(pairs, 8)), 256, 0, 0, s, p);
