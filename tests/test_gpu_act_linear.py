@@ -228,6 +228,35 @@ def test_onto_the_residual(dev, torch, act, rows, K, N, ld, offsets):
     assert torch.equal(c.res[live], apart[live]) and torch.equal(c.res[~live], was[~live])
 
 
+@pytest.mark.parametrize("rows,K,N", [(3, 256, 128), (60, 512, 256), (900, 512, 768), (40, 90, 40)])
+@pytest.mark.parametrize("up", [False, True])
+def test_gathered_and_swiglu_rows_as_the_plain_call(dev, torch, rows, K, N, up):
+    """Rows by index, SwiGLU of two operands, groups: what the plain call gives, bit for bit, where the epilogue adds
+    nothing; and the residual on top of it, rounded once more."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn(rows // 2 + 1, K, device="cuda", generator=g).bfloat16()
+    u = torch.randn(rows // 2 + 1, K, device="cuda", generator=g).bfloat16() if up else None
+    index = torch.randint(0, rows // 2 + 3, (rows,), device="cuda", generator=g, dtype=torch.int32)  # some past the rows
+    offsets = torch.tensor([0, rows // 3, rows // 3, rows - 1], device="cuda", dtype=torch.int32)
+    ld = (K + 15) // 16 * 16
+    w = torch.randint(-127, 128, (3, N, ld), device="cuda", generator=g, dtype=torch.int8)
+    ws = torch.rand(3, N, device="cuda", generator=g) * 0.01
+    res = torch.randn(rows, N, device="cuda", generator=g)
+    need = vb.int8_workspace_bytes(rows, K)
+    scratch = torch.empty(need, device="cuda", dtype=torch.uint8)
+    y = [torch.full((rows, N), 9.0, device="cuda") for _ in range(3)]
+    kw = dict(x_type=KIND["bf16"], x_rows=x.shape[0], row_index_ptr=index.data_ptr(), up_ptr=u.data_ptr() if up else 0,
+              swiglu_limit=2.0 if up else 0.0, offsets_ptr=offsets.data_ptr(), ws_ptr=scratch.data_ptr(), ws_bytes=need,
+              stream=LEGACY)
+    weights = vb.Int8Weights(w.data_ptr(), ws.data_ptr(), N, K, groups=3, stride=ld)
+    dev.int8_linear_device(weights, x.data_ptr(), rows, y[0].data_ptr(), **kw)
+    dev.int8_linear_act_device(weights, x.data_ptr(), rows, y[1].data_ptr(), **kw)
+    dev.int8_linear_act_device(weights, x.data_ptr(), rows, y[2].data_ptr(), residual_ptr=res.data_ptr(), **kw)
+    assert torch.equal(y[0], y[1])
+    live = slice(0, rows - 1)
+    assert torch.equal(y[2][live], y[0][live] + res[live]) and bool((y[2][rows - 1] == 9).all())
+
+
 def test_rows_that_are_not_finite(dev, torch):
     """A row of NaN or infinities is NaN in its own outputs and nowhere else, through every activation."""
     for rows in (3, 300):

@@ -99,12 +99,12 @@ def forward(dev, torch, x, r, w, *, xt, rt, eps=EPS, h=None, y=None, q=None, sca
 
 
 SIZES = [(1, 1), (1, 7), (3, 8), (1, 4096), (2, 2048), (5, 1411), (64, 64), (33, 96), (300, 1000), (9, 4100), (130, 4096),
-         (2100, 512), (1, 16384), (7, 12345), (3, 40000)]
+         (2100, 512), (1, 16384), (7, 12345), (3, 40000), (200, 1), (70, 3), (1000, 5), (65, 2049), (70, 8191)]
 
 
 @pytest.mark.parametrize("xt,rt", PAIRS)
 @pytest.mark.parametrize("rows,cols", SIZES)
-@pytest.mark.parametrize("pad,shift", [(0, 0), (8, 0), (3, 1)])
+@pytest.mark.parametrize("pad,shift", [(0, 0), (8, 0), (3, 0), (3, 1)])
 def test_norm_matches_the_formula(dev, torch, rows, cols, xt, rt, pad, shift):
     g = torch.Generator(device="cuda").manual_seed(rows * 131 + cols)
     x = rows_of(torch, g, rows, cols, xt, 1.0, pad, shift)
@@ -246,7 +246,7 @@ def backward(dev, torch, dy, h, w, dh, *, xt, rt, eps=EPS, dx=None, dr=None, dw=
 
 @pytest.mark.parametrize("xt,rt", PAIRS)
 @pytest.mark.parametrize("rows,cols", SIZES + [(1500, 2048), (5000, 64), (1000, 1411)])
-@pytest.mark.parametrize("pad,shift", [(0, 0), (8, 0), (3, 1)])
+@pytest.mark.parametrize("pad,shift", [(0, 0), (8, 0), (3, 0), (3, 1)])
 def test_gradient_matches_the_formula(dev, torch, rows, cols, xt, rt, pad, shift):
     g = torch.Generator(device="cuda").manual_seed(rows * 17 + cols)
     dy = rows_of(torch, g, rows, cols, xt, 1.0, pad, shift)

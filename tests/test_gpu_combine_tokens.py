@@ -167,7 +167,8 @@ TYPES = [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f1
          ("bf16", "f16"), ("f16", "bf16")]
 SHAPES = [(1, 1, 1, 1, "even"), (1, 8, 64, 4096, "distinct"), (64, 8, 256, 2048, "dropped"), (7, 6, 16, 1411, "dropped"),
           (200, 3, 8, 40, "skewed"), (1000, 8, 64, 1024, "dropped"), (5, 64, 8, 520, "dropped"), (12, 2, 4, 9001, "none"),
-          (3, 9, 4, 20000, "even"), (17, 17, 40, 256, "distinct"), (4000, 1, 3, 128, "dropped")]
+          (3, 9, 4, 20000, "even"), (17, 17, 40, 256, "distinct"), (4000, 1, 3, 128, "dropped"), (900, 4, 8, 7, "dropped"),
+          (600, 5, 16, 1003, "even")]
 
 
 def placed(dev, torch, T, k, E, how, seed):
@@ -179,7 +180,7 @@ def placed(dev, torch, T, k, E, how, seed):
 
 @pytest.mark.parametrize("kind,out_kind", TYPES)
 @pytest.mark.parametrize("T,k,E,H,how", SHAPES)
-@pytest.mark.parametrize("pad,shift", [(0, 0), (8, 0), (3, 1)])
+@pytest.mark.parametrize("pad,shift", [(0, 0), (8, 0), (3, 0), (3, 1)])
 def test_combine(dev, torch, T, k, E, H, how, kind, out_kind, pad, shift):
     elem_row, n, where = placed(dev, torch, T, k, E, how, T + H)
     g = torch.Generator(device="cuda").manual_seed(T + H)
