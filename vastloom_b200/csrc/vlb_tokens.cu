@@ -72,8 +72,16 @@ struct Piece {
     Part part[kParts];
     __device__ __forceinline__ static uint32_t shift_of(const E* row, int32_t c) { return Part::shift_of(row, c); }
     __device__ __forceinline__ void load(const E* row, int32_t c, uint32_t shift) {
+        if constexpr (kParts == 2u && !SHIFTED) {  // one access: two of 16 bytes would each take half of every sector
+            uint32_t *a = part[0].x.v, *b = part[1].x.v;
+            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3])
+                         : "l"(row + c)
+                         : "memory");
+        } else {
 #pragma unroll
-        for (uint32_t i = 0; i < kParts; ++i) part[i].load(row, c + (int32_t)(i * kPart), shift);
+            for (uint32_t i = 0; i < kParts; ++i) part[i].load(row, c + (int32_t)(i * kPart), shift);
+        }
     }
     __device__ __forceinline__ void get(uint32_t shift, float (&f)[V]) const {
 #pragma unroll
@@ -531,6 +539,15 @@ __global__ void __launch_bounds__(256, 2) combine_kernel(const CombineParams p, 
             } else if (p.residual) {
                 add_each<V>(1.f, res, c, p.H, acc[i]);
             }
+            if constexpr (V * sizeof(O) == 32u && !SHIFTED) {
+                if (inside(c, V, p.H)) {
+                    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + c), "f"(acc[i][0]),
+                                 "f"(acc[i][1]), "f"(acc[i][2]), "f"(acc[i][3]), "f"(acc[i][4]), "f"(acc[i][5]), "f"(acc[i][6]),
+                                 "f"(acc[i][7])
+                                 : "memory");
+                    continue;
+                }
+            }
             store_piece<V>(out + c, acc[i], c, p.H);
         }
     }
@@ -682,7 +699,7 @@ cudaError_t sort_rows(const SortParams& p, bool few, cudaStream_t s) {
 // Pieces of 16 bytes of the rows; of the others, 32, 16 or 8.
 template <typename T, typename O>
 bool on_pieces(const void* rows, size_t rows_stride, const void* other, size_t other_stride) {
-    constexpr uint32_t V = 16u / sizeof(T), kOther = V * sizeof(O) < 16u ? V * sizeof(O) : 16u;
+    constexpr uint32_t V = 16u / sizeof(T), kOther = V * sizeof(O);
     return on(rows, rows_stride * sizeof(T), 16) && on(other, other_stride * sizeof(O), kOther);
 }
 
