@@ -438,9 +438,9 @@ __global__ void __launch_bounds__(256) sort_few_kernel(const SortParams p, uint3
 
 // LANES lanes (a warp, or 8 for short rows) take a segment of a token, KEEP pieces of V columns a lane (16 bytes of the
 // rows), summed in registers over the slots in order, SLOTS slots' loads in flight. Pieces lie on the boundaries of out.
-// HBM-bound: 16,384 x 8 of 2048 bf16 onto f32 126 us (5.6 TB/s; with branches between the loads 463), of 1001 bf16 84.
+// HBM-bound: 16,384 x 8 of 2048 bf16 onto f32 115 us (6.1 TB/s; with branches between the loads 463), of 1001 bf16 83.
 template <typename T, typename O, uint32_t LANES, uint32_t KEEP, uint32_t SLOTS, bool SHIFTED>
-__global__ void __launch_bounds__(256, 2) combine_kernel(const CombineParams p, uint32_t segments) {
+__global__ void __launch_bounds__(256, SLOTS > 2u ? 2 : SHIFTED ? 3 : 4) combine_kernel(const CombineParams p, uint32_t segments) {
     constexpr uint32_t V = 16u / sizeof(T), kItems = 256u / LANES;
     constexpr int32_t kStep = LANES * V;
     const uint32_t lane = threadIdx.x % LANES;
@@ -555,10 +555,11 @@ __global__ void __launch_bounds__(256, 2) combine_kernel(const CombineParams p, 
 
 // ROW lanes (a warp; 8 for short rows; the CTA where pairs are few) take a pair: its row in pieces of its own
 // boundaries (of drows where they are written), dout beside it, which the pairs of a token share in L1. HBM-bound: 8192 x 8
-// of 2048 bf16 89 us (5.3 TB/s); eight pieces in flight instead of four gain 2 % there and lose 20 % on rows of 128.
+// of 2048 bf16 89 us (5.3 TB/s). Two pieces in flight in 32 warps an SM: 32,768 x 8 of 128 bf16 38 us, four pieces in 24
+// warps 48; 16,384 x 8 of 2048 195 and 202, 256 x 8 7.6 and 6.9. Shifted, 16 warps: 16,384 x 8 of 1001 168, 24 warps 178.
 template <typename T, typename O, uint32_t ROW, bool SHIFTED>
-__global__ void __launch_bounds__(256, SHIFTED ? 2 : 3) combine_grad_kernel(const CombineGradParams p) {
-    constexpr uint32_t V = 16u / sizeof(T), kRows = 256u / ROW, kAtOnce = SHIFTED && sizeof(O) > sizeof(T) ? 2u : 4u;
+__global__ void __launch_bounds__(256, SHIFTED ? 2 : 4) combine_grad_kernel(const CombineGradParams p) {
+    constexpr uint32_t V = 16u / sizeof(T), kRows = 256u / ROW, kAtOnce = !SHIFTED || sizeof(O) > sizeof(T) ? 2u : 4u;
     __shared__ float scratch[2][8];
     const uint32_t tid = threadIdx.x % ROW;
     const uint64_t pairs = (uint64_t)p.T * p.k;
@@ -713,14 +714,13 @@ cudaError_t combine_typed(const CombineParams& p, cudaStream_t s) {
         const uint32_t segments = (pieces + lanes * keep - 1u) / (lanes * keep);
         return launch_chained(kernel, dim3(item_blocks((uint64_t)p.T * segments, lanes)), 256, 0, 0, s, p, segments);
     };
-    // 256 bytes a lane in flight; shifted pieces take twice the registers
-    constexpr uint32_t kKeep = 4u, kShiftedKeep = sizeof(T) == 4u ? 4u : 2u, kShiftedSlots = sizeof(T) == 4u ? 2u : 4u;
-    if (pieces <= 16u)
-        return whole ? run(combine_kernel<T, O, 8, 2, 4, false>, 8, 2) : run(combine_kernel<T, O, 8, 2, kShiftedSlots, true>, 8, 2);
+    if (pieces <= 16u) return whole ? run(combine_kernel<T, O, 8, 2, 2, false>, 8, 2) : run(combine_kernel<T, O, 8, 2, 2, true>, 8, 2);
     if ((uint64_t)p.T * pieces <= (1u << 17))  // few tokens: a piece a lane, all slots at once
         return whole ? run(combine_kernel<T, O, 32, 1, 8, false>, 32, 1) : run(combine_kernel<T, O, 32, 1, 4, true>, 32, 1);
-    return whole ? run(combine_kernel<T, O, 32, kKeep, 4, false>, 32, kKeep)
-                 : run(combine_kernel<T, O, 32, kShiftedKeep, kShiftedSlots, true>, 32, kShiftedKeep);
+    // Two pieces of two slots a lane in flight and 32 warps an SM (shifted 24) rather than more of both and 16 warps: 16,384
+    // tokens of 2048 bf16 onto f32 with 8 slots 129 us (four of four 137), with two 66 (86); shifted,
+    // of 1001 bf16, 83 us, in 16 warps 92, one piece of two or four slots 89 and 100.
+    return whole ? run(combine_kernel<T, O, 32, 2, 2, false>, 32, 2) : run(combine_kernel<T, O, 32, 2, 2, true>, 32, 2);
 }
 
 template <typename T, typename O>
