@@ -690,7 +690,8 @@ int vlb_add_rms_norm_device(vlb_handle* h, const vlb_add_rms_norm_desc* desc, vo
  * dresidual (residual_type) are the same numbers, each rounded once; of one type, one of them is
  * enough. Any of dx, dresidual and dweight may be NULL, not all; dx may be dy's memory and dresidual
  * dh's. Sums over rows run in a fixed order: equal inputs give equal bits. rows = 0 gives a dweight of
- * zeros. ws: vlb_add_rms_norm_grad_workspace_bytes(rows, cols), 16-byte aligned, for dweight alone. */
+ * zeros. ws: vlb_add_rms_norm_grad_workspace_bytes(rows, cols), 16-byte aligned, for dweight alone; calls that
+ * may overlap (two streams, two graphs) bring one each. */
 typedef struct vlb_add_rms_norm_grad_desc {
     const void* dy;              /* [rows] rows of type */
     uint64_t dy_stride;
@@ -756,7 +757,7 @@ typedef struct vlb_sort_tokens_desc {
     int32_t type;
     uint32_t reserved0;
 } vlb_sort_tokens_desc;
-/* Never falls as T, k or E rise. */
+/* Never falls as T, k or E rise. Calls that may overlap (two streams, two graphs) bring one workspace each. */
 uint64_t vlb_sort_tokens_workspace_bytes(uint32_t T, uint32_t k, uint32_t E);
 int vlb_sort_tokens_device(vlb_handle* h, const vlb_sort_tokens_desc* desc, void* stream);
 
@@ -789,7 +790,7 @@ int vlb_combine_device(vlb_handle* h, const vlb_combine_desc* desc, void* stream
  *     drows[elem_row[t][s]] = weights[t][s] dout[t],   dweights[t][s] = sum_c dout[t]_c rows[elem_row[t][s]]_c
  * dweights is 0 where elem_row >= n_rows; rows of drows that no pair names are left as they were. Each
  * row is named once at most, as vlb_sort_tokens_device leaves it (of a row named twice, drows holds
- * either pair's). rows (for dweights alone) and drows of `type`, dout of out_type; drows may be the
+ * either pair's, element by element). rows (for dweights alone) and drows of `type`, dout of out_type; drows may be the
  * rows' own memory (same address and stride). drows or dweights may be NULL, not both. Sums run in a
  * fixed order. */
 typedef struct vlb_combine_grad_desc {
