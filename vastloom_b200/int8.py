@@ -60,6 +60,8 @@ class Int8Experts:
         dev = self.dev
         sources = [s if isinstance(s, Matrix) else np.ascontiguousarray(s, dtype=np.float32) for s in sources]
         shapes = [(s.rows, s.cols) if isinstance(s, Matrix) else s.shape for s in sources]
+        if any(len(shape) != 2 for shape in shapes):
+            raise ValueError(f"a source must be a matrix, not of shape {next(s for s in shapes if len(s) != 2)}")
         n, cols = sum(shape[0] for shape in shapes), shapes[0][1]
         if (any(shape[1] != self.cols for shape in shapes) or not 0 <= row0 <= self.rows - n or
                 not 0 <= group < self.weights.groups or (order is not None and (order.size != n or len(set(shapes)) > 1))):
