@@ -5,7 +5,7 @@
 //   gradient   n = h s,  g = dy w,  d = s (g - n mean(g n)) + dh,  dw = sum over rows of dy n
 //
 // Both move every element once and do a dozen operations on it: HBM bounds them. The sums are in 32 bits.
-// Where the squares pass them (h above 1.8e19) the row is taken again with h lifted by 2^-70.
+// Where the squares pass them (h above 1.8e19) the row is taken again with h lifted by 2^-100.
 //
 // Rows come as pieces of V neighbouring elements (16 bytes of the wider type), ROW threads a row, KEEP pieces
 // a thread. A matrix whose stride is no multiple of V has its rows at V different offsets from a 16-byte
@@ -25,7 +25,10 @@
 namespace vlb {
 namespace {
 
-constexpr float kNormLift = 0x1p-70f;
+// Holds over the whole range: the largest h becomes 2^28, and 2^30 such squares stay below 2^86; a row that gets
+// here has a sum of 2^128 at least, lifted 2^-72 and its mean 2^-102, far above the subnormals (eps, where lifted it
+// underflows, is below 2^-45 of the mean). s itself is subnormal once the mean passes 2^252: within 2^-22 then.
+constexpr float kNormLift = 0x1p-100f;
 
 // The rings' shared memory an SM, threads and CTAs an SM, and depth: as many rows as a CTA's share holds of
 // `bytes` a thread, at most 6.
