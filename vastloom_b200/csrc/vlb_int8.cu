@@ -39,6 +39,9 @@ __device__ __forceinline__ float swiglu(float g, float u, float limit) {
 // z = sum * x_scale * w_scale + bias, y = row_weight * act(z) + residual, the same operations in the same
 // order in every form of the product.
 
+// Added where there is no residual: it leaves every value as it is, a -0 too, as the tiles' plain product does.
+constexpr float kNoResidual = -0.f;
+
 __device__ __forceinline__ float epi_sum(int32_t sum, float x_scale, float w_scale, float bias) {
     return fmaf((float)sum * x_scale, w_scale, bias);
 }
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(256) int8_linear_kernel(const Int8LinearParams
                         const float a = pairs ? swiglu(z, up, p.act_limit) : activate(z, p.act);
                         const float res = p.residual
                                               ? to_float(static_cast<const TY*>(p.residual)[(size_t)r * p.residual_stride + c])
-                                              : 0.f;
+                                              : kNoResidual;
                         static_cast<TY*>(p.y)[(size_t)r * p.y_stride + c] = from_float<TY>(fmaf(rw, a, res));
                     }
                     continue;
@@ -641,7 +644,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(GROUPED)) int8_few_ker
                 else
                     a = activate(a, l.act);
                 const uint32_t to = pairs ? c / 2u : c;
-                const float res = l.residual ? load_typed(l.residual, r * l.residual_stride + to, y_type) : 0.f;
+                const float res = l.residual ? load_typed(l.residual, r * l.residual_stride + to, y_type) : kNoResidual;
                 store_typed(l.y, r * l.y_stride + to, fmaf(l.row_weight ? l.row_weight[r] : 1.f, a, res), y_type);
             }
             if (n + 2u * kFewWarps < n_end) fetch_scales(n + 2u * kFewWarps);
@@ -1291,7 +1294,7 @@ __global__ void __launch_bounds__(mm_threads(MODE, EPI, sizeof(TY)), 1) int8_mma
                                 if (n + i >= l.out_cols || (pairs && (i & 1u))) continue;
                                 const uint32_t to = pairs ? (n + i) / 2u : n + i;
                                 const float a = pairs ? swiglu(z[i], z[i | 1u], l.act_limit) : activate(z[i], l.act);
-                                const float res = from ? to_float(from[r * l.residual_stride + to]) : 0.f;
+                                const float res = from ? to_float(from[r * l.residual_stride + to]) : kNoResidual;
                                 static_cast<TY*>(l.y)[r * l.y_stride + to] = from_float<TY>(fmaf(rw, a, res));
                             }
                             continue;
