@@ -551,34 +551,35 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(GROUPED)) int8_few_ker
         const auto value = [&](uint32_t c) {
             return q.up ? row_value<T, true>(q, base + c) : row_value<T, false>(q, base + c);
         };
-        // a lane's first kFewKeep elements stay in registers between the row's maximum and its rounding
+        // a lane's first kFewKeep elements stay in registers between the row's maximum and its rounding, four at a time
+        // as far as the row goes (all sixteen for a row of 512 took a lone one 2.7 -> 2.8 us, of SwiGLU 3.0 -> 3.5)
         constexpr uint32_t kFewKeep = 16;
         float kept[kFewKeep];
         const uint32_t step = row_warps * 32u;
+        const auto each = [&](auto&& f) {
+#pragma unroll
+            for (uint32_t i0 = 0; i0 < kFewKeep; i0 += 4u) {
+                if (i0 * step >= pitch) break;
+#pragma unroll
+                for (uint32_t i = i0; i < i0 + 4u; ++i) f(i);
+            }
+        };
         uint32_t most = 0;
         {
-            T a[kFewKeep];  // all loads first
-#pragma unroll
-            for (uint32_t i = 0; i < kFewKeep; ++i) {
-                a[i] = from_float<T>(0.f);
-                if (have && part + i * step < l.cols) a[i] = static_cast<const T*>(q.x)[base + part + i * step];
-            }
+            T a[kFewKeep], b[kFewKeep];  // all loads first
+            const auto load = [&](const void* from, uint32_t i) {
+                const uint32_t c = part + i * step;
+                return have && c < l.cols ? static_cast<const T*>(from)[base + c] : from_float<T>(0.f);
+            };
+            each([&](uint32_t i) { a[i] = load(q.x, i); });
             if (q.up) {
-                T b[kFewKeep];
-#pragma unroll
-                for (uint32_t i = 0; i < kFewKeep; ++i) {
-                    b[i] = from_float<T>(0.f);
-                    if (have && part + i * step < l.cols) b[i] = static_cast<const T*>(q.up)[base + part + i * step];
-                }
-#pragma unroll
-                for (uint32_t i = 0; i < kFewKeep; ++i) kept[i] = swiglu(to_float(a[i]), to_float(b[i]), q.limit);
+                each([&](uint32_t i) { b[i] = load(q.up, i); });
+                each([&](uint32_t i) { kept[i] = swiglu(to_float(a[i]), to_float(b[i]), q.limit); });
             } else {
-#pragma unroll
-                for (uint32_t i = 0; i < kFewKeep; ++i) kept[i] = to_float(a[i]);
+                each([&](uint32_t i) { kept[i] = to_float(a[i]); });
             }
         }
-#pragma unroll
-        for (uint32_t i = 0; i < kFewKeep; ++i) most = max(most, __float_as_uint(kept[i]) & 0x7fffffffu);
+        each([&](uint32_t i) { most = max(most, __float_as_uint(kept[i]) & 0x7fffffffu); });
         if (have)
 #pragma unroll 8
             for (uint32_t c = part + kFewKeep * step; c < l.cols; c += step)
@@ -588,9 +589,9 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(GROUPED)) int8_few_ker
         __syncthreads();
         const RowStep st = row_step(top[m]);
         if (m < rows && part == 0) scale[m] = !EPI && l.row_weight ? st.scale * l.row_weight[r] : st.scale;
-#pragma unroll
-        for (uint32_t i = 0; i < kFewKeep; ++i)
+        each([&](uint32_t i) {
             if (part + i * step < pitch) xs[m * pitch + part + i * step] = (int8_t)quant_byte(kept[i], st);
+        });
 #pragma unroll 8
         for (uint32_t c = part + kFewKeep * step; c < pitch; c += step)
             xs[m * pitch + c] = (int8_t)(have && c < l.cols ? quant_byte(value(c), st) : 0u);
