@@ -1789,7 +1789,7 @@ static int int8_linear(vlb_handle* h, const vlb_int8_linear_desc* desc, const vl
             return bad("a pointer is not aligned to its elements");
         if (d.w_stride < d.cols || d.y_stride < y_cols || d.w_stride > (1ull << 38) || d.y_stride > (1ull << 38))
             return bad("a stride is out of range");
-        Int8LinearParams p{};
+        Int8ActParams p{};
         p.row_weight = d.row_weight;
         p.w = d.w;
         p.w_scale = d.w_scale;

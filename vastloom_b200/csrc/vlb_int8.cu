@@ -42,6 +42,9 @@ __device__ __forceinline__ float swiglu(float g, float u, float limit) {
 // Added where there is no residual: it leaves every value as it is, a -0 too, as the tiles' plain product does.
 constexpr float kNoResidual = -0.f;
 
+template <bool EPI>
+using LinearParams = std::conditional_t<EPI, Int8ActParams, Int8LinearParams>;
+
 __device__ __forceinline__ float epi_sum(int32_t sum, float x_scale, float w_scale, float bias) {
     return fmaf((float)sum * x_scale, w_scale, bias);
 }
@@ -374,7 +377,7 @@ __device__ __forceinline__ uint32_t load_word(const int8_t* row, uint32_t c, uin
 }
 
 template <typename TY, bool EPI>
-__global__ void __launch_bounds__(256) int8_linear_kernel(const Int8LinearParams p) {
+__global__ void __launch_bounds__(256) int8_linear_kernel(const LinearParams<EPI> p) {
     __shared__ uint32_t xs[kGenTile][kGenK / 4 + 1], ws[kGenTile][kGenK / 4 + 1];
     tc::grid_dependency_wait();
     tc::grid_launch_dependents();
@@ -480,7 +483,7 @@ __device__ __forceinline__ void store_typed(void* y, size_t at, float v, int typ
 
 // T: the rows' type, int8_t for rows that are integers already. ROWS: rows of a block.
 template <typename T, uint32_t ROWS, bool EPI, bool GROUPED>
-__global__ void __launch_bounds__(kFewThreads, few_blocks(GROUPED)) int8_few_kernel(const Int8LinearParams l, const Int8QuantParams q, int y_type,
+__global__ void __launch_bounds__(kFewThreads, few_blocks(GROUPED)) int8_few_kernel(const LinearParams<EPI> l, const Int8QuantParams q, int y_type,
                                                                uint32_t channels) {
     constexpr uint32_t kFewPieces = few_pieces(GROUPED);
     extern __shared__ __align__(16) unsigned char few_smem[];
@@ -522,14 +525,16 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(GROUPED)) int8_few_ker
     // of a SwiGLU pair both), not after the sums
     [[maybe_unused]] float ws[2] = {}, bs[2] = {};
     [[maybe_unused]] const auto fetch_scales = [&](uint32_t n) {
-        const bool pairs = l.act == VLB_ACT_SWIGLU;
-        const uint32_t c = n + (pairs ? 0u : lane / ROWS);
-        const size_t at = (size_t)g * l.out_cols + c;
+        if constexpr (EPI) {
+            const bool pairs = l.act == VLB_ACT_SWIGLU;
+            const uint32_t c = n + (pairs ? 0u : lane / ROWS);
+            const size_t at = (size_t)g * l.out_cols + c;
 #pragma unroll
-        for (uint32_t i = 0; i < 2u; ++i) {
-            if (lane >= 2u * ROWS || c + i >= l.out_cols || (i && !pairs)) continue;
-            ws[i] = l.w_scale[at + i];
-            if (l.bias) bs[i] = l.bias[at + i];
+            for (uint32_t i = 0; i < 2u; ++i) {
+                if (lane >= 2u * ROWS || c + i >= l.out_cols || (i && !pairs)) continue;
+                ws[i] = l.w_scale[at + i];
+                if (l.bias) bs[i] = l.bias[at + i];
+            }
         }
     };
     if (EPI && n < n_end) fetch_scales(n);
@@ -688,9 +693,10 @@ constexpr uint32_t kMmMaxStages = 12;
 constexpr uint32_t kMmSmemLimit = 227u * 1024u;
 constexpr uint64_t kMmWaitNs = 2000000000ull;
 
+template <bool EPI>
 struct Int8MmaParams {
     CUtensorMap wmap, xmap;
-    Int8LinearParams l;
+    LinearParams<EPI> l;
     uint32_t width;     // most tokens a tile takes (a multiple of 16)
     uint32_t box;       // rows of the token operand's TMA box
     uint32_t stages, x_stage;
@@ -762,7 +768,8 @@ __device__ __forceinline__ void mm_fail(volatile uint32_t* abort, const Int8Line
     mm_report(l);
 }
 
-__device__ __forceinline__ MmTile mm_tile(const MmShared& sh, const Int8MmaParams& p, uint32_t t) {
+template <bool EPI>
+__device__ __forceinline__ MmTile mm_tile(const MmShared& sh, const Int8MmaParams<EPI>& p, uint32_t t) {
     const uint32_t u = t / p.ct;
     uint32_t a = 0, b = p.l.groups;  // last g with first[g] <= u; groups without rows have no tiles
     while (b - a > 1u) {
@@ -777,16 +784,138 @@ __device__ __forceinline__ MmTile mm_tile(const MmShared& sh, const Int8MmaParam
     return MmTile{a, sh.lo[a] + j * each + min(j, more), each + (j < more ? 1u : 0u), c * p.channels};
 }
 
+// A tile's way out with an epilogue (functions of their own: as lambdas of the kernel, which without an epilogue does
+// not call them, they cost that form 0.2 us a launch).
+
+// Whether `ok` holds in the four warps of a turn; each of them comes here once a tile, its waits behind it.
+__device__ __forceinline__ bool all_of_turn(bool ok, uint32_t warp) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %1, 0;\n\t"
+        "barrier.cta.red.and.pred p, %2, 128, q;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(all)
+        : "r"(ok ? 1u : 0u), "r"(1u + (warp >> 2))
+        : "memory");
+    return all != 0;
+}
+
+// 16 tokens from c on of the CTA's 128 channels (64 columns of y for SwiGLU), with an epilogue: the four warps of a
+// turn. act(z) goes to shared memory, and comes back in rows of y: 16 bytes a thread of neighbouring columns, with
+// the residual's loaded before. (Stored from where the sums are, a channel a lane, the tokens' rows are 64 bytes a
+// store: 4096 x 4096 x 4096 f16 with GELU and a residual 88 us, so 68.)
+template <typename TY, bool PAIR, bool WIDE_Y>
+__device__ __forceinline__ void finish(const Int8ActParams& l, float* out, const float (&v)[16], const MmTile& tile, uint32_t c,
+                                       uint32_t warp, uint32_t rank, const float* ts, const float* rw, float cs, float bias) {
+    constexpr uint32_t E = 16u / sizeof(TY);
+    const uint32_t lane = threadIdx.x & 31u, quad = warp & 3u, turn = warp >> 2, t = threadIdx.x & 127u, count = min(tile.count - c, 16u);
+    const auto put = [&](auto act, auto whole) {
+        constexpr int ACT = decltype(act)::value;
+        // WIDE: 16 bytes a thread; rows of y at any offset: neighbouring lanes on neighbouring columns
+        constexpr bool PAIRS = ACT == VLB_ACT_SWIGLU, WIDE = decltype(whole)::value;
+        constexpr uint32_t kEach = WIDE ? E : 1u, kCols = PAIRS ? 64u : 128u;
+        constexpr uint32_t kPitch = PAIRS ? 80u : 128u;  // the pitch keeps pairs off each other's banks
+        constexpr uint32_t kAcross = kCols / kEach, kRows = 128u / kAcross, kPasses = 16u / kRows;
+        float* at = out + turn * (16u * kMmChannels);
+        const uint32_t y_cols = PAIRS ? l.out_cols / 2u : l.out_cols;
+        const uint32_t col = (tile.channel0 + (PAIR ? rank * kMmChannels : 0u)) / (PAIRS ? 2u : 1u) + t % kAcross * kEach;
+        const uint32_t n_cols = col < y_cols ? min(kEach, y_cols - col) : 0u;
+        const uint32_t row0 = t / kAcross, rows = n_cols ? count : 0u;  // of this thread: row0, row0 + kRows, ..
+        const size_t r0 = tile.row0 + c + row0;
+        Pack<TY, kEach> res[kPasses];
+        if (l.residual) {
+            const TY* from = static_cast<const TY*>(l.residual) + r0 * l.residual_stride + col;
+#pragma unroll
+            for (uint32_t i = 0; i < kPasses; ++i) {
+                if (row0 + i * kRows < rows) {
+                    if (n_cols == kEach) {
+                        res[i] = *reinterpret_cast<const Pack<TY, kEach>*>(from);
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < kEach; ++j)
+                            if (j < n_cols) res[i].v[j] = from[j];
+                    }
+                }
+                from += kRows * l.residual_stride;
+            }
+        }
+        const float4* t4 = reinterpret_cast<const float4*>(ts + c);
+        const uint32_t odd = lane & 1u;  // of a pair's lanes the even one takes the even tokens
+#pragma unroll
+        for (uint32_t i0 = 0; i0 < 16u; i0 += 4u) {
+            const float4 s4 = t4[i0 / 4u];
+            float z[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; ++j) z[j] = epi_sum(__float_as_int(v[i0 + j]), (&s4.x)[j], cs, bias);
+            if constexpr (PAIRS) {
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; j += 2u) {  // one exchange for two tokens
+                    const float other = __shfl_xor_sync(0xffffffffu, odd ? z[j] : z[j + 1u], 1);
+                    at[(i0 + j + odd) * kPitch + 16u * quad + lane / 2u] =
+                        swiglu(odd ? other : z[j], odd ? z[j + 1u] : other, l.act_limit);
+                }
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; ++j) at[(i0 + j) * kPitch + 32u * quad + lane] = activate<ACT>(z[j]);
+            }
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(1u + turn) : "memory");
+        TY* y = static_cast<TY*>(l.y) + r0 * l.y_stride + col;
+#pragma unroll
+        for (uint32_t i = 0; i < kPasses; ++i) {
+            const uint32_t row = row0 + i * kRows;
+            float f[kEach];
+            const Pack<float, kEach> sums = *reinterpret_cast<const Pack<float, kEach>*>(at + row * kPitch + t % kAcross * kEach);
+            unpack(sums, f);
+            const float w = rw[c + row];
+            if (l.residual) {
+                float g[kEach];
+                unpack(res[i], g);
+#pragma unroll
+                for (uint32_t j = 0; j < kEach; ++j) f[j] = fmaf(w, f[j], g[j]);
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < kEach; ++j) f[j] *= w;
+            }
+            const Pack<TY, kEach> row_y = pack<TY>(f);
+            if (row < rows) {
+                if (n_cols == kEach) {
+                    *reinterpret_cast<Pack<TY, kEach>*>(y) = row_y;
+                } else {
+#pragma unroll
+                    for (uint32_t j = 0; j < kEach; ++j)
+                        if (j < n_cols) y[j] = row_y.v[j];
+                }
+            }
+            y += kRows * l.y_stride;
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(1u + turn) : "memory");
+    };
+    // one branch for all of them, whose chains then run side by side
+    const auto by_act = [&](auto whole) {
+        switch (l.act) {
+            case VLB_ACT_RELU: return put(std::integral_constant<int, VLB_ACT_RELU>{}, whole);
+            case VLB_ACT_SILU: return put(std::integral_constant<int, VLB_ACT_SILU>{}, whole);
+            case VLB_ACT_GELU: return put(std::integral_constant<int, VLB_ACT_GELU>{}, whole);
+            case VLB_ACT_GELU_TANH: return put(std::integral_constant<int, VLB_ACT_GELU_TANH>{}, whole);
+            case VLB_ACT_SWIGLU: return put(std::integral_constant<int, VLB_ACT_SWIGLU>{}, whole);
+            default: return put(std::integral_constant<int, VLB_ACT_NONE>{}, whole);
+        }
+    };
+    by_act(std::integral_constant<bool, WIDE_Y>{});
+}
+
 // WIDE_Y: with an epilogue, rows of y and of the residual lie on 16-byte boundaries (a kernel of its own: the other form's
 // registers would spill into it).
 template <typename TY, Mm MODE, bool EPI, bool WIDE_Y>
-__global__ void __launch_bounds__(mm_threads(MODE, EPI, sizeof(TY)), 1) int8_mma_kernel(const __grid_constant__ Int8MmaParams p) {
+__global__ void __launch_bounds__(mm_threads(MODE, EPI, sizeof(TY)), 1) int8_mma_kernel(const __grid_constant__ Int8MmaParams<EPI> p) {
     constexpr bool SPLIT = MODE == Mm::kSplit, PAIR = MODE == Mm::kPair;
     constexpr uint32_t kEpi = mm_epi_warps(MODE, EPI, sizeof(TY));
     extern __shared__ __align__(1024) unsigned char mm_smem[];
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
     const uint32_t smem = tc::smem_u32(mm_smem), stage_bytes = kMmWStage + p.x_stage;
-    const Int8LinearParams& l = p.l;
+    const LinearParams<EPI>& l = p.l;
     MmShared sh;
     {
         unsigned char* at = mm_smem + p.stages * stage_bytes;
@@ -1012,122 +1141,6 @@ __global__ void __launch_bounds__(mm_threads(MODE, EPI, sizeof(TY)), 1) int8_mma
         ++it;
         return true;
     };
-    // Whether `ok` holds in the four warps of a turn; each of them comes here once a tile, its waits behind it.
-    [[maybe_unused]] auto all_of_turn = [&](bool ok) -> bool {
-        uint32_t all;
-        asm volatile(
-            "{\n\t.reg .pred p, q;\n\t"
-            "setp.ne.u32 q, %1, 0;\n\t"
-            "barrier.cta.red.and.pred p, %2, 128, q;\n\t"
-            "selp.b32 %0, 1, 0, p;\n\t}"
-            : "=r"(all)
-            : "r"(ok ? 1u : 0u), "r"(1u + (warp >> 2))
-            : "memory");
-        return all != 0;
-    };
-    // 16 tokens from c on of the CTA's 128 channels (64 columns of y for SwiGLU), with an epilogue: the four warps of a
-    // turn. act(z) goes to shared memory, and comes back in rows of y: 16 bytes a thread of neighbouring columns, with
-    // the residual's loaded before. (Stored from where the sums are, a channel a lane, the tokens' rows are 64 bytes a
-    // store: 4096 x 4096 x 4096 f16 with GELU and a residual 88 us, so 68.)
-    [[maybe_unused]] auto finish = [&](const float (&v)[16], const MmTile& tile, uint32_t c, const float* ts, const float* rw,
-                                       float cs, float bias) {
-        constexpr uint32_t E = 16u / sizeof(TY);
-        const uint32_t turn = warp >> 2, t = tid & 127u, count = min(tile.count - c, 16u);
-        const auto put = [&](auto act, auto whole) {
-            constexpr int ACT = decltype(act)::value;
-            // WIDE: 16 bytes a thread; rows of y at any offset: neighbouring lanes on neighbouring columns
-            constexpr bool PAIRS = ACT == VLB_ACT_SWIGLU, WIDE = decltype(whole)::value;
-            constexpr uint32_t kEach = WIDE ? E : 1u, kCols = PAIRS ? 64u : 128u;
-            constexpr uint32_t kPitch = PAIRS ? 80u : 128u;  // the pitch keeps pairs off each other's banks
-            constexpr uint32_t kAcross = kCols / kEach, kRows = 128u / kAcross, kPasses = 16u / kRows;
-            float* at = sh.out + turn * (16u * kMmChannels);
-            const uint32_t y_cols = PAIRS ? l.out_cols / 2u : l.out_cols;
-            const uint32_t col = (tile.channel0 + (PAIR ? rank * kMmChannels : 0u)) / (PAIRS ? 2u : 1u) + t % kAcross * kEach;
-            const uint32_t n_cols = col < y_cols ? min(kEach, y_cols - col) : 0u;
-            const uint32_t row0 = t / kAcross, rows = n_cols ? count : 0u;  // of this thread: row0, row0 + kRows, ..
-            const size_t r0 = tile.row0 + c + row0;
-            Pack<TY, kEach> res[kPasses];
-            if (l.residual) {
-                const TY* from = static_cast<const TY*>(l.residual) + r0 * l.residual_stride + col;
-#pragma unroll
-                for (uint32_t i = 0; i < kPasses; ++i) {
-                    if (row0 + i * kRows < rows) {
-                        if (n_cols == kEach) {
-                            res[i] = *reinterpret_cast<const Pack<TY, kEach>*>(from);
-                        } else {
-#pragma unroll
-                            for (uint32_t j = 0; j < kEach; ++j)
-                                if (j < n_cols) res[i].v[j] = from[j];
-                        }
-                    }
-                    from += kRows * l.residual_stride;
-                }
-            }
-            const float4* t4 = reinterpret_cast<const float4*>(ts + c);
-            const uint32_t odd = lane & 1u;  // of a pair's lanes the even one takes the even tokens
-#pragma unroll
-            for (uint32_t i0 = 0; i0 < 16u; i0 += 4u) {
-                const float4 s4 = t4[i0 / 4u];
-                float z[4];
-#pragma unroll
-                for (uint32_t j = 0; j < 4u; ++j) z[j] = epi_sum(__float_as_int(v[i0 + j]), (&s4.x)[j], cs, bias);
-                if constexpr (PAIRS) {
-#pragma unroll
-                    for (uint32_t j = 0; j < 4u; j += 2u) {  // one exchange for two tokens
-                        const float other = __shfl_xor_sync(0xffffffffu, odd ? z[j] : z[j + 1u], 1);
-                        at[(i0 + j + odd) * kPitch + 16u * quad + lane / 2u] =
-                            swiglu(odd ? other : z[j], odd ? z[j + 1u] : other, l.act_limit);
-                    }
-                } else {
-#pragma unroll
-                    for (uint32_t j = 0; j < 4u; ++j) at[(i0 + j) * kPitch + 32u * quad + lane] = activate<ACT>(z[j]);
-                }
-            }
-            asm volatile("bar.sync %0, 128;" ::"r"(1u + turn) : "memory");
-            TY* y = static_cast<TY*>(l.y) + r0 * l.y_stride + col;
-#pragma unroll
-            for (uint32_t i = 0; i < kPasses; ++i) {
-                const uint32_t row = row0 + i * kRows;
-                float f[kEach];
-                const Pack<float, kEach> sums = *reinterpret_cast<const Pack<float, kEach>*>(at + row * kPitch + t % kAcross * kEach);
-                unpack(sums, f);
-                const float w = rw[c + row];
-                if (l.residual) {
-                    float g[kEach];
-                    unpack(res[i], g);
-#pragma unroll
-                    for (uint32_t j = 0; j < kEach; ++j) f[j] = fmaf(w, f[j], g[j]);
-                } else {
-#pragma unroll
-                    for (uint32_t j = 0; j < kEach; ++j) f[j] *= w;
-                }
-                const Pack<TY, kEach> out = pack<TY>(f);
-                if (row < rows) {
-                    if (n_cols == kEach) {
-                        *reinterpret_cast<Pack<TY, kEach>*>(y) = out;
-                    } else {
-#pragma unroll
-                        for (uint32_t j = 0; j < kEach; ++j)
-                            if (j < n_cols) y[j] = out.v[j];
-                    }
-                }
-                y += kRows * l.y_stride;
-            }
-            asm volatile("bar.sync %0, 128;" ::"r"(1u + turn) : "memory");
-        };
-        // one branch for all of them, whose chains then run side by side
-        const auto by_act = [&](auto whole) {
-            switch (l.act) {
-                case VLB_ACT_RELU: return put(std::integral_constant<int, VLB_ACT_RELU>{}, whole);
-                case VLB_ACT_SILU: return put(std::integral_constant<int, VLB_ACT_SILU>{}, whole);
-                case VLB_ACT_GELU: return put(std::integral_constant<int, VLB_ACT_GELU>{}, whole);
-                case VLB_ACT_GELU_TANH: return put(std::integral_constant<int, VLB_ACT_GELU_TANH>{}, whole);
-                case VLB_ACT_SWIGLU: return put(std::integral_constant<int, VLB_ACT_SWIGLU>{}, whole);
-                default: return put(std::integral_constant<int, VLB_ACT_NONE>{}, whole);
-            }
-        };
-        by_act(std::integral_constant<bool, WIDE_Y>{});
-    };
     auto epilogue = [&]() -> bool {
         const uint32_t buf = it & 1u, use = it >> 1;
         const float* ts = sh.scale + buf * kMmMaxTokens;
@@ -1136,7 +1149,7 @@ __global__ void __launch_bounds__(mm_threads(MODE, EPI, sizeof(TY)), 1) int8_mma
         const float cs = sh.channel[buf * kMmChannels + 32u * quad + lane];
         const uint32_t n = tile.channel0 + (PAIR ? rank * kMmChannels : 0u) + 32u * quad + lane;
         ok = ok && __all_sync(0xffffffffu, mm_wait(sh.acc_full + buf, use & 1u, sh.abort));
-        if constexpr (EPI) ok = all_of_turn(ok);  // the four warps go on to their barriers, or give up, together
+        if constexpr (EPI) ok = all_of_turn(ok, warp);  // the four warps go on to their barriers, or give up, together
         if (ok) {
             tc::fence_after_sync();
             const uint32_t src = tmem + buf * p.acc_cols + ((32u * quad) << 16);
@@ -1146,7 +1159,7 @@ __global__ void __launch_bounds__(mm_threads(MODE, EPI, sizeof(TY)), 1) int8_mma
                     float v[16];
                     tc::tmem_ld16(src + c, v);
                     tc::tmem_wait_ld();
-                    finish(v, tile, c, ts, sh.weight + buf * kMmMaxTokens, cs, bias);
+                    finish<TY, PAIR, WIDE_Y>(l, sh.out, v, tile, c, warp, rank, ts, sh.weight + buf * kMmMaxTokens, cs, bias);
                 }
             }
             // 32 columns (tokens) at a time, the warps of a lane quarter taking turns
@@ -1242,7 +1255,7 @@ __global__ void __launch_bounds__(mm_threads(MODE, EPI, sizeof(TY)), 1) int8_mma
                 for (uint32_t i = 0; i < 4u; ++i) {
                     const uint32_t n = tile.channel0 + 4u * lane + i;
                     cs[i] = n < l.out_cols ? l.w_scale[(size_t)tile.g * l.out_cols + n] : 0.f;
-                    if (EPI && l.bias && n < l.out_cols) bs[i] = l.bias[(size_t)tile.g * l.out_cols + n];
+                    if constexpr (EPI) bs[i] = l.bias && n < l.out_cols ? l.bias[(size_t)tile.g * l.out_cols + n] : 0.f;
                 }
                 if (ok) {
                     tc::fence_after_sync();
@@ -1370,7 +1383,7 @@ cudaError_t quantize_type(const Int8QuantParams& p, cudaStream_t s) {
 }
 
 template <typename TY, bool EPI>
-cudaError_t general_type(const Int8LinearParams& p, cudaStream_t s) {
+cudaError_t general_type(const LinearParams<EPI>& p, cudaStream_t s) {
     const uint32_t tiles_n = (p.out_cols + kGenTile - 1u) / kGenTile, tiles_r = (p.rows + kGenTile - 1u) / kGenTile;
     const dim3 grid(tiles_n, tiles_r < 1024u ? tiles_r : 1024u, p.groups < 1024u ? p.groups : 1024u);
     return launch_chained(int8_linear_kernel<TY, EPI>, grid, 256, 0, 0, s, p);
@@ -1411,7 +1424,8 @@ bool tma_rows(const int8_t* p, size_t stride) {
 }
 
 // Tile width, split or pairs of a product on the tensor cores. Returns the mode.
-Mm mma_plan(Int8MmaParams& p, uint32_t sms, size_t y_size) {
+template <bool EPI>
+Mm mma_plan(Int8MmaParams<EPI>& p, uint32_t sms, size_t y_size) {
     const Int8LinearParams& l = p.l;
     p.nk = (l.cols + kMmKc - 1u) / kMmKc;
     const auto split_of = [&](uint64_t tiles) {
@@ -1482,14 +1496,14 @@ Mm mma_plan(Int8MmaParams& p, uint32_t sms, size_t y_size) {
     p.acc_cols = p.width < 32u ? 32u : p.width;
     p.tmem_cols = 32;
     while (p.tmem_cols < (mode == Mm::kSplit ? 1u : 2u) * p.acc_cols) p.tmem_cols *= 2u;
-    const uint32_t room = kMmSmemLimit - 1024u - mm_fixed_bytes(l.groups, mode, l.act != kInt8NoEpilogue, y_size);
+    const uint32_t room = kMmSmemLimit - 1024u - mm_fixed_bytes(l.groups, mode, EPI, y_size);
     p.stages = room / (kMmWStage + p.x_stage);
     if (p.stages > kMmMaxStages) p.stages = kMmMaxStages;
     return mode;
 }
 
 template <typename TY, Mm MODE, bool EPI>
-cudaError_t mma_launch(const Int8MmaParams& p, uint32_t sms, bool wide, cudaStream_t s) {
+cudaError_t mma_launch(const Int8MmaParams<EPI>& p, uint32_t sms, bool wide, cudaStream_t s) {
     constexpr bool kForms = EPI && MODE != Mm::kSplit;  // a split's sums take another way out
     auto* kernel = wide && kForms ? int8_mma_kernel<TY, MODE, EPI, kForms> : int8_mma_kernel<TY, MODE, EPI, false>;
     const uint32_t in_cluster = MODE == Mm::kSplit ? p.split : MODE == Mm::kPair ? 2u : 1u;
@@ -1510,7 +1524,7 @@ constexpr uint32_t kFewRows = 8, kFewGroupedRows = 24, kFewElements = 8192;
 constexpr uint64_t kFewWork = 1u << 24;
 
 template <typename T, uint32_t ROWS, bool EPI, bool GROUPED = false>
-cudaError_t few_launch(const Int8LinearParams& l, const Int8QuantParams& q, int y_type, uint32_t sms, cudaStream_t s) {
+cudaError_t few_launch(const LinearParams<EPI>& l, const Int8QuantParams& q, int y_type, uint32_t sms, cudaStream_t s) {
     auto* kernel = int8_few_kernel<T, ROWS, EPI, GROUPED>;
     const size_t smem = (size_t)ROWS * ((l.cols + 15u) / 16u * 16u);
     if (smem > kFewDefaultSmem) {
@@ -1525,7 +1539,7 @@ cudaError_t few_launch(const Int8LinearParams& l, const Int8QuantParams& q, int 
 }
 
 template <typename T, bool EPI>
-cudaError_t few_rows(const Int8LinearParams& l, const Int8QuantParams& q, int y_type, cudaStream_t s) {
+cudaError_t few_rows(const LinearParams<EPI>& l, const Int8QuantParams& q, int y_type, cudaStream_t s) {
     const uint32_t rows = l.rows, sms = sm_count();
     if (l.offsets) return few_launch<T, 1, EPI, true>(l, q, y_type, sms, s);
     if (rows <= 1u) return few_launch<T, 1, EPI>(l, q, y_type, sms, s);
@@ -1535,15 +1549,16 @@ cudaError_t few_rows(const Int8LinearParams& l, const Int8QuantParams& q, int y_
 }
 
 template <typename TY, bool EPI>
-cudaError_t linear_type(const Int8LinearParams& l, bool after_quantize, cudaStream_t s) {
+cudaError_t linear_type(const LinearParams<EPI>& l, bool after_quantize, cudaStream_t s) {
     if (tma_rows(l.w, l.w_stride) && tma_rows(l.x, l.x_stride)) {
-        Int8MmaParams p{};
+        Int8MmaParams<EPI> p{};
         p.l = l;
         p.early = after_quantize;
         const auto on16 = [](const void* at, size_t stride) {
             return reinterpret_cast<uintptr_t>(at) % 16u == 0 && stride * sizeof(TY) % 16u == 0;
         };
-        const bool wide = EPI && on16(l.y, l.y_stride) && (!l.residual || on16(l.residual, l.residual_stride));
+        bool wide = false;
+        if constexpr (EPI) wide = on16(l.y, l.y_stride) && (!l.residual || on16(l.residual, l.residual_stride));
         const uint32_t sms = sm_count();
         const Mm mode = mma_plan(p, sms, sizeof(TY));
         if (encode_rows(&p.wmap, l.w, (uint64_t)l.groups * l.out_cols, l.cols, l.w_stride, kMmChannels) &&
@@ -1582,7 +1597,7 @@ bool int8_few(const Int8LinearParams& l) {
 }
 
 template <bool EPI>
-static cudaError_t few_typed(const Int8LinearParams& l, const Int8QuantParams& q, int x_type, int y_type, cudaStream_t s) {
+static cudaError_t few_typed(const LinearParams<EPI>& l, const Int8QuantParams& q, int x_type, int y_type, cudaStream_t s) {
     switch (x_type) {
         case VLB_DTYPE_F32: return few_rows<float, EPI>(l, q, y_type, s);
         case VLB_DTYPE_F16: return few_rows<__half, EPI>(l, q, y_type, s);
@@ -1590,12 +1605,12 @@ static cudaError_t few_typed(const Int8LinearParams& l, const Int8QuantParams& q
         default: return few_rows<int8_t, EPI>(l, q, y_type, s);
     }
 }
-cudaError_t launch_int8_few(const Int8LinearParams& l, const Int8QuantParams& q, int x_type, int y_type, cudaStream_t s) {
+cudaError_t launch_int8_few(const Int8ActParams& l, const Int8QuantParams& q, int x_type, int y_type, cudaStream_t s) {
     return l.act == kInt8NoEpilogue ? few_typed<false>(l, q, x_type, y_type, s) : few_typed<true>(l, q, x_type, y_type, s);
 }
 
 template <bool EPI>
-static cudaError_t linear_typed(const Int8LinearParams& p, int y_type, bool after_quantize, cudaStream_t s) {
+static cudaError_t linear_typed(const LinearParams<EPI>& p, int y_type, bool after_quantize, cudaStream_t s) {
     switch (y_type) {
         case VLB_DTYPE_F32: return linear_type<float, EPI>(p, after_quantize, s);
         case VLB_DTYPE_F16: return linear_type<__half, EPI>(p, after_quantize, s);
@@ -1603,7 +1618,7 @@ static cudaError_t linear_typed(const Int8LinearParams& p, int y_type, bool afte
         default: return cudaErrorInvalidValue;
     }
 }
-cudaError_t launch_int8_linear(const Int8LinearParams& p, int y_type, bool after_quantize, cudaStream_t s) {
+cudaError_t launch_int8_linear(const Int8ActParams& p, int y_type, bool after_quantize, cudaStream_t s) {
     return p.act == kInt8NoEpilogue ? linear_typed<false>(p, y_type, after_quantize, s)
                                     : linear_typed<true>(p, y_type, after_quantize, s);
 }

@@ -163,7 +163,10 @@ struct Int8LinearParams {
     uint32_t* error;           // the handle's word in host memory: 1 once a wait has run out
     size_t x_stride, w_stride, y_stride;
     uint32_t rows, cols, out_cols, groups;
-    // the epilogue of vlb_int8_linear_act_device; act < 0: none of it
+};
+// With the epilogue of vlb_int8_linear_act_device; act < 0: none of it, and the kernels get the part above alone (they
+// read what they are given anew at each launch: 32 bytes more took one row of 512 x 512 2.02 -> 2.08 us).
+struct Int8ActParams : Int8LinearParams {
     const float* bias;         // [groups x out_cols] or null
     const void* residual;      // rows of y's type or null
     size_t residual_stride;
@@ -177,9 +180,9 @@ cudaError_t launch_int8_quantize(const Int8QuantParams& p, int x_type, cudaStrea
 // A product of few rows in one launch, its rows quantized on the way (q: their source, x_type I8:
 // unused); int8_few: whether it takes the call.
 bool int8_few(const Int8LinearParams& l);
-cudaError_t launch_int8_few(const Int8LinearParams& l, const Int8QuantParams& q, int x_type, int y_type, cudaStream_t s);
+cudaError_t launch_int8_few(const Int8ActParams& l, const Int8QuantParams& q, int x_type, int y_type, cudaStream_t s);
 // after_quantize: launch_int8_quantize went before it on the stream (the product may start beside it)
-cudaError_t launch_int8_linear(const Int8LinearParams& p, int y_type, bool after_quantize, cudaStream_t s);
+cudaError_t launch_int8_linear(const Int8ActParams& p, int y_type, bool after_quantize, cudaStream_t s);
 
 // ---- the router's balance loss (vlb_balance.cu) ----
 struct BalanceParams {
