@@ -454,7 +454,9 @@ __global__ void __launch_bounds__(256) int8_linear_kernel(const LinearParams<EPI
 constexpr uint32_t kFewThreads = 256, kFewWarps = kFewThreads / 32u;
 // Pieces of a channel in flight, and blocks an SM. A group's row has registers for twice the blocks, whose set-up then
 // overlaps (16 rows of 64 experts' 2048 x 2048: 4 pieces and 2 blocks 19.2 us, 2 and 4 14.8); one row of one matrix fills
-// no more than two an SM (4096 x 4096: 2 pieces and 4 blocks 6.8 us, 4 and 2 6.2).
+// no more than two an SM (int8 rows, 2 pieces and 4 blocks / 4 and 2: 512 x 512 2.0 / 1.9 us, 2048 x 2048 3.4 / 2.9, 4096 x
+// 4096 6.0 / 5.2, 8192 x 8192 13.8 / 13.8). 128 registers are short of 4 and 8 rows with an epilogue: 56 to 92 bytes
+// a thread spill.
 __host__ __device__ constexpr uint32_t few_pieces(bool grouped) { return grouped ? 2u : 4u; }
 __host__ __device__ constexpr uint32_t few_blocks(bool grouped) { return grouped ? 4u : 2u; }
 constexpr uint32_t kFewSmem = 64u * 1024u;
@@ -682,9 +684,10 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(GROUPED)) int8_few_ker
 
 enum class Mm { kOne, kSplit, kPair };
 constexpr uint32_t kMmChannels = 128, kMmMaxTokens = 256, kMmKc = 128;
-// Warps that take the sums to memory: more where an epilogue's operations come on top, as many as registers are for
-// (elements of 2 bytes 16, of 4 12; what 8 warps hold in flight does not cover the operations' latency: 4096 x 4096 x 4096
-// f16 with GELU 96 us with 8, 67 with 16).
+// Warps that take the sums to memory: more where an epilogue's operations come on top (elements of 2 bytes 16, of 4 12;
+// what 8 warps hold in flight does not cover the operations' latency: 4096 x 4096 x 4096 f16 with GELU 96 us with 8, 67
+// with 16). The registers that leaves are enough where rows of y lie on 16 bytes (up to 8 bytes a thread spill); off
+// them 2-byte elements spill 204 bytes a thread, in pairs 156.
 __host__ __device__ constexpr uint32_t mm_epi_warps(Mm mode, bool epi, size_t element) {
     return !epi || mode == Mm::kSplit ? 8u : element == 2u ? 16u : 12u;
 }

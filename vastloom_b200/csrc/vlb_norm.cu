@@ -248,9 +248,11 @@ __global__ void __launch_bounds__(ROW) add_norm_kernel(const NormParams p) {
     }
 }
 
-// Many rows: persistent CTAs, DEPTH rows ahead on their way to shared memory, since the registers that h and w
+// Many rows: persistent CTAs, DEPTH - 1 rows ahead on their way to shared memory, since the registers that h and w
 // take leave too few threads to hold enough loads in flight themselves. 16,384 x 4096 bf16, h and y written:
-// a CTA a row from registers 126 us, rings 85 (6.3 TB/s).
+// a CTA a row from registers 126 us, rings 85 (6.3 TB/s). Rows of f32 past 8192 columns fill a ring (DEPTH 1) and none
+// is ahead; it still reads each row once, which registers do not: 2048 x 12,288 f32 76 us for 90, 2048 x 16,384 95 for
+// 131 (5.3 and 5.7 TB/s).
 template <typename T, typename R, uint32_t ROW, uint32_t KEEP, uint32_t DEPTH, bool SHIFTED>
 __global__ void __launch_bounds__(norm_threads(ROW), norm_ctas(ROW, KEEP * 16u / sizeof(R), SHIFTED)) add_norm_ring_kernel(const NormParams p) {
     constexpr uint32_t V = 16u / sizeof(R), kThreads = norm_threads(ROW), kRows = kThreads / ROW, kStep = ROW * V;
@@ -432,8 +434,9 @@ __global__ void __launch_bounds__(ROW) norm_grad_kernel(const NormGradParams p) 
     if (p.dw) norm_grad_part<V, ROW, KEEP, ROW>(p, c0, acc, nullptr);
 }
 
-// Many rows, as add_norm_ring_kernel; a CTA an SM, so that few parts are left. 8192 x 4096 bf16 with dh and dw:
-// from registers 156 us, rings 49 with the sum of the parts (5.5 TB/s).
+// Many rows, as add_norm_ring_kernel (rows past 8192 columns with an f32 residual fill a ring too: 2048 x 16,384 f32 93 us,
+// read again 220); a CTA an SM, so that few parts are left. 8192 x 4096 bf16 with dh and dw: from registers 156 us,
+// rings 48 with the sum of the parts (5.6 TB/s).
 template <typename T, typename R, uint32_t ROW, uint32_t KEEP, uint32_t DEPTH, bool SHIFTED>
 __global__ void __launch_bounds__(kGradThreads, 1) norm_grad_ring_kernel(const NormGradParams p) {
     constexpr uint32_t V = 16u / sizeof(R), kThreads = kGradThreads, kRows = kThreads / ROW, kStep = ROW * V;
@@ -600,7 +603,10 @@ struct Shape {
     static constexpr uint32_t V = V_, ROW = ROW_, KEEP = KEEP_;
 };
 
-// Rows from which a ring pays: below, a CTA of more threads a row is over sooner.
+// Rows from which rings are taken. Below, a CTA of more threads a row is over sooner (registers / ring: 32 x 2048 f32 1.9 /
+// 2.2 us, gradient 3.8 / 5.5); at 64 that still holds for short rows (64 x 2048 f32 2.0 / 2.3, gradient 4.0 / 5.6; 64 x
+// 4096 bf16 2.4 / 2.4, 7.0 / 7.1) and no longer for long ones (64 x 16,384 f32 8.9 / 7.5, 23.6 / 12.7; 64 x 8192 bf16
+// 4.3 / 3.9, 11.9 / 8.3). From 512 rows on rings are ahead or within a tenth at every width from 256 to 16,384.
 constexpr uint32_t kNormRingRows = 64, kGradRingRows = 64;
 
 template <typename T, typename R>

@@ -715,11 +715,14 @@ cudaError_t combine_typed(const CombineParams& p, cudaStream_t s) {
         return launch_chained(kernel, dim3(item_blocks((uint64_t)p.T * segments, lanes)), 256, 0, 0, s, p, segments);
     };
     if (pieces <= 16u) return whole ? run(combine_kernel<T, O, 8, 2, 2, false>, 8, 2) : run(combine_kernel<T, O, 8, 2, 2, true>, 8, 2);
-    if ((uint64_t)p.T * pieces <= (1u << 17))  // few tokens: a piece a lane, all slots at once
+    // few tokens: a piece a lane, all slots at once (8 slots of 2048 bf16 onto f32, this way / below: 64 tokens 3.4 / 4.5 us,
+    // 256 5.1 / 6.7, 512 9.2 / 7.8; of two slots, which need no more in flight, 64 3.0 / 2.6, 512 7.8 / 4.6)
+    if ((uint64_t)p.T * pieces <= (1u << 17))
         return whole ? run(combine_kernel<T, O, 32, 1, 8, false>, 32, 1) : run(combine_kernel<T, O, 32, 1, 4, true>, 32, 1);
     // Two pieces of two slots a lane in flight and 32 warps an SM (shifted 24) rather than more of both and 16 warps: 16,384
     // tokens of 2048 bf16 onto f32 with 8 slots 129 us (four of four 137), with two 66 (86); shifted,
-    // of 1001 bf16, 83 us, in 16 warps 92, one piece of two or four slots 89 and 100.
+    // of 1001 bf16, 83 us, in 16 warps 92, one piece of two or four slots 89 and 100. The 64 (80) registers of so many warps
+    // spill: 16-bit rows onto f32 48 bytes a thread, shifted 124, onto 16 bits 84; f32 12 and 48.
     return whole ? run(combine_kernel<T, O, 32, 2, 2, false>, 32, 2) : run(combine_kernel<T, O, 32, 2, 2, true>, 32, 2);
 }
 
